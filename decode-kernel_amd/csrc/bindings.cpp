@@ -60,6 +60,8 @@ void check_gemv_inputs(const torch::Tensor& packed, const torch::Tensor& scales,
 
 }  // namespace
 
+#include "bindings_kv.hpp"
+
 torch::Tensor gemv_common(const torch::Tensor& packed, const torch::Tensor& scales,
                           const torch::Tensor& x, int version, int split_k, bool reuse_weights, int warps_per_row);
 
@@ -390,5 +392,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("workspace_bytes", &workspace_bytes, "Device workspace bytes a GEMV call needs",
         py::arg("M"), py::arg("K"), py::arg("B"), py::arg("version") = 5, py::arg("split_k") = 4,
         py::arg("reuse_weights") = false, py::arg("warps_per_row") = 1);
+  define_kv(m);
   m.attr("ABI_VERSION") = dk_abi_version();
 }

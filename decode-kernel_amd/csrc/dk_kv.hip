@@ -1,0 +1,565 @@
+// The paged 8-bit key/value cache: planning a step, appending and reading.
+// Layouts in dk_kv.hpp, contracts in include/decode_kernel/dk_kv.h.
+#include <hip/hip_runtime.h>
+
+#include "dk_host.hpp"
+#include "dk_kv.hpp"
+
+namespace dk {
+
+// ---------------------------------------------------------------------------
+// Plan: from request lengths to offsets, pages and slots, in one launch.
+//
+// Every workgroup scans all requests into LDS (tokens, then pages, since the
+// pages follow from the tokens that fit) and then serves its own tokens, one
+// a thread: the request by bisection, the page from the table or, for a page
+// that the step opens, from the free list at the rank that the scan gives. A
+// token at a page's first place writes the table's entry, so no token waits
+// for another. A few kilobytes: latency alone.
+// ---------------------------------------------------------------------------
+constexpr int kPlanThreads = 256;
+
+// Exclusive scan of one value a thread; the total in *total.
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, T* wave_sums, T* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  T inc = v;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const T o = __shfl_up(inc, d);
+    if (lane >= d) inc += o;
+  }
+  __syncthreads();  // wave_sums may be in use from the scan before
+  if (lane == 63) wave_sums[wave] = inc;
+  __syncthreads();
+  T before = 0, sum = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; ++w) {
+    if (w < wave) before += wave_sums[w];
+    sum += wave_sums[w];
+  }
+  *total = sum;
+  return before + inc - v;
+}
+
+struct PlanArgs {
+  int32_t* tables;
+  const int32_t* held;
+  const int32_t* added;
+  const int32_t* free_pages;
+  const int32_t* free_count;
+  int64_t* slots;
+  int32_t* positions;
+  int32_t* query_offsets;
+  int32_t* seq_lens;
+  int32_t* free_count_out;
+  int width, requests, capacity, page_shift, tokens;
+};
+
+__device__ __forceinline__ int pages_of(long long tokens, int shift) {
+  return (int)((tokens + (1 << shift) - 1) >> shift);
+}
+
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
+  __shared__ int offs[DK_KV_MAX_REQUESTS + 1];   // where request b's tokens start
+  __shared__ int ranks[DK_KV_MAX_REQUESTS];      // pages opened before request b
+  __shared__ long long token_sums[kPlanThreads / 64];
+  __shared__ int page_sums[kPlanThreads / 64];
+  const int tid = threadIdx.x;
+  const int each = (a.requests + kPlanThreads - 1) / kPlanThreads;
+  const int b0 = min(tid * each, a.requests), b1 = min(b0 + each, a.requests);
+  const long long room = (long long)a.width << a.page_shift;
+
+  long long mine = 0, all;
+  for (int b = b0; b < b1; ++b) mine += max(a.added[b], 0);
+  long long at = block_scan(mine, token_sums, &all);
+  for (int b = b0; b < b1; ++b) {
+    offs[b] = (int)min(at, (long long)a.tokens);
+    at += max(a.added[b], 0);
+  }
+  if (tid == 0) offs[a.requests] = (int)min(all, (long long)a.tokens);
+  __syncthreads();
+
+  int pages = 0, opened;
+  for (int b = b0; b < b1; ++b) {
+    const long long had = max(a.held[b], 0);
+    const long long len = min(had + offs[b + 1] - offs[b], room);
+    ranks[b] = pages;
+    pages += max(pages_of(len, a.page_shift) - pages_of(had, a.page_shift), 0);
+    if (blockIdx.x == 0) {
+      a.seq_lens[b] = (int)len;
+      a.query_offsets[b] = offs[b];
+    }
+  }
+  const int first = block_scan(pages, page_sums, &opened);
+  for (int b = b0; b < b1; ++b) ranks[b] += first;
+  if (blockIdx.x == 0 && tid == 0) {
+    a.query_offsets[a.requests] = offs[a.requests];
+    *a.free_count_out = *a.free_count - opened;
+  }
+  __syncthreads();
+
+  const int t = blockIdx.x * kPlanThreads + tid;
+  if (t >= a.tokens) return;
+  if (t >= offs[a.requests]) {
+    a.slots[t] = -1;
+    a.positions[t] = -1;
+    return;
+  }
+  int lo = 0, hi = a.requests - 1;  // the first request that ends after t
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (offs[mid + 1] > t) hi = mid;
+    else lo = mid + 1;
+  }
+  const long long had = max(a.held[lo], 0);
+  const long long pos = had + t - offs[lo];
+  const long long col = pos >> a.page_shift;
+  const int in_page = (int)(pos & ((1 << a.page_shift) - 1));
+  long long slot = -1;
+  if (col < a.width) {
+    int32_t* entry = a.tables + (long long)lo * a.width + col;
+    const int fresh = (int)col - pages_of(had, a.page_shift);
+    int page;
+    if (fresh >= 0) {
+      const int i = min(*a.free_count, a.capacity) - 1 - (ranks[lo] + fresh);
+      page = i >= 0 ? a.free_pages[i] : -1;
+      if (in_page == 0) *entry = page;
+    } else {
+      page = *entry;
+    }
+    if (page >= 0) slot = ((long long)page << a.page_shift) + in_page;
+  }
+  a.slots[t] = slot;
+  a.positions[t] = (int)min(pos, (long long)INT32_MAX);
+}
+
+// ---------------------------------------------------------------------------
+// Append: one wave quantises one run (a page's new tokens) of one head, keys
+// or values. A workgroup looks for runs that start among its `scan` tokens.
+// ---------------------------------------------------------------------------
+struct AppendArgs {
+  KvView c;
+  const uint16_t* k;
+  const uint16_t* v;
+  long long kt, kh, vt, vh;  // strides of tokens and heads, elements
+  const int64_t* slots;
+  int tokens;
+};
+
+constexpr int kAppendWaves = 4;
+
+// The new tokens of one page: token t0 + i goes to place off + i, for i < n
+// with bit i of hi:lo (the others have no slot).
+struct Run {
+  unsigned long long lo, hi;
+  int t0, n, page, off;
+  __device__ __forceinline__ bool has(int i) const { return ((i < 64 ? lo : hi) >> (i & 63)) & 1; }
+};
+
+// Largest of non-negative floats as bits: NaN above infinity above the rest.
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d));
+  return v;
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float f) {
+  return __builtin_bit_cast(uint32_t, f) & 0x7FFFFFFFu;
+}
+
+__device__ __forceinline__ int quantise(float x, float inv) {
+  // fminf/fmaxf drop a NaN, so a code is in range whatever comes in.
+  return (int)fminf(fmaxf(rintf(x * inv), -kCodeMax), kCodeMax);
+}
+
+__device__ __forceinline__ uint32_t requantise_word(uint32_t w, float ratio) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r |= ((uint32_t)quantise((float)code_of(w, i), ratio) & 0xFFu) << (8 * i);
+  return r;
+}
+
+// The scale a page gets, from the old one and the new tokens' largest bits.
+struct PageScale {
+  float scale, inv, ratio;
+  bool grew;
+};
+__device__ __forceinline__ PageScale page_scale(float old, uint32_t amax) {
+  PageScale s;
+  // An infinity counts as a NaN: the page's values for this head are NaN then.
+  const float top = amax >= 0x7F800000u ? __builtin_nanf("")
+                                        : __builtin_bit_cast(float, amax) * (1.0f / kCodeMax);
+  const uint32_t ob = abs_bits(old), tb = abs_bits(top);
+  s.grew = tb > ob;
+  s.scale = __builtin_bit_cast(float, max(ob, tb));
+  s.inv = s.scale >= 0x1p-126f ? 1.0f / s.scale : 0.0f;
+  s.ratio = old * s.inv;
+  return s;
+}
+
+template <int D, bool kBf16>
+__device__ void append_keys(const AppendArgs& a, const Run& run, int head, int lane) {
+  const int n = run.n, off = run.off;
+  constexpr int kC = D / 16;  // 16-element pieces a token
+  const int P = 1 << a.c.page_shift;
+  const uint16_t* x = a.k + (long long)run.t0 * a.kt + (long long)head * a.kh;
+  uint32_t amax = 0;
+  for (int u = lane; u < n * kC; u += 64) {
+    if (!run.has(u / kC)) continue;
+    const uint4* p = reinterpret_cast<const uint4*>(x + (long long)(u / kC) * a.kt + (u % kC) * 16);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 w = p[h];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t we = e == 0 ? w.x : e == 1 ? w.y : e == 2 ? w.z : w.w;
+        amax = max(amax, max(abs_bits(pair_lo<kBf16>(we)), abs_bits(pair_hi<kBf16>(we))));
+      }
+    }
+  }
+  amax = wave_max_bits(amax);
+  const long long ph = (long long)run.page * a.c.heads + head;
+  const float old = off == 0 ? 0.0f : a.c.ks[ph];
+  const PageScale s = page_scale(old, amax);
+  uint4* codes = reinterpret_cast<uint4*>(a.c.k + ph * D * P);
+  if (s.grew) {
+    for (int u = lane; u < off * kC; u += 64) {
+      uint4* c = codes + (u % kC) * P + u / kC;
+      uint4 w = *c;
+      w = make_uint4(requantise_word(w.x, s.ratio), requantise_word(w.y, s.ratio),
+                     requantise_word(w.z, s.ratio), requantise_word(w.w, s.ratio));
+      *c = w;
+    }
+    if (lane == 0) a.c.ks[ph] = s.scale;
+  } else if (off == 0 && lane == 0) {
+    a.c.ks[ph] = s.scale;
+  }
+  for (int u = lane; u < n * kC; u += 64) {
+    if (!run.has(u / kC)) continue;
+    const uint4* p = reinterpret_cast<const uint4*>(x + (long long)(u / kC) * a.kt + (u % kC) * 16);
+    uint32_t out[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 w = p[h];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t we = e == 0 ? w.x : e == 1 ? w.y : e == 2 ? w.z : w.w;
+        const uint32_t lo = (uint32_t)quantise(pair_lo<kBf16>(we), s.inv) & 0xFFu;
+        const uint32_t hi = (uint32_t)quantise(pair_hi<kBf16>(we), s.inv) & 0xFFu;
+        out[2 * h + e / 2] |= (lo | hi << 8) << (16 * (e & 1));
+      }
+    }
+    codes[(u % kC) * P + off + u / kC] = make_uint4(out[0], out[1], out[2], out[3]);
+  }
+}
+
+// Values: a lane has two elements of 16 consecutive tokens of the page, which
+// are two 16-byte pieces, so the transposition costs no shuffle.
+template <int D, bool kBf16>
+__device__ void append_values(const AppendArgs& a, const Run& run, int head, int lane) {
+  const int n = run.n, off = run.off;
+  constexpr int kPairs = D / 2;
+  constexpr int kSide = 64 / kPairs;  // groups of 16 tokens a wave does at once
+  const int P = 1 << a.c.page_shift;
+  const int d = 2 * (lane % kPairs);
+  const uint16_t* x = a.v + (long long)run.t0 * a.vt + (long long)head * a.vh + d;
+  const int g0 = off >> 4, g1 = (off + n + 15) >> 4;
+  uint32_t amax = 0;
+  for (int g = g0 + lane / kPairs; g < g1; g += kSide) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int t = g * 16 + i - off;
+      if (t >= 0 && t < n && run.has(t)) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(x + (long long)t * a.vt);
+        amax = max(amax, max(abs_bits(pair_lo<kBf16>(w)), abs_bits(pair_hi<kBf16>(w))));
+      }
+    }
+  }
+  amax = wave_max_bits(amax);
+  const long long ph = (long long)run.page * a.c.heads + head;
+  const float old = off == 0 ? 0.0f : a.c.vs[ph];
+  const PageScale s = page_scale(old, amax);
+  if (lane == 0 && (s.grew || off == 0)) a.c.vs[ph] = s.scale;
+  uint4* codes = reinterpret_cast<uint4*>(a.c.v + ph * D * P + (long long)d * P);
+  const int row = P / 16;  // pieces from one element to the next
+  for (int g = (s.grew ? 0 : g0) + lane / kPairs; g < g1; g += kSide) {
+    uint32_t w[2][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const uint4 c = codes[r * row + g];
+      w[r][0] = c.x, w[r][1] = c.y, w[r][2] = c.z, w[r][3] = c.w;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int t = g * 16 + i - off;
+      const int sh = 8 * (i & 3);
+      if (t < 0) {
+        if (s.grew) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            uint32_t& y = w[r][i >> 2];
+            const uint32_t q = (uint32_t)quantise((float)code_of(y, i & 3), s.ratio) & 0xFFu;
+            y = (y & ~(0xFFu << sh)) | q << sh;
+          }
+        }
+      } else if (t < n && run.has(t)) {
+        const uint32_t xx = *reinterpret_cast<const uint32_t*>(x + (long long)t * a.vt);
+        const uint32_t q0 = (uint32_t)quantise(pair_lo<kBf16>(xx), s.inv) & 0xFFu;
+        const uint32_t q1 = (uint32_t)quantise(pair_hi<kBf16>(xx), s.inv) & 0xFFu;
+        w[0][i >> 2] = (w[0][i >> 2] & ~(0xFFu << sh)) | q0 << sh;
+        w[1][i >> 2] = (w[1][i >> 2] & ~(0xFFu << sh)) | q1 << sh;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) codes[r * row + g] = make_uint4(w[r][0], w[r][1], w[r][2], w[r][3]);
+  }
+}
+
+__device__ __forceinline__ bool in_cache(const AppendArgs& a, long long slot) {
+  return slot >= 0 && slot >> a.c.page_shift < a.c.pages;
+}
+
+// Whether token t, which has a slot, is its page's first one in this step.
+__device__ __forceinline__ bool starts_run(const AppendArgs& a, int t, long long slot) {
+  const int off = (int)(slot & ((1 << a.c.page_shift) - 1));
+  for (int k = 1; k <= min(t, off); ++k) {  // back over tokens without a slot
+    const long long s = a.slots[t - k];
+    if (s == slot - k) return false;
+    if (in_cache(a, s)) return true;
+  }
+  return true;
+}
+
+template <int D, bool kBf16>
+__global__ __launch_bounds__(kAppendWaves * 64) void append_kernel(AppendArgs a, int scan) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int head = blockIdx.y;
+  const int base = blockIdx.x * scan;  // scan <= 64
+  const int P = 1 << a.c.page_shift;
+  bool starts = false;
+  if (lane < scan && lane < a.tokens - base) {
+    const long long slot = a.slots[base + lane];
+    starts = in_cache(a, slot) && starts_run(a, base + lane, slot);
+  }
+  unsigned long long mask = __ballot(starts);
+  for (int i = 0; mask; ++i, mask &= mask - 1) {
+    if (i % kAppendWaves != wave) continue;
+    Run run;
+    run.t0 = base + __builtin_ctzll(mask);
+    const long long slot = a.slots[run.t0];
+    run.page = (int)(slot >> a.c.page_shift);
+    run.off = (int)(slot & (P - 1));
+    // The tokens that follow on in the page, over those without a slot.
+    run.n = 0;
+    const int most = min(P - run.off, a.tokens - run.t0);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const int j = 64 * w + lane;
+      const long long s = j < most ? a.slots[run.t0 + j] : 0;
+      const bool mine = j < most && s == slot + j;
+      const bool on = mine || (j < most && !in_cache(a, s));
+      const unsigned long long follow = run.n == 64 * w ? __ballot(on) : 0;
+      const int c = follow == ~0ull ? 64 : __builtin_ctzll(~follow);
+      run.n += c;
+      (w ? run.hi : run.lo) = __ballot(mine) & (c == 64 ? ~0ull : (1ull << c) - 1);
+    }
+    if (blockIdx.z == 0)
+      append_keys<D, kBf16>(a, run, head, lane);
+    else
+      append_values<D, kBf16>(a, run, head, lane);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Read: 16 lanes a token and head, 8 elements a lane.
+// ---------------------------------------------------------------------------
+struct ReadArgs {
+  KvView c;
+  const int64_t* slots;
+  void* k;
+  void* v;
+  int tokens;
+};
+
+template <int kDtype>
+__device__ __forceinline__ void store8(void* out, long long at, const float (&x)[8]) {
+  if constexpr (kDtype == DK_KV_F32) {
+    float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
+    o[0] = make_float4(x[0], x[1], x[2], x[3]);
+    o[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = to_half_bits<kDtype>(x[2 * i]) | (uint32_t)to_half_bits<kDtype>(x[2 * i + 1]) << 16;
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+template <int D, int kDtype>
+__global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
+  constexpr int kLanes = D / 8;
+  const int P = 1 << a.c.page_shift;
+  const int head = blockIdx.y;
+  const int t = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const int d = threadIdx.x % kLanes * 8;
+  if (t >= a.tokens) return;
+  const long long slot = a.slots[t];
+  const long long page = slot >> a.c.page_shift;
+  const int off = (int)(slot & (P - 1));
+  const bool ok = slot >= 0 && page < a.c.pages;
+  const long long ph = ok ? page * a.c.heads + head : 0;
+  const long long out = ((long long)t * a.c.heads + head) * D + d;
+  float x[8] = {};
+  if (blockIdx.z == 0) {
+    if (ok) {
+      const uint2 w = *reinterpret_cast<const uint2*>(a.c.k + ph * D * P + ((d / 16) * P + off) * 16 + d % 16);
+      const float s = a.c.ks[ph];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = (float)code_of(i < 4 ? w.x : w.y, i & 3) * s;
+    }
+    store8<kDtype>(a.k, out, x);
+  } else {
+    if (ok) {
+      const int8_t* c = a.c.v + ph * D * P + (long long)d * P + off;
+      const float s = a.c.vs[ph];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = (float)c[i * P] * s;
+    }
+    store8<kDtype>(a.v, out, x);
+  }
+}
+
+}  // namespace dk
+
+namespace {
+
+bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+int page_shift(int page_size) {
+  switch (page_size) {
+    case 16: return 4;
+    case 32: return 5;
+    case 64: return 6;
+    case 128: return 7;
+    default: return -1;
+  }
+}
+
+}  // namespace
+
+namespace dk {
+
+int kv_view(const dk_kv_cache* c, KvView* view) {
+  if (!c) return set_error(DK_ERR_INVALID_ARGUMENT, "cache must not be NULL");
+  const int shift = page_shift(c->page_size);
+  if (shift < 0)
+    return set_error(DK_ERR_INVALID_ARGUMENT, "page_size=%d must be 16, 32, 64 or 128", c->page_size);
+  if (c->head_size != 64 && c->head_size != 128)
+    return set_error(DK_ERR_INVALID_ARGUMENT, "head_size=%d must be 64 or 128", c->head_size);
+  if (c->pages < 0 || c->heads < 1 || c->heads > 65535)
+    return set_error(DK_ERR_INVALID_ARGUMENT, "the cache needs pages >= 0 and 1..65535 heads");
+  if (c->pages > 0) {
+    if (!c->k_codes || !c->v_codes || !c->k_scales || !c->v_scales)
+      return set_error(DK_ERR_INVALID_ARGUMENT, "the cache's codes and scales must not be NULL");
+    if (!aligned(c->k_codes, 16) || !aligned(c->v_codes, 16) || !aligned(c->k_scales, 4) ||
+        !aligned(c->v_scales, 4))
+      return set_error(DK_ERR_INVALID_ARGUMENT,
+                       "the cache's codes must be 16-byte and its scales 4-byte aligned");
+  }
+  *view = KvView{c->k_codes, c->v_codes, c->k_scales, c->v_scales, c->pages, c->heads, shift};
+  return DK_OK;
+}
+
+}  // namespace dk
+
+extern "C" int dk_kv_plan(int32_t* tables, int table_width, const int32_t* held,
+                          const int32_t* added, int requests, const int32_t* free_pages,
+                          int free_capacity, const int32_t* free_count, int page_size,
+                          int num_tokens, int64_t* slots, int32_t* positions,
+                          int32_t* query_offsets, int32_t* seq_lens, int32_t* free_count_out,
+                          hipStream_t stream) {
+  const int shift = page_shift(page_size);
+  if (shift < 0)
+    return dk::set_error(DK_ERR_INVALID_ARGUMENT, "page_size=%d must be 16, 32, 64 or 128", page_size);
+  if (requests < 0 || requests > DK_KV_MAX_REQUESTS)
+    return dk::set_error(DK_ERR_INVALID_ARGUMENT, "requests must be in [0, %d]", DK_KV_MAX_REQUESTS);
+  if (table_width < 0 || num_tokens < 0 || free_capacity < 0)
+    return dk::set_error(DK_ERR_INVALID_ARGUMENT,
+                         "table_width, num_tokens and free_capacity must be >= 0");
+  if (((long long)table_width << shift) > INT32_MAX)
+    return dk::set_error(DK_ERR_INVALID_ARGUMENT, "table_width * page_size must fit in int32");
+  if (!query_offsets || !free_count || !free_count_out ||
+      (requests > 0 && (!held || !added || !seq_lens)) ||
+      (requests > 0 && table_width > 0 && !tables) || (num_tokens > 0 && (!slots || !positions)) ||
+      (free_capacity > 0 && !free_pages))
+    return dk::set_error(DK_ERR_INVALID_ARGUMENT, "plan's arrays must not be NULL");
+  if (free_count == free_count_out)
+    return dk::set_error(DK_ERR_INVALID_ARGUMENT, "free_count_out must not be free_count");
+  const dk::PlanArgs a{tables, held, added, free_pages, free_count, slots, positions,
+                       query_offsets, seq_lens, free_count_out, table_width, requests,
+                       free_capacity, shift, num_tokens};
+  const unsigned blocks = num_tokens == 0 ? 1u : (unsigned)((num_tokens - 1) / dk::kPlanThreads + 1);
+  hipLaunchKernelGGL(dk::plan_kernel, dim3(blocks), dim3(dk::kPlanThreads), 0, stream, a);
+  return dk::check_launch("plan launch");
+}
+
+extern "C" int dk_kv_append(const dk_kv_cache* cache, const void* k, const void* v, int dtype,
+                            long long k_token_stride, long long k_head_stride,
+                            long long v_token_stride, long long v_head_stride,
+                            const int64_t* slots, int num_tokens, hipStream_t stream) {
+  dk::KvView view;
+  if (const int rc = dk::kv_view(cache, &view)) return rc;
+  if (dtype != DK_KV_F16 && dtype != DK_KV_BF16)
+    return dk::set_error(DK_ERR_INVALID_ARGUMENT, "k and v must be fp16 or bf16");
+  if (num_tokens < 0) return dk::set_error(DK_ERR_INVALID_ARGUMENT, "num_tokens must be >= 0");
+  if (num_tokens == 0 || cache->pages == 0) return DK_OK;
+  if (!k || !v || !slots) return dk::set_error(DK_ERR_INVALID_ARGUMENT, "k, v and slots must not be NULL");
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(slots, 8))
+    return dk::set_error(DK_ERR_INVALID_ARGUMENT, "k and v must be 16-byte, slots 8-byte aligned");
+  if (k_token_stride % 8 || k_head_stride % 8 || v_token_stride % 8 || v_head_stride % 8)
+    return dk::set_error(DK_ERR_INVALID_ARGUMENT, "the strides of k and v must be multiples of 8");
+  const dk::AppendArgs a{view, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
+                         k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots,
+                         num_tokens};
+  const int scan = num_tokens <= 1024 ? 4 : 16;
+  const dim3 grid((unsigned)((num_tokens - 1) / scan + 1), (unsigned)view.heads, 2);
+  const dim3 block(dk::kAppendWaves * 64);
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a, scan); };
+  if (cache->head_size == 64)
+    dtype == DK_KV_BF16 ? launch(dk::append_kernel<64, true>) : launch(dk::append_kernel<64, false>);
+  else
+    dtype == DK_KV_BF16 ? launch(dk::append_kernel<128, true>) : launch(dk::append_kernel<128, false>);
+  return dk::check_launch("append launch");
+}
+
+extern "C" int dk_kv_read(const dk_kv_cache* cache, const int64_t* slots, int num_tokens, int dtype,
+                          void* k, void* v, hipStream_t stream) {
+  dk::KvView view;
+  if (const int rc = dk::kv_view(cache, &view)) return rc;
+  if (dtype != DK_KV_F16 && dtype != DK_KV_BF16 && dtype != DK_KV_F32)
+    return dk::set_error(DK_ERR_INVALID_ARGUMENT, "dtype must be fp16, bf16 or fp32");
+  if (num_tokens < 0) return dk::set_error(DK_ERR_INVALID_ARGUMENT, "num_tokens must be >= 0");
+  if (num_tokens == 0) return DK_OK;
+  if (!k || !v || !slots) return dk::set_error(DK_ERR_INVALID_ARGUMENT, "k, v and slots must not be NULL");
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(slots, 8))
+    return dk::set_error(DK_ERR_INVALID_ARGUMENT, "k and v must be 16-byte, slots 8-byte aligned");
+  const dk::ReadArgs a{view, slots, k, v, num_tokens};
+  auto launch = [&](auto kernel, int lanes) {
+    const int each = 256 / lanes;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((num_tokens - 1) / each + 1), (unsigned)view.heads, 2),
+                       dim3(256), 0, stream, a);
+  };
+  if (cache->head_size == 64) {
+    if (dtype == DK_KV_F16) launch(dk::read_kernel<64, DK_KV_F16>, 8);
+    else if (dtype == DK_KV_BF16) launch(dk::read_kernel<64, DK_KV_BF16>, 8);
+    else launch(dk::read_kernel<64, DK_KV_F32>, 8);
+  } else {
+    if (dtype == DK_KV_F16) launch(dk::read_kernel<128, DK_KV_F16>, 16);
+    else if (dtype == DK_KV_BF16) launch(dk::read_kernel<128, DK_KV_BF16>, 16);
+    else launch(dk::read_kernel<128, DK_KV_F32>, 16);
+  }
+  return dk::check_launch("read launch");
+}

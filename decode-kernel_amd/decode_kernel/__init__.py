@@ -9,7 +9,9 @@ and calling `gemv` without the built extension raises ImportError.
 `mlp_decode`, `gate_up_silu` and `QuantizedMLP` (decode_kernel.mlp) run a
 Llama-style MLP decode step on the same kernels (include/decode_kernel/dk_mlp.h);
 `repack_paired` / `gemv_paired` (decode_kernel.layout) use the kernel-native
-paired weight layout.
+paired weight layout. `KVCache`, `plan_kv_step`, `append_kv`, `read_kv` and
+`attend_kv` (decode_kernel.kv) are the paged 8-bit key/value cache and the
+attention over it (include/decode_kernel/dk_kv.h).
 """
 
 from __future__ import annotations
@@ -19,20 +21,27 @@ from typing import Optional
 import torch
 
 from ._native import ext as _ext
+from .kv import KVCache, KVStep, append_kv, attend_kv, plan_kv_step, read_kv
 from .layout import gemv_paired, repack_paired, unpack_paired
 from .mlp import QuantizedMLP, gate_up_silu, mlp_decode
 from .quantize import GROUP_SIZE, dequantize, quantize_and_pack
 
 __all__ = [
     "GROUP_SIZE",
+    "KVCache",
+    "KVStep",
     "QuantizedMLP",
+    "append_kv",
+    "attend_kv",
     "cuda_available",
     "dequantize",
     "gate_up_silu",
     "gemv",
     "gemv_paired",
     "mlp_decode",
+    "plan_kv_step",
     "quantize_and_pack",
+    "read_kv",
     "repack_paired",
     "unpack_paired",
     "w4a16_linear",

@@ -1,4 +1,4 @@
-"""ctypes view of the C ABI in include/decode_kernel/dk_gemv.h and dk_mlp.h.
+"""ctypes view of the C ABI in include/decode_kernel/dk_gemv.h, dk_mlp.h and dk_kv.h.
 
 This is the binding a non-torch host (or a maintainer wiring the library into
 another runtime) would write: plain pointers, sizes and a hipStream_t handle.
@@ -41,6 +41,24 @@ class LaunchInfo(ctypes.Structure):
         ("launches", ctypes.c_int),
     ]
 
+
+class KvCache(ctypes.Structure):
+    """Mirror of dk_kv_cache."""
+
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p),
+        ("v_codes", ctypes.c_void_p),
+        ("k_scales", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p),
+        ("pages", ctypes.c_int),
+        ("heads", ctypes.c_int),
+        ("head_size", ctypes.c_int),
+        ("page_size", ctypes.c_int),
+    ]
+
+
+DK_KV_F16, DK_KV_BF16, DK_KV_F32 = 0, 1, 2
+DK_KV_MAX_REQUESTS = 4096
 
 # name -> (restype, argtypes); the export list checked against the header.
 _P = ctypes.c_void_p
@@ -103,6 +121,27 @@ _SIGNATURES = {
         ctypes.c_int,
         [_P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_int, ctypes.c_int, ctypes.c_int, _P,
          ctypes.c_size_t, _P],
+    ),
+    "dk_kv_plan": (
+        ctypes.c_int,
+        [_P, ctypes.c_int, _P, _P, ctypes.c_int, _P, ctypes.c_int, _P, ctypes.c_int,
+         ctypes.c_int, _P, _P, _P, _P, _P, _P],
+    ),
+    "dk_kv_append": (
+        ctypes.c_int,
+        [ctypes.POINTER(KvCache), _P, _P, ctypes.c_int, ctypes.c_longlong, ctypes.c_longlong,
+         ctypes.c_longlong, ctypes.c_longlong, _P, ctypes.c_int, _P],
+    ),
+    "dk_kv_read": (
+        ctypes.c_int,
+        [ctypes.POINTER(KvCache), _P, ctypes.c_int, ctypes.c_int, _P, _P, _P],
+    ),
+    "dk_kv_attend_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 8),
+    "dk_kv_attend": (
+        ctypes.c_int,
+        [_P, ctypes.c_int, ctypes.c_longlong, ctypes.c_longlong, ctypes.POINTER(KvCache), _P,
+         ctypes.c_int, _P, _P, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+         ctypes.c_float, ctypes.c_int, _P, _P, ctypes.c_size_t, _P],
     ),
     "dk_d2d_copy": (ctypes.c_int, [_P, _P, ctypes.c_size_t, _P]),
     "dk_stream_read": (ctypes.c_int, [_P, _P, ctypes.c_size_t, ctypes.c_int, _P]),
