@@ -14,6 +14,8 @@
 // registers that P goes in, and a page's scales are one value a lane.
 #include <hip/hip_runtime.h>
 
+#include <atomic>
+
 #include "dk_host.hpp"
 #include "dk_kv.hpp"
 
@@ -22,7 +24,7 @@ namespace dk {
 int kv_view(const dk_kv_cache* c, KvView* view);
 
 constexpr int kTile = 64;          // keys of a tile
-constexpr int kAttendWaves = 4;
+constexpr int kWorkgroups = 256;   // one a CU
 constexpr float kNegInf = -__builtin_huge_valf();
 // A row's maximum is moved only when a tile passes it by this much (base 2):
 // P stays below 2^8, far inside fp16, and the usual tile rescales nothing.
@@ -37,18 +39,18 @@ struct AttendArgs {
   const int32_t* lens;
   const int32_t* offsets;
   float* partials;
-  int4* starts;
+  unsigned long long* flags;  // two a workgroup, as its pieces
+  unsigned long long gen;
   float scale_log2;
   int width, tokens, requests, group, bf16, causal;
 };
 
-// One sequence's share of the work.
+// One sequence: its queries, its keys, its row tiles and tiles of keys.
 struct Seq {
   int q0, n, len, row_tiles, tiles;
 };
 
-template <int NT>
-__device__ __forceinline__ Seq sequence(const AttendArgs& a, int b) {
+__device__ __forceinline__ Seq sequence(const AttendArgs& a, int b, int rows_a_tile) {
   Seq s;
   s.q0 = b, s.n = 1;
   if (a.offsets) {
@@ -56,7 +58,7 @@ __device__ __forceinline__ Seq sequence(const AttendArgs& a, int b) {
     s.n = max(min(a.offsets[b + 1], a.tokens) - s.q0, 0);
   }
   s.len = min((long long)max(a.lens[b], 0), (long long)a.width << a.c.page_shift);
-  s.row_tiles = (int)(((long long)s.n * a.group + 16 * NT - 1) / (16 * NT));
+  s.row_tiles = (int)(((long long)s.n * a.group + rows_a_tile - 1) / rows_a_tile);
   s.tiles = max((s.len + kTile - 1) / kTile, 1);  // an empty sequence's rows are written too
   return s;
 }
@@ -76,8 +78,7 @@ __device__ __forceinline__ h8_t codes_to_f16(uint32_t lo, uint32_t hi) {
 }
 
 // Eight elements of a query as fp32.
-__device__ __forceinline__ void load_q8(const uint16_t* p, int bf16, float (&x)[8]) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void q_floats(const uint4& w, int bf16, float (&x)[8]) {
   const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -96,13 +97,43 @@ __device__ __forceinline__ float pow2i(int e) {
   return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23);
 }
 
+// The four lane groups' values against each other: exchanges of half rows of
+// registers, no LDS on the way.
 __device__ __forceinline__ float max_groups(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+  const auto h = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v),
+                                                  __builtin_bit_cast(uint32_t, v), false, false);
+  v = fmaxf(__builtin_bit_cast(float, (uint32_t)h[0]), __builtin_bit_cast(float, (uint32_t)h[1]));
+  const auto q = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v),
+                                                  __builtin_bit_cast(uint32_t, v), false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)q[0]), __builtin_bit_cast(float, (uint32_t)q[1]));
 }
 __device__ __forceinline__ float sum_groups(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+  const auto h = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v),
+                                                  __builtin_bit_cast(uint32_t, v), false, false);
+  v = __builtin_bit_cast(float, (uint32_t)h[0]) + __builtin_bit_cast(float, (uint32_t)h[1]);
+  const auto q = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v),
+                                                  __builtin_bit_cast(uint32_t, v), false, false);
+  return __builtin_bit_cast(float, (uint32_t)q[0]) + __builtin_bit_cast(float, (uint32_t)q[1]);
+}
+
+// The 16 lanes of a row against each other.
+__device__ __forceinline__ float max_row(float v) {
+  v = fmaxf(v, dpp<0xB1>(v));   // quad_perm [1,0,3,2]
+  v = fmaxf(v, dpp<0x4E>(v));   // quad_perm [2,3,0,1]
+  v = fmaxf(v, dpp<0x141>(v));  // row_half_mirror
+  return fmaxf(v, dpp<0x140>(v));  // row_mirror
+}
+__device__ __forceinline__ float sum_row(float v) {
+  v += dpp<0xB1>(v);
+  v += dpp<0x4E>(v);
+  v += dpp<0x141>(v);
+  return v + dpp<0x140>(v);
+}
+__device__ __forceinline__ int max_row(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false));
+  return max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false));
 }
 
 __device__ __forceinline__ void store_half4(const AttendArgs& a, uint16_t* at, const float (&x)[4]) {
@@ -122,156 +153,280 @@ __device__ __forceinline__ uint16_t* out_row(const AttendArgs& a, const Seq& s, 
   return a.out + ((long long)(s.q0 + i) * ((long long)a.c.heads * a.group) + head) * D;
 }
 
+// ---------------------------------------------------------------------------
+// Few rows: bound by the cache's bytes.
+//
+// The work is (sequence, key/value head, row tile, tile of keys), in that
+// order. Every wave of the card's 256 workgroups takes an equal share of it,
+// whatever the sequences' lengths are; an item (one row tile with all its
+// keys) costs kItemCost tiles on top, for the latency of its start. A wave
+// writes what it has of a whole item, and leaves the piece of an item it
+// shares, at its start or its end, in LDS; the workgroup joins the pieces of
+// an item, and an item that several workgroups share goes through the
+// workspace, where the last one to arrive adds the pieces up in their order.
+// ---------------------------------------------------------------------------
+constexpr int kItemCost = 1;
+
 template <int D, int NT>
-struct AttendLds {
+struct Few {
   static constexpr int kRows = 16 * NT;
-  static constexpr int kStride = D + 4;
-  float o[kAttendWaves][kRows][kStride];
-  float m[kAttendWaves][kRows];
-  float l[kAttendWaves][kRows];
-  long long sums[kAttendWaves];
-  int found;
-  long long found_base;
+  static constexpr int kWaves = D * NT > 128 ? 4 : 8;  // as many as LDS holds two pieces of
+  static constexpr int kThreads = kWaves * 64;
+  static constexpr int kPiece = kRows * (D + 2);  // floats of a piece in the workspace
+  struct Piece {
+    int b, item, tile0, tile1;
+    int start;  // of the item in the work
+  };
+  struct Shared {  // an item that several workgroups have pieces of
+    int b, item, wg0, pieces;
+    Seq s;
+  };
+  struct Lds {
+    float o[kWaves][2][kRows][D + 4];
+    float m[kWaves][2][kRows];
+    float l[kWaves][2][kRows];
+    Piece piece[kWaves][2];
+    Seq of_piece[kWaves][2];
+    float w[kRows][16];  // weights of the pieces being joined
+    float sum[kRows];
+    Shared shared[2];
+    int last[2];
+  };
+  // In the place of o: maxima, then weights, and sums of an item's pieces.
+  static constexpr int kMostPieces = kWorkgroups;
+  static_assert(2 * kMostPieces * kRows + kThreads * 4 <= kWaves * 2 * kRows * (D + 4), "");
 };
 
-// The keys tile0 .. tile1 of one (sequence, key/value head, row tile): the
-// waves take tiles in turn and leave their O, m and l in LDS.
+// What a wave holds of a row tile: lane (g, n) the sums of column n over
+// elements 16 d + 4 g + v, its maximum, and l over its own keys alone.
 template <int D, int NT>
-__device__ void attend_tiles(const AttendArgs& a, AttendLds<D, NT>& lds, const Seq& s, int b, int h,
-                             int rt, int tile0, int tile1, int lane, int wave) {
-  constexpr int kJ = D / 64;  // 16-byte pieces of a key a lane holds
-  constexpr int kD = D / 16;
-  const int n16 = lane & 15, g = lane >> 4;
-  const int shift = a.c.page_shift, P = 1 << shift;
-  const int rows = s.n * a.group;
+struct Sums {
+  f4_t o[NT][D / 16];
+  float m[NT], l[NT];
+};
 
-  // This lane's columns: the row, the keys it sees, its query as fp16.
-  h8_t qf[NT][kJ][2];
-  float qs[NT], m[NT], l[NT];
-  int limit[NT], most = 0, least = INT32_MAX;
+// The queries of a row tile as the product's right operand, in fp16 times a
+// power of two, and what multiplies a column's scores.
+template <int D, int NT>
+struct Queries {
+  h8_t f[NT][D / 64][2];
+  float scale[NT];
+  int limit[NT];    // keys that a column's row sees
+  int most, least;  // of all columns with a row
+};
+
+// A column's eight elements each as they lie in memory, on their way.
+template <int D, int NT>
+struct RawQueries {
+  uint4 w[NT][D / 64][2];
+};
+
+template <int D, int NT>
+__device__ __forceinline__ void load_queries(const AttendArgs& a, const Seq& s, int h, int rt, int lane,
+                                             RawQueries<D, NT>& raw, Queries<D, NT>& y) {
+  const int n16 = lane & 15, g = lane >> 4;
+  const int rows = s.n * a.group;
+  int most = 0, least = INT32_MAX;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int r = (rt * NT + t) * 16 + n16;
     const bool real = r < rows;
     const int i = real ? r / a.group : 0;
-    limit[t] = !real ? 0 : a.causal ? s.len - s.n + i + 1 : s.len;
+    y.limit[t] = !real ? 0 : a.causal ? s.len - s.n + i + 1 : s.len;
     const uint16_t* q = a.q + (long long)(s.q0 + i) * a.qt +
-                        ((long long)h * a.group + (real ? r - i * a.group : 0)) * a.qh;
-    float x[kJ][2][8];
+                        ((long long)h * a.group + (real ? r - i * a.group : 0)) * a.qh + 16 * g;
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) raw.w[t][j][e] = *reinterpret_cast<const uint4*>(q + 64 * j + 8 * e);
+    most = max(most, y.limit[t]);
+    least = min(least, real ? y.limit[t] : INT32_MAX);
+  }
+  y.most = __builtin_amdgcn_readfirstlane(max_row(most));
+  y.least = -__builtin_amdgcn_readfirstlane(max_row(-least));
+}
+
+template <int D, int NT>
+__device__ __forceinline__ void convert_queries(const AttendArgs& a, const RawQueries<D, NT>& raw,
+                                                Queries<D, NT>& y) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
     float amax = 0;
 #pragma unroll
-    for (int j = 0; j < kJ; ++j)
+    for (int j = 0; j < D / 64; ++j)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        load_q8(q + 16 * (4 * j + g) + 8 * e, a.bf16, x[j][e]);
+        float x[8];
+        q_floats(raw.w[t][j][e], a.bf16, x);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(x[j][e][k]));
+        for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(x[k]));
       }
     const int ex = row_exponent(max_groups(amax));
     const float f = pow2i(ex);
 #pragma unroll
+    for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x[8];
+        q_floats(raw.w[t][j][e], a.bf16, x);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y.f[t][j][e][k] = (_Float16)(x[k] * f);
+      }
+    y.scale[t] = a.scale_log2 * pow2i(-ex);
+  }
+}
+
+// The pages of a tile that this lane's key pieces and value pieces lie on, -1
+// where there is none.
+struct Pages {
+  int k, v;
+};
+__device__ __forceinline__ Pages tile_pages(const AttendArgs& a, const int32_t* table, int len,
+                                            int key0, int lane) {
+  const int kt = key0 + 16 * ((lane & 15) >> 2), vt = key0 + 16 * (lane >> 4);
+  Pages p;
+  p.k = kt < len ? table[kt >> a.c.page_shift] : -1;
+  p.v = vt < len ? table[vt >> a.c.page_shift] : -1;
+  return p;
+}
+
+// Keys tile0 .. tile1 of one item. The loads run a step ahead of the products:
+// the next tile's keys go out when this one's scores are done, its values when
+// this one's sums are, and page numbers a tile before them, so that a wave
+// always has 8 KiB or more in flight.
+template <int D, int NT>
+__device__ __forceinline__ void attend_piece(const AttendArgs& a, const Seq& s, int b, int h, int rt,
+                                             int tile0, int tile1, int lane, Sums<D, NT>& y) {
+  constexpr int kJ = D / 64;  // 16-byte pieces of a key a lane holds
+  constexpr int kD = D / 16;
+  const int n16 = lane & 15, g = lane >> 4;
+  const int shift = a.c.page_shift, P = 1 << shift;
+  Queries<D, NT> q;
+  const int32_t* table = a.tables + (long long)b * a.width;
+  Pages next = tile_pages(a, table, s.len, tile0 * kTile, lane);
+  RawQueries<D, NT> raw;
+  load_queries<D, NT>(a, s, h, rt, lane, raw, q);
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    y.m[t] = kNegInf;
+    y.l[t] = 0;
+#pragma unroll
+    for (int d = 0; d < kD; ++d) y.o[t][d] = f4_t{0, 0, 0, 0};
+  }
+  tile1 = min(tile1, (q.most + kTile - 1) / kTile);
+  if (tile0 >= tile1) return;
+
+  const long long page_bytes = (long long)a.c.heads * D * P;
+  const int8_t* kh = a.c.k + (long long)h * D * P + (g * P + (n16 & 3)) * 16;
+  const int8_t* vh = a.c.v + (long long)h * D * P + n16 * P;
+  const float* ksh = a.c.ks + h;
+  const float* vsh = a.c.vs + h;
+  uint4 kw[4][kJ], vw[kD];
+  float sk, sv;
+  bool have;
+  int vpage;
+  // Where the next tile's pieces are; a page that is not there is read as
+  // page 0 and masked.
+  const int8_t* kb;
+  const int8_t* vb;
+  auto locate = [&](int key0) {
+    const int kt = key0 + 16 * (n16 >> 2), vt = key0 + 16 * g;
+    const int kp = next.k >= 0 && next.k < a.c.pages ? next.k : 0;
+    have = next.v >= 0 && next.v < a.c.pages;
+    vpage = have ? next.v : 0;
+    kb = kh + kp * page_bytes + (kt & (P - 1)) * 16;
+    vb = vh + vpage * page_bytes + (vt & (P - 1));
+  };
+  auto load_keys = [&] {
+#pragma unroll
     for (int j = 0; j < kJ; ++j)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) qf[t][j][e][k] = (_Float16)(x[j][e][k] * f);
-    qs[t] = a.scale_log2 * pow2i(-ex);
-    m[t] = kNegInf;
-    l[t] = 0;
-    most = max(most, limit[t]);
-    least = min(least, real ? limit[t] : INT32_MAX);
-  }
-#pragma unroll
-  for (int d = 1; d < 16; d *= 2) {
-    most = max(most, __shfl_xor(most, d));
-    least = min(least, __shfl_xor(least, d));
-  }
-  most = __builtin_amdgcn_readfirstlane(most);
-  least = __builtin_amdgcn_readfirstlane(least);
-
-  f4_t o[NT][kD] = {};
-  const int32_t* table = a.tables + (long long)b * a.width;
-  const long long page_bytes = (long long)a.c.heads * D * P;
-  const long long head_bytes = (long long)h * D * P;
-
-  for (int tile = tile0 + wave; tile < tile1; tile += kAttendWaves) {
-    const int key0 = tile * kTile;
-    if (key0 >= most) break;
-    // The page of this lane's key pieces (A rows 4 i + v of group n16 / 4)
-    // and of its value pieces and scales (group g).
-    const int kt = key0 + 16 * (n16 >> 2), vt = key0 + 16 * g;
-    const int kcol = kt >> shift, vcol = vt >> shift;
-    int kp = kcol < a.width && kt < s.len ? table[kcol] : -1;
-    int vp = vcol < a.width && vt < s.len ? table[vcol] : -1;
-    const bool have = vp >= 0 && vp < a.c.pages;
-    kp = kp >= 0 && kp < a.c.pages ? kp : 0;
-    vp = have ? vp : 0;
-    const int8_t* kb = a.c.k + kp * page_bytes + head_bytes + ((kt & (P - 1)) + (n16 & 3)) * 16;
-    const int8_t* vb = a.c.v + vp * page_bytes + head_bytes + n16 * P + (vt & (P - 1));
-    uint4 kw[4][kJ], vw[kD];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < kJ; ++j)
-        kw[i][j] = *reinterpret_cast<const uint4*>(kb + ((4 * j + g) * P + 4 * i) * 16);
+      for (int i = 0; i < 4; ++i)
+        kw[i][j] = *reinterpret_cast<const uint4*>(kb + (4 * j * P + 4 * i) * 16);
+    sk = ksh[(long long)vpage * a.c.heads];
+    sv = vsh[(long long)vpage * a.c.heads];
+  };
+  auto load_values = [&] {
 #pragma unroll
     for (int d = 0; d < kD; ++d) vw[d] = *reinterpret_cast<const uint4*>(vb + 16 * d * P);
-    const float sk = a.c.ks[(long long)vp * a.c.heads + h];
-    const float sv = have ? a.c.vs[(long long)vp * a.c.heads + h] : 0.0f;
+  };
+  locate(tile0 * kTile);
+  load_keys();
+  load_values();
+  next = tile_pages(a, table, s.len, (tile0 + 1) * kTile, lane);
+  convert_queries<D, NT>(a, raw, q);
 
-    f4_t st[NT][4] = {};
+  for (int tile = tile0; tile < tile1; ++tile) {
+    const int key0 = tile * kTile;
+    const bool more = tile + 1 < tile1;
+    f4_t st[NT][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) {
+      for (int i = 0; i < 4; ++i) st[t][i] = f4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < kJ; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
         const h8_t k0 = codes_to_f16(kw[i][j].x, kw[i][j].y);
         const h8_t k1 = codes_to_f16(kw[i][j].z, kw[i][j].w);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          st[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qf[t][j][0], st[t][i], 0, 0, 0);
-          st[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qf[t][j][1], st[t][i], 0, 0, 0);
+          st[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q.f[t][j][0], st[t][i], 0, 0, 0);
+          st[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q.f[t][j][1], st[t][i], 0, 0, 0);
         }
       }
+    const float ck = sk;
+    const bool here = have;
+    const float cv = here ? sv : 0.0f;
+    if (more) {
+      locate(key0 + kTile);
+      load_keys();
+      next = tile_pages(a, table, s.len, key0 + 2 * kTile, lane);
+    }
 
     // Value scales relative to the tile's largest, so that P in fp16 keeps
     // its bits whatever the values' size is; exactly 1 on a page alone.
-    float top = max_groups(sv < __builtin_huge_valf() ? sv : 0.0f);
+    float top = max_groups(cv < __builtin_huge_valf() ? cv : 0.0f);
     top = top > 0 ? top : 1.0f;
-    const float rel = sv / top;
+    const float rel = cv / top;
 
-    const bool whole = key0 + kTile <= least && __all(have);
+    const bool whole = key0 + kTile <= q.least && __all(here);
     h8_t pf[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const float c = sk * qs[t];
-      float x[4][4], tm = kNegInf;
+      const float c = ck * q.scale[t];
+      float x[16], tm = kNegInf;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int k = 0; k < 16; ++k) x[k] = st[t][k >> 2][k & 3] * c;
+      const int left = here ? q.limit[t] - key0 - 16 * g : 0;  // keys seen of this lane's 16
+      if (!whole) {
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          x[i][v] = st[t][i][v] * c;
-          if (!whole && !(have && vt + 4 * i + v < limit[t])) x[i][v] = kNegInf;
-          tm = fmaxf(tm, x[i][v]);
-        }
-      if (__any(tm > m[t] + kLazy)) {
-        const float mn = fmaxf(m[t], max_groups(tm));
-        const float alpha = mn == kNegInf ? 1.0f : exp2f(m[t] - mn);
-        l[t] *= alpha;
-#pragma unroll
-        for (int d = 0; d < kD; ++d) o[t][d] *= alpha;
-        m[t] = mn;
+        for (int k = 0; k < 16; ++k) x[k] = k < left ? x[k] : kNegInf;
       }
-      const float base = m[t] == kNegInf ? 0.0f : m[t];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int k = 0; k < 16; ++k) tm = fmaxf(tm, x[k]);
+      if (__any(tm > y.m[t] + kLazy)) {
+        const float mn = fmaxf(y.m[t], max_groups(tm));
+        const float alpha = mn == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(y.m[t] - mn);
+        y.l[t] *= alpha;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const float p = exp2f(x[i][v] - base);
-          l[t] += p;
-          // A key that is not seen has p = 0 on a page of any scale.
-          const float w = x[i][v] == kNegInf ? 0.0f : p * rel;
-          pf[t][i >> 1][4 * (i & 1) + v] = (_Float16)w;
-        }
+        for (int d = 0; d < kD; ++d) y.o[t][d] *= alpha;
+        y.m[t] = mn;
+      }
+      const float base = y.m[t] == kNegInf ? 0.0f : y.m[t];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        x[k] = __builtin_amdgcn_exp2f(x[k] - base);
+        y.l[t] += x[k];
+        x[k] *= rel;
+      }
+      if (!whole) {  // a key that is not seen has weight 0 on a page of any scale
+#pragma unroll
+        for (int k = 0; k < 16; ++k) x[k] = k < left ? x[k] : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < 16; ++k) pf[t][k >> 3][k & 7] = (_Float16)x[k];
     }
 #pragma unroll
     for (int d = 0; d < kD; ++d) {
@@ -279,178 +434,419 @@ __device__ void attend_tiles(const AttendArgs& a, AttendLds<D, NT>& lds, const S
       const h8_t v1 = codes_to_f16(vw[d].z, vw[d].w);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        f4_t y = {};
-        y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[t][0], y, 0, 0, 0);
-        y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[t][1], y, 0, 0, 0);
+        f4_t z = {0, 0, 0, 0};
+        z = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[t][0], z, 0, 0, 0);
+        z = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[t][1], z, 0, 0, 0);
 #pragma unroll
-        for (int v = 0; v < 4; ++v) o[t][d][v] = fmaf(top, y[v], o[t][d][v]);
+        for (int v = 0; v < 4; ++v) y.o[t][d][v] = fmaf(top, z[v], y.o[t][d][v]);
       }
     }
+    if (more) load_values();
   }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) y.l[t] = sum_groups(y.l[t]);
+}
 
+// Whether all pieces of an item are in the workspace. A workgroup sets its own
+// piece's flag to the call's number when its stores are acknowledged, waits
+// for that too, and looks at all flags of the item: the one whose flag is set
+// last sees them all. Two that set theirs at once may both, and then write the
+// same rows with the same bits. Nothing but the call's number counts as set,
+// so the workspace needs no clearing; who sees them all clears them, and a
+// replay of the same captured call starts clean. Relaxed accesses at agent
+// scope go past the XCDs' L2s (see take_ticket in dk_kernels.hpp). One atomic
+// counter an item instead took 32 workgroups that arrive together 12 us more.
+__device__ __forceinline__ void set_flag(unsigned long long* f, unsigned long long v) {
+  __hip_atomic_store(f, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ bool flags_set(const unsigned long long* flags, unsigned long long gen, int wg0,
+                                          int pieces, int lane) {
+  bool all = true;
+  for (int k = lane; k < pieces; k += 64)
+    all &= __hip_atomic_load(flags + 2 * (wg0 + k) + (k == 0), __ATOMIC_RELAXED,
+                             __HIP_MEMORY_SCOPE_AGENT) == gen;
+  return __all(all);
+}
+
+// Two floats at once.
+__device__ __forceinline__ void store_agent2(float* p, float x, float y) {
+  const unsigned long long w = __builtin_bit_cast(uint32_t, x) | (unsigned long long)__builtin_bit_cast(uint32_t, y) << 32;
+  __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load_agent2(const float* p) {
+  const unsigned long long w = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p),
+                                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__builtin_bit_cast(float, (uint32_t)w), __builtin_bit_cast(float, (uint32_t)(w >> 32)));
+}
+
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+
+// The last workgroup to arrive adds an item's pieces up, in their order, and
+// writes its rows. The place of o in LDS is free by then.
+template <int D, int NT>
+__device__ __forceinline__ void join_pieces(const AttendArgs& a, typename Few<D, NT>::Lds& lds,
+                                            const typename Few<D, NT>::Shared& x0, int tid) {
+  using F = Few<D, NT>;
+  constexpr int kRows = F::kRows, kUnits = D / 4;
+  const Seq s = x0.s;
+  const int wg0 = x0.wg0, pieces = x0.pieces;
+  const int h = x0.item / s.row_tiles, rt = x0.item % s.row_tiles;
+  const int rows = min(kRows, s.n * a.group - rt * kRows);
+  const int lane = tid & 63, wave = tid >> 6;
+  float* ms = &lds.o[0][0][0][0];           // [row][piece]
+  float* ls = ms + F::kMostPieces * kRows;  // the same
+  float* xs = ls + F::kMostPieces * kRows;  // [thread][4]
+  auto piece = [&](int k) { return a.partials + (2LL * (wg0 + k) + (k == 0)) * F::kPiece; };
+  if (pieces <= 16) {  // no need of LDS: each thread takes all pieces, eight at once
+    for (int u = tid; u < rows * kUnits; u += F::kThreads) {
+      const int r = u / kUnits, d = u % kUnits * 4;
+      float mx = kNegInf, sum = 0, x[4] = {};
+      for (int k0 = 0; k0 < pieces; k0 += 8) {
+        float2 ml[8], o[8][2];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int r = 16 * t + n16;
-    const float sum = sum_groups(l[t]);
-    if (g == 0) {
-      lds.m[wave][r] = m[t];
-      lds.l[wave][r] = sum;
+        for (int k = 0; k < 8; ++k) {
+          ml[k] = make_float2(kNegInf, 0.0f);
+          o[k][0] = o[k][1] = make_float2(0.0f, 0.0f);
+          if (k0 + k < pieces) {
+            const float* p = piece(k0 + k);
+            ml[k] = load_agent2(p + kRows * D + 2 * r);
+            o[k][0] = load_agent2(p + r * D + d);
+            o[k][1] = load_agent2(p + r * D + d + 2);
+          }
+        }
+        const float old = mx;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mx = fmaxf(mx, ml[k].x);
+        const float f = old == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(old - mx);
+        sum *= f;  // a NaN stays
+#pragma unroll
+        for (int v = 0; v < 4; ++v) x[v] *= f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float w = ml[k].x == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ml[k].x - mx);
+          sum += w * ml[k].y;
+          x[0] = fmaf(w, o[k][0].x, x[0]);
+          x[1] = fmaf(w, o[k][0].y, x[1]);
+          x[2] = fmaf(w, o[k][1].x, x[2]);
+          x[3] = fmaf(w, o[k][1].y, x[3]);
+        }
+      }
+      sum = inverse_sum(sum);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) x[v] *= sum;
+      store_half4(a, out_row<D>(a, s, h, rt * kRows + r) + d, x);
     }
+    return;
+  }
+  __syncthreads();
+  for (int u = tid; u < pieces * kRows; u += F::kThreads) {
+    const int k = u / kRows, r = u % kRows;
+    if (r >= rows) continue;
+    const float2 ml = load_agent2(piece(k) + kRows * D + 2 * r);
+    ms[r * F::kMostPieces + k] = ml.x;
+    ls[r * F::kMostPieces + k] = ml.y;
+  }
+  __syncthreads();
+  for (int r = wave; r < rows; r += F::kWaves) {
+    float* m = ms + r * F::kMostPieces;
+    float mx = kNegInf, sum = 0;
+    for (int k = lane; k < pieces; k += 64) mx = fmaxf(mx, m[k]);
+    for (int d = 32; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
+    for (int k = lane; k < pieces; k += 64) {
+      const float w = m[k] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m[k] - mx);
+      m[k] = w;
+      sum += w * ls[r * F::kMostPieces + k];  // a NaN stays
+    }
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+    if (lane == 0) lds.sum[r] = inverse_sum(sum);
+  }
+  __syncthreads();
+  // Where rows leave threads over, they take the pieces in `parts` turns.
+  const int units = rows * kUnits;
+  const int parts = max(F::kThreads / units, 1);
+  const int part = units < F::kThreads ? tid / units : 0;
+  for (int u0 = 0; u0 < units; u0 += F::kThreads) {
+    const int u = units < F::kThreads ? tid % units : u0 + tid;
+    const int r = u / kUnits, d = u % kUnits * 4;
+    const bool on = part < parts && u < units;
+    float x[4] = {};
+    if (on) {
+      for (int k0 = part; k0 < pieces; k0 += 8 * parts) {
+        float2 o[8][2];
 #pragma unroll
-    for (int d = 0; d < kD; ++d)
-      *reinterpret_cast<f4_t*>(&lds.o[wave][r][16 * d + 4 * g]) = o[t][d];
+        for (int e = 0; e < 8; ++e) {
+          const float* p = piece(min(k0 + e * parts, pieces - 1)) + r * D + d;
+          o[e][0] = load_agent2(p);
+          o[e][1] = load_agent2(p + 2);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (k0 + e * parts >= pieces) break;
+          const float w = ms[r * F::kMostPieces + k0 + e * parts];
+          x[0] = fmaf(w, o[e][0].x, x[0]);
+          x[1] = fmaf(w, o[e][0].y, x[1]);
+          x[2] = fmaf(w, o[e][1].x, x[2]);
+          x[3] = fmaf(w, o[e][1].y, x[3]);
+        }
+      }
+    }
+    if (parts > 1) {
+      if (on) *reinterpret_cast<f4_t*>(xs + 4 * tid) = f4_t{x[0], x[1], x[2], x[3]};
+      __syncthreads();
+      if (on && part == 0)
+        for (int k = 1; k < parts; ++k) {
+          const f4_t y = *reinterpret_cast<const f4_t*>(xs + 4 * (tid + k * units));
+#pragma unroll
+          for (int v = 0; v < 4; ++v) x[v] += y[v];
+        }
+    }
+    if (on && part == 0) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) x[v] *= lds.sum[r];
+      store_half4(a, out_row<D>(a, s, h, rt * kRows + r) + d, x);
+    }
   }
 }
 
-// The work is (sequence, key/value head, row tile, tile of keys), in that
-// order; a workgroup takes an equal share of it, whatever the lengths are.
-// What a share holds of an item that others share goes to the workspace, and
-// attend_join adds it up.
+// Inclusive sums over the wave.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
+__device__ __forceinline__ Seq lane_seq(const Seq& s, int lane) {
+  Seq u;
+  u.q0 = __builtin_amdgcn_readlane(s.q0, lane);
+  u.n = __builtin_amdgcn_readlane(s.n, lane);
+  u.len = __builtin_amdgcn_readlane(s.len, lane);
+  u.row_tiles = __builtin_amdgcn_readlane(s.row_tiles, lane);
+  u.tiles = __builtin_amdgcn_readlane(s.tiles, lane);
+  return u;
+}
+
+__device__ __forceinline__ Seq uniform_seq(const Seq& s) {
+  Seq u;
+  u.q0 = __builtin_amdgcn_readfirstlane(s.q0);
+  u.n = __builtin_amdgcn_readfirstlane(s.n);
+  u.len = __builtin_amdgcn_readfirstlane(s.len);
+  u.row_tiles = __builtin_amdgcn_readfirstlane(s.row_tiles);
+  u.tiles = __builtin_amdgcn_readfirstlane(s.tiles);
+  return u;
+}
+
 template <int D, int NT>
-__global__ __launch_bounds__(kAttendWaves * 64) void attend_kernel(AttendArgs a) {
-  using Lds = AttendLds<D, NT>;
-  constexpr int kRows = Lds::kRows;
-  __shared__ Lds lds;
+__global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs a) {
+  using F = Few<D, NT>;
+  constexpr int kRows = F::kRows, kWaves = F::kWaves, kSlots = 2 * F::kWaves;
+  __shared__ typename F::Lds lds;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wg = blockIdx.x;
 
-  // Every workgroup adds up all sequences' work to find its own.
-  const int each = (a.requests + 255) / 256;
-  const int b0 = min(tid * each, a.requests), b1 = min(b0 + each, a.requests);
-  long long mine = 0;
-  for (int b = b0; b < b1; ++b) {
-    const Seq s = sequence<NT>(a, b);
-    mine += (long long)a.c.heads * s.row_tiles * s.tiles;
-  }
-  long long inc = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const long long o = __shfl_up(inc, d);
-    if (lane >= d) inc += o;
-  }
-  if (lane == 63) lds.sums[wave] = inc;
-  __syncthreads();
-  long long total = 0, before = inc - mine;
-#pragma unroll
-  for (int w = 0; w < kAttendWaves; ++w) {
-    if (w < wave) before += lds.sums[w];
-    total += lds.sums[w];
-  }
-  const long long share = max((total + gridDim.x - 1) / gridDim.x, (long long)kAttendWaves);
-  const long long begin = wg * share, end = min(begin + share, total);
-  if (tid == 0) a.starts[wg] = make_int4(-1, 0, 0, 0);
-  if (begin >= end) return;
-  if (begin >= before && begin < before + mine) {
-    long long base = before;
-    for (int b = b0; b < b1; ++b) {
-      const Seq s = sequence<NT>(a, b);
-      const long long w = (long long)a.c.heads * s.row_tiles * s.tiles;
-      if (begin < base + w) {
-        lds.found = b;
-        lds.found_base = base;
-        break;
-      }
-      base += w;
-    }
-  }
-  __syncthreads();
-  int b = lds.found;
-  long long base = lds.found_base;
+  if (lane < 2) lds.piece[wave][lane].b = -1;
+  if (tid < 2) lds.shared[tid].pieces = 0;
 
-  for (long long cur = begin; cur < end;) {
-    const Seq s = sequence<NT>(a, b);
-    const long long w = (long long)a.c.heads * s.row_tiles * s.tiles;
-    if (cur >= base + w) {
-      base += w;
-      ++b;
-      continue;
-    }
-    const long long local = cur - base;
-    const int item = (int)(local / s.tiles), tile0 = (int)(local % s.tiles);
-    const int tile1 = (int)min((long long)s.tiles, tile0 + (end - cur));
-    const int h = item / s.row_tiles, rt = item % s.row_tiles;
-    attend_tiles<D, NT>(a, lds, s, b, h, rt, tile0, tile1, lane, wave);
-    __syncthreads();
-
-    const bool shared = tile0 > 0 || tile1 < s.tiles;
-    const int slot = 2 * wg + (cur == begin ? 0 : 1);
-    float* part = a.partials + (long long)slot * kRows * (D + 2);
-    const int rows = min(kRows, s.n * a.group - rt * kRows);
-    for (int u = tid; u < rows * (D / 4); u += 256) {
-      const int r = u / (D / 4), d = u % (D / 4) * 4;
-      float mx = kNegInf;
-#pragma unroll
-      for (int k = 0; k < kAttendWaves; ++k) mx = fmaxf(mx, lds.m[k][r]);
-      float sum = 0, x[4] = {};
-#pragma unroll
-      for (int k = 0; k < kAttendWaves; ++k) {
-        const float f = lds.m[k][r] == kNegInf ? 0.0f : exp2f(lds.m[k][r] - mx);
-        sum += f * lds.l[k][r];
-        if (f == 0.0f) continue;  // a wave without keys
-        const f4_t y = *reinterpret_cast<const f4_t*>(&lds.o[k][r][d]);
-#pragma unroll
-        for (int v = 0; v < 4; ++v) x[v] = fmaf(f, y[v], x[v]);
+  // Every wave adds up all sequences' work to find its own, by itself: the
+  // lanes take `each` sequences in a row, then those of the block that the
+  // share starts in one by one. The host has seen to it that the sum fits.
+  auto cost = [&](const Seq& s) { return a.c.heads * s.row_tiles * (s.tiles + kItemCost); };
+  const int each = (a.requests + 63) / 64;
+  int b = lane * each;
+  Seq s{};
+  int work = 0;
+  for (int k = 0; k < each && b + k < a.requests; ++k) {
+    s = sequence(a, b + k, kRows);
+    work += cost(s);
+  }
+  int upto = wave_scan(work);
+  const int total = __builtin_amdgcn_readlane(upto, 63);
+  // A wave's share, and the workgroup's.
+  const int share = max((int)(((unsigned)total + kWorkgroups * kWaves - 1) / (kWorkgroups * kWaves)), 1);
+  const int group_share = share * kWaves;
+  if (wg >= (total + group_share - 1) / group_share) return;
+  const int begin = wg * group_share + wave * share, end = min(begin + share, total);
+  int base = 0;
+  if (begin < end) {
+    int at = __builtin_ctzll(__ballot(begin < upto));
+    base = __builtin_amdgcn_readlane(upto - work, at);
+    b = at * each;
+    if (each > 1) {
+      int first = b;
+      for (;; first += 64) {
+        const bool real = first + lane < min(b + each, a.requests);
+        s = sequence(a, real ? first + lane : 0, kRows);
+        work = real ? cost(s) : 0;
+        upto = wave_scan(work);
+        if (begin < base + __builtin_amdgcn_readlane(upto, 63)) break;
+        base += __builtin_amdgcn_readlane(upto, 63);
       }
-      if (shared) {
-        *reinterpret_cast<f4_t*>(part + r * D + d) = f4_t{x[0], x[1], x[2], x[3]};
-        if (d == 0) {
-          part[kRows * D + r] = mx;
-          part[kRows * D + kRows + r] = sum;
+      at = __builtin_ctzll(__ballot(begin < base + upto));
+      base += __builtin_amdgcn_readlane(upto - work, at);
+      b = first + at;
+    }
+    s = lane_seq(s, at);
+    for (int cur = begin; cur < end;) {
+      const int c = cost(s);
+      if (cur >= base + c) {
+        base += c;
+        s = sequence(a, ++b, kRows);
+        continue;
+      }
+      const int units = s.tiles + kItemCost;
+      const int item = (unsigned)(cur - base) / (unsigned)units, at = cur - base - item * units;
+      const int stop = min(units, at + (end - cur));
+      cur += stop - at;
+      const int tile0 = max(at - kItemCost, 0), tile1 = stop - kItemCost;
+      if (tile0 >= tile1) continue;  // the item's start alone
+      const int h = (unsigned)item / (unsigned)s.row_tiles, rt = item - h * s.row_tiles;
+      Sums<D, NT> y;
+      attend_piece<D, NT>(a, s, b, h, rt, tile0, tile1, lane, y);
+      const int n16 = lane & 15, g = lane >> 4;
+      if (tile0 == 0 && tile1 == s.tiles) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const int r = (rt * NT + t) * 16 + n16;
+          if (r >= s.n * a.group) continue;
+          const float inv = inverse_sum(y.l[t]);
+          uint16_t* out = out_row<D>(a, s, h, r) + 4 * g;
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) {
+            const float x[4] = {y.o[t][d][0] * inv, y.o[t][d][1] * inv, y.o[t][d][2] * inv,
+                                y.o[t][d][3] * inv};
+            store_half4(a, out + 16 * d, x);
+          }
         }
       } else {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int slot = tile0 == 0 ? 1 : 0;  // at the share's end, or its start
 #pragma unroll
-        for (int v = 0; v < 4; ++v) x[v] *= inv;
-        store_half4(a, out_row<D>(a, s, h, rt * kRows + r) + d, x);
+        for (int t = 0; t < NT; ++t) {
+          const int r = 16 * t + n16;
+          if (g == 0) {
+            lds.m[wave][slot][r] = y.m[t];
+            lds.l[wave][slot][r] = y.l[t];
+          }
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d)
+            *reinterpret_cast<f4_t*>(&lds.o[wave][slot][r][16 * d + 4 * g]) = y.o[t][d];
+        }
+        if (lane == 0) {
+          lds.piece[wave][slot] = typename F::Piece{b, item, tile0, tile1, base + item * units};
+          lds.of_piece[wave][slot] = s;
+        }
       }
     }
-    if (shared && tile0 == 0 && tid == 0) {
-      // The pieces that follow are the first ones of the next workgroups.
-      const int more = (int)((s.tiles - tile1 + share - 1) / share);
-      a.starts[wg] = make_int4(b, item, slot, more);
+  }
+  __syncthreads();
+
+  // Pieces of one item stand in a row: a wave's end and the next one's start.
+  // Lane i looks at piece i.
+  typename F::Piece piece{-1, 0, 0, 0, 0};
+  if (lane < kSlots) piece = lds.piece[lane / 2][lane % 2];
+  const uint32_t filled = (uint32_t)__ballot(piece.b >= 0);
+  const uint32_t below = filled & ((1u << (lane & 31)) - 1);
+  const int prev = below ? 31 - __builtin_clz(below) : 0;
+  const int prev_b = __shfl(piece.b, prev), prev_item = __shfl(piece.item, prev);  // by every lane
+  const bool same = below && prev_b == piece.b && prev_item == piece.item;
+  const uint32_t starts = (uint32_t)__ballot(piece.b >= 0 && !same);
+  for (uint32_t todo = starts; todo; todo &= todo - 1) {
+    const int i = __builtin_ctz(todo);
+    const uint32_t after = todo & (todo - 1);
+    const uint32_t group = filled & ~((1u << i) - 1) & (after ? (after & -after) - 1 : ~0u);
+    const int last_piece = 31 - __builtin_clz(group);
+    const int b = __builtin_amdgcn_readlane(piece.b, i);
+    const int item = __builtin_amdgcn_readlane(piece.item, i);
+    const int tile0 = __builtin_amdgcn_readlane(piece.tile0, i);
+    const int tile1 = __builtin_amdgcn_readlane(piece.tile1, last_piece);
+    const int start = __builtin_amdgcn_readlane(piece.start, i);
+    const Seq s = uniform_seq(lds.of_piece[i / 2][i % 2]);
+    const int h = (unsigned)item / (unsigned)s.row_tiles, rt = item - h * s.row_tiles;
+    const int rows = min(kRows, s.n * a.group - rt * kRows);
+    const bool whole = tile0 == 0 && tile1 == s.tiles;
+    float* part = a.partials + (2LL * wg + (tile0 == 0)) * F::kPiece;
+    // Weights: 16 lanes a row, a lane a piece.
+    for (int u = tid; u < kRows * 16; u += F::kThreads) {
+      const int r = u >> 4, p = u & 15;
+      const bool on = group >> p & 1;
+      const float m = on ? lds.m[p / 2][p % 2][r] : kNegInf;
+      const float l = on ? lds.l[p / 2][p % 2][r] : 0.0f;
+      const float mx = max_row(m);
+      const float w = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
+      const float sum = sum_row(w * l);  // a NaN stays
+      lds.w[r][p] = w;
+      if (p == 0) {
+        lds.sum[r] = inverse_sum(sum);
+        if (!whole && r < rows) store_agent2(part + kRows * D + 2 * r, mx, sum);
+      }
     }
     __syncthreads();
-    cur += tile1 - tile0;
+    for (int u = tid; u < rows * (D / 4); u += F::kThreads) {
+      const int r = u / (D / 4), d = u % (D / 4) * 4;
+      float x[4] = {};
+      for (uint32_t k = group; k;) {  // four pieces' loads at once
+        f4_t o[4];
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int p = k ? __builtin_ctz(k) : last_piece;
+          o[e] = *reinterpret_cast<const f4_t*>(&lds.o[p / 2][p % 2][r][d]);
+          w[e] = k ? lds.w[r][p] : 0.0f;
+          k &= k - 1;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) x[v] = fmaf(w[e], o[e][v], x[v]);
+      }
+      if (whole) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) x[v] *= lds.sum[r];
+        store_half4(a, out_row<D>(a, s, h, rt * kRows + r) + d, x);
+      } else {
+        store_agent2(part + r * D + d, x[0], x[1]);
+        store_agent2(part + r * D + d + 2, x[2], x[3]);
+      }
+    }
+    if (!whole && tid == 0) {
+      // The item's pieces are the end of the workgroup that its first tile
+      // falls to and the starts of those after it.
+      const int wg0 = tile0 == 0 ? wg : (start + kItemCost) / group_share;
+      const int last = (start + s.tiles + kItemCost - 1) / group_share;
+      lds.shared[tile0 == 0] = typename F::Shared{b, item, wg0, last - wg0 + 1, s};
+    }
+    __syncthreads();  // w and sum are free again
   }
-}
 
-// Adds up the pieces of the item that starts in workgroup blockIdx.x and
-// goes on in the next ones, in their order. A workgroup does four rows.
-template <int D, int NT>
-__global__ __launch_bounds__(4 * (D / 4)) void attend_join(AttendArgs a) {
-  constexpr int kRows = 16 * NT;
-  const int4 start = a.starts[blockIdx.x];
-  if (start.x < 0) return;
-  const Seq s = sequence<NT>(a, start.x);
-  const int h = start.y / s.row_tiles, rt = start.y % s.row_tiles;
-  const int r = blockIdx.y * 4 + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
-  if (r >= min(kRows, s.n * a.group - rt * kRows)) return;
-  const long long size = (long long)kRows * (D + 2);
-  float mx = kNegInf, sum = 0, x[4] = {};
-  for (int k = 0; k <= start.w; ++k) {
-    const float* part = a.partials + (k == 0 ? (long long)start.z : 2LL * (blockIdx.x + k)) * size;
-    const float pm = part[kRows * D + r], pl = part[kRows * D + kRows + r];
-    const f4_t y = *reinterpret_cast<const f4_t*>(part + r * D + d);
-    const float mn = fmaxf(mx, pm);
-    const float fo = mx == kNegInf ? 0.0f : exp2f(mx - mn);
-    const float fn = pm == kNegInf ? 0.0f : exp2f(pm - mn);
-    sum = sum * fo + pl * fn;
-#pragma unroll
-    for (int v = 0; v < 4; ++v) x[v] = x[v] * fo + (fn == 0.0f ? 0.0f : y[v] * fn);
-    mx = mn;
+  // At most two items of a workgroup are shared, at its start and at its end.
+  __builtin_amdgcn_s_waitcnt(0);  // this wave's stores to the workspace
+  __syncthreads();
+  if (wave < 2) {
+    const typename F::Shared x = lds.shared[wave];
+    bool all = false;
+    if (x.pieces > 0) {
+      if (lane == 0) set_flag(a.flags + 2 * wg + wave, a.gen);
+      __builtin_amdgcn_s_waitcnt(0);
+      all = flags_set(a.flags, a.gen, x.wg0, x.pieces, lane);
+    }
+    if (lane == 0) lds.last[wave] = all;
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-  for (int v = 0; v < 4; ++v) x[v] *= inv;
-  store_half4(a, out_row<D>(a, s, h, rt * kRows + r) + d, x);
+  __syncthreads();
+  for (int k = 0; k < 2; ++k) {
+    if (!lds.last[k]) continue;
+    const typename F::Shared x = lds.shared[k];
+    join_pieces<D, NT>(a, lds, x, tid);
+    for (int p = tid; p < x.pieces; p += F::kThreads)
+      set_flag(a.flags + 2 * (x.wg0 + p) + (p == 0), 0);
+  }
 }
 
 }  // namespace dk
 
 namespace {
-
-constexpr int kWorkgroups = 512;  // two a CU
 
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
@@ -459,9 +855,16 @@ int column_tiles(int max_query_len, int group) {
   return (long long)max_query_len * group <= 16 ? 1 : 2;
 }
 
+// The number of a call, which never comes again in a process: what its pieces'
+// flags hold when they are set.
+unsigned long long next_call() {
+  static std::atomic<unsigned long long> calls{0x9D8E6B1F37A95C41ull};  // no count that memory may hold
+  return calls.fetch_add(1, std::memory_order_relaxed);
+}
+
 size_t workspace(int nt, int head_size) {
-  return (size_t)kWorkgroups * sizeof(int4) +
-         (size_t)kWorkgroups * 2 * 16 * nt * (head_size + 2) * sizeof(float);
+  return (size_t)dk::kWorkgroups * 2 * sizeof(unsigned long long) +
+         (size_t)dk::kWorkgroups * 2 * 16 * nt * (head_size + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -510,6 +913,11 @@ extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
   if (q_token_stride % 8 || q_head_stride % 8)
     return dk::set_error(DK_ERR_INVALID_ARGUMENT, "the strides of q must be multiples of 8");
   const int group = q_heads / view.heads;
+  // Work is counted in 31 bits: heads, row tiles and tiles of keys.
+  const double most = (double)view.heads * ((double)num_tokens * group / 16 + requests) *
+                      (((double)table_width * cache->page_size) / dk::kTile + 2);
+  if (most > 1 << 30)
+    return dk::set_error(DK_ERR_UNSUPPORTED, "heads * queries * keys too large");
   const int nt = column_tiles(max_query_len, group);
   if (workspace_bytes < workspace(nt, cache->head_size))
     return dk::set_error(DK_ERR_INVALID_ARGUMENT, "the workspace has %zu of %zu bytes",
@@ -523,8 +931,9 @@ extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
   a.tables = tables;
   a.lens = seq_lens;
   a.offsets = query_offsets;
-  a.starts = static_cast<int4*>(workspace_ptr);
-  a.partials = reinterpret_cast<float*>(a.starts + kWorkgroups);
+  a.flags = static_cast<unsigned long long*>(workspace_ptr);
+  a.gen = next_call();
+  a.partials = reinterpret_cast<float*>(a.flags + 2 * dk::kWorkgroups);
   a.scale_log2 = scale * 1.44269504088896340736f;
   a.width = cache->pages > 0 ? table_width : 0;  // no pages, no keys
   a.tokens = num_tokens;
@@ -532,16 +941,15 @@ extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
   a.group = group;
   a.bf16 = dtype == DK_KV_BF16;
   a.causal = causal != 0;
-  auto launch = [&](auto main, auto join) {
-    hipLaunchKernelGGL(main, dim3(kWorkgroups), dim3(dk::kAttendWaves * 64), 0, stream, a);
-    hipLaunchKernelGGL(join, dim3(kWorkgroups, 4 * nt), dim3(cache->head_size), 0, stream, a);
+  auto launch = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, dim3(dk::kWorkgroups), dim3(threads), 0, stream, a);
   };
   if (cache->head_size == 64) {
-    if (nt == 1) launch(dk::attend_kernel<64, 1>, dk::attend_join<64, 1>);
-    else launch(dk::attend_kernel<64, 2>, dk::attend_join<64, 2>);
+    if (nt == 1) launch(dk::attend_few<64, 1>, dk::Few<64, 1>::kThreads);
+    else launch(dk::attend_few<64, 2>, dk::Few<64, 2>::kThreads);
   } else {
-    if (nt == 1) launch(dk::attend_kernel<128, 1>, dk::attend_join<128, 1>);
-    else launch(dk::attend_kernel<128, 2>, dk::attend_join<128, 2>);
+    if (nt == 1) launch(dk::attend_few<128, 1>, dk::Few<128, 1>::kThreads);
+    else launch(dk::attend_few<128, 2>, dk::Few<128, 2>::kThreads);
   }
   return dk::check_launch("attend launch");
 }
