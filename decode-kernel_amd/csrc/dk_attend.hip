@@ -14,6 +14,7 @@
 // registers that P goes in, and a page's scales are one value a lane.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "dk_host.hpp"
@@ -43,6 +44,7 @@ struct AttendArgs {
   unsigned long long gen;
   float scale_log2;
   int width, tokens, requests, group, bf16, causal;
+  int few_rows;  // sequences of more rows are attend_many's
 };
 
 // One sequence: its queries, its keys, its row tiles and tiles of keys.
@@ -50,7 +52,7 @@ struct Seq {
   int q0, n, len, row_tiles, tiles;
 };
 
-__device__ __forceinline__ Seq sequence(const AttendArgs& a, int b, int rows_a_tile) {
+__device__ __forceinline__ Seq sequence(const AttendArgs& a, int b, int rows_a_tile, bool many) {
   Seq s;
   s.q0 = b, s.n = 1;
   if (a.offsets) {
@@ -58,7 +60,8 @@ __device__ __forceinline__ Seq sequence(const AttendArgs& a, int b, int rows_a_t
     s.n = max(min(a.offsets[b + 1], a.tokens) - s.q0, 0);
   }
   s.len = min((long long)max(a.lens[b], 0), (long long)a.width << a.c.page_shift);
-  s.row_tiles = (int)(((long long)s.n * a.group + rows_a_tile - 1) / rows_a_tile);
+  const int rows = s.n * a.group;
+  s.row_tiles = (rows > a.few_rows) == many ? (rows + rows_a_tile - 1) / rows_a_tile : 0;
   s.tiles = max((s.len + kTile - 1) / kTile, 1);  // an empty sequence's rows are written too
   return s;
 }
@@ -116,6 +119,18 @@ __device__ __forceinline__ float sum_groups(float v) {
   return __builtin_bit_cast(float, (uint32_t)q[0]) + __builtin_bit_cast(float, (uint32_t)q[1]);
 }
 
+// The wave's halves against each other.
+__device__ __forceinline__ float max_halves(float v) {
+  const auto h = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v),
+                                                  __builtin_bit_cast(uint32_t, v), false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)h[0]), __builtin_bit_cast(float, (uint32_t)h[1]));
+}
+__device__ __forceinline__ float sum_halves(float v) {
+  const auto h = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v),
+                                                  __builtin_bit_cast(uint32_t, v), false, false);
+  return __builtin_bit_cast(float, (uint32_t)h[0]) + __builtin_bit_cast(float, (uint32_t)h[1]);
+}
+
 // The 16 lanes of a row against each other.
 __device__ __forceinline__ float max_row(float v) {
   v = fmaxf(v, dpp<0xB1>(v));   // quad_perm [1,0,3,2]
@@ -134,6 +149,11 @@ __device__ __forceinline__ int max_row(int v) {
   v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
   v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false));
   return max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false));
+}
+// Of lanes 0..31, in lane 0.
+__device__ __forceinline__ int max_half_wave(int v) {
+  v = max_row(v);
+  return max(v, __builtin_amdgcn_readlane(v, 16));
 }
 
 __device__ __forceinline__ void store_half4(const AttendArgs& a, uint16_t* at, const float (&x)[4]) {
@@ -660,7 +680,7 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
   Seq s{};
   int work = 0;
   for (int k = 0; k < each && b + k < a.requests; ++k) {
-    s = sequence(a, b + k, kRows);
+    s = sequence(a, b + k, kRows, false);
     work += cost(s);
   }
   int upto = wave_scan(work);
@@ -679,7 +699,7 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
       int first = b;
       for (;; first += 64) {
         const bool real = first + lane < min(b + each, a.requests);
-        s = sequence(a, real ? first + lane : 0, kRows);
+        s = sequence(a, real ? first + lane : 0, kRows, false);
         work = real ? cost(s) : 0;
         upto = wave_scan(work);
         if (begin < base + __builtin_amdgcn_readlane(upto, 63)) break;
@@ -694,7 +714,7 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
       const int c = cost(s);
       if (cur >= base + c) {
         base += c;
-        s = sequence(a, ++b, kRows);
+        s = sequence(a, ++b, kRows, false);
         continue;
       }
       const int units = s.tiles + kItemCost;
@@ -844,15 +864,476 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
   }
 }
 
+// ---------------------------------------------------------------------------
+// Many rows (prompts): bound by the matrix products.
+//
+// A workgroup of eight waves takes 256 rows of one sequence and key/value head
+// over the tiles of keys, 32 rows a wave, v_mfma_f32_32x32x16_f16. It turns a
+// tile's codes into fp16 in LDS once for all its rows (a thread 16 bytes of
+// keys and of values), two tiles in turn: while one is multiplied, the next is
+// converted and the one after is on its way. Rows of a product's right operand
+// are a wave's lanes, so a row's maximum and sum need one exchange of the
+// wave's halves, and P goes from the first product's registers into the
+// second's. Values lie in LDS in the order in which lanes hold P's tokens.
+//
+// A page's value scale goes into P relative to a power of two, `unit`, that
+// follows the scales within 2^6: P keeps fp16's bits whatever the values' size
+// is, and the sums are only rescaled when the unit moves.
+//
+// The work is (sequence, head, row tile, tile of keys), with the tiles past a
+// row tile's last visible key left out; the workgroups take equal shares, and
+// pieces of an item that two or more share meet as those of attend_few do.
+// ---------------------------------------------------------------------------
+constexpr int kManyRows = 256;
+constexpr int kManyThreads = 512;
+constexpr int kManyItemCost = 2;
+
+typedef float f16_t __attribute__((ext_vector_type(16)));
+
+template <int D>
+struct Many {
+  static constexpr int kPiece = kManyRows * (D + 2);      // floats in the workspace
+  static constexpr int kBlock = D * 16 + 16;              // bytes of eight tokens' values, spread over the banks
+  struct Lds {
+    alignas(16) char k[2][D / 8][kTile][16];  // eight elements of a key
+    alignas(16) char v[2][8 * kBlock];        // [(16 tokens, half)][element][8 tokens]
+    float ks[2][4], vs[2][4];                 // scales of a tile's 16-token groups; -1: no page
+    int last;
+  };
+};
+
+// sum of floor((a i + b) / m) over i < n
+__device__ __forceinline__ int floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
+  unsigned sum = 0;
+  while (n > 0) {
+    if (a >= m) {
+      sum += n * (n - 1) / 2 * (a / m);
+      a %= m;
+    }
+    if (b >= m) {
+      sum += n * (b / m);
+      b %= m;
+    }
+    const unsigned top = a * n + b;
+    if (top < m) break;
+    n = top / m;
+    b = top % m;
+    const unsigned t = m;
+    m = a;
+    a = t;
+  }
+  return (int)sum;
+}
+
+// Whether a sequence's row tiles see different numbers of keys.
+__device__ __forceinline__ bool slanted(const AttendArgs& a, const Seq& s) {
+  return a.causal && s.n <= s.len && s.row_tiles > 1;
+}
+
+// Tiles of keys that row tile rt sees: its last row's token sees
+// len - n + ceil((rt + 1) 256 / group) keys, or all.
+__device__ __forceinline__ int tiles_seen(const AttendArgs& a, const Seq& s, int rt) {
+  if (!slanted(a, s) || rt >= s.row_tiles - 1) return s.tiles;
+  const unsigned G = a.group;
+  return ((unsigned)(s.len - s.n) * G + (rt + 1) * kManyRows + kTile * G - 1) / (kTile * G);
+}
+
+// The work of one head of a sequence.
+__device__ __forceinline__ int head_cost(const AttendArgs& a, const Seq& s) {
+  if (!slanted(a, s)) return s.row_tiles * (s.tiles + kManyItemCost);
+  const unsigned G = a.group;
+  return s.row_tiles * kManyItemCost + s.tiles +
+         floor_sum(s.row_tiles - 1, kTile * G, kManyRows,
+                   (unsigned)(s.len - s.n) * G + kManyRows + kTile * G - 1);
+}
+
+template <int D>
+__global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
+  using M = Many<D>;
+  constexpr int kK = D / 16, kDt = D / 32;
+  __shared__ typename M::Lds lds;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n32 = lane & 31, hh = lane >> 5;
+  const int wg = blockIdx.x;
+  const int shift = a.c.page_shift, P = 1 << shift;
+
+  // This workgroup's share, found by every wave for itself as in attend_few.
+  const int each = (a.requests + 63) / 64;
+  int b = lane * each;
+  Seq s{};
+  int work = 0;
+  for (int k = 0; k < each && b + k < a.requests; ++k) {
+    s = sequence(a, b + k, kManyRows, true);
+    work += a.c.heads * head_cost(a, s);
+  }
+  int upto = wave_scan(work);
+  const int total = __builtin_amdgcn_readlane(upto, 63);
+  const int share = max((int)(((unsigned)total + kWorkgroups - 1) / kWorkgroups), 1);
+  const int begin = wg * share, end = min(begin + share, total);
+  if (begin >= end) return;
+  int at = __builtin_ctzll(__ballot(begin < upto));
+  int base = __builtin_amdgcn_readlane(upto - work, at);
+  b = at * each;
+  if (each > 1) {
+    int first = b;
+    for (;; first += 64) {
+      const bool real = first + lane < min(b + each, a.requests);
+      s = sequence(a, real ? first + lane : 0, kManyRows, true);
+      work = real ? a.c.heads * head_cost(a, s) : 0;
+      upto = wave_scan(work);
+      if (begin < base + __builtin_amdgcn_readlane(upto, 63)) break;
+      base += __builtin_amdgcn_readlane(upto, 63);
+    }
+    at = __builtin_ctzll(__ballot(begin < base + upto));
+    base += __builtin_amdgcn_readlane(upto - work, at);
+    b = first + at;
+  }
+  s = lane_seq(s, at);
+
+  // The item that the share starts in, and where: head, row tile.
+  int per_head = __builtin_amdgcn_readfirstlane(head_cost(a, s));
+  int h = (begin - base) / per_head, rt = 0;
+  base += h * per_head;
+  for (;; rt += 64) {
+    const int u = rt + lane < s.row_tiles ? tiles_seen(a, s, rt + lane) + kManyItemCost : 0;
+    const int scan = wave_scan(u);
+    const int all = __builtin_amdgcn_readlane(scan, 63);
+    if (begin < base + all) {
+      const int i = __builtin_ctzll(__ballot(begin < base + scan));
+      base += __builtin_amdgcn_readlane(scan - u, i);
+      rt += i;
+      break;
+    }
+    base += all;
+  }
+
+  for (int cur = begin; cur < end;) {
+    const int tiles = tiles_seen(a, s, rt);
+    const int units = tiles + kManyItemCost;
+    const int from = cur - base, stop = min(units, from + (end - cur));
+    const int tile0 = max(from - kManyItemCost, 0), tile1 = stop - kManyItemCost;
+    const int start = base;
+    cur += stop - from;
+    if (tile0 < tile1) {
+      const int row0 = rt * kManyRows + wave * 32;
+      const int rows = s.n * a.group;
+      const int32_t* table = a.tables + (long long)b * a.width;
+
+      // Loads of a tile: keys of token lane, piece `wave`; values of 16 tokens
+      // of one element. With 64 elements half the waves load each.
+      const bool loads_k = D == 128 || wave < 4, loads_v = D == 128 || wave >= 4;
+      const int kc = wave & (kK - 1);
+      const int vd = (D == 128 ? wave : wave & 3) * 16 + (lane >> 2), vq = lane & 3;
+      const long long page_bytes = (long long)a.c.heads * D * P;
+      uint4 kraw = zero4(), vraw = zero4();
+      float sraw = 0;
+      int kpage = -1, vpage = -1, spage = -1;
+      auto load_pages = [&](int tile) {
+        const int kt = tile * kTile + lane, vt = tile * kTile + 16 * vq;
+        kpage = tile < tile1 && kt < s.len ? table[kt >> shift] : -1;
+        vpage = tile < tile1 && vt < s.len ? table[vt >> shift] : -1;
+      };
+      auto load_codes = [&](int tile) {
+        const int kt = tile * kTile + lane, vt = tile * kTile + 16 * vq;
+        const int kp = kpage >= 0 && kpage < a.c.pages ? kpage : 0;
+        const int vp = vpage >= 0 && vpage < a.c.pages ? vpage : 0;
+        spage = vpage == vp ? vp : -1;
+        if (tile >= tile1 || tile * kTile >= s.len) return;  // nothing is there
+        if (loads_k)
+          kraw = *reinterpret_cast<const uint4*>(a.c.k + kp * page_bytes +
+                                                 ((long long)h * D + kc * 16) * P + (kt & (P - 1)) * 16);
+        if (loads_v)
+          vraw = *reinterpret_cast<const uint4*>(a.c.v + vp * page_bytes +
+                                                 ((long long)h * D + vd) * P + (vt & (P - 1)));
+        // Lanes 0..3 of two waves bring the scales of their 16 tokens.
+        if (wave == 0 || wave == 1) {
+          const float* scales = wave == 0 ? a.c.ks : a.c.vs;
+          sraw = scales[(long long)vp * a.c.heads + h];
+        }
+      };
+      auto store_codes = [&](int buf) {
+        if (loads_k) {
+          *reinterpret_cast<h8_t*>(lds.k[buf][2 * kc][lane]) = codes_to_f16(kraw.x, kraw.y);
+          *reinterpret_cast<h8_t*>(lds.k[buf][2 * kc + 1][lane]) = codes_to_f16(kraw.z, kraw.w);
+        }
+        if (loads_v) {
+          char* v = lds.v[buf] + 2 * vq * M::kBlock + vd * 16;
+          *reinterpret_cast<h8_t*>(v) = codes_to_f16(vraw.x, vraw.z);
+          *reinterpret_cast<h8_t*>(v + M::kBlock) = codes_to_f16(vraw.y, vraw.w);
+        }
+        if (wave < 2 && lane < 4) (wave == 0 ? lds.ks : lds.vs)[buf][lane] = spage >= 0 ? sraw : -1.0f;
+      };
+
+      load_pages(tile0);
+      // The queries of this wave's rows.
+      h8_t qf[kK];
+      float qs;
+      int limit, least, most;
+      {
+        const int r = row0 + n32;
+        const bool real = r < rows;
+        const int i = real ? r / a.group : 0;
+        limit = !real ? 0 : a.causal ? s.len - s.n + i + 1 : s.len;
+        const uint16_t* q = a.q + (long long)(s.q0 + i) * a.qt +
+                            ((long long)h * a.group + (real ? r - i * a.group : 0)) * a.qh + 8 * hh;
+        uint4 raw[kK];
+#pragma unroll
+        for (int k = 0; k < kK; ++k) raw[k] = *reinterpret_cast<const uint4*>(q + 16 * k);
+        load_codes(tile0);
+        load_pages(tile0 + 1);
+        float amax = 0;
+#pragma unroll
+        for (int k = 0; k < kK; ++k) {
+          float x[8];
+          q_floats(raw[k], a.bf16, x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
+        }
+        const int ex = row_exponent(max_halves(amax));
+        const float f = a.scale_log2 < 0 ? -pow2i(ex) : pow2i(ex);
+#pragma unroll
+        for (int k = 0; k < kK; ++k) {
+          float x[8];
+          q_floats(raw[k], a.bf16, x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) qf[k][e] = (_Float16)(x[e] * f);
+        }
+        qs = fabsf(a.scale_log2) * pow2i(-ex);
+        most = __builtin_amdgcn_readfirstlane(max_half_wave(limit));
+        least = -__builtin_amdgcn_readfirstlane(max_half_wave(real ? -limit : -INT32_MAX));
+      }
+
+      f16_t o[kDt];
+      float m = kNegInf, l = 0, unit = 0;
+#pragma unroll
+      for (int d = 0; d < kDt; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[d][v] = 0;
+      __syncthreads();  // the buffers may be in use by the item before
+      store_codes(tile0 & 1);
+      load_codes(tile0 + 1);
+      load_pages(tile0 + 2);
+      __syncthreads();
+
+      for (int tile = tile0; tile < tile1; ++tile) {
+        const int buf = tile & 1, key0 = tile * kTile;
+        if (tile + 1 < tile1) {
+          store_codes(buf ^ 1);
+          load_codes(tile + 2);
+          load_pages(tile + 3);
+        }
+        if (key0 < most) {
+          f16_t st[2];
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) st[t][v] = 0;
+#pragma unroll
+          for (int k = 0; k < kK; ++k)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const h8_t kf = *reinterpret_cast<const h8_t*>(lds.k[buf][2 * k + hh][32 * t + n32]);
+              st[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[k], st[t], 0, 0, 0);
+            }
+          // Group q of 16 tokens: registers 8 (q % 2) .. of st[q / 2].
+          float ck[4], rel[4];
+          float top = 0;
+          bool missing = false;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            ck[q] = lds.ks[buf][q] * qs;
+            rel[q] = lds.vs[buf][q];
+            missing |= lds.ks[buf][q] == -1.0f;
+            if (rel[q] < __builtin_huge_valf()) top = fmaxf(top, rel[q]);
+          }
+          float alpha = 1.0f;
+          bool move = false;
+          if (top > 0 && !(top <= 64.0f * unit && top * 64.0f >= unit)) {
+            const float was = unit;
+            unit = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, top) & 0x7F800000u);
+            if (unit == 0.0f) unit = 0x1p-126f;
+            alpha = was / unit;
+            move = true;
+          }
+          const float per_unit = unit > 0 ? 1.0f / unit : 0.0f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) rel[q] *= per_unit;
+
+          const bool masked = key0 + kTile > least || missing;
+          // Places of this lane's tokens in the tile: 16 q + 8 (e / 4) + 4 hh + e % 4.
+          const int left = limit - key0 - 4 * hh;
+          if (masked) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const bool there = lds.ks[buf][q] != -1.0f;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float x = st[q >> 1][8 * (q & 1) + e];
+                st[q >> 1][8 * (q & 1) + e] =
+                    there && 16 * q + 8 * (e >> 2) + (e & 3) < left ? x * ck[q] : kNegInf;
+              }
+              ck[q] = 1.0f;
+            }
+          }
+          float tm = kNegInf;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float g = st[q >> 1][8 * (q & 1)];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) g = fmaxf(g, st[q >> 1][8 * (q & 1) + e]);
+            tm = fmaxf(tm, g * ck[q]);
+          }
+          if (__any(tm > m + kLazy)) {
+            const float mn = fmaxf(m, max_halves(tm));
+            const float f = mn == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            l *= f;
+            alpha *= f;
+            m = mn;
+            move = true;
+          }
+          if (move) {
+#pragma unroll
+            for (int d = 0; d < kDt; ++d) o[d] *= alpha;
+          }
+          const float sub = m == kNegInf ? 0.0f : -m;
+          h8_t pf[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const bool there = !masked || lds.ks[buf][q] != -1.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float p = __builtin_amdgcn_exp2f(fmaf(st[q >> 1][8 * (q & 1) + e], ck[q], sub));
+              l += p;
+              float w = p * rel[q];
+              if (masked && !(there && 16 * q + 8 * (e >> 2) + (e & 3) < left)) w = 0.0f;
+              pf[q][e] = (_Float16)w;
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int d = 0; d < kDt; ++d) {
+              const h8_t vf = *reinterpret_cast<const h8_t*>(lds.v[buf] + (2 * q + hh) * M::kBlock +
+                                                             (32 * d + n32) * 16);
+              o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[q], o[d], 0, 0, 0);
+            }
+        }
+        __syncthreads();
+      }
+
+      l = sum_halves(l);
+#pragma unroll
+      for (int d = 0; d < kDt; ++d) o[d] *= unit;  // 0 where no page had a scale above 0
+      const int r = row0 + n32;
+      bool write = true;
+      if (tile0 > 0 || tile1 < tiles) {
+        // A piece, as the registers lie: [wave][pair of registers][lane].
+        auto place = [&](int k, int pair) {
+          return a.partials + (2LL * k) * M::kPiece + ((wave * (8 * kDt) + pair) * 64 + lane) * 2;
+        };
+        auto stats = [&](int k) {
+          return a.partials + (2LL * k) * M::kPiece + kManyRows * D + (wave * 32 + n32) * 2;
+        };
+        const int own = tile0 == 0 ? 1 : 0;
+        float* slot = place(wg, 0) + own * M::kPiece;
+#pragma unroll
+        for (int d = 0; d < kDt; ++d)
+#pragma unroll
+          for (int v = 0; v < 8; ++v) store_agent2(slot + (8 * d + v) * 128, o[d][2 * v], o[d][2 * v + 1]);
+        if (hh == 0) store_agent2(stats(wg) + own * M::kPiece, m, l);
+        const int wg0 = tile0 == 0 ? wg : (start + kManyItemCost) / share;
+        const int pieces = (start + units - 1) / share - wg0 + 1;
+        __builtin_amdgcn_s_waitcnt(0);  // this wave's stores to the workspace
+        __syncthreads();
+        if (wave == 0) {
+          if (lane == 0) set_flag(a.flags + 2 * wg + own, a.gen);
+          __builtin_amdgcn_s_waitcnt(0);
+          const bool all = flags_set(a.flags, a.gen, wg0, pieces, lane);
+          if (lane == 0) lds.last = all;
+        }
+        __syncthreads();
+        write = lds.last;
+        if (write) {
+          m = kNegInf, l = 0;
+#pragma unroll
+          for (int d = 0; d < kDt; ++d)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[d][v] = 0;
+          for (int k = 0; k < pieces; ++k) {
+            const long long off = k == 0 ? M::kPiece : 0;
+            const float2 ml = load_agent2(stats(wg0 + k) + off);
+            const float* p = place(wg0 + k, 0) + off;
+            float2 x[kDt][8];
+#pragma unroll
+            for (int d = 0; d < kDt; ++d)
+#pragma unroll
+              for (int v = 0; v < 8; ++v) x[d][v] = load_agent2(p + (8 * d + v) * 128);
+            const float mn = fmaxf(m, ml.x);
+            const float fo = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+            const float fn = ml.x == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
+            l = l * fo + ml.y * fn;  // a NaN stays
+            m = mn;
+#pragma unroll
+            for (int d = 0; d < kDt; ++d)
+#pragma unroll
+              for (int v = 0; v < 8; ++v) {
+                o[d][2 * v] = fmaf(o[d][2 * v], fo, x[d][v].x * fn);
+                o[d][2 * v + 1] = fmaf(o[d][2 * v + 1], fo, x[d][v].y * fn);
+              }
+          }
+          for (int k = tid; k < pieces; k += kManyThreads)
+            set_flag(a.flags + 2 * (wg0 + k) + (k == 0), 0);
+        }
+      }
+      if (write && r < rows) {
+        const float inv = inverse_sum(l);
+        uint16_t* out = out_row<D>(a, s, h, r) + 4 * hh;
+#pragma unroll
+        for (int d = 0; d < kDt; ++d)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const float x[4] = {o[d][4 * v] * inv, o[d][4 * v + 1] * inv, o[d][4 * v + 2] * inv,
+                                o[d][4 * v + 3] * inv};
+            store_half4(a, out + 32 * d + 8 * v, x);
+          }
+      }
+    }
+    // On to the next item.
+    base += units;
+    if (++rt == s.row_tiles && cur < end) {
+      rt = 0;
+      if (++h == a.c.heads) {
+        h = 0;
+        do {
+          s = sequence(a, ++b, kManyRows, true);
+        } while (s.row_tiles == 0);
+      }
+    }
+  }
+}
+
 }  // namespace dk
 
 namespace {
 
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-// Column tiles of a wave: 16 rows where no sequence has more.
-int column_tiles(int max_query_len, int group) {
-  return (long long)max_query_len * group <= 16 ? 1 : 2;
+// Which kernels a call runs and what they need. Sequences of at most 32 rows
+// (queries times the group) are attend_few's, which takes 16 of them at a time
+// where no sequence has more, larger ones attend_many's; a call that by its
+// sizes can have one kind alone runs one kernel, which then takes every size.
+struct Dispatch {
+  bool few, many;
+  int nt;
+};
+Dispatch dispatch(int num_tokens, int requests, int group, int max_query_len) {
+  Dispatch d;
+  const long long rows = (long long)std::min(max_query_len, num_tokens) * group;
+  d.many = rows > 32;
+  d.few = !d.many || requests > 1;
+  d.nt = rows <= 16 ? 1 : 2;
+  return d;
 }
 
 // The number of a call, which never comes again in a process: what its pieces'
@@ -862,9 +1343,15 @@ unsigned long long next_call() {
   return calls.fetch_add(1, std::memory_order_relaxed);
 }
 
-size_t workspace(int nt, int head_size) {
-  return (size_t)dk::kWorkgroups * 2 * sizeof(unsigned long long) +
-         (size_t)dk::kWorkgroups * 2 * 16 * nt * (head_size + 2) * sizeof(float);
+size_t flags_bytes() { return (size_t)dk::kWorkgroups * 2 * sizeof(unsigned long long); }
+
+// Flags and pieces of each kernel that runs.
+size_t workspace_bytes_of(const Dispatch& d, int head_size) {
+  size_t rows = 0;
+  if (d.few) rows += 16 * d.nt;
+  if (d.many) rows += dk::kManyRows;
+  return flags_bytes() * (d.few + d.many) +
+         (size_t)dk::kWorkgroups * 2 * rows * (head_size + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -874,8 +1361,8 @@ extern "C" size_t dk_kv_attend_workspace_bytes(int num_tokens, int requests, int
                                                int max_query_len) {
   (void)table_width;
   (void)page_size;
-  if (num_tokens <= 0 || requests <= 0 || heads <= 0 || q_heads <= 0) return 0;
-  return workspace(column_tiles(max_query_len, q_heads / heads), head_size);
+  if (num_tokens <= 0 || requests <= 0 || heads <= 0 || q_heads <= 0 || head_size <= 0) return 0;
+  return workspace_bytes_of(dispatch(num_tokens, requests, q_heads / heads, max_query_len), head_size);
 }
 
 extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
@@ -918,10 +1405,12 @@ extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
                       (((double)table_width * cache->page_size) / dk::kTile + 2);
   if (most > 1 << 30)
     return dk::set_error(DK_ERR_UNSUPPORTED, "heads * queries * keys too large");
-  const int nt = column_tiles(max_query_len, group);
-  if (workspace_bytes < workspace(nt, cache->head_size))
+  if (((double)table_width * cache->page_size + num_tokens + dk::kTile) * group > 1 << 30)
+    return dk::set_error(DK_ERR_UNSUPPORTED, "keys * q_heads / heads too large");
+  const Dispatch d = dispatch(num_tokens, requests, group, max_query_len);
+  if (workspace_bytes < workspace_bytes_of(d, cache->head_size))
     return dk::set_error(DK_ERR_INVALID_ARGUMENT, "the workspace has %zu of %zu bytes",
-                         workspace_bytes, workspace(nt, cache->head_size));
+                         workspace_bytes, workspace_bytes_of(d, cache->head_size));
   dk::AttendArgs a{};
   a.c = view;
   a.q = static_cast<const uint16_t*>(q);
@@ -931,9 +1420,7 @@ extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
   a.tables = tables;
   a.lens = seq_lens;
   a.offsets = query_offsets;
-  a.flags = static_cast<unsigned long long*>(workspace_ptr);
   a.gen = next_call();
-  a.partials = reinterpret_cast<float*>(a.flags + 2 * dk::kWorkgroups);
   a.scale_log2 = scale * 1.44269504088896340736f;
   a.width = cache->pages > 0 ? table_width : 0;  // no pages, no keys
   a.tokens = num_tokens;
@@ -941,15 +1428,27 @@ extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
   a.group = group;
   a.bf16 = dtype == DK_KV_BF16;
   a.causal = causal != 0;
-  auto launch = [&](auto kernel, int threads) {
+  char* ws = static_cast<char*>(workspace_ptr);
+  auto launch = [&](auto kernel, int threads, int rows) {
+    a.flags = reinterpret_cast<unsigned long long*>(ws);
+    a.partials = reinterpret_cast<float*>(ws + flags_bytes());
     hipLaunchKernelGGL(kernel, dim3(dk::kWorkgroups), dim3(threads), 0, stream, a);
+    ws += flags_bytes() + (size_t)dk::kWorkgroups * 2 * rows * (cache->head_size + 2) * sizeof(float);
   };
-  if (cache->head_size == 64) {
-    if (nt == 1) launch(dk::attend_few<64, 1>, dk::Few<64, 1>::kThreads);
-    else launch(dk::attend_few<64, 2>, dk::Few<64, 2>::kThreads);
-  } else {
-    if (nt == 1) launch(dk::attend_few<128, 1>, dk::Few<128, 1>::kThreads);
-    else launch(dk::attend_few<128, 2>, dk::Few<128, 2>::kThreads);
+  if (d.many) {
+    a.few_rows = d.few ? 32 : 0;
+    if (cache->head_size == 64) launch(dk::attend_many<64>, dk::kManyThreads, dk::kManyRows);
+    else launch(dk::attend_many<128>, dk::kManyThreads, dk::kManyRows);
+  }
+  if (d.few) {
+    a.few_rows = d.many ? 32 : INT32_MAX;
+    if (cache->head_size == 64) {
+      if (d.nt == 1) launch(dk::attend_few<64, 1>, dk::Few<64, 1>::kThreads, 16);
+      else launch(dk::attend_few<64, 2>, dk::Few<64, 2>::kThreads, 32);
+    } else {
+      if (d.nt == 1) launch(dk::attend_few<128, 1>, dk::Few<128, 1>::kThreads, 16);
+      else launch(dk::attend_few<128, 2>, dk::Few<128, 2>::kThreads, 32);
+    }
   }
   return dk::check_launch("attend launch");
 }
