@@ -947,6 +947,21 @@ __device__ __forceinline__ int head_cost(const AttendArgs& a, const Seq& s) {
                    (unsigned)(s.len - s.n) * G + kManyRows + kTile * G - 1);
 }
 
+constexpr int kAhead = 4;
+
+// Keeps the compiler to this order: kAhead loads from LDS, then a product and
+// a load in turn. Left to itself it put every load right before its product.
+template <int kProducts, int kLoadsAhead>
+__device__ __forceinline__ void interleave_loads() {
+  __builtin_amdgcn_sched_group_barrier(0x100, kLoadsAhead, 0);  // LDS reads
+#pragma unroll
+  for (int i = 0; i < kProducts - kLoadsAhead; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, kLoadsAhead, 0);
+}
+
 template <int D>
 __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
   using M = Many<D>;
@@ -1129,23 +1144,31 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int v = 0; v < 16; ++v) st[t][v] = 0;
+          // Operands come from LDS kAhead products ahead of their own.
+          h8_t kf[kAhead];
+          auto load_k = [&](int i) {
+            kf[i % kAhead] =
+                *reinterpret_cast<const h8_t*>(lds.k[buf][i / 2 * 2 + hh][32 * (i % 2) + n32]);
+          };
 #pragma unroll
-          for (int k = 0; k < kK; ++k)
+          for (int i = 0; i < kAhead; ++i) load_k(i);
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              const h8_t kf = *reinterpret_cast<const h8_t*>(lds.k[buf][2 * k + hh][32 * t + n32]);
-              st[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[k], st[t], 0, 0, 0);
-            }
+          for (int i = 0; i < 2 * kK; ++i) {
+            st[i % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i % kAhead], qf[i / 2], st[i % 2], 0, 0, 0);
+            if (i + kAhead < 2 * kK) load_k(i + kAhead);
+          }
+          interleave_loads<2 * kK, kAhead>();
           // Group q of 16 tokens: registers 8 (q % 2) .. of st[q / 2].
           float ck[4], rel[4];
           float top = 0;
-          bool missing = false;
+          bool missing = false, finite = true;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             ck[q] = lds.ks[buf][q] * qs;
             rel[q] = lds.vs[buf][q];
             missing |= lds.ks[buf][q] == -1.0f;
             if (rel[q] < __builtin_huge_valf()) top = fmaxf(top, rel[q]);
+            else finite = false;
           }
           float alpha = 1.0f;
           bool move = false;
@@ -1160,18 +1183,19 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) rel[q] *= per_unit;
 
-          const bool masked = key0 + kTile > least || missing;
           // Places of this lane's tokens in the tile: 16 q + 8 (e / 4) + 4 hh + e % 4.
           const int left = limit - key0 - 4 * hh;
+          auto seen = [&](int q, int e) {
+            return lds.ks[buf][q] != -1.0f && 16 * q + 8 * (e >> 2) + (e & 3) < left;
+          };
+          const bool masked = key0 + kTile > least || missing;
           if (masked) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const bool there = lds.ks[buf][q] != -1.0f;
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
                 const float x = st[q >> 1][8 * (q & 1) + e];
-                st[q >> 1][8 * (q & 1) + e] =
-                    there && 16 * q + 8 * (e >> 2) + (e & 3) < left ? x * ck[q] : kNegInf;
+                st[q >> 1][8 * (q & 1) + e] = seen(q, e) ? x * ck[q] : kNegInf;
               }
               ck[q] = 1.0f;
             }
@@ -1199,25 +1223,32 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
           const float sub = m == kNegInf ? 0.0f : -m;
           h8_t pf[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const bool there = !masked || lds.ks[buf][q] != -1.0f;
+          for (int q = 0; q < 4; ++q)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const float p = __builtin_amdgcn_exp2f(fmaf(st[q >> 1][8 * (q & 1) + e], ck[q], sub));
               l += p;
-              float w = p * rel[q];
-              if (masked && !(there && 16 * q + 8 * (e >> 2) + (e & 3) < left)) w = 0.0f;
-              pf[q][e] = (_Float16)w;
+              pf[q][e] = (_Float16)(p * rel[q]);
             }
+          if (masked && !finite) {  // a key that is not seen has weight 0 on a page of any scale
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) pf[q][e] = seen(q, e) ? pf[q][e] : (_Float16)0.0f;
           }
+          h8_t vf[kAhead];
+          auto load_v = [&](int i) {
+            vf[i % kAhead] = *reinterpret_cast<const h8_t*>(
+                lds.v[buf] + (2 * (i / kDt) + hh) * M::kBlock + (32 * (i % kDt) + n32) * 16);
+          };
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int i = 0; i < kAhead; ++i) load_v(i);
 #pragma unroll
-            for (int d = 0; d < kDt; ++d) {
-              const h8_t vf = *reinterpret_cast<const h8_t*>(lds.v[buf] + (2 * q + hh) * M::kBlock +
-                                                             (32 * d + n32) * 16);
-              o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[q], o[d], 0, 0, 0);
-            }
+          for (int i = 0; i < 4 * kDt; ++i) {
+            o[i % kDt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i % kAhead], pf[i / kDt], o[i % kDt], 0, 0, 0);
+            if (i + kAhead < 4 * kDt) load_v(i + kAhead);
+          }
+          interleave_loads<4 * kDt, kAhead>();
         }
         __syncthreads();
       }
