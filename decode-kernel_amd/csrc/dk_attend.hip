@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "dk_host.hpp"
 #include "dk_kv.hpp"
@@ -870,8 +871,7 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
 // A workgroup of eight waves takes 256 rows of one sequence and key/value head
 // over the tiles of keys, 32 rows a wave, v_mfma_f32_32x32x16_f16. It turns a
 // tile's codes into fp16 in LDS once for all its rows (a thread 16 bytes of
-// keys and of values), two tiles in turn: while one is multiplied, the next is
-// converted and the one after is on its way. Rows of a product's right operand
+// keys and of values), two tiles ahead of the products. Rows of a product's right operand
 // are a wave's lanes, so a row's maximum and sum need one exchange of the
 // wave's halves, and P goes from the first product's registers into the
 // second's. Values lie in LDS in the order in which lanes hold P's tokens.
@@ -895,9 +895,11 @@ struct Many {
   static constexpr int kPiece = kManyRows * (D + 2);      // floats in the workspace
   static constexpr int kBlock = D * 16 + 16;              // bytes of eight tokens' values, spread over the banks
   struct Lds {
-    alignas(16) char k[2][D / 8][kTile][16];  // eight elements of a key
-    alignas(16) char v[2][8 * kBlock];        // [(16 tokens, half)][element][8 tokens]
-    float ks[2][4], vs[2][4];                 // scales of a tile's 16-token groups; -1: no page
+    // Three tiles in turn: one is multiplied by P while the next is multiplied
+    // by Q and the one after is written, with the workgroup's halves apart.
+    alignas(16) char k[3][D / 8][kTile][16];  // eight elements of a key
+    alignas(16) char v[3][8 * kBlock];        // [(16 tokens, half)][element][8 tokens]
+    float ks[3][4], vs[3][4];                 // scales of a tile's 16-token groups; -1: no page
     int last;
   };
 };
@@ -947,6 +949,14 @@ __device__ __forceinline__ int head_cost(const AttendArgs& a, const Seq& s) {
                    (unsigned)(s.len - s.n) * G + kManyRows + kTile * G - 1);
 }
 
+// A workgroup barrier for what is in LDS alone: __syncthreads() also waits for
+// every load from memory under way, the next tiles' codes among them.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 constexpr int kAhead = 4;
 
 // Keeps the compiler to this order: kAhead loads from LDS, then a product and
@@ -958,6 +968,7 @@ __device__ __forceinline__ void interleave_loads() {
   for (int i = 0; i < kProducts - kLoadsAhead; ++i) {
     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
     __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, 0, 0);  // VALU: the next tile's codes
   }
   __builtin_amdgcn_sched_group_barrier(0x008, kLoadsAhead, 0);
 }
@@ -1036,55 +1047,61 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
       const int32_t* table = a.tables + (long long)b * a.width;
 
       // Loads of a tile: keys of token lane, piece `wave`; values of 16 tokens
-      // of one element. With 64 elements half the waves load each.
-      const bool loads_k = D == 128 || wave < 4, loads_v = D == 128 || wave >= 4;
+      // of one element. With 64 elements half the waves load each. They run
+      // for every tile, past the last one too (of the last key's page): loads
+      // under a condition would be waited for where the ways meet again.
+      const bool loads_k = D == 128 || wave < 4;
       const int kc = wave & (kK - 1);
       const int vd = (D == 128 ? wave : wave & 3) * 16 + (lane >> 2), vq = lane & 3;
-      const long long page_bytes = (long long)a.c.heads * D * P;
-      uint4 kraw = zero4(), vraw = zero4();
-      float sraw = 0;
-      int kpage = -1, vpage = -1, spage = -1;
+      const uint32_t page_bytes = (uint32_t)a.c.heads * D * P;  // under 2^31
+      const int8_t* kbase = a.c.k + (uint32_t)((h * D + kc * 16) * P);
+      const int8_t* vbase = a.c.v + (uint32_t)((h * D + vd) * P);
+      const float* sbase = (wave == 0 ? a.c.ks : a.c.vs) + h;
+      uint4 kraw, vraw;
+      float sraw;
+      int kpage, vpage, spage;
+      const int last = s.len - 1;
       auto load_pages = [&](int tile) {
-        const int kt = tile * kTile + lane, vt = tile * kTile + 16 * vq;
-        kpage = tile < tile1 && kt < s.len ? table[kt >> shift] : -1;
-        vpage = tile < tile1 && vt < s.len ? table[vt >> shift] : -1;
+        kpage = table[min(tile * kTile + lane, last) >> shift];
+        vpage = table[min(tile * kTile + 16 * vq, last) >> shift];
       };
       auto load_codes = [&](int tile) {
-        const int kt = tile * kTile + lane, vt = tile * kTile + 16 * vq;
-        const int kp = kpage >= 0 && kpage < a.c.pages ? kpage : 0;
-        const int vp = vpage >= 0 && vpage < a.c.pages ? vpage : 0;
-        spage = vpage == vp ? vp : -1;
-        if (tile >= tile1 || tile * kTile >= s.len) return;  // nothing is there
-        if (loads_k)
-          kraw = *reinterpret_cast<const uint4*>(a.c.k + kp * page_bytes +
-                                                 ((long long)h * D + kc * 16) * P + (kt & (P - 1)) * 16);
-        if (loads_v)
-          vraw = *reinterpret_cast<const uint4*>(a.c.v + vp * page_bytes +
-                                                 ((long long)h * D + vd) * P + (vt & (P - 1)));
-        // Lanes 0..3 of two waves bring the scales of their 16 tokens.
-        if (wave == 0 || wave == 1) {
-          const float* scales = wave == 0 ? a.c.ks : a.c.vs;
-          sraw = scales[(long long)vp * a.c.heads + h];
+        const uint32_t kp = kpage >= 0 && kpage < a.c.pages ? kpage : 0;
+        const uint32_t vp = vpage >= 0 && vpage < a.c.pages ? vpage : 0;
+        const int kin = (tile * kTile + lane) & (P - 1), vin = (tile * kTile + 16 * vq) & (P - 1);
+        spage = vpage;
+        if constexpr (D == 128) {
+          kraw = *reinterpret_cast<const uint4*>(kbase + kin * 16 + (unsigned long long)kp * page_bytes);
+          vraw = *reinterpret_cast<const uint4*>(vbase + vin + (unsigned long long)vp * page_bytes);
+        } else {
+          kraw = *reinterpret_cast<const uint4*>((loads_k ? kbase + kin * 16 : vbase + vin) +
+                                                 (unsigned long long)(loads_k ? kp : vp) * page_bytes);
+          vraw = kraw;
         }
+        sraw = sbase[(unsigned long long)vp * (uint32_t)a.c.heads];
       };
       auto store_codes = [&](int buf) {
         if (loads_k) {
-          *reinterpret_cast<h8_t*>(lds.k[buf][2 * kc][lane]) = codes_to_f16(kraw.x, kraw.y);
-          *reinterpret_cast<h8_t*>(lds.k[buf][2 * kc + 1][lane]) = codes_to_f16(kraw.z, kraw.w);
+          auto& k = lds.k[buf];
+          *reinterpret_cast<h8_t*>(k[2 * kc][lane]) = codes_to_f16(kraw.x, kraw.y);
+          *reinterpret_cast<h8_t*>(k[2 * kc + 1][lane]) = codes_to_f16(kraw.z, kraw.w);
         }
-        if (loads_v) {
+        if (D == 128 || !loads_k) {
           char* v = lds.v[buf] + 2 * vq * M::kBlock + vd * 16;
           *reinterpret_cast<h8_t*>(v) = codes_to_f16(vraw.x, vraw.z);
           *reinterpret_cast<h8_t*>(v + M::kBlock) = codes_to_f16(vraw.y, vraw.w);
         }
-        if (wave < 2 && lane < 4) (wave == 0 ? lds.ks : lds.vs)[buf][lane] = spage >= 0 ? sraw : -1.0f;
+        // The scales of 16 tokens each, by lanes 0..3 of two waves.
+        if (wave < 2 && lane < 4)
+          (wave == 0 ? lds.ks : lds.vs)[buf][lane] = spage >= 0 && spage < a.c.pages ? sraw : -1.0f;
       };
 
-      load_pages(tile0);
+      const bool keys = s.len > 0;  // a sequence without keys has no page to read
+      if (keys) load_pages(tile0);
       // The queries of this wave's rows.
       h8_t qf[kK];
       float qs;
-      int limit, least, most;
+      int limit, least;
       {
         const int r = row0 + n32;
         const bool real = r < rows;
@@ -1095,8 +1112,10 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
         uint4 raw[kK];
 #pragma unroll
         for (int k = 0; k < kK; ++k) raw[k] = *reinterpret_cast<const uint4*>(q + 16 * k);
-        load_codes(tile0);
-        load_pages(tile0 + 1);
+        if (keys) {
+          load_codes(tile0);
+          load_pages(tile0 + 1);
+        }
         float amax = 0;
 #pragma unroll
         for (int k = 0; k < kK; ++k) {
@@ -1115,142 +1134,166 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
           for (int e = 0; e < 8; ++e) qf[k][e] = (_Float16)(x[e] * f);
         }
         qs = fabsf(a.scale_log2) * pow2i(-ex);
-        most = __builtin_amdgcn_readfirstlane(max_half_wave(limit));
         least = -__builtin_amdgcn_readfirstlane(max_half_wave(real ? -limit : -INT32_MAX));
       }
 
-      f16_t o[kDt];
-      float m = kNegInf, l = 0, unit = 0;
+      // Sums, and what the fast way through a tile compares with: `bound` the
+      // score that moves a row's maximum, `sub` what is taken off a score.
+      f16_t o[kDt], st[2];
+      h8_t pf[4];
+      float m = kNegInf, bound = kNegInf, sub = 0, l = 0;
+      float unit = 0, per_unit = 0;
 #pragma unroll
       for (int d = 0; d < kDt; ++d)
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[d][v] = 0;
-      __syncthreads();  // the buffers may be in use by the item before
-      store_codes(tile0 & 1);
-      load_codes(tile0 + 1);
-      load_pages(tile0 + 2);
-      __syncthreads();
 
-      for (int tile = tile0; tile < tile1; ++tile) {
-        const int buf = tile & 1, key0 = tile * kTile;
-        if (tile + 1 < tile1) {
-          store_codes(buf ^ 1);
-          load_codes(tile + 2);
-          load_pages(tile + 3);
-        }
-        if (key0 < most) {
-          f16_t st[2];
+      // Products of the values of `vbuf` with P, then of the keys of `kbuf`
+      // with Q: operands come from LDS kAhead products ahead of their own.
+      auto products = [&](auto with_values, auto with_keys, int vbuf, int kbuf) {
+        constexpr int kV = decltype(with_values)::value ? 4 * kDt : 0;
+        constexpr int kN = kV + (decltype(with_keys)::value ? 2 * kK : 0);
+        const char* v = lds.v[vbuf] + hh * M::kBlock + n32 * 16;
+        const char* k = &lds.k[kbuf][hh][n32][0];
+        h8_t ring[kAhead];
+        auto load = [&](int i) {
+          const char* from = i < kV ? v + 2 * (i / kDt) * M::kBlock + 32 * (i % kDt) * 16
+                                    : k + (2 * ((i - kV) / 2) * kTile + 32 * ((i - kV) % 2)) * 16;
+          ring[i % kAhead] = *reinterpret_cast<const h8_t*>(from);
+        };
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) load(i);
+        if constexpr (decltype(with_keys)::value) {
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) st[t][v] = 0;
-          // Operands come from LDS kAhead products ahead of their own.
-          h8_t kf[kAhead];
-          auto load_k = [&](int i) {
-            kf[i % kAhead] =
-                *reinterpret_cast<const h8_t*>(lds.k[buf][i / 2 * 2 + hh][32 * (i % 2) + n32]);
-          };
+            for (int e = 0; e < 16; ++e) st[t][e] = 0;
+        }
 #pragma unroll
-          for (int i = 0; i < kAhead; ++i) load_k(i);
+        for (int i = 0; i < kN; ++i) {
+          const h8_t x = ring[i % kAhead];
+          if (i < kV)
+            o[i % kDt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pf[i / kDt], o[i % kDt], 0, 0, 0);
+          else
+            st[(i - kV) % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qf[(i - kV) / 2], st[(i - kV) % 2], 0, 0, 0);
+          if (i + kAhead < kN) load(i + kAhead);
+        }
+        interleave_loads<kN, kAhead>();
+      };
+
+      // P of a tile from its scores.
+      auto weights = [&](int tile, int buf) {
+        const int key0 = tile * kTile;
+        const f4_t cs = *reinterpret_cast<const f4_t*>(lds.ks[buf]);
+        const f4_t vs = *reinterpret_cast<const f4_t*>(lds.vs[buf]);
+        float ck[4], rel[4];
+        const float top = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+        const float bottom = fminf(fminf(cs[0], cs[1]), fminf(cs[2], cs[3]));  // -1: a page is missing
+        float alpha = 1.0f;
+        bool move = false;
+        if (__builtin_expect(!(top * 64.0f >= unit && top <= unit * 64.0f), 0)) {  // the unit moves, or there is none
+          float t = 0;
 #pragma unroll
-          for (int i = 0; i < 2 * kK; ++i) {
-            st[i % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i % kAhead], qf[i / 2], st[i % 2], 0, 0, 0);
-            if (i + kAhead < 2 * kK) load_k(i + kAhead);
-          }
-          interleave_loads<2 * kK, kAhead>();
-          // Group q of 16 tokens: registers 8 (q % 2) .. of st[q / 2].
-          float ck[4], rel[4];
-          float top = 0;
-          bool missing = false, finite = true;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            ck[q] = lds.ks[buf][q] * qs;
-            rel[q] = lds.vs[buf][q];
-            missing |= lds.ks[buf][q] == -1.0f;
-            if (rel[q] < __builtin_huge_valf()) top = fmaxf(top, rel[q]);
-            else finite = false;
-          }
-          float alpha = 1.0f;
-          bool move = false;
-          if (top > 0 && !(top <= 64.0f * unit && top * 64.0f >= unit)) {
+          for (int q = 0; q < 4; ++q) t = fmaxf(t, vs[q] < __builtin_huge_valf() ? vs[q] : 0.0f);
+          if (t > 0 && !(t * 64.0f >= unit && t <= unit * 64.0f)) {
             const float was = unit;
-            unit = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, top) & 0x7F800000u);
-            if (unit == 0.0f) unit = 0x1p-126f;
+            unit = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, t) & 0x7F800000u);
+            unit = fmaxf(unit, 0x1p-120f);
             alpha = was / unit;
             move = true;
+            per_unit = 1.0f / unit;
           }
-          const float per_unit = unit > 0 ? 1.0f / unit : 0.0f;
+        }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) rel[q] *= per_unit;
-
-          // Places of this lane's tokens in the tile: 16 q + 8 (e / 4) + 4 hh + e % 4.
-          const int left = limit - key0 - 4 * hh;
-          auto seen = [&](int q, int e) {
-            return lds.ks[buf][q] != -1.0f && 16 * q + 8 * (e >> 2) + (e & 3) < left;
-          };
-          const bool masked = key0 + kTile > least || missing;
-          if (masked) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const float x = st[q >> 1][8 * (q & 1) + e];
-                st[q >> 1][8 * (q & 1) + e] = seen(q, e) ? x * ck[q] : kNegInf;
-              }
-              ck[q] = 1.0f;
-            }
-          }
-          float tm = kNegInf;
+        for (int q = 0; q < 4; ++q) {
+          ck[q] = cs[q] * qs;
+          rel[q] = vs[q] * per_unit;
+        }
+        bool fix = false;
+        // Places of this lane's tokens in the tile: 16 q + 8 (e / 4) + 4 hh + e % 4.
+        int left = limit - key0 - 4 * hh;
+        auto seen = [&](int q, int e) { return cs[q] != -1.0f && 16 * q + 8 * (e >> 2) + (e & 3) < left; };
+        if (__builtin_expect(key0 + kTile > least || bottom < 0, 0)) {
+          asm volatile("" : "+v"(left));  // keeps the comparisons in here
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            float g = st[q >> 1][8 * (q & 1)];
 #pragma unroll
-            for (int e = 1; e < 8; ++e) g = fmaxf(g, st[q >> 1][8 * (q & 1) + e]);
-            tm = fmaxf(tm, g * ck[q]);
+            for (int e = 0; e < 8; ++e) {
+              const float x = st[q >> 1][8 * (q & 1) + e];
+              st[q >> 1][8 * (q & 1) + e] = seen(q, e) ? x * ck[q] : kNegInf;
+            }
+            ck[q] = 1.0f;
           }
-          if (__any(tm > m + kLazy)) {
-            const float mn = fmaxf(m, max_halves(tm));
-            const float f = mn == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-            l *= f;
-            alpha *= f;
-            m = mn;
-            move = true;
-          }
-          if (move) {
+          fix = !(fabsf(vs[0]) + fabsf(vs[1]) + fabsf(vs[2]) + fabsf(vs[3]) < __builtin_huge_valf());
+        }
+        float tm = kNegInf;
 #pragma unroll
-            for (int d = 0; d < kDt; ++d) o[d] *= alpha;
+        for (int q = 0; q < 4; ++q) {
+          float g = st[q >> 1][8 * (q & 1)];
+#pragma unroll
+          for (int e = 1; e < 8; ++e) g = fmaxf(g, st[q >> 1][8 * (q & 1) + e]);
+          tm = fmaxf(tm, g * ck[q]);
+        }
+        if (__builtin_expect(__any(tm > bound), 0)) {
+          const float mn = fmaxf(m, max_halves(tm));
+          const float f = mn == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+          l *= f;
+          alpha *= f;
+          m = mn;
+          bound = mn + kLazy;
+          sub = mn == kNegInf ? 0.0f : -mn;
+          move = true;
+        }
+        if (__builtin_expect(move, 0)) {
+#pragma unroll
+          for (int d = 0; d < kDt; ++d) o[d] *= alpha;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(st[q >> 1][8 * (q & 1) + e], ck[q], sub));
+            l += p;
+            pf[q][e] = (_Float16)(p * rel[q]);
           }
-          const float sub = m == kNegInf ? 0.0f : -m;
-          h8_t pf[4];
+        if (__builtin_expect(fix, 0)) {  // a key that is not seen has weight 0 on a page of any scale
+          asm volatile("" : "+v"(left));
 #pragma unroll
           for (int q = 0; q < 4; ++q)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float p = __builtin_amdgcn_exp2f(fmaf(st[q >> 1][8 * (q & 1) + e], ck[q], sub));
-              l += p;
-              pf[q][e] = (_Float16)(p * rel[q]);
-            }
-          if (masked && !finite) {  // a key that is not seen has weight 0 on a page of any scale
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-              for (int e = 0; e < 8; ++e) pf[q][e] = seen(q, e) ? pf[q][e] : (_Float16)0.0f;
-          }
-          h8_t vf[kAhead];
-          auto load_v = [&](int i) {
-            vf[i % kAhead] = *reinterpret_cast<const h8_t*>(
-                lds.v[buf] + (2 * (i / kDt) + hh) * M::kBlock + (32 * (i % kDt) + n32) * 16);
-          };
-#pragma unroll
-          for (int i = 0; i < kAhead; ++i) load_v(i);
-#pragma unroll
-          for (int i = 0; i < 4 * kDt; ++i) {
-            o[i % kDt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i % kAhead], pf[i / kDt], o[i % kDt], 0, 0, 0);
-            if (i + kAhead < 4 * kDt) load_v(i + kAhead);
-          }
-          interleave_loads<4 * kDt, kAhead>();
+            for (int e = 0; e < 8; ++e) pf[q][e] = seen(q, e) ? pf[q][e] : (_Float16)0.0f;
         }
-        __syncthreads();
+      };
+
+      if (keys) {
+        constexpr std::true_type kYes;
+        constexpr std::false_type kNo;
+        // Tile tile0 + i is in buffer i % 3: the one before this one, this one
+        // and the next.
+        int prev = 2, buf = 0, next = 1;
+        lds_barrier();  // the buffers may be in use by the item before
+        store_codes(0);
+        load_codes(tile0 + 1);
+        load_pages(tile0 + 2);
+        lds_barrier();
+        // The workgroup's two halves, a wave of each on every SIMD, run half a
+        // tile apart: while one multiplies, the other works out its weights.
+        // Both pass the same barriers.
+        if (wave >= 4) lds_barrier();
+        for (int tile = tile0; tile < tile1; ++tile) {
+          if (tile > tile0) products(kYes, kNo, prev, buf);
+          products(kNo, kYes, prev, buf);
+          store_codes(next);
+          load_codes(tile + 2);
+          load_pages(tile + 3);
+          lds_barrier();
+          weights(tile, buf);
+          lds_barrier();
+          const int free = prev;
+          prev = buf, buf = next, next = free;
+        }
+        products(kYes, kNo, prev, buf);
+        if (wave < 4) lds_barrier();
       }
 
       l = sum_halves(l);
