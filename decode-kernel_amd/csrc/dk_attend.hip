@@ -886,7 +886,7 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
 // ---------------------------------------------------------------------------
 constexpr int kManyRows = 256;
 constexpr int kManyThreads = 512;
-constexpr int kManyItemCost = 2;
+constexpr int kManyItemCost = 6;
 
 typedef float f16_t __attribute__((ext_vector_type(16)));
 
@@ -899,7 +899,9 @@ struct Many {
     // by Q and the one after is written, with the workgroup's halves apart.
     alignas(16) char k[3][D / 8][kTile][16];  // eight elements of a key
     alignas(16) char v[3][8 * kBlock];        // [(16 tokens, half)][element][8 tokens]
-    float ks[3][4], vs[3][4];                 // scales of a tile's 16-token groups; -1: no page
+    // Scales of a tile's 16-token groups, keys and values; -1: no page. The
+    // last one is where lanes that bring none write.
+    float scales[2][3][4], none;
     int last;
   };
 };
@@ -958,20 +960,6 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 constexpr int kAhead = 4;
-
-// Keeps the compiler to this order: kAhead loads from LDS, then a product and
-// a load in turn. Left to itself it put every load right before its product.
-template <int kProducts, int kLoadsAhead>
-__device__ __forceinline__ void interleave_loads() {
-  __builtin_amdgcn_sched_group_barrier(0x100, kLoadsAhead, 0);  // LDS reads
-#pragma unroll
-  for (int i = 0; i < kProducts - kLoadsAhead; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
-    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(0x002, 0, 0);  // VALU: the next tile's codes
-  }
-  __builtin_amdgcn_sched_group_barrier(0x008, kLoadsAhead, 0);
-}
 
 template <int D>
 __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
@@ -1057,7 +1045,7 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
       const int8_t* kbase = a.c.k + (uint32_t)((h * D + kc * 16) * P);
       const int8_t* vbase = a.c.v + (uint32_t)((h * D + vd) * P);
       const float* sbase = (wave == 0 ? a.c.ks : a.c.vs) + h;
-      uint4 kraw, vraw;
+      uint4 kraw, vraw;  // with 64 elements kraw alone, of keys or values
       float sraw;
       int kpage, vpage, spage;
       const int last = s.len - 1;
@@ -1065,35 +1053,50 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
         kpage = table[min(tile * kTile + lane, last) >> shift];
         vpage = table[min(tile * kTile + 16 * vq, last) >> shift];
       };
-      auto load_codes = [&](int tile) {
+      // In eight steps, to go between products.
+      auto load_codes = [&](int tile, int step) {
+        const int kin = (tile * kTile + lane) & (P - 1), vin = (tile * kTile + 16 * vq) & (P - 1);
         const uint32_t kp = kpage >= 0 && kpage < a.c.pages ? kpage : 0;
         const uint32_t vp = vpage >= 0 && vpage < a.c.pages ? vpage : 0;
-        const int kin = (tile * kTile + lane) & (P - 1), vin = (tile * kTile + 16 * vq) & (P - 1);
-        spage = vpage;
-        if constexpr (D == 128) {
-          kraw = *reinterpret_cast<const uint4*>(kbase + kin * 16 + (unsigned long long)kp * page_bytes);
-          vraw = *reinterpret_cast<const uint4*>(vbase + vin + (unsigned long long)vp * page_bytes);
+        if (step == 0) {
+          if constexpr (D == 128)
+            kraw = *reinterpret_cast<const uint4*>(kbase + kin * 16 + (unsigned long long)kp * page_bytes);
+          else
+            kraw = *reinterpret_cast<const uint4*>((loads_k ? kbase + kin * 16 : vbase + vin) +
+                                                   (unsigned long long)(loads_k ? kp : vp) * page_bytes);
+        } else if (step == 1) {
+          if constexpr (D == 128)
+            vraw = *reinterpret_cast<const uint4*>(vbase + vin + (unsigned long long)vp * page_bytes);
         } else {
-          kraw = *reinterpret_cast<const uint4*>((loads_k ? kbase + kin * 16 : vbase + vin) +
-                                                 (unsigned long long)(loads_k ? kp : vp) * page_bytes);
-          vraw = kraw;
+          spage = vpage;
+          sraw = sbase[(unsigned long long)vp * (uint32_t)a.c.heads];
         }
-        sraw = sbase[(unsigned long long)vp * (uint32_t)a.c.heads];
       };
-      auto store_codes = [&](int buf) {
-        if (loads_k) {
-          auto& k = lds.k[buf];
-          *reinterpret_cast<h8_t*>(k[2 * kc][lane]) = codes_to_f16(kraw.x, kraw.y);
-          *reinterpret_cast<h8_t*>(k[2 * kc + 1][lane]) = codes_to_f16(kraw.z, kraw.w);
-        }
-        if (D == 128 || !loads_k) {
-          char* v = lds.v[buf] + 2 * vq * M::kBlock + vd * 16;
-          *reinterpret_cast<h8_t*>(v) = codes_to_f16(vraw.x, vraw.z);
-          *reinterpret_cast<h8_t*>(v + M::kBlock) = codes_to_f16(vraw.y, vraw.w);
-        }
-        // The scales of 16 tokens each, by lanes 0..3 of two waves.
-        if (wave < 2 && lane < 4)
-          (wave == 0 ? lds.ks : lds.vs)[buf][lane] = spage >= 0 && spage < a.c.pages ? sraw : -1.0f;
+      auto store_codes = [&](int buf, int step) {
+        const uint4 v = D == 128 ? vraw : kraw;
+        char* vat = lds.v[buf] + 2 * vq * M::kBlock + vd * 16;
+        if (step == 0 && loads_k)
+          *reinterpret_cast<h8_t*>(lds.k[buf][2 * kc][lane]) = codes_to_f16(kraw.x, kraw.y);
+        else if (step == 1 && loads_k)
+          *reinterpret_cast<h8_t*>(lds.k[buf][2 * kc + 1][lane]) = codes_to_f16(kraw.z, kraw.w);
+        else if (step == 2 && (D == 128 || !loads_k))
+          *reinterpret_cast<h8_t*>(vat) = codes_to_f16(v.x, v.z);
+        else if (step == 3 && (D == 128 || !loads_k))
+          *reinterpret_cast<h8_t*>(vat + M::kBlock) = codes_to_f16(v.y, v.w);
+        else if (step == 4)  // the scales of 16 tokens each, by lanes 0..3 of two waves
+          (&lds.scales[0][0][0])[wave < 2 && lane < 4 ? wave * 12 + buf * 4 + lane : 24] =
+              spage >= 0 && spage < a.c.pages ? sraw : -1.0f;
+      };
+      // Step `step` of 9: tile's successor out of the registers into `buf`, the
+      // one after it into them, and that one's successor's pages.
+      auto move_codes = [&](int tile, int buf, int step) {
+        if (step < 5) store_codes(buf, step);
+        else if (step < 8) load_codes(tile + 2, step - 5);
+        else if (step == 8) load_pages(tile + 3);
+      };
+      auto move_all = [&](int tile, int buf) {
+#pragma unroll
+        for (int i = 0; i < 9; ++i) move_codes(tile, buf, i);
       };
 
       const bool keys = s.len > 0;  // a sequence without keys has no page to read
@@ -1113,7 +1116,8 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
 #pragma unroll
         for (int k = 0; k < kK; ++k) raw[k] = *reinterpret_cast<const uint4*>(q + 16 * k);
         if (keys) {
-          load_codes(tile0);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) load_codes(tile0, i);
           load_pages(tile0 + 1);
         }
         float amax = 0;
@@ -1150,7 +1154,7 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
 
       // Products of the values of `vbuf` with P, then of the keys of `kbuf`
       // with Q: operands come from LDS kAhead products ahead of their own.
-      auto products = [&](auto with_values, auto with_keys, int vbuf, int kbuf) {
+      auto products = [&](auto with_values, auto with_keys, int vbuf, int kbuf, auto between) {
         constexpr int kV = decltype(with_values)::value ? 4 * kDt : 0;
         constexpr int kN = kV + (decltype(with_keys)::value ? 2 * kK : 0);
         const char* v = lds.v[vbuf] + hh * M::kBlock + n32 * 16;
@@ -1177,15 +1181,16 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
           else
             st[(i - kV) % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qf[(i - kV) / 2], st[(i - kV) % 2], 0, 0, 0);
           if (i + kAhead < kN) load(i + kAhead);
+          between(i);
+          __builtin_amdgcn_sched_barrier(0);  // the compiler puts loads right before their products
         }
-        interleave_loads<kN, kAhead>();
       };
 
       // P of a tile from its scores.
       auto weights = [&](int tile, int buf) {
         const int key0 = tile * kTile;
-        const f4_t cs = *reinterpret_cast<const f4_t*>(lds.ks[buf]);
-        const f4_t vs = *reinterpret_cast<const f4_t*>(lds.vs[buf]);
+        const f4_t cs = *reinterpret_cast<const f4_t*>(lds.scales[0][buf]);
+        const f4_t vs = *reinterpret_cast<const f4_t*>(lds.scales[1][buf]);
         float ck[4], rel[4];
         const float top = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
         const float bottom = fminf(fminf(cs[0], cs[1]), fminf(cs[2], cs[3]));  // -1: a page is missing
@@ -1272,27 +1277,23 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
         // and the next.
         int prev = 2, buf = 0, next = 1;
         lds_barrier();  // the buffers may be in use by the item before
-        store_codes(0);
-        load_codes(tile0 + 1);
-        load_pages(tile0 + 2);
+        move_all(tile0 - 1, 0);
         lds_barrier();
         // The workgroup's two halves, a wave of each on every SIMD, run half a
         // tile apart: while one multiplies, the other works out its weights.
         // Both pass the same barriers.
         if (wave >= 4) lds_barrier();
+        auto nothing = [](int) {};
         for (int tile = tile0; tile < tile1; ++tile) {
-          if (tile > tile0) products(kYes, kNo, prev, buf);
-          products(kNo, kYes, prev, buf);
-          store_codes(next);
-          load_codes(tile + 2);
-          load_pages(tile + 3);
+          if (tile > tile0) products(kYes, kNo, prev, buf, nothing);
+          products(kNo, kYes, prev, buf, [&](int i) { move_codes(tile, next, i); });
           lds_barrier();
           weights(tile, buf);
           lds_barrier();
           const int free = prev;
           prev = buf, buf = next, next = free;
         }
-        products(kYes, kNo, prev, buf);
+        products(kYes, kNo, prev, buf, nothing);
         if (wave < 4) lds_barrier();
       }
 
