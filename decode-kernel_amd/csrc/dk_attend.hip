@@ -899,9 +899,9 @@ struct Many {
     // by Q and the one after is written, with the workgroup's halves apart.
     alignas(16) char k[3][D / 8][kTile][16];  // eight elements of a key
     alignas(16) char v[3][8 * kBlock];        // [(16 tokens, half)][element][8 tokens]
-    // Scales of a tile's 16-token groups, keys and values; -1: no page. The
-    // last one is where lanes that bring none write.
-    float scales[2][3][4], none;
+    // Scales of a tile's 16-token groups, keys and values; -1: no page. Lanes
+    // that bring none write to the second one.
+    float scales[2][3][4], none[24];
     int last;
   };
 };
@@ -960,6 +960,13 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 constexpr int kAhead = 4;
+
+// Uniform loads through it are scalar loads, stores elsewhere or not: what is
+// read so (tables, scales) no kernel here writes while it is read.
+template <typename T>
+__device__ __forceinline__ const __attribute__((address_space(4))) T* as_constant(const T* p) {
+  return (const __attribute__((address_space(4))) T*)(uintptr_t)p;
+}
 
 template <int D>
 __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
@@ -1034,73 +1041,75 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
       const int rows = s.n * a.group;
       const int32_t* table = a.tables + (long long)b * a.width;
 
-      // Loads of a tile: keys of token lane, piece `wave`; values of 16 tokens
-      // of one element. With 64 elements half the waves load each. They run
-      // for every tile, past the last one too (of the last key's page): loads
-      // under a condition would be waited for where the ways meet again.
+      // A wave loads 16 tokens of a tile, group `wave % 4`: half of their keys'
+      // pieces and of their values' elements, or with 64 elements all of the
+      // one or the other. Its page is uniform, so addresses cost no vector
+      // instruction. Loads run for every tile, past the last one too (of the
+      // last key's page): under a condition they would be waited for where the
+      // ways meet again.
       const bool loads_k = D == 128 || wave < 4;
-      const int kc = wave & (kK - 1);
-      const int vd = (D == 128 ? wave : wave & 3) * 16 + (lane >> 2), vq = lane & 3;
+      const int own = wave & 3, half = wave >> 2;
+      const int kc = (D == 128 ? 4 * half : 0) + (lane >> 4), vd = (D == 128 ? 64 * half : 0) + lane;
       const uint32_t page_bytes = (uint32_t)a.c.heads * D * P;  // under 2^31
-      const int8_t* kbase = a.c.k + (uint32_t)((h * D + kc * 16) * P);
-      const int8_t* vbase = a.c.v + (uint32_t)((h * D + vd) * P);
-      const float* sbase = (wave == 0 ? a.c.ks : a.c.vs) + h;
+      const uint32_t head_bytes = (uint32_t)h * D * P;
+      const uint32_t kat = (kc * P + (lane & 15)) * 16, vat = vd * P;
       uint4 kraw, vraw;  // with 64 elements kraw alone, of keys or values
-      float sraw;
-      int kpage, vpage, spage;
+      float ksraw, vsraw;
+      int page, page_of_raw;
       const int last = s.len - 1;
-      auto load_pages = [&](int tile) {
-        kpage = table[min(tile * kTile + lane, last) >> shift];
-        vpage = table[min(tile * kTile + 16 * vq, last) >> shift];
+      auto load_page = [&](int tile) {
+        page = as_constant(table)[min(tile * kTile + 16 * own, last) >> shift];
       };
-      // In eight steps, to go between products.
+      auto load_scales = [&] {  // of `page`
+        page_of_raw = page;
+        const uint32_t at = page >= 0 && page < a.c.pages ? page : 0;
+        ksraw = as_constant(a.c.ks)[(unsigned long long)at * (uint32_t)a.c.heads + h];
+        vsraw = as_constant(a.c.vs)[(unsigned long long)at * (uint32_t)a.c.heads + h];
+      };
       auto load_codes = [&](int tile, int step) {
-        const int kin = (tile * kTile + lane) & (P - 1), vin = (tile * kTile + 16 * vq) & (P - 1);
-        const uint32_t kp = kpage >= 0 && kpage < a.c.pages ? kpage : 0;
-        const uint32_t vp = vpage >= 0 && vpage < a.c.pages ? vpage : 0;
+        const uint32_t in = (tile * kTile + 16 * own) & (P - 1);
+        const unsigned long long at =
+            (unsigned long long)(uint32_t)(page >= 0 && page < a.c.pages ? page : 0) * page_bytes + head_bytes;
         if (step == 0) {
           if constexpr (D == 128)
-            kraw = *reinterpret_cast<const uint4*>(kbase + kin * 16 + (unsigned long long)kp * page_bytes);
+            kraw = *reinterpret_cast<const uint4*>(a.c.k + (at + in * 16) + kat);
           else
-            kraw = *reinterpret_cast<const uint4*>((loads_k ? kbase + kin * 16 : vbase + vin) +
-                                                   (unsigned long long)(loads_k ? kp : vp) * page_bytes);
-        } else if (step == 1) {
-          if constexpr (D == 128)
-            vraw = *reinterpret_cast<const uint4*>(vbase + vin + (unsigned long long)vp * page_bytes);
-        } else {
-          spage = vpage;
-          sraw = sbase[(unsigned long long)vp * (uint32_t)a.c.heads];
+            kraw = *reinterpret_cast<const uint4*>((loads_k ? a.c.k + (at + in * 16) : a.c.v + (at + in)) +
+                                                   (loads_k ? kat : vat));
+        } else if (D == 128) {
+          vraw = *reinterpret_cast<const uint4*>(a.c.v + (at + in) + vat);
         }
       };
+      char* const kto = lds.k[0][2 * kc][16 * own + (lane & 15)];
+      char* const vto = lds.v[0] + 2 * own * M::kBlock + vd * 16;
+      float* const sto = wave < 4 && lane == 0 ? &lds.scales[0][0][own] : lds.none;
       auto store_codes = [&](int buf, int step) {
         const uint4 v = D == 128 ? vraw : kraw;
-        char* vat = lds.v[buf] + 2 * vq * M::kBlock + vd * 16;
+        char* k = kto + buf * (int)sizeof(lds.k[0]);
+        char* w = vto + buf * (int)sizeof(lds.v[0]);
         if (step == 0 && loads_k)
-          *reinterpret_cast<h8_t*>(lds.k[buf][2 * kc][lane]) = codes_to_f16(kraw.x, kraw.y);
+          *reinterpret_cast<h8_t*>(k) = codes_to_f16(kraw.x, kraw.y);
         else if (step == 1 && loads_k)
-          *reinterpret_cast<h8_t*>(lds.k[buf][2 * kc + 1][lane]) = codes_to_f16(kraw.z, kraw.w);
+          *reinterpret_cast<h8_t*>(k + kTile * 16) = codes_to_f16(kraw.z, kraw.w);
         else if (step == 2 && (D == 128 || !loads_k))
-          *reinterpret_cast<h8_t*>(vat) = codes_to_f16(v.x, v.z);
+          *reinterpret_cast<h8_t*>(w) = codes_to_f16(v.x, v.z);
         else if (step == 3 && (D == 128 || !loads_k))
-          *reinterpret_cast<h8_t*>(vat + M::kBlock) = codes_to_f16(v.y, v.w);
-        else if (step == 4)  // the scales of 16 tokens each, by lanes 0..3 of two waves
-          (&lds.scales[0][0][0])[wave < 2 && lane < 4 ? wave * 12 + buf * 4 + lane : 24] =
-              spage >= 0 && spage < a.c.pages ? sraw : -1.0f;
+          *reinterpret_cast<h8_t*>(w + M::kBlock) = codes_to_f16(v.y, v.w);
+        else if (step == 4) {
+          const bool there = page_of_raw >= 0 && page_of_raw < a.c.pages;
+          sto[buf * 4] = there ? ksraw : -1.0f;
+          sto[buf * 4 + 12] = there ? vsraw : -1.0f;
+        }
       };
-      // Step `step` of 9: tile's successor out of the registers into `buf`, the
-      // one after it into them, and that one's successor's pages.
+      // Steps to go between products: tile's successor out of the registers into
+      // `buf`, the one after it into them.
       auto move_codes = [&](int tile, int buf, int step) {
         if (step < 5) store_codes(buf, step);
-        else if (step < 8) load_codes(tile + 2, step - 5);
-        else if (step == 8) load_pages(tile + 3);
-      };
-      auto move_all = [&](int tile, int buf) {
-#pragma unroll
-        for (int i = 0; i < 9; ++i) move_codes(tile, buf, i);
+        else if (step < 7) load_codes(tile + 2, step - 5);
       };
 
       const bool keys = s.len > 0;  // a sequence without keys has no page to read
-      if (keys) load_pages(tile0);
+      if (keys) load_page(tile0);
       // The queries of this wave's rows.
       h8_t qf[kK];
       float qs;
@@ -1116,9 +1125,10 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
 #pragma unroll
         for (int k = 0; k < kK; ++k) raw[k] = *reinterpret_cast<const uint4*>(q + 16 * k);
         if (keys) {
-#pragma unroll
-          for (int i = 0; i < 3; ++i) load_codes(tile0, i);
-          load_pages(tile0 + 1);
+          load_codes(tile0, 0);
+          load_codes(tile0, 1);
+          load_scales();
+          load_page(tile0 + 1);
         }
         float amax = 0;
 #pragma unroll
@@ -1187,10 +1197,11 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
       };
 
       // P of a tile from its scores.
-      auto weights = [&](int tile, int buf) {
+      auto weights = [&](int tile, int buf, auto meanwhile) {
         const int key0 = tile * kTile;
         const f4_t cs = *reinterpret_cast<const f4_t*>(lds.scales[0][buf]);
         const f4_t vs = *reinterpret_cast<const f4_t*>(lds.scales[1][buf]);
+        meanwhile();
         float ck[4], rel[4];
         const float top = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
         const float bottom = fminf(fminf(cs[0], cs[1]), fminf(cs[2], cs[3]));  // -1: a page is missing
@@ -1277,18 +1288,27 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
         // and the next.
         int prev = 2, buf = 0, next = 1;
         lds_barrier();  // the buffers may be in use by the item before
-        move_all(tile0 - 1, 0);
+#pragma unroll
+        for (int i = 0; i < 7; ++i) move_codes(tile0 - 1, 0, i);
+        load_scales();
+        load_page(tile0 + 2);
         lds_barrier();
         // The workgroup's two halves, a wave of each on every SIMD, run half a
         // tile apart: while one multiplies, the other works out its weights.
-        // Both pass the same barriers.
+        // Both pass the same barriers. Who multiplies issues first: its few
+        // vector instructions would hold its products up (340 against 322 us).
         if (wave >= 4) lds_barrier();
         auto nothing = [](int) {};
         for (int tile = tile0; tile < tile1; ++tile) {
+          __builtin_amdgcn_s_setprio(1);
           if (tile > tile0) products(kYes, kNo, prev, buf, nothing);
           products(kNo, kYes, prev, buf, [&](int i) { move_codes(tile, next, i); });
+          __builtin_amdgcn_s_setprio(0);
           lds_barrier();
-          weights(tile, buf);
+          weights(tile, buf, [&] {
+            load_scales();  // of the tile that is in the registers next
+            load_page(tile + 3);
+          });
           lds_barrier();
           const int free = prev;
           prev = buf, buf = next, next = free;

@@ -135,8 +135,16 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Append: one wave quantises one run (a page's new tokens) of one head, keys
-// or values. A workgroup looks for runs that start among its `scan` tokens.
+// Append: bound by bytes for prompts, by latency for decode.
+//
+// A run is the step's tokens of one page; for one head, keys or values. Its
+// tokens fall into groups of 16 places of the page. A group's elements stay in
+// a wave's registers from the largest one's search to the codes' store, so
+// they are read once, and everything that a run needs is asked for at once
+// (elements, old scale, codes beside the new ones): two trips to memory after
+// the slots. A workgroup looks for runs that start among its `scan` tokens;
+// runs within one group go to its waves in turn, longer ones to all of them.
+// 8003 prompt tokens, 8 heads of 128, pages of 64: see the design's table.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
   KvView c;
@@ -154,7 +162,9 @@ constexpr int kAppendWaves = 4;
 struct Run {
   unsigned long long lo, hi;
   int t0, n, page, off;
-  __device__ __forceinline__ bool has(int i) const { return ((i < 64 ? lo : hi) >> (i & 63)) & 1; }
+  __device__ __forceinline__ bool has(int i) const {
+    return i >= 0 && i < n && (((i < 64 ? lo : hi) >> (i & 63)) & 1);
+  }
 };
 
 // Largest of non-negative floats as bits: NaN above infinity above the rest.
@@ -168,15 +178,15 @@ __device__ __forceinline__ uint32_t abs_bits(float f) {
   return __builtin_bit_cast(uint32_t, f) & 0x7FFFFFFFu;
 }
 
-__device__ __forceinline__ int quantise(float x, float inv) {
+__device__ __forceinline__ uint32_t quantise(float x, float inv) {
   // fminf/fmaxf drop a NaN, so a code is in range whatever comes in.
-  return (int)fminf(fmaxf(rintf(x * inv), -kCodeMax), kCodeMax);
+  return (uint32_t)(int)fminf(fmaxf(rintf(x * inv), -kCodeMax), kCodeMax) & 0xFFu;
 }
 
 __device__ __forceinline__ uint32_t requantise_word(uint32_t w, float ratio) {
   uint32_t r = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r |= ((uint32_t)quantise((float)code_of(w, i), ratio) & 0xFFu) << (8 * i);
+  for (int i = 0; i < 4; ++i) r |= quantise((float)code_of(w, i), ratio) << (8 * i);
   return r;
 }
 
@@ -198,122 +208,190 @@ __device__ __forceinline__ PageScale page_scale(float old, uint32_t amax) {
   return s;
 }
 
-template <int D, bool kBf16>
-__device__ void append_keys(const AppendArgs& a, const Run& run, int head, int lane) {
-  const int n = run.n, off = run.off;
-  constexpr int kC = D / 16;  // 16-element pieces a token
-  const int P = 1 << a.c.page_shift;
-  const uint16_t* x = a.k + (long long)run.t0 * a.kt + (long long)head * a.kh;
-  uint32_t amax = 0;
-  for (int u = lane; u < n * kC; u += 64) {
-    if (!run.has(u / kC)) continue;
-    const uint4* p = reinterpret_cast<const uint4*>(x + (long long)(u / kC) * a.kt + (u % kC) * 16);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint4 w = p[h];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t we = e == 0 ? w.x : e == 1 ? w.y : e == 2 ? w.z : w.w;
-        amax = max(amax, max(abs_bits(pair_lo<kBf16>(we)), abs_bits(pair_hi<kBf16>(we))));
-      }
-    }
-  }
-  amax = wave_max_bits(amax);
-  const long long ph = (long long)run.page * a.c.heads + head;
-  const float old = off == 0 ? 0.0f : a.c.ks[ph];
-  const PageScale s = page_scale(old, amax);
-  uint4* codes = reinterpret_cast<uint4*>(a.c.k + ph * D * P);
-  if (s.grew) {
-    for (int u = lane; u < off * kC; u += 64) {
-      uint4* c = codes + (u % kC) * P + u / kC;
-      uint4 w = *c;
-      w = make_uint4(requantise_word(w.x, s.ratio), requantise_word(w.y, s.ratio),
-                     requantise_word(w.z, s.ratio), requantise_word(w.w, s.ratio));
-      *c = w;
-    }
-    if (lane == 0) a.c.ks[ph] = s.scale;
-  } else if (off == 0 && lane == 0) {
-    a.c.ks[ph] = s.scale;
-  }
-  for (int u = lane; u < n * kC; u += 64) {
-    if (!run.has(u / kC)) continue;
-    const uint4* p = reinterpret_cast<const uint4*>(x + (long long)(u / kC) * a.kt + (u % kC) * 16);
-    uint32_t out[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint4 w = p[h];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t we = e == 0 ? w.x : e == 1 ? w.y : e == 2 ? w.z : w.w;
-        const uint32_t lo = (uint32_t)quantise(pair_lo<kBf16>(we), s.inv) & 0xFFu;
-        const uint32_t hi = (uint32_t)quantise(pair_hi<kBf16>(we), s.inv) & 0xFFu;
-        out[2 * h + e / 2] |= (lo | hi << 8) << (16 * (e & 1));
-      }
-    }
-    codes[(u % kC) * P + off + u / kC] = make_uint4(out[0], out[1], out[2], out[3]);
-  }
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pair_max_bits(uint32_t w) {
+  return max(abs_bits(pair_lo<kBf16>(w)), abs_bits(pair_hi<kBf16>(w)));
+}
+template <bool kBf16>
+__device__ __forceinline__ uint32_t quantise_pair(uint32_t w, float inv) {
+  return quantise(pair_lo<kBf16>(w), inv) | quantise(pair_hi<kBf16>(w), inv) << 8;
 }
 
-// Values: a lane has two elements of 16 consecutive tokens of the page, which
-// are two 16-byte pieces, so the transposition costs no shuffle.
+// A group's keys: a lane has 16 elements of a token, kUnits times.
 template <int D, bool kBf16>
-__device__ void append_values(const AppendArgs& a, const Run& run, int head, int lane) {
-  const int n = run.n, off = run.off;
-  constexpr int kPairs = D / 2;
-  constexpr int kSide = 64 / kPairs;  // groups of 16 tokens a wave does at once
-  const int P = 1 << a.c.page_shift;
-  const int d = 2 * (lane % kPairs);
-  const uint16_t* x = a.v + (long long)run.t0 * a.vt + (long long)head * a.vh + d;
-  const int g0 = off >> 4, g1 = (off + n + 15) >> 4;
-  uint32_t amax = 0;
-  for (int g = g0 + lane / kPairs; g < g1; g += kSide) {
+struct KeyGroup {
+  static constexpr int kC = D / 16, kUnits = kC / 4;
+  uint4 w[kUnits][2];
+
+  static __device__ __forceinline__ int place(int g, int u, int lane) { return 16 * g + (64 * u + lane) / kC; }
+
+  __device__ __forceinline__ void load(const AppendArgs& a, const Run& run, int head, int g, int lane) {
+    const uint16_t* x = a.k + (long long)run.t0 * a.kt + (long long)head * a.kh + lane % kC * 16;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int t = g * 16 + i - off;
-      if (t >= 0 && t < n && run.has(t)) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(x + (long long)t * a.vt);
-        amax = max(amax, max(abs_bits(pair_lo<kBf16>(w)), abs_bits(pair_hi<kBf16>(w))));
-      }
+    for (int u = 0; u < kUnits; ++u) {
+      const int t = place(g, u, lane) - run.off;
+      const bool on = run.has(t);
+      const uint4* p = reinterpret_cast<const uint4*>(x + (long long)(on ? t : 0) * a.kt);
+      w[u][0] = on ? p[0] : zero4();
+      w[u][1] = on ? p[1] : zero4();
     }
   }
-  amax = wave_max_bits(amax);
-  const long long ph = (long long)run.page * a.c.heads + head;
-  const float old = off == 0 ? 0.0f : a.c.vs[ph];
-  const PageScale s = page_scale(old, amax);
-  if (lane == 0 && (s.grew || off == 0)) a.c.vs[ph] = s.scale;
-  uint4* codes = reinterpret_cast<uint4*>(a.c.v + ph * D * P + (long long)d * P);
-  const int row = P / 16;  // pieces from one element to the next
-  for (int g = (s.grew ? 0 : g0) + lane / kPairs; g < g1; g += kSide) {
-    uint32_t w[2][4];
+  __device__ __forceinline__ uint32_t max_bits() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        m = max(max(m, max(pair_max_bits<kBf16>(w[u][h].x), pair_max_bits<kBf16>(w[u][h].y))),
+                max(pair_max_bits<kBf16>(w[u][h].z), pair_max_bits<kBf16>(w[u][h].w)));
+    return m;
+  }
+  __device__ __forceinline__ void store(const AppendArgs& a, const Run& run, long long ph, int g, int lane,
+                                        const PageScale& s) const {
+    const int P = 1 << a.c.page_shift;
+    uint4* codes = reinterpret_cast<uint4*>(a.c.k + ph * D * P) + lane % kC * P;
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int at = place(g, u, lane);
+      if (!run.has(at - run.off)) continue;
+      uint32_t q[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        q[2 * h] = quantise_pair<kBf16>(w[u][h].x, s.inv) | quantise_pair<kBf16>(w[u][h].y, s.inv) << 16;
+        q[2 * h + 1] = quantise_pair<kBf16>(w[u][h].z, s.inv) | quantise_pair<kBf16>(w[u][h].w, s.inv) << 16;
+      }
+      codes[at] = make_uint4(q[0], q[1], q[2], q[3]);
+    }
+  }
+  // The page's earlier tokens of a group, where the scale grew.
+  static __device__ __forceinline__ void requantise(const AppendArgs& a, const Run& run, long long ph, int g,
+                                                    int lane, const PageScale& s) {
+    const int P = 1 << a.c.page_shift;
+    uint4* codes = reinterpret_cast<uint4*>(a.c.k + ph * D * P) + lane % kC * P;
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int at = place(g, u, lane);
+      if (at >= run.off) continue;
+      const uint4 c = codes[at];
+      codes[at] = make_uint4(requantise_word(c.x, s.ratio), requantise_word(c.y, s.ratio),
+                             requantise_word(c.z, s.ratio), requantise_word(c.w, s.ratio));
+    }
+  }
+};
+
+// A group's values: a lane has two elements of kTok consecutive places, which
+// are two runs of bytes in the cache, so the transposition costs no shuffle.
+// `old` is what lies there, asked for where not every place is written.
+template <int D, bool kBf16>
+struct ValueGroup {
+  static constexpr int kTok = D / 8, kWords = kTok / 4;
+  typedef uint32_t words_t __attribute__((ext_vector_type(kWords)));
+  uint32_t w[kTok];
+  words_t old[2];
+
+  static __device__ __forceinline__ int place(int g, int lane) { return 16 * g + lane / (D / 2) * kTok; }
+  static __device__ __forceinline__ words_t* row(const AppendArgs& a, long long ph, int g, int lane, int r) {
+    const int P = 1 << a.c.page_shift;
+    return reinterpret_cast<words_t*>(a.c.v + ph * D * P + (long long)(lane % (D / 2) * 2 + r) * P + place(g, lane));
+  }
+  __device__ __forceinline__ void load(const AppendArgs& a, const Run& run, int head, int g, int lane) {
+    const uint16_t* x = a.v + (long long)run.t0 * a.vt + (long long)head * a.vh + lane % (D / 2) * 2;
+    bool all = true;
+#pragma unroll
+    for (int i = 0; i < kTok; ++i) {
+      const int t = place(g, lane) + i - run.off;
+      const bool on = run.has(t);
+      all &= on;
+      w[i] = on ? *reinterpret_cast<const uint32_t*>(x + (long long)t * a.vt) : 0u;
+    }
+    if (!all) {
+      const long long ph = (long long)run.page * a.c.heads + head;
+      old[0] = *row(a, ph, g, lane, 0);
+      old[1] = *row(a, ph, g, lane, 1);
+    }
+  }
+  __device__ __forceinline__ uint32_t max_bits() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kTok; ++i) m = max(m, pair_max_bits<kBf16>(w[i]));
+    return m;
+  }
+  __device__ __forceinline__ void store(const AppendArgs& a, const Run& run, long long ph, int g, int lane,
+                                        const PageScale& s) {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+      uint32_t c[2] = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = place(g, lane) + 4 * k + i - run.off;
+        const bool on = run.has(t);
+        const uint32_t q = quantise_pair<kBf16>(w[4 * k + i], s.inv);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          uint32_t y = q >> (8 * r) & 0xFFu;
+          if (!on) {
+            y = old[r][k] >> (8 * i) & 0xFFu;
+            if (t < 0 && s.grew) y = quantise((float)code_of(old[r][k], i), s.ratio);
+          }
+          c[r] |= y << (8 * i);
+        }
+      }
+      old[0][k] = c[0];
+      old[1][k] = c[1];
+    }
+    *row(a, ph, g, lane, 0) = old[0];
+    *row(a, ph, g, lane, 1) = old[1];
+  }
+  // A group of earlier tokens alone, where the scale grew.
+  static __device__ __forceinline__ void requantise(const AppendArgs& a, const Run& run, long long ph, int g,
+                                                    int lane, const PageScale& s) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const uint4 c = codes[r * row + g];
-      w[r][0] = c.x, w[r][1] = c.y, w[r][2] = c.z, w[r][3] = c.w;
+      words_t* at = row(a, ph, g, lane, r);
+      words_t c = *at;
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) c[k] = requantise_word(c[k], s.ratio);
+      *at = c;
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int t = g * 16 + i - off;
-      const int sh = 8 * (i & 3);
-      if (t < 0) {
-        if (s.grew) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            uint32_t& y = w[r][i >> 2];
-            const uint32_t q = (uint32_t)quantise((float)code_of(y, i & 3), s.ratio) & 0xFFu;
-            y = (y & ~(0xFFu << sh)) | q << sh;
-          }
-        }
-      } else if (t < n && run.has(t)) {
-        const uint32_t xx = *reinterpret_cast<const uint32_t*>(x + (long long)t * a.vt);
-        const uint32_t q0 = (uint32_t)quantise(pair_lo<kBf16>(xx), s.inv) & 0xFFu;
-        const uint32_t q1 = (uint32_t)quantise(pair_hi<kBf16>(xx), s.inv) & 0xFFu;
-        w[0][i >> 2] = (w[0][i >> 2] & ~(0xFFu << sh)) | q0 << sh;
-        w[1][i >> 2] = (w[1][i >> 2] & ~(0xFFu << sh)) | q1 << sh;
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) codes[r * row + g] = make_uint4(w[r][0], w[r][1], w[r][2], w[r][3]);
   }
+};
+
+// One run by `waves` waves, the workgroup's all or this one alone. With pages
+// of at most 128 places a wave of four has at most two groups of a run.
+template <typename Group, bool kKeys>
+__device__ void append_run(const AppendArgs& a, const Run& run, int head, int wave, int waves, int lane,
+                           uint32_t* shared_max) {
+  const long long ph = (long long)run.page * a.c.heads + head;
+  float* scales = kKeys ? a.c.ks : a.c.vs;
+  const int g0 = run.off >> 4, g1 = (run.off + run.n + 15) >> 4;
+  const float old = run.off == 0 ? 0.0f : scales[ph];
+  Group x[2];
+  uint32_t amax = 0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    if (g0 + wave + j * waves < g1) x[j].load(a, run, head, g0 + wave + j * waves, lane);
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    if (g0 + wave + j * waves < g1) amax = max(amax, x[j].max_bits());
+  amax = wave_max_bits(amax);
+  if (waves > 1) {
+    __syncthreads();  // the run before may still be read
+    if (lane == 0) shared_max[wave] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kAppendWaves; ++w) amax = max(amax, shared_max[w]);
+  }
+  const PageScale s = page_scale(old, amax);
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    if (g0 + wave + j * waves < g1) x[j].store(a, run, ph, g0 + wave + j * waves, lane, s);
+  if (s.grew) {
+    // Earlier tokens: all their groups, but for values the one that they share
+    // with new tokens, which is written whole above.
+    const int stop = kKeys ? (run.off + 15) >> 4 : g0;
+    for (int g = wave; g < stop; g += waves) Group::requantise(a, run, ph, g, lane, s);
+  }
+  if (wave == 0 && lane == 0 && (s.grew || run.off == 0)) scales[ph] = s.scale;
 }
 
 __device__ __forceinline__ bool in_cache(const AppendArgs& a, long long slot) {
@@ -333,6 +411,7 @@ __device__ __forceinline__ bool starts_run(const AppendArgs& a, int t, long long
 
 template <int D, bool kBf16>
 __global__ __launch_bounds__(kAppendWaves * 64) void append_kernel(AppendArgs a, int scan) {
+  __shared__ uint32_t shared_max[kAppendWaves];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int head = blockIdx.y;
@@ -343,9 +422,14 @@ __global__ __launch_bounds__(kAppendWaves * 64) void append_kernel(AppendArgs a,
     const long long slot = a.slots[base + lane];
     starts = in_cache(a, slot) && starts_run(a, base + lane, slot);
   }
-  unsigned long long mask = __ballot(starts);
-  for (int i = 0; mask; ++i, mask &= mask - 1) {
-    if (i % kAppendWaves != wave) continue;
+  auto append = [&](const Run& run, int w, int waves) {
+    if (blockIdx.z == 0)
+      append_run<KeyGroup<D, kBf16>, true>(a, run, head, w, waves, lane, shared_max);
+    else
+      append_run<ValueGroup<D, kBf16>, false>(a, run, head, w, waves, lane, shared_max);
+  };
+  int i = 0;
+  for (unsigned long long mask = __ballot(starts); mask; ++i, mask &= mask - 1) {
     Run run;
     run.t0 = base + __builtin_ctzll(mask);
     const long long slot = a.slots[run.t0];
@@ -365,15 +449,17 @@ __global__ __launch_bounds__(kAppendWaves * 64) void append_kernel(AppendArgs a,
       run.n += c;
       (w ? run.hi : run.lo) = __ballot(mine) & (c == 64 ? ~0ull : (1ull << c) - 1);
     }
-    if (blockIdx.z == 0)
-      append_keys<D, kBf16>(a, run, head, lane);
-    else
-      append_values<D, kBf16>(a, run, head, lane);
+    if ((run.off & 15) + run.n > 16) append(run, wave, kAppendWaves);
+    else if (i % kAppendWaves == wave) append(run, 0, 1);
   }
 }
 
 // ---------------------------------------------------------------------------
-// Read: 16 lanes a token and head, 8 elements a lane.
+// Read: bound by bytes, two thirds of them written. A lane has 8 elements of
+// four tokens, so that a wave writes rows of 128 and 256 bytes. Keys: 8 bytes
+// of each token. Values lie the other way round: four tokens' bytes of each
+// element in one word where the tokens follow each other in a page, turned
+// round in registers; else byte by byte.
 // ---------------------------------------------------------------------------
 struct ReadArgs {
   KvView c;
@@ -383,18 +469,28 @@ struct ReadArgs {
   int tokens;
 };
 
+typedef float read_f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t read_u4 __attribute__((ext_vector_type(4)));
+
+// Eight codes, two words, times a scale.
 template <int kDtype>
-__device__ __forceinline__ void store8(void* out, long long at, const float (&x)[8]) {
+__device__ __forceinline__ void store_codes(void* out, long long at, uint32_t lo, uint32_t hi, float s) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = (float)code_of(i < 4 ? lo : hi, i & 3) * s;
+    asm("" : "+v"(x[i]));  // in fp32, also where the product could go into fp16 in one instruction
+  }
   if constexpr (kDtype == DK_KV_F32) {
-    float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
-    o[0] = make_float4(x[0], x[1], x[2], x[3]);
-    o[1] = make_float4(x[4], x[5], x[6], x[7]);
+    read_f4* o = reinterpret_cast<read_f4*>(static_cast<float*>(out) + at);
+    __builtin_nontemporal_store(read_f4{x[0], x[1], x[2], x[3]}, o);
+    __builtin_nontemporal_store(read_f4{x[4], x[5], x[6], x[7]}, o + 1);
   } else {
-    uint32_t w[4];
+    read_u4 w;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       w[i] = to_half_bits<kDtype>(x[2 * i]) | (uint32_t)to_half_bits<kDtype>(x[2 * i + 1]) << 16;
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    __builtin_nontemporal_store(w, reinterpret_cast<read_u4*>(static_cast<uint16_t*>(out) + at));
   }
 }
 
@@ -403,33 +499,78 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
   constexpr int kLanes = D / 8;
   const int P = 1 << a.c.page_shift;
   const int head = blockIdx.y;
-  const int t = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const int t0 = (blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes) * 4;
   const int d = threadIdx.x % kLanes * 8;
-  if (t >= a.tokens) return;
-  const long long slot = a.slots[t];
-  const long long page = slot >> a.c.page_shift;
-  const int off = (int)(slot & (P - 1));
-  const bool ok = slot >= 0 && page < a.c.pages;
-  const long long ph = ok ? page * a.c.heads + head : 0;
-  const long long out = ((long long)t * a.c.heads + head) * D + d;
-  float x[8] = {};
-  if (blockIdx.z == 0) {
-    if (ok) {
-      const uint2 w = *reinterpret_cast<const uint2*>(a.c.k + ph * D * P + ((d / 16) * P + off) * 16 + d % 16);
-      const float s = a.c.ks[ph];
+  if (t0 >= a.tokens) return;
+  const int n = min(4, a.tokens - t0);
+  long long slot[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = (float)code_of(i < 4 ? w.x : w.y, i & 3) * s;
-    }
-    store8<kDtype>(a.k, out, x);
-  } else {
-    if (ok) {
-      const int8_t* c = a.c.v + ph * D * P + (long long)d * P + off;
-      const float s = a.c.vs[ph];
+  for (int i = 0; i < 4; ++i) slot[i] = a.slots[t0 + min(i, n - 1)];
+  bool ok[4];
+  long long ph[4];
+  float scale[4];
+  const float* scales = blockIdx.z == 0 ? a.c.ks : a.c.vs;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = (float)c[i * P] * s;
-    }
-    store8<kDtype>(a.v, out, x);
+  for (int i = 0; i < 4; ++i) {
+    const long long page = slot[i] >> a.c.page_shift;
+    ok[i] = slot[i] >= 0 && page < a.c.pages;
+    ph[i] = ok[i] ? page * a.c.heads + head : 0;
+    scale[i] = ok[i] ? scales[ph[i]] : 0.0f;
   }
+  uint32_t lo[4] = {}, hi[4] = {};
+  if (blockIdx.z == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (ok[i]) {
+        const int off = (int)(slot[i] & (P - 1));
+        const uint2 w = *reinterpret_cast<const uint2*>(a.c.k + ph[i] * D * P + ((d / 16) * P + off) * 16 + d % 16);
+        lo[i] = w.x, hi[i] = w.y;
+      }
+  } else {
+    const int off = (int)(slot[0] & (P - 1));
+    const bool follow = n == 4 && ok[0] && off + 3 < P && slot[1] == slot[0] + 1 &&
+                        slot[2] == slot[0] + 2 && slot[3] == slot[0] + 3;
+    if (follow) {
+      const int8_t* c = a.c.v + ph[0] * D * P + (long long)d * P + (off & ~3);
+      const int by = off & 3;
+      uint32_t w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = *reinterpret_cast<const uint32_t*>(c + e * P);
+      if (by)  // the four tokens lie in two words
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          w[e] = __builtin_amdgcn_alignbyte(*reinterpret_cast<const uint32_t*>(c + e * P + 4), w[e], by);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // four elements of four tokens, turned round
+        const uint32_t ab = __builtin_amdgcn_perm(w[4 * h + 1], w[4 * h], 0x05010400u);
+        const uint32_t cd = __builtin_amdgcn_perm(w[4 * h + 3], w[4 * h + 2], 0x05010400u);
+        const uint32_t ef = __builtin_amdgcn_perm(w[4 * h + 1], w[4 * h], 0x07030602u);
+        const uint32_t gh = __builtin_amdgcn_perm(w[4 * h + 3], w[4 * h + 2], 0x07030602u);
+        uint32_t* to = h ? hi : lo;
+        to[0] = __builtin_amdgcn_perm(cd, ab, 0x05040100u);
+        to[1] = __builtin_amdgcn_perm(cd, ab, 0x07060302u);
+        to[2] = __builtin_amdgcn_perm(gh, ef, 0x05040100u);
+        to[3] = __builtin_amdgcn_perm(gh, ef, 0x07060302u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (ok[i]) {
+          const uint8_t* c = reinterpret_cast<const uint8_t*>(a.c.v) + ph[i] * D * P + (long long)d * P +
+                             (slot[i] & (P - 1));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            lo[i] |= (uint32_t)c[e * P] << (8 * e);
+            hi[i] |= (uint32_t)c[(e + 4) * P] << (8 * e);
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < n)
+      store_codes<kDtype>(blockIdx.z == 0 ? a.k : a.v, ((long long)(t0 + i) * a.c.heads + head) * D + d,
+                          lo[i], hi[i], scale[i]);
 }
 
 }  // namespace dk
@@ -548,7 +689,7 @@ extern "C" int dk_kv_read(const dk_kv_cache* cache, const int64_t* slots, int nu
     return dk::set_error(DK_ERR_INVALID_ARGUMENT, "k and v must be 16-byte, slots 8-byte aligned");
   const dk::ReadArgs a{view, slots, k, v, num_tokens};
   auto launch = [&](auto kernel, int lanes) {
-    const int each = 256 / lanes;
+    const int each = 256 / lanes * 4;
     hipLaunchKernelGGL(kernel, dim3((unsigned)((num_tokens - 1) / each + 1), (unsigned)view.heads, 2),
                        dim3(256), 0, stream, a);
   };

@@ -94,8 +94,9 @@ int dk_kv_append(const dk_kv_cache* cache, const void* k, const void* v, int dty
                  long long v_head_stride, const int64_t* slots, int num_tokens,
                  hipStream_t stream);
 
-/* k and v [num_tokens, heads, head_size] = code * scale at slots, rounded once
- * to dtype (F16, BF16 or F32); zeros for a slot outside the cache. */
+/* k and v [num_tokens, heads, head_size] = code * scale at slots, in fp32 and
+ * from there rounded to dtype (F16, BF16 or F32); zeros for a slot outside the
+ * cache. */
 int dk_kv_read(const dk_kv_cache* cache, const int64_t* slots, int num_tokens, int dtype, void* k,
                void* v, hipStream_t stream);
 
