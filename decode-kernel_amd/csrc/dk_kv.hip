@@ -2,6 +2,8 @@
 // Layouts in dk_kv.hpp, contracts in include/decode_kernel/dk_kv.h.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "dk_host.hpp"
 #include "dk_kv.hpp"
 
@@ -320,10 +322,12 @@ struct ValueGroup {
                                         const PageScale& s) {
 #pragma unroll
     for (int k = 0; k < kWords; ++k) {
+      const int first = place(g, lane) + 4 * k - run.off;
+      if (!s.grew && (first + 4 <= 0 || first >= run.n)) continue;  // as it lies
       uint32_t c[2] = {0, 0};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int t = place(g, lane) + 4 * k + i - run.off;
+        const int t = first + i;
         const bool on = run.has(t);
         const uint32_t q = quantise_pair<kBf16>(w[4 * k + i], s.inv);
 #pragma unroll
@@ -357,22 +361,23 @@ struct ValueGroup {
 };
 
 // One run by `waves` waves, the workgroup's all or this one alone. With pages
-// of at most 128 places a wave of four has at most two groups of a run.
+// of at most 128 places a wave of four has at most two groups of a run, and a
+// wave alone runs within one.
 template <typename Group, bool kKeys>
-__device__ void append_run(const AppendArgs& a, const Run& run, int head, int wave, int waves, int lane,
-                           uint32_t* shared_max) {
+__device__ __forceinline__ void append_run(const AppendArgs& a, const Run& run, int head, int wave, int waves,
+                                           int lane, uint32_t* shared_max) {
   const long long ph = (long long)run.page * a.c.heads + head;
   float* scales = kKeys ? a.c.ks : a.c.vs;
-  const int g0 = run.off >> 4, g1 = (run.off + run.n + 15) >> 4;
+  const int g0 = (run.off >> 4) + wave, g1 = (run.off + run.n + 15) >> 4;
   const float old = run.off == 0 ? 0.0f : scales[ph];
   Group x[2];
   uint32_t amax = 0;
 #pragma unroll
   for (int j = 0; j < 2; ++j)
-    if (g0 + wave + j * waves < g1) x[j].load(a, run, head, g0 + wave + j * waves, lane);
+    if (g0 + j * waves < g1) x[j].load(a, run, head, g0 + j * waves, lane);
 #pragma unroll
   for (int j = 0; j < 2; ++j)
-    if (g0 + wave + j * waves < g1) amax = max(amax, x[j].max_bits());
+    if (g0 + j * waves < g1) amax = max(amax, x[j].max_bits());
   amax = wave_max_bits(amax);
   if (waves > 1) {
     __syncthreads();  // the run before may still be read
@@ -384,14 +389,65 @@ __device__ void append_run(const AppendArgs& a, const Run& run, int head, int wa
   const PageScale s = page_scale(old, amax);
 #pragma unroll
   for (int j = 0; j < 2; ++j)
-    if (g0 + wave + j * waves < g1) x[j].store(a, run, ph, g0 + wave + j * waves, lane, s);
+    if (g0 + j * waves < g1) x[j].store(a, run, ph, g0 + j * waves, lane, s);
   if (s.grew) {
     // Earlier tokens: all their groups, but for values the one that they share
     // with new tokens, which is written whole above.
-    const int stop = kKeys ? (run.off + 15) >> 4 : g0;
+    const int stop = kKeys ? (run.off + 15) >> 4 : run.off >> 4;
     for (int g = wave; g < stop; g += waves) Group::requantise(a, run, ph, g, lane, s);
   }
   if (wave == 0 && lane == 0 && (s.grew || run.off == 0)) scales[ph] = s.scale;
+}
+
+// One run by this wave alone, token by token, two elements a lane: little code
+// for runs of one or a few tokens, whose time is latency (a workgroup fetches
+// its instructions cold).
+template <int D, bool kBf16, bool kKeys>
+__device__ __forceinline__ void append_few(const AppendArgs& a, const Run& run, int head, int lane) {
+  constexpr int kSide = 128 / D;  // tokens at once
+  const int P = 1 << a.c.page_shift;
+  const int d = lane % (D / 2) * 2, side = lane / (D / 2);
+  const long long ph = (long long)run.page * a.c.heads + head;
+  float* scales = kKeys ? a.c.ks : a.c.vs;
+  int8_t* codes = (kKeys ? a.c.k : a.c.v) + ph * D * P;
+  const long long stride = kKeys ? a.kt : a.vt;
+  const uint16_t* x = (kKeys ? a.k + (long long)head * a.kh : a.v + (long long)head * a.vh) +
+                      (long long)run.t0 * stride + d;
+  const float old = run.off == 0 ? 0.0f : scales[ph];
+  auto load = [&](int t) {
+    return run.has(t) ? *reinterpret_cast<const uint32_t*>(x + (long long)t * stride) : 0u;
+  };
+  const uint32_t first = load(side);
+  uint32_t amax = pair_max_bits<kBf16>(first);
+#pragma unroll 4
+  for (int t = side + kSide; t < run.n; t += kSide) amax = max(amax, pair_max_bits<kBf16>(load(t)));
+  const PageScale s = page_scale(old, wave_max_bits(amax));
+  for (int t = side; t < run.n; t += kSide) {
+    if (!run.has(t)) continue;
+    const uint32_t q = quantise_pair<kBf16>(t == side ? first : load(t), s.inv);
+    const int at = run.off + t;
+    if (kKeys) {
+      *reinterpret_cast<uint16_t*>(codes + (d / 16 * P + at) * 16 + d % 16) = (uint16_t)q;
+    } else {
+      codes[d * P + at] = (int8_t)q;
+      codes[(d + 1) * P + at] = (int8_t)(q >> 8);
+    }
+  }
+  if (s.grew) {  // the page's earlier tokens, of which a word with new ones is done by bytes
+    const int words = kKeys ? run.off * (D / 4) : (run.off + 3) / 4 * D;
+    for (int u = lane; u < words; u += 64) {
+      const int tok = kKeys ? u / (D / 4) : u / D * 4;
+      uint32_t* w = reinterpret_cast<uint32_t*>(
+          kKeys ? codes + (u % (D / 4) / 4 * P + tok) * 16 + u % 4 * 4 : codes + u % D * P + tok);
+      if (kKeys || tok + 4 <= run.off) {
+        *w = requantise_word(*w, s.ratio);
+      } else {
+        int8_t* c = reinterpret_cast<int8_t*>(w);
+        for (int i = 0; tok + i < run.off; ++i) c[i] = (int8_t)quantise((float)c[i], s.ratio);
+      }
+    }
+  }
+  if (lane == 0 && (s.grew || run.off == 0)) scales[ph] = s.scale;
 }
 
 __device__ __forceinline__ bool in_cache(const AppendArgs& a, long long slot) {
@@ -409,7 +465,7 @@ __device__ __forceinline__ bool starts_run(const AppendArgs& a, int t, long long
   return true;
 }
 
-template <int D, bool kBf16>
+template <int D, bool kBf16, bool kFew>
 __global__ __launch_bounds__(kAppendWaves * 64) void append_kernel(AppendArgs a, int scan) {
   __shared__ uint32_t shared_max[kAppendWaves];
   const int lane = threadIdx.x & 63;
@@ -422,12 +478,6 @@ __global__ __launch_bounds__(kAppendWaves * 64) void append_kernel(AppendArgs a,
     const long long slot = a.slots[base + lane];
     starts = in_cache(a, slot) && starts_run(a, base + lane, slot);
   }
-  auto append = [&](const Run& run, int w, int waves) {
-    if (blockIdx.z == 0)
-      append_run<KeyGroup<D, kBf16>, true>(a, run, head, w, waves, lane, shared_max);
-    else
-      append_run<ValueGroup<D, kBf16>, false>(a, run, head, w, waves, lane, shared_max);
-  };
   int i = 0;
   for (unsigned long long mask = __ballot(starts); mask; ++i, mask &= mask - 1) {
     Run run;
@@ -449,8 +499,18 @@ __global__ __launch_bounds__(kAppendWaves * 64) void append_kernel(AppendArgs a,
       run.n += c;
       (w ? run.hi : run.lo) = __ballot(mine) & (c == 64 ? ~0ull : (1ull << c) - 1);
     }
-    if ((run.off & 15) + run.n > 16) append(run, wave, kAppendWaves);
-    else if (i % kAppendWaves == wave) append(run, 0, 1);
+    const bool all = !kFew && (run.off & 15) + run.n > 16;  // more than a group
+    if (!all && i % kAppendWaves != wave) continue;
+    if constexpr (kFew) {
+      if (blockIdx.z == 0) append_few<D, kBf16, true>(a, run, head, lane);
+      else append_few<D, kBf16, false>(a, run, head, lane);
+    } else {
+      const int w = all ? wave : 0, waves = all ? kAppendWaves : 1;
+      if (blockIdx.z == 0)
+        append_run<KeyGroup<D, kBf16>, true>(a, run, head, w, waves, lane, shared_max);
+      else
+        append_run<ValueGroup<D, kBf16>, false>(a, run, head, w, waves, lane, shared_max);
+    }
   }
 }
 
@@ -665,14 +725,21 @@ extern "C" int dk_kv_append(const dk_kv_cache* cache, const void* k, const void*
   const dk::AppendArgs a{view, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
                          k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots,
                          num_tokens};
-  const int scan = num_tokens <= 1024 ? 4 : 16;
+  // Few tokens are mostly runs of one, whose time is latency; many are mostly
+  // whole pages.
+  const bool few = num_tokens <= 256;
+  const int scan = few ? 4 : 16;
   const dim3 grid((unsigned)((num_tokens - 1) / scan + 1), (unsigned)view.heads, 2);
   const dim3 block(dk::kAppendWaves * 64);
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a, scan); };
-  if (cache->head_size == 64)
-    dtype == DK_KV_BF16 ? launch(dk::append_kernel<64, true>) : launch(dk::append_kernel<64, false>);
-  else
-    dtype == DK_KV_BF16 ? launch(dk::append_kernel<128, true>) : launch(dk::append_kernel<128, false>);
+  auto pick = [&](auto d, auto bf16) {
+    constexpr int kD = decltype(d)::value;
+    constexpr bool kBf16 = decltype(bf16)::value;
+    few ? launch(dk::append_kernel<kD, kBf16, true>) : launch(dk::append_kernel<kD, kBf16, false>);
+  };
+  auto by_type = [&](auto d) { dtype == DK_KV_BF16 ? pick(d, std::true_type{}) : pick(d, std::false_type{}); };
+  if (cache->head_size == 64) by_type(std::integral_constant<int, 64>{});
+  else by_type(std::integral_constant<int, 128>{});
   return dk::check_launch("append launch");
 }
 
