@@ -413,7 +413,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs& a, const Seq& s, 
     const float rel = cv / top;
 
     const bool whole = key0 + kTile <= q.least && __all(here);
-    h8_t pf[NT][2];
+    h8_t pf[NT][2], pl[NT][2];  // P in fp16 and what that leaves of it
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const float c = ck * q.scale[t];
@@ -447,7 +447,10 @@ __device__ __forceinline__ void attend_piece(const AttendArgs& a, const Seq& s, 
         for (int k = 0; k < 16; ++k) x[k] = k < left ? x[k] : 0.0f;
       }
 #pragma unroll
-      for (int k = 0; k < 16; ++k) pf[t][k >> 3][k & 7] = (_Float16)x[k];
+      for (int k = 0; k < 16; ++k) {
+        pf[t][k >> 3][k & 7] = (_Float16)x[k];
+        pl[t][k >> 3][k & 7] = (_Float16)(x[k] - (float)pf[t][k >> 3][k & 7]);
+      }
     }
 #pragma unroll
     for (int d = 0; d < kD; ++d) {
@@ -458,6 +461,8 @@ __device__ __forceinline__ void attend_piece(const AttendArgs& a, const Seq& s, 
         f4_t z = {0, 0, 0, 0};
         z = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[t][0], z, 0, 0, 0);
         z = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[t][1], z, 0, 0, 0);
+        z = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[t][0], z, 0, 0, 0);
+        z = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[t][1], z, 0, 0, 0);
 #pragma unroll
         for (int v = 0; v < 4; ++v) y.o[t][d][v] = fmaf(top, z[v], y.o[t][d][v]);
       }
