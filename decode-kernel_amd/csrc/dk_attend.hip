@@ -973,7 +973,10 @@ __device__ __forceinline__ const __attribute__((address_space(4))) T* as_constan
   return (const __attribute__((address_space(4))) T*)(uintptr_t)p;
 }
 
-template <int D>
+// kLow: P in two fp16 parts. For fp16 results, whose rounding is as coarse as
+// P's: their error against 64 bits was up to 1.6 times the rounding's, and is
+// the rounding's so. bf16 results do not show it.
+template <int D, bool kLow>
 __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
   using M = Many<D>;
   constexpr int kK = D / 16, kDt = D / 32;
@@ -1159,7 +1162,7 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
       // Sums, and what the fast way through a tile compares with: `bound` the
       // score that moves a row's maximum, `sub` what is taken off a score.
       f16_t o[kDt], st[2];
-      h8_t pf[4];
+      h8_t pf[4], pl[4];  // pl: what rounding to pf leaves
       float m = kNegInf, bound = kNegInf, sub = 0, l = 0;
       float unit = 0, per_unit = 0;
 #pragma unroll
@@ -1188,16 +1191,33 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) st[t][e] = 0;
         }
-#pragma unroll
-        for (int i = 0; i < kN; ++i) {
-          const h8_t x = ring[i % kAhead];
-          if (i < kV)
-            o[i % kDt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pf[i / kDt], o[i % kDt], 0, 0, 0);
-          else
-            st[(i - kV) % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qf[(i - kV) / 2], st[(i - kV) % 2], 0, 0, 0);
+        auto step = [&](int i) {  // the operand after the ring's in the place of product i's
           if (i + kAhead < kN) load(i + kAhead);
-          between(i);
-          __builtin_amdgcn_sched_barrier(0);  // the compiler puts loads right before their products
+          between(i - kV);
+          // The compiler puts loads right before their products.
+          __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (int q = 0; q < kV / kDt; ++q) {
+#pragma unroll
+          for (int d = 0; d < kDt; ++d) {
+            const h8_t x = ring[(q * kDt + d) % kAhead];
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pf[q], o[d], 0, 0, 0);
+            if constexpr (!kLow) step(q * kDt + d);
+          }
+          if constexpr (kLow)  // after the others, whose sums they wait for
+#pragma unroll
+            for (int d = 0; d < kDt; ++d) {
+              const h8_t x = ring[(q * kDt + d) % kAhead];
+              o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl[q], o[d], 0, 0, 0);
+              step(q * kDt + d);
+            }
+        }
+#pragma unroll
+        for (int i = kV; i < kN; ++i) {
+          const int k = i - kV;
+          st[k % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[i % kAhead], qf[k / 2], st[k % 2], 0, 0, 0);
+          step(i);
         }
       };
 
@@ -1275,14 +1295,19 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
           for (int e = 0; e < 8; ++e) {
             const float p = __builtin_amdgcn_exp2f(fmaf(st[q >> 1][8 * (q & 1) + e], ck[q], sub));
             l += p;
-            pf[q][e] = (_Float16)(p * rel[q]);
+            const float w = p * rel[q];
+            pf[q][e] = (_Float16)w;
+            if constexpr (kLow) pl[q][e] = (_Float16)fmaf((float)pf[q][e], -1.0f, w);
           }
         if (__builtin_expect(fix, 0)) {  // a key that is not seen has weight 0 on a page of any scale
           asm volatile("" : "+v"(left));
 #pragma unroll
           for (int q = 0; q < 4; ++q)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) pf[q][e] = seen(q, e) ? pf[q][e] : (_Float16)0.0f;
+            for (int e = 0; e < 8; ++e) {
+              pf[q][e] = seen(q, e) ? pf[q][e] : (_Float16)0.0f;
+              if constexpr (kLow) pl[q][e] = seen(q, e) ? pl[q][e] : (_Float16)0.0f;
+            }
         }
       };
 
@@ -1502,7 +1527,7 @@ extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
   const int group = q_heads / view.heads;
   // Work is counted in 31 bits: heads, row tiles and tiles of keys.
   const double most = (double)view.heads * ((double)num_tokens * group / 16 + requests) *
-                      (((double)table_width * cache->page_size) / dk::kTile + 2);
+                      (((double)table_width * cache->page_size) / dk::kTile + 8);
   if (most > 1 << 30)
     return dk::set_error(DK_ERR_UNSUPPORTED, "heads * queries * keys too large");
   if (((double)table_width * cache->page_size + num_tokens + dk::kTile) * group > 1 << 30)
@@ -1537,8 +1562,12 @@ extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
   };
   if (d.many) {
     a.few_rows = d.few ? 32 : 0;
-    if (cache->head_size == 64) launch(dk::attend_many<64>, dk::kManyThreads, dk::kManyRows);
-    else launch(dk::attend_many<128>, dk::kManyThreads, dk::kManyRows);
+    auto pick = [&](auto low) {
+      if (cache->head_size == 64) launch(dk::attend_many<64, decltype(low)::value>, dk::kManyThreads, dk::kManyRows);
+      else launch(dk::attend_many<128, decltype(low)::value>, dk::kManyThreads, dk::kManyRows);
+    };
+    if (a.bf16) pick(std::false_type{});
+    else pick(std::true_type{});
   }
   if (d.few) {
     a.few_rows = d.many ? 32 : INT32_MAX;
