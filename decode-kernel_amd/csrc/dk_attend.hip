@@ -58,7 +58,7 @@ __device__ __forceinline__ Seq sequence(const AttendArgs& a, int b, int rows_a_t
   s.q0 = b, s.n = 1;
   if (a.offsets) {
     s.q0 = min(max(a.offsets[b], 0), a.tokens);
-    s.n = max(min(a.offsets[b + 1], a.tokens) - s.q0, 0);
+    s.n = max(min(max(a.offsets[b + 1], 0), a.tokens) - s.q0, 0);
   }
   s.len = min((long long)max(a.lens[b], 0), (long long)a.width << a.c.page_shift);
   const int rows = s.n * a.group;

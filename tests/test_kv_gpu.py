@@ -168,6 +168,21 @@ def test_append(spans, page, heads, d, dtype):
         assert (off <= step * (0.5 + 1e-5)).all()
 
 
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("page,heads,d", [(16, 2, 64), (32, 1, 128), (64, 2, 128), (128, 1, 64), (128, 2, 128)])
+def test_append_many_tokens(page, heads, d, dtype):
+    # Past 256 tokens: long runs on all waves of a workgroup, runs of one token
+    # among them, tokens without a slot inside, at a start and at an end.
+    spans = [(0, 300), (5, 1), (page - 1, 1), (9, page + 30), (0, 1), (3, 2), (0, page), (14, 5), (1, 200)]
+    rng, pages, slots, x = _append_case(page + d, page, heads, d, spans)
+    assert len(slots) > 256
+    for lo, hi in ((7, 9), (297, 301), (350, 351), (len(slots) - 4, len(slots) - 1)):
+        slots[lo:hi] = -1
+    before = _random_cache(rng, pages, page, heads, d)
+    xt = [_dev(a, DTYPES[dtype]) for a in x]
+    _check_append(_cache(*before), before, [a.float().cpu().numpy() for a in xt], xt, slots)
+
+
 def test_append_scale_kept_and_grown():
     # One request's tokens one by one: scales only grow, and each stored value
     # is within half a step of the scale at its writing plus half a step for
@@ -409,6 +424,61 @@ def test_attend_prompt(new, group, page):
 
 def test_attend_long_sequence_with_short_ones():
     _attend_case(1, [20000, 3, 0, 64, 1], None, 2, 8, 128, 64, "fp16")
+
+
+@pytest.mark.parametrize("new", [None, [90, 3]])
+@pytest.mark.parametrize("scale", [-0.09, 0.0, 0.5])
+def test_attend_scale(new, scale):
+    # Any factor: a negative one turns the scores round, 0 takes the mean.
+    from decode_kernel import attend_kv
+
+    rng = np.random.default_rng(12)
+    lens, heads, group, d, page = [150, 700], 2, 3, 64, 32
+    tables, pages = _tables(rng, lens, page)
+    host = _random_cache(rng, pages, page, heads, d)
+    counts = new or [1, 1]
+    offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    q = _dev(rng.standard_normal((offsets[-1], heads * group, d)).astype(np.float16))
+    got = attend_kv(q, _cache(*host), _dev(tables), _dev(np.array(lens, np.int32)),
+                    None if new is None else _dev(offsets), max(counts), scale=scale)
+    ref, spread = kv_oracle.attend(q.float().cpu().numpy(), *host, tables, lens, offsets, scale, True)
+    _check(got, ref, spread, max(lens), 127 * host[3].max(), torch.float16)
+
+
+@pytest.mark.parametrize("new", [None, [100]])
+def test_attend_zero_pages(new):
+    # Pages whose scales are 0: their keys score 0, their values add nothing.
+    rng = np.random.default_rng(13)
+    lens, page = [230], 16
+    tables, pages = _tables(rng, lens, page)
+    host = _random_cache(rng, pages, page, 2, 128)
+    host[2][tables[0, 3]] = 0
+    host[3][tables[0, :9]] = 0
+    _attend_case(13, lens, new, 2, 2, 128, page, "fp16", host=host, tables=tables)
+    host[3][:] = 0
+    got, _ = _attend_case(13, lens, new, 2, 2, 128, page, "fp16", host=host, tables=tables)
+    assert not got.any()
+
+
+def test_attend_queries_that_belong_to_nobody():
+    # Offsets that leave queries out at the end, and ones that are no offsets:
+    # what is in range is right, nothing else is touched or read.
+    from decode_kernel import attend_kv
+
+    rng = np.random.default_rng(14)
+    lens = [100, 60]
+    tables, pages = _tables(rng, lens, 16)
+    host = _random_cache(rng, pages, 16, 1, 64)
+    q = _dev(rng.standard_normal((50, 2, 64)).astype(np.float16))
+    lens_d = _dev(np.array(lens, np.int32))
+    for offsets, n in (([0, 3, 40], 40), ([0, 1, 2], 2)):
+        got = attend_kv(q, _cache(*host), _dev(tables), lens_d, _dev(np.array(offsets, np.int32)), 37)
+        ref, spread = kv_oracle.attend(q.float().cpu().numpy(), *host, tables, lens, offsets, 0.125, True)
+        assert np.isnan(ref[n:]).all()
+        _check(got[:n], ref[:n], spread[:n], 100, 127 * host[3].max(), torch.float16)
+    wild = _dev(np.array([-5, 2**30, -(2**31)], np.int32))
+    attend_kv(q, _cache(*host), _dev(tables), _dev(np.array([-7, 2**31 - 1], np.int32)), wild, 50)
+    torch.cuda.synchronize()
 
 
 def test_attend_sharp_scores():
