@@ -1444,20 +1444,30 @@ namespace {
 
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-// Which kernels a call runs and what they need. Sequences of at most 32 rows
-// (queries times the group) are attend_few's, which takes 16 of them at a time
-// where no sequence has more, larger ones attend_many's; a call that by its
-// sizes can have one kind alone runs one kernel, which then takes every size.
+// Which kernels a call runs and what they need. Sequences of at most 128 rows
+// (queries times the group) are attend_few's, larger ones attend_many's. fp16,
+// head size 128, 8 heads, us of the two kernels at 64, 128 and 256 rows:
+//   64 sequences of 4000 keys   182 / 363   354 / 377   704 / 404
+//    8 sequences of 4000 keys    38 / 68     54 / 71     97 / 77
+//    1 sequence of 30000 keys    47 / 115    70 / 117   102 / 122
+//   64 sequences of 500 keys     32 / 59     61 / 66    114 / 79
+// A call that by its sizes can have one kind alone runs one kernel, which then
+// takes every size. attend_few takes 32 rows at a time where sequences have
+// more than 16 and there are 32 sequences and heads to share the card (64 x 8,
+// 4000 keys, 64 rows: 182 us against 205 for 16 at a time); with fewer, pieces
+// of 16 rows are joined sooner (1 x 8, 30000 keys, 32 rows: 33 against 65).
+constexpr int kFewRows = 128;
+
 struct Dispatch {
   bool few, many;
   int nt;
 };
-Dispatch dispatch(int num_tokens, int requests, int group, int max_query_len) {
+Dispatch dispatch(int num_tokens, int requests, int heads, int group, int max_query_len) {
   Dispatch d;
   const long long rows = (long long)std::min(max_query_len, num_tokens) * group;
-  d.many = rows > 32;
+  d.many = rows > kFewRows;
   d.few = !d.many || requests > 1;
-  d.nt = rows <= 16 ? 1 : 2;
+  d.nt = rows <= 16 || (long long)heads * requests < 32 ? 1 : 2;
   return d;
 }
 
@@ -1487,7 +1497,8 @@ extern "C" size_t dk_kv_attend_workspace_bytes(int num_tokens, int requests, int
   (void)table_width;
   (void)page_size;
   if (num_tokens <= 0 || requests <= 0 || heads <= 0 || q_heads <= 0 || head_size <= 0) return 0;
-  return workspace_bytes_of(dispatch(num_tokens, requests, q_heads / heads, max_query_len), head_size);
+  return workspace_bytes_of(dispatch(num_tokens, requests, heads, q_heads / heads, max_query_len),
+                            head_size);
 }
 
 extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
@@ -1532,7 +1543,7 @@ extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
     return dk::set_error(DK_ERR_UNSUPPORTED, "heads * queries * keys too large");
   if (((double)table_width * cache->page_size + num_tokens + dk::kTile) * group > 1 << 30)
     return dk::set_error(DK_ERR_UNSUPPORTED, "keys * q_heads / heads too large");
-  const Dispatch d = dispatch(num_tokens, requests, group, max_query_len);
+  const Dispatch d = dispatch(num_tokens, requests, view.heads, group, max_query_len);
   if (workspace_bytes < workspace_bytes_of(d, cache->head_size))
     return dk::set_error(DK_ERR_INVALID_ARGUMENT, "the workspace has %zu of %zu bytes",
                          workspace_bytes, workspace_bytes_of(d, cache->head_size));
@@ -1561,7 +1572,7 @@ extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
     ws += flags_bytes() + (size_t)dk::kWorkgroups * 2 * rows * (cache->head_size + 2) * sizeof(float);
   };
   if (d.many) {
-    a.few_rows = d.few ? 32 : 0;
+    a.few_rows = d.few ? kFewRows : 0;
     auto pick = [&](auto low) {
       if (cache->head_size == 64) launch(dk::attend_many<64, decltype(low)::value>, dk::kManyThreads, dk::kManyRows);
       else launch(dk::attend_many<128, decltype(low)::value>, dk::kManyThreads, dk::kManyRows);
@@ -1570,7 +1581,7 @@ extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
     else pick(std::true_type{});
   }
   if (d.few) {
-    a.few_rows = d.many ? 32 : INT32_MAX;
+    a.few_rows = d.many ? kFewRows : INT32_MAX;
     if (cache->head_size == 64) {
       if (d.nt == 1) launch(dk::attend_few<64, 1>, dk::Few<64, 1>::kThreads, 16);
       else launch(dk::attend_few<64, 2>, dk::Few<64, 2>::kThreads, 32);

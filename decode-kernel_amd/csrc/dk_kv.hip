@@ -2,8 +2,6 @@
 // Layouts in dk_kv.hpp, contracts in include/decode_kernel/dk_kv.h.
 #include <hip/hip_runtime.h>
 
-#include <type_traits>
-
 #include "dk_host.hpp"
 #include "dk_kv.hpp"
 
@@ -17,7 +15,8 @@ namespace dk {
 // a thread: the request by bisection, the page from the table or, for a page
 // that the step opens, from the free list at the rank that the scan gives. A
 // token at a page's first place writes the table's entry, so no token waits
-// for another. A few kilobytes: latency alone.
+// for another. A few kilobytes, so latency alone: 3.9 us for 256 requests with
+// a token each, 4.6 for 37 with 30011.
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 256;
 
@@ -145,8 +144,10 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
 // they are read once, and everything that a run needs is asked for at once
 // (elements, old scale, codes beside the new ones): two trips to memory after
 // the slots. A workgroup looks for runs that start among its `scan` tokens;
-// runs within one group go to its waves in turn, longer ones to all of them.
-// 8003 prompt tokens, 8 heads of 128, pages of 64: see the design's table.
+// runs of few tokens or within one group go to its waves in turn, longer ones
+// to all of them. 8003 prompt tokens, 8 heads of 128, pages of 64: 49.5 MB in
+// 22 us (2.2 TB/s); 10 us would be the rate of a large copy. One wave a run,
+// with the elements read twice, took 53.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
   KvView c;
@@ -399,9 +400,10 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, const Run& run, 
   if (wave == 0 && lane == 0 && (s.grew || run.off == 0)) scales[ph] = s.scale;
 }
 
-// One run by this wave alone, token by token, two elements a lane: little code
-// for runs of one or a few tokens, whose time is latency (a workgroup fetches
-// its instructions cold).
+// A run of few tokens by this wave alone, token by token, two elements a lane:
+// little code, since its time is latency and a workgroup fetches its
+// instructions cold (200 runs of one token and 8 heads: 7 us, on append_run 10).
+constexpr int kFewTokens = 8;
 template <int D, bool kBf16, bool kKeys>
 __device__ __forceinline__ void append_few(const AppendArgs& a, const Run& run, int head, int lane) {
   constexpr int kSide = 128 / D;  // tokens at once
@@ -465,7 +467,7 @@ __device__ __forceinline__ bool starts_run(const AppendArgs& a, int t, long long
   return true;
 }
 
-template <int D, bool kBf16, bool kFew>
+template <int D, bool kBf16>
 __global__ __launch_bounds__(kAppendWaves * 64) void append_kernel(AppendArgs a, int scan) {
   __shared__ uint32_t shared_max[kAppendWaves];
   const int lane = threadIdx.x & 63;
@@ -499,17 +501,16 @@ __global__ __launch_bounds__(kAppendWaves * 64) void append_kernel(AppendArgs a,
       run.n += c;
       (w ? run.hi : run.lo) = __ballot(mine) & (c == 64 ? ~0ull : (1ull << c) - 1);
     }
-    const bool all = !kFew && (run.off & 15) + run.n > 16;  // more than a group
+    const bool all = run.n > kFewTokens && (run.off & 15) + run.n > 16;  // more than a group
     if (!all && i % kAppendWaves != wave) continue;
-    if constexpr (kFew) {
+    const int w = all ? wave : 0, waves = all ? kAppendWaves : 1;
+    if (run.n <= kFewTokens) {
       if (blockIdx.z == 0) append_few<D, kBf16, true>(a, run, head, lane);
       else append_few<D, kBf16, false>(a, run, head, lane);
+    } else if (blockIdx.z == 0) {
+      append_run<KeyGroup<D, kBf16>, true>(a, run, head, w, waves, lane, shared_max);
     } else {
-      const int w = all ? wave : 0, waves = all ? kAppendWaves : 1;
-      if (blockIdx.z == 0)
-        append_run<KeyGroup<D, kBf16>, true>(a, run, head, w, waves, lane, shared_max);
-      else
-        append_run<ValueGroup<D, kBf16>, false>(a, run, head, w, waves, lane, shared_max);
+      append_run<ValueGroup<D, kBf16>, false>(a, run, head, w, waves, lane, shared_max);
     }
   }
 }
@@ -519,7 +520,9 @@ __global__ __launch_bounds__(kAppendWaves * 64) void append_kernel(AppendArgs a,
 // four tokens, so that a wave writes rows of 128 and 256 bytes. Keys: 8 bytes
 // of each token. Values lie the other way round: four tokens' bytes of each
 // element in one word where the tokens follow each other in a page, turned
-// round in registers; else byte by byte.
+// round in registers; else byte by byte. 65000 tokens of 8 heads of 128, 400 MB
+// in 93 us (4.3 TB/s; a large copy has 5.0), 5000 of 32 heads, 123 MB in 25.5
+// (4.8); single bytes of the values took 178 and 50.
 // ---------------------------------------------------------------------------
 struct ReadArgs {
   KvView c;
@@ -725,21 +728,17 @@ extern "C" int dk_kv_append(const dk_kv_cache* cache, const void* k, const void*
   const dk::AppendArgs a{view, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
                          k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots,
                          num_tokens};
-  // Few tokens are mostly runs of one, whose time is latency; many are mostly
-  // whole pages.
-  const bool few = num_tokens <= 256;
-  const int scan = few ? 4 : 16;
+  // A workgroup's runs of one token go round its four waves: no more than four
+  // where they may be most of the step; more where whole pages are, of which
+  // one workgroup in many finds the start.
+  const int scan = num_tokens <= 2048 ? 4 : 16;
   const dim3 grid((unsigned)((num_tokens - 1) / scan + 1), (unsigned)view.heads, 2);
   const dim3 block(dk::kAppendWaves * 64);
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a, scan); };
-  auto pick = [&](auto d, auto bf16) {
-    constexpr int kD = decltype(d)::value;
-    constexpr bool kBf16 = decltype(bf16)::value;
-    few ? launch(dk::append_kernel<kD, kBf16, true>) : launch(dk::append_kernel<kD, kBf16, false>);
-  };
-  auto by_type = [&](auto d) { dtype == DK_KV_BF16 ? pick(d, std::true_type{}) : pick(d, std::false_type{}); };
-  if (cache->head_size == 64) by_type(std::integral_constant<int, 64>{});
-  else by_type(std::integral_constant<int, 128>{});
+  if (cache->head_size == 64)
+    dtype == DK_KV_BF16 ? launch(dk::append_kernel<64, true>) : launch(dk::append_kernel<64, false>);
+  else
+    dtype == DK_KV_BF16 ? launch(dk::append_kernel<128, true>) : launch(dk::append_kernel<128, false>);
   return dk::check_launch("append launch");
 }
 
