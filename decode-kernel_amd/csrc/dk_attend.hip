@@ -5,13 +5,16 @@
 //   s_j = scale q.k_j,  o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),
 // in one pass with a running m (fp32, base 2). The rows of one key/value head
 // and sequence (the group's query heads times the sequence's queries) are
-// the columns of matrix products over a tile of 64 keys:
-//   S^T [64 keys, 16 rows] = K Q^T,   O^T [elements, 16 rows] += V^T P^T,
-// v_mfma_f32_16x16x32_f16 throughout. Codes are whole numbers up to 127,
-// exact in fp16; a page's scale multiplies S after, P before, the product.
-// Which key a product's row is, is free, so lane group g (16 lanes) takes the
-// keys 16 g .. 16 g + 15 of the tile in both products: S comes out in the
-// registers that P goes in, and a page's scales are one value a lane.
+// the columns of two matrix products over a tile of 64 keys,
+//   S^T [64 keys, rows] = K Q^T,   O^T [elements, rows] += V^T P^T,
+// on fp16 MFMAs with fp32 sums. Codes are whole numbers up to 127, exact in
+// fp16; a page's scale multiplies S after, P before, the product. Which key a
+// row of the first product is, is free: it is chosen so that S comes out in
+// the registers that P goes into the second product from. Scales are taken to
+// be at least 0 (or NaN), as append leaves them.
+//
+// attend_few reads the cache once and is bound by that; attend_many keeps the
+// matrix units busy for long query rows. Which one takes a sequence: dispatch.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -185,6 +188,19 @@ __device__ __forceinline__ uint16_t* out_row(const AttendArgs& a, const Seq& s, 
 // shares, at its start or its end, in LDS; the workgroup joins the pieces of
 // an item, and an item that several workgroups share goes through the
 // workspace, where the last one to arrive adds the pieces up in their order.
+//
+// v_mfma_f32_16x16x32_f16, 16 rows to a product: lane group g (16 lanes) takes
+// the keys 16 g .. 16 g + 15 of the tile in both products, and a page's scales
+// are one value a lane. P goes in as two fp16 parts, which costs nothing here.
+//
+// 131071 keys of 8 heads of 128 for one token (8 rows a head): 268 MB in 59 us,
+// 4.5 TB/s (a large read has 6.1). The tiles themselves run at 6.9 TB/s; 5 us
+// go by before them (lengths, page numbers, first codes: three trips to
+// memory) and 10 after (joining in LDS, flags, joining 32 workgroups' pieces).
+// 64 ragged sequences in pages of 16: 185 MB in 45 us. 700 keys of 32 heads:
+// 14 us, all of it such trips. Equal shares a workgroup instead of a wave, its
+// four waves on one item, took 50 us and more where short sequences stand
+// together, and a second launch to join 5 us more.
 // ---------------------------------------------------------------------------
 constexpr int kItemCost = 1;
 
@@ -876,10 +892,10 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
 // A workgroup of eight waves takes 256 rows of one sequence and key/value head
 // over the tiles of keys, 32 rows a wave, v_mfma_f32_32x32x16_f16. It turns a
 // tile's codes into fp16 in LDS once for all its rows (a thread 16 bytes of
-// keys and of values), two tiles ahead of the products. Rows of a product's right operand
-// are a wave's lanes, so a row's maximum and sum need one exchange of the
-// wave's halves, and P goes from the first product's registers into the
-// second's. Values lie in LDS in the order in which lanes hold P's tokens.
+// keys and of values), a tile ahead of the products. Rows of a product's right
+// operand are a wave's lanes, so a row's maximum and sum need one exchange of
+// the wave's halves. Values lie in LDS in the order in which lanes hold P's
+// tokens.
 //
 // A page's value scale goes into P relative to a power of two, `unit`, that
 // follows the scales within 2^6: P keeps fp16's bits whatever the values' size
@@ -888,10 +904,19 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
 // The work is (sequence, head, row tile, tile of keys), with the tiles past a
 // row tile's last visible key left out; the workgroups take equal shares, and
 // pieces of an item that two or more share meet as those of attend_few do.
+//
+// A prompt of 4096 tokens, 64 query and 8 key/value heads, fp16: 275 GFLOP in
+// 415 us, 660 TFLOP/s, with the products for P's second part on top; 501 tokens
+// on each of three long contexts, bf16: 281 GFLOP in 306 us, 918 TFLOP/s (a
+// large library product has 1200). Per tile the vector instructions of two
+// waves (scores to weights 230, codes 50 each) take about as long as their
+// products, at half of the matrix slots and a clock that falls to 1.7 GHz.
+// Operand loads next to their products, in the compiler's order, cost a
+// quarter; without the halves' shift 383 us instead of 328 for the second.
 // ---------------------------------------------------------------------------
 constexpr int kManyRows = 256;
 constexpr int kManyThreads = 512;
-constexpr int kManyItemCost = 6;
+constexpr int kManyItemCost = 6;  // an item's start and end against a tile, measured
 
 typedef float f16_t __attribute__((ext_vector_type(16)));
 
