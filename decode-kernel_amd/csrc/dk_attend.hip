@@ -183,8 +183,9 @@ __device__ __forceinline__ uint16_t* out_row(const AttendArgs& a, const Seq& s, 
 // The work is (sequence, key/value head, row tile, tile of keys), in that
 // order. Every wave of the card's 256 workgroups takes an equal share of it,
 // whatever the sequences' lengths are; an item (one row tile with all its
-// keys) costs kItemCost tiles on top, for the latency of its start. A wave
-// writes what it has of a whole item, and leaves the piece of an item it
+// keys) costs kItemCost tiles on top, for the latency of its start. Where
+// items are few and short, a workgroup's share is one item (kAloneTiles). A
+// wave writes what it has of a whole item, and leaves the piece of an item it
 // shares, at its start or its end, in LDS; the workgroup joins the pieces of
 // an item, and an item that several workgroups share goes through the
 // workspace, where the last one to arrive adds the pieces up in their order.
@@ -198,11 +199,22 @@ __device__ __forceinline__ uint16_t* out_row(const AttendArgs& a, const Seq& s, 
 // go by before them (lengths, page numbers, first codes: three trips to
 // memory) and 10 after (joining in LDS, flags, joining 32 workgroups' pieces).
 // 64 ragged sequences in pages of 16: 185 MB in 45 us. 700 keys of 32 heads:
-// 14 us, all of it such trips. Equal shares a workgroup instead of a wave, its
+// 13 us, all of it such trips. Equal shares a workgroup instead of a wave, its
 // four waves on one item, took 50 us and more where short sequences stand
 // together, and a second launch to join 5 us more.
 // ---------------------------------------------------------------------------
 constexpr int kItemCost = 1;
+
+// With no more items than workgroups, each goes to one of its own where that
+// makes a wave's share longer by no more than this many tiles (of a workgroup
+// of eight waves; twice as many of four): a tile costs 2.5 us where a wave has
+// few, meeting through the workspace 4 to 7. us, shared / alone, fp16, heads of
+// 128, pages of 64, at 200, 500, 700, 1500 and 3000 keys:
+//    1 sequence, 32 heads                14.9/9.0  14.9/10.8  14.5/13.2  15/19  13/24
+//   16 sequences, 8 x 8 heads            15.7/9.2  15.3/11.1  15.2/13.7  20/-   23/-
+//   32 sequences, 8 x 8 heads            15.8/9.3  19.5/11.7  19.2/15.5  28/22  34/35
+//    8 sequences, 8 x 8, four queries    23.9/16   24.8/19    19.4/20    28/30  26/-
+constexpr int kAloneTiles = 1;
 
 template <int D, int NT>
 struct Few {
@@ -650,6 +662,17 @@ __device__ __forceinline__ void join_pieces(const AttendArgs& a, typename Few<D,
   }
 }
 
+// Of whole numbers >= 0, in lane 63.
+__device__ __forceinline__ int wave_max(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
+  return v;
+}
+
 // Inclusive sums over the wave.
 __device__ __forceinline__ int wave_scan(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
@@ -696,19 +719,33 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
   // Every wave adds up all sequences' work to find its own, by itself: the
   // lanes take `each` sequences in a row, then those of the block that the
   // share starts in one by one. The host has seen to it that the sum fits.
-  auto cost = [&](const Seq& s) { return a.c.heads * s.row_tiles * (s.tiles + kItemCost); };
+  int each_units = 0;  // of every item, if they are one workgroup's each
+  auto units_of = [&](const Seq& s) { return each_units ? each_units : s.tiles + kItemCost; };
+  auto cost = [&](const Seq& s) { return a.c.heads * s.row_tiles * units_of(s); };
   const int each = (a.requests + 63) / 64;
   int b = lane * each;
   Seq s{};
-  int work = 0;
+  int work = 0, items = 0, longest = 0;
   for (int k = 0; k < each && b + k < a.requests; ++k) {
     s = sequence(a, b + k, kRows, false);
     work += cost(s);
+    items += a.c.heads * s.row_tiles;
+    longest = max(longest, s.row_tiles ? s.tiles : 0);
   }
   int upto = wave_scan(work);
-  const int total = __builtin_amdgcn_readlane(upto, 63);
-  // A wave's share, and the workgroup's.
-  const int share = max((int)(((unsigned)total + kWorkgroups * kWaves - 1) / (kWorkgroups * kWaves)), 1);
+  int total = __builtin_amdgcn_readlane(upto, 63);
+  // A wave's share, and below the workgroup's.
+  int share = max((int)(((unsigned)total + kWorkgroups * kWaves - 1) / (kWorkgroups * kWaves)), 1);
+  const int items_upto = wave_scan(items), most_items = __builtin_amdgcn_readlane(items_upto, 63);
+  longest = __builtin_amdgcn_readlane(wave_max(longest), 63);
+  const int alone = (longest + kItemCost + kWaves - 1) / kWaves;  // a wave's share of the longest item
+  if (most_items <= kWorkgroups && alone <= share + kAloneTiles * 8 / kWaves) {
+    share = alone;
+    each_units = share * kWaves;
+    work = items * each_units;
+    upto = items_upto * each_units;
+    total = most_items * each_units;
+  }
   const int group_share = share * kWaves;
   if (wg >= (total + group_share - 1) / group_share) return;
   const int begin = wg * group_share + wave * share, end = min(begin + share, total);
@@ -739,12 +776,12 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
         s = sequence(a, ++b, kRows, false);
         continue;
       }
-      const int units = s.tiles + kItemCost;
+      const int units = units_of(s);
       const int item = (unsigned)(cur - base) / (unsigned)units, at = cur - base - item * units;
       const int stop = min(units, at + (end - cur));
       cur += stop - at;
-      const int tile0 = max(at - kItemCost, 0), tile1 = stop - kItemCost;
-      if (tile0 >= tile1) continue;  // the item's start alone
+      const int tile0 = max(at - kItemCost, 0), tile1 = min(stop - kItemCost, s.tiles);
+      if (tile0 >= tile1) continue;  // the item's start alone, or past its end
       const int h = (unsigned)item / (unsigned)s.row_tiles, rt = item - h * s.row_tiles;
       Sums<D, NT> y;
       attend_piece<D, NT>(a, s, b, h, rt, tile0, tile1, lane, y);

@@ -426,6 +426,26 @@ def test_attend_long_sequence_with_short_ones():
     _attend_case(1, [20000, 3, 0, 64, 1], None, 2, 8, 128, 64, "fp16")
 
 
+@pytest.mark.parametrize("b,heads", [(1, 1), (63, 1), (65, 2), (64, 4), (200, 1), (255, 1), (256, 1), (257, 1), (129, 2)])
+@pytest.mark.parametrize("longest", [1, 63, 448, 449, 960, 961])
+def test_attend_items_of_one_workgroup(b, heads, longest):
+    # To 256 items of a few tiles each (448, 960 keys: the last that make two
+    # shares' worth for eight waves), and just past that; idle ones among them.
+    rng = np.random.default_rng(b)
+    lens = [int(x) for x in rng.integers(0, longest + 1, b)]
+    lens[b // 3] = longest
+    _attend_case(b, lens, [int(x) for x in rng.integers(0, 3, b)], heads, 2, 64 if b % 2 else 128, 32, "fp16")
+
+
+@pytest.mark.parametrize("group", [1, 3, 8])
+@pytest.mark.parametrize("d,page,dtype", [(128, 16, "bf16"), (64, 64, "fp16"), (128, 128, "fp16"), (64, 32, "bf16")])
+def test_attend_several_queries_beside_a_long_sequence(d, page, dtype, group):
+    # The long one has the shares cut across the short ones' items.
+    lens = [300, 40, 3001, 64, 0, 5, 130, 333, 1, 65]
+    new = [1, 16, 1, 7, 2, 9, 0, 15, 1, 12]
+    _attend_case(group, lens, new, 2, group, d, page, dtype)
+
+
 @pytest.mark.parametrize("new", [None, [90, 3]])
 @pytest.mark.parametrize("scale", [-0.09, 0.0, 0.5])
 def test_attend_scale(new, scale):
