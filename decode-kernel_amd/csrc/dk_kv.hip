@@ -728,10 +728,18 @@ extern "C" int dk_kv_append(const dk_kv_cache* cache, const void* k, const void*
   const dk::AppendArgs a{view, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
                          k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots,
                          num_tokens};
-  // A workgroup's runs of one token go round its four waves: no more than four
-  // where they may be most of the step; more where whole pages are, of which
-  // one workgroup in many finds the start.
-  const int scan = num_tokens <= 2048 ? 4 : 16;
+  // Tokens that a workgroup looks for runs among: about 12 workgroups a CU. Runs
+  // of one token go round its four waves, and one of four waves finds few of
+  // them; of whole pages one workgroup in many finds the start, and the others
+  // cost their launch. 8 heads of 128, us by 4 / 16 / 32 tokens:
+  //   2 prompts, 2000 tokens   19 / 10 / 12    300 sequences, a token each   11 / 16 / 23
+  //   4 prompts, 4000 tokens   44 / 17 / 15    600 sequences, a token each   17 / 19 / 28
+  //   2 prompts, 60000 tokens  - / 229 / 125; 64 tokens take 115, but 30 instead
+  //   of 22 for 2000 tokens of 32 heads, where each has a run or two: only far on
+  const long long rows = (long long)num_tokens * view.heads;
+  int scan = 4;
+  while (scan < 32 && rows > 1536LL * scan) scan *= 2;
+  if (rows > 1 << 18) scan = 64;
   const dim3 grid((unsigned)((num_tokens - 1) / scan + 1), (unsigned)view.heads, 2);
   const dim3 block(dk::kAppendWaves * 64);
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a, scan); };
