@@ -84,6 +84,16 @@ __device__ __forceinline__ h8_t codes_to_f16(uint32_t lo, uint32_t hi) {
   return r;
 }
 
+// Two weights as their first fp16 parts. The second part is what these very
+// bits leave: without the asm the compiler rounds a product to fp16 twice, from
+// fp32 for the first part and exactly where that is taken off again, which
+// differ on ties: one weight in some ten thousand was half a step of fp16 off.
+__device__ __forceinline__ h2_t first_parts(float x, float y) {
+  uint32_t w = __builtin_bit_cast(uint32_t, h2_t{(_Float16)x, (_Float16)y});
+  asm("" : "+v"(w));
+  return as_h2(w);
+}
+
 // Eight elements of a query as fp32.
 __device__ __forceinline__ void q_floats(const uint4& w, int bf16, float (&x)[8]) {
   const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
@@ -475,9 +485,13 @@ __device__ __forceinline__ void attend_piece(const AttendArgs& a, const Seq& s, 
         for (int k = 0; k < 16; ++k) x[k] = k < left ? x[k] : 0.0f;
       }
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        pf[t][k >> 3][k & 7] = (_Float16)x[k];
-        pl[t][k >> 3][k & 7] = (_Float16)(x[k] - (float)pf[t][k >> 3][k & 7]);
+      for (int k = 0; k < 16; k += 2) {
+        const h2_t f = first_parts(x[k], x[k + 1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          pf[t][k >> 3][(k & 7) + i] = f[i];
+          pl[t][k >> 3][(k & 7) + i] = (_Float16)(x[k + i] - (float)f[i]);
+        }
       }
     }
 #pragma unroll
@@ -1354,12 +1368,20 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(st[q >> 1][8 * (q & 1) + e], ck[q], sub));
-            l += p;
-            const float w = p * rel[q];
-            pf[q][e] = (_Float16)w;
-            if constexpr (kLow) pl[q][e] = (_Float16)fmaf((float)pf[q][e], -1.0f, w);
+          for (int e = 0; e < 8; e += 2) {
+            float w[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float p = __builtin_amdgcn_exp2f(fmaf(st[q >> 1][8 * (q & 1) + e + i], ck[q], sub));
+              l += p;
+              w[i] = p * rel[q];
+            }
+            const h2_t f = first_parts(w[0], w[1]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              pf[q][e + i] = f[i];
+              if constexpr (kLow) pl[q][e + i] = (_Float16)fmaf((float)f[i], -1.0f, w[i]);
+            }
           }
         if (__builtin_expect(fix, 0)) {  // a key that is not seen has weight 0 on a page of any scale
           asm volatile("" : "+v"(left));

@@ -1,0 +1,69 @@
+"""What attention over the paged cache rounds, held against 64 bits closer
+than tests/test_kv_gpu.py does. The bound, per output, with a = sum p |v| / sum p:
+
+    half a step of the output's type + 2^-14 a + keys floor 127 top
+
+* the rounding of the result;
+* the fp32 of scores, weights and sums. A score's terms add up to about 10 in
+  base 2 here, each rounded at 2^-24 of that a few times, and up to 2000 tiles
+  of keys are added up, each rounded at 2^-24 of the sum: under 2^-14 in all.
+  A weight goes into the second product as two fp16 parts, 2^-22 of it off;
+* where those two parts end: a weight under `floor` of its row's largest is
+  lost, times a value of the largest scale of its tile of 64 keys, `top`.
+  2^-36 with few rows, 2^-30 with many (where one unit holds for tiles whose
+  scales are within 2^6 of each other).
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv_oracle
+from test_kv_gpu import DTYPES, _cache, _dev, _half_step, _random_cache, _tables
+
+pytestmark = pytest.mark.gpu
+
+FEW, MANY = 2.0**-36, 2.0**-30
+
+
+def _attend(q, host, tables, lens, new, dtype, floor, scale=None, top=None, causal=True, batch=1, heads=1):
+    """Runs attend_kv on one batch and holds it against the bound; `top` is
+    the largest value scale of tiles that have a say (default: of all). The
+    sequences stand `batch` times in the call, and the heads `heads` times in
+    the cache, so that each goes through one share of the work in one piece."""
+    from decode_kernel import attend_kv
+
+    offsets = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    many = np.concatenate([[0], np.cumsum(new * batch)]).astype(np.int32)
+    q = _dev(q.astype(np.float32), DTYPES[dtype])
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    cache = _cache(*(np.tile(a, (1,) * (a.ndim - 1 - (a.ndim > 2)) + (heads,) + (1,) * (a.ndim > 2)) for a in host))
+    got = attend_kv(q.repeat(batch, heads, 1), cache, _dev(np.tile(tables, (batch, 1))),
+                    torch.tensor(lens * batch, dtype=torch.int32, device="cuda"), _dev(many), max(new), scale=scale, causal=causal)
+    ref, spread = kv_oracle.attend(q.double().cpu().numpy(), *host, tables, lens, offsets, scale, causal)
+    top = host[3].max() if top is None else top
+    got = got.double().view(batch, q.shape[0], heads, q.shape[1], -1).cpu().numpy()
+    ref, spread = ref[None, :, None], spread[None, :, None]
+    bound = _half_step(ref, DTYPES[dtype]) + 2.0**-14 * spread + max(lens) * floor * 127 * top
+    assert np.isfinite(got).all()
+    err = np.abs(got - ref)
+    off = err > bound
+    assert not off.any(), f"{off.sum()} of {off.size} outputs off, worst {(err / bound).max():.2f} bounds, " \
+                          f"first {np.argwhere(off)[:3].tolist()}"
+    return got, ref
+
+
+@pytest.mark.parametrize("dtype", ["fp16"])
+@pytest.mark.parametrize("d,page,group", [(128, 16, 8), (64, 64, 3), (128, 128, 1)])
+@pytest.mark.parametrize("new,floor", [([1, 1], FEW), ([9, 4], FEW), ([300, 129], MANY), ([200, 500], MANY)])
+def test_results_are_as_exact_as_their_rounding(new, floor, d, page, group, dtype):
+    # Prompts from their first token on: rows of two and three keys show a
+    # weight's rounding whole.
+    rng = np.random.default_rng(d + page)
+    new = [n * 8 // group if floor == MANY else n for n in new]
+    lens = list(new) if floor == MANY else [70, 700]
+    tables, pages = _tables(rng, lens, page)
+    host = _random_cache(rng, pages, page, 2, d)
+    _attend(rng.standard_normal((sum(new), 2 * group, d)), host, tables, lens, new, dtype, floor)
