@@ -1049,10 +1049,10 @@ __device__ __forceinline__ const __attribute__((address_space(4))) T* as_constan
   return (const __attribute__((address_space(4))) T*)(uintptr_t)p;
 }
 
-// kLow: P in two fp16 parts. For fp16 results, whose rounding is as coarse as
-// P's: their error against 64 bits was up to 1.6 times the rounding's, and is
-// the rounding's so. bf16 results do not show it.
-template <int D, bool kLow>
+// P goes in as two fp16 parts here too, which doubles the second product. With
+// one, results were up to 4.4 (bf16) and 1.6 (fp16) times their own rounding
+// away from 64 bits where few keys carry a row; with two they are not.
+template <int D>
 __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
   using M = Many<D>;
   constexpr int kK = D / 16, kDt = D / 32;
@@ -1279,15 +1279,13 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
           for (int d = 0; d < kDt; ++d) {
             const h8_t x = ring[(q * kDt + d) % kAhead];
             o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pf[q], o[d], 0, 0, 0);
-            if constexpr (!kLow) step(q * kDt + d);
           }
-          if constexpr (kLow)  // after the others, whose sums they wait for
 #pragma unroll
-            for (int d = 0; d < kDt; ++d) {
-              const h8_t x = ring[(q * kDt + d) % kAhead];
-              o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl[q], o[d], 0, 0, 0);
-              step(q * kDt + d);
-            }
+          for (int d = 0; d < kDt; ++d) {  // after the others, whose sums they wait for
+            const h8_t x = ring[(q * kDt + d) % kAhead];
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl[q], o[d], 0, 0, 0);
+            step(q * kDt + d);
+          }
         }
 #pragma unroll
         for (int i = kV; i < kN; ++i) {
@@ -1380,7 +1378,7 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               pf[q][e + i] = f[i];
-              if constexpr (kLow) pl[q][e + i] = (_Float16)fmaf((float)f[i], -1.0f, w[i]);
+              pl[q][e + i] = (_Float16)fmaf((float)f[i], -1.0f, w[i]);
             }
           }
         if (__builtin_expect(fix, 0)) {  // a key that is not seen has weight 0 on a page of any scale
@@ -1390,7 +1388,7 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               pf[q][e] = seen(q, e) ? pf[q][e] : (_Float16)0.0f;
-              if constexpr (kLow) pl[q][e] = seen(q, e) ? pl[q][e] : (_Float16)0.0f;
+              pl[q][e] = seen(q, e) ? pl[q][e] : (_Float16)0.0f;
             }
         }
       };
@@ -1657,12 +1655,8 @@ extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
   };
   if (d.many) {
     a.few_rows = d.few ? kFewRows : 0;
-    auto pick = [&](auto low) {
-      if (cache->head_size == 64) launch(dk::attend_many<64, decltype(low)::value>, dk::kManyThreads, dk::kManyRows);
-      else launch(dk::attend_many<128, decltype(low)::value>, dk::kManyThreads, dk::kManyRows);
-    };
-    if (a.bf16) pick(std::false_type{});
-    else pick(std::true_type{});
+    if (cache->head_size == 64) launch(dk::attend_many<64>, dk::kManyThreads, dk::kManyRows);
+    else launch(dk::attend_many<128>, dk::kManyThreads, dk::kManyRows);
   }
   if (d.few) {
     a.few_rows = d.many ? kFewRows : INT32_MAX;

@@ -55,7 +55,7 @@ def _attend(q, host, tables, lens, new, dtype, floor, scale=None, top=None, caus
     return got, ref
 
 
-@pytest.mark.parametrize("dtype", ["fp16"])
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
 @pytest.mark.parametrize("d,page,group", [(128, 16, 8), (64, 64, 3), (128, 128, 1)])
 @pytest.mark.parametrize("new,floor", [([1, 1], FEW), ([9, 4], FEW), ([300, 129], MANY), ([200, 500], MANY)])
 def test_results_are_as_exact_as_their_rounding(new, floor, d, page, group, dtype):
