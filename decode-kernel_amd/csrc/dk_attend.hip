@@ -114,6 +114,11 @@ __device__ __forceinline__ float pow2i(int e) {
   return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23);
 }
 
+// Of a value >= 0; 0 below the normal range.
+__device__ __forceinline__ float floor_pow2(float v) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0x7F800000u);
+}
+
 // The four lane groups' values against each other: exchanges of half rows of
 // registers, no LDS on the way.
 __device__ __forceinline__ float max_groups(float v) {
@@ -1312,10 +1317,17 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
           for (int q = 0; q < 4; ++q) t = fmaxf(t, vs[q] < __builtin_huge_valf() ? vs[q] : 0.0f);
           if (t > 0 && !(t * 64.0f >= unit && t <= unit * 64.0f)) {
             const float was = unit;
-            unit = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, t) & 0x7F800000u);
-            unit = fmaxf(unit, 0x1p-120f);
+            unit = fmaxf(floor_pow2(t), 0x1p-120f);
+            if (unit < was) {  // not so far that the sums overflow: what such a tile adds is nothing to them
+              float most = 0;
+#pragma unroll
+              for (int d = 0; d < kDt; ++d)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(o[d][v]));
+              unit = fminf(fmaxf(unit, floor_pow2(was * (max_halves(most) * 0x1p-99f))), was);
+            }
             alpha = was / unit;
-            move = true;
+            move = unit != was;
             per_unit = 1.0f / unit;
           }
         }

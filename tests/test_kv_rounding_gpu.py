@@ -55,6 +55,11 @@ def _attend(q, host, tables, lens, new, dtype, floor, scale=None, top=None, caus
     return got, ref
 
 
+# Times a sequence and a head of it stand in a call, so that each wave (few
+# rows) or workgroup (many) has an item whole.
+WHOLE = {FEW: dict(batch=256, heads=8), MANY: dict(batch=32, heads=8)}
+
+
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
 @pytest.mark.parametrize("d,page,group", [(128, 16, 8), (64, 64, 3), (128, 128, 1)])
 @pytest.mark.parametrize("new,floor", [([1, 1], FEW), ([9, 4], FEW), ([300, 129], MANY), ([200, 500], MANY)])
@@ -67,3 +72,54 @@ def test_results_are_as_exact_as_their_rounding(new, floor, d, page, group, dtyp
     tables, pages = _tables(rng, lens, page)
     host = _random_cache(rng, pages, page, 2, d)
     _attend(rng.standard_normal((sum(new), 2 * group, d)), host, tables, lens, new, dtype, floor)
+
+
+def _tile_scales(tile_scales, page, zero=(), heads=1, d=64):
+    """Pages in order whose value scale is given tile by tile of 64 keys; in
+    tiles `zero` all codes are 0."""
+    rng = np.random.default_rng(len(tile_scales))
+    each = max(64 // page, 1)
+    scales = np.repeat(np.asarray(tile_scales, np.float64), each)[:: max(page // 64, 1)]
+    host = list(_random_cache(rng, len(scales), page, heads, d))
+    host[1] = np.clip(np.rint(60 + 30 * rng.standard_normal(host[1].shape)), -127, 127).astype(np.int8)
+    host[3] = np.repeat(scales[:, None], heads, 1).astype(np.float32)
+    for t in zero:
+        host[1][t * each * 64 // max(page, 64): (t + 1) * each * 64 // max(page, 64)] = 0
+    return rng, host, np.arange(len(scales), dtype=np.int32)[None], len(scales) * page
+
+
+ONE = 1 / 38
+TILES = {
+    "34": [ONE] * 60 + [1e-34 / 127] + [ONE] * 5,
+    "37": [ONE] * 60 + [1e-37 / 127] + [ONE] * 5,
+    "both": [ONE] * 40 + [1e-34 / 127] + [ONE] * 8 + [1e-37 / 127] + [ONE] * 3,
+    "last": [ONE] * 60 + [1e-34 / 127] * 2,
+    "first": [1e-34 / 127] * 3 + [ONE] * 20,
+    "first37": [1e-37 / 127] * 3 + [ONE] * 20,
+    "large": [2000.0] * 20 + [1e-34 / 127] * 2 + [2000.0],
+    "down": list(10.0 ** -np.arange(0, 36, 1.5)),
+    "up": list(10.0 ** -np.arange(0, 36, 1.5))[::-1],
+    "steps": [ONE, ONE * 40, ONE / 40, ONE * 900, ONE / 900, ONE * 20000, ONE / 20000] * 4,
+    "tiny": [1e-34 / 127] * 20,
+}
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("new,floor", [(1, FEW), (20, FEW), (140, MANY), (256, MANY)])
+@pytest.mark.parametrize("which", sorted(TILES))
+def test_value_scales_of_any_ratio(which, new, floor, page):
+    # bf16 values reach down to 1e-38: pages of such values among ordinary
+    # ones, whichever comes first.
+    rng, host, tables, n = _tile_scales(TILES[which], page)
+    q = rng.standard_normal((new, 1, 64))
+    _attend(q, host, tables, [n], [new], "bf16", floor, causal=False)
+    _attend(q, host, tables, [n], [new], "bf16", floor, causal=False, **WHOLE[floor])
+
+
+@pytest.mark.parametrize("new,floor", [(1, FEW), (140, MANY)])
+@pytest.mark.parametrize("tiny", [1e-20, 1e-30])
+def test_small_values_after_zeros_on_large_pages(tiny, new, floor):
+    # Nothing has been summed when the scales fall: what follows is all there is.
+    rng, host, tables, n = _tile_scales([ONE] * 6 + [tiny] * 6 + [ONE] * 3, 16, zero=[*range(6), 12, 13, 14])
+    got, ref = _attend(rng.standard_normal((new, 1, 64)), host, tables, [n], [new], "bf16", floor, causal=False, top=tiny, **WHOLE[floor])
+    assert np.abs(ref).max() > tiny and np.abs(got).max() > tiny
