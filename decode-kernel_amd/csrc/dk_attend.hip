@@ -31,9 +31,11 @@ int kv_view(const dk_kv_cache* c, KvView* view);
 constexpr int kTile = 64;          // keys of a tile
 constexpr int kWorkgroups = 256;   // one a CU
 constexpr float kNegInf = -__builtin_huge_valf();
-// A row's maximum is moved only when a tile passes it by this much (base 2):
-// P stays below 2^8, far inside fp16, and the usual tile rescales nothing.
-constexpr float kLazy = 8.0f;
+// A row's maximum is moved only when a tile passes it by this much (base 2), so
+// that the usual tile rescales nothing: P stays below 2^kLazy. Times 2^kLift it
+// fills fp16 upwards, whose second part ends at 2^-25: a weight is kept down to
+// 2^-36 of the row's largest, where 131072 of them add 2^-19.
+constexpr float kLazy = 4.0f, kLift = 11.0f, kLower = 0x1p-11f;  // kLower: what undoes the lift
 
 struct AttendArgs {
   KvView c;
@@ -454,6 +456,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs& a, const Seq& s, 
     float top = max_groups(cv < __builtin_huge_valf() ? cv : 0.0f);
     top = top > 0 ? top : 1.0f;
     const float rel = cv / top;
+    const float lowered = top * kLower;  // 12 bits at the least scale that has codes, 2^-126
 
     const bool whole = key0 + kTile <= q.least && __all(here);
     h8_t pf[NT][2], pl[NT][2];  // P in fp16 and what that leaves of it
@@ -478,13 +481,15 @@ __device__ __forceinline__ void attend_piece(const AttendArgs& a, const Seq& s, 
         for (int d = 0; d < kD; ++d) y.o[t][d] *= alpha;
         y.m[t] = mn;
       }
-      const float base = y.m[t] == kNegInf ? 0.0f : y.m[t];
+      const float base = y.m[t] == kNegInf ? 0.0f : y.m[t] - kLift;
+      float sum = 0;  // the tile's by itself: small weights are not lost one by one beside large ones
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
         x[k] = __builtin_amdgcn_exp2f(x[k] - base);
-        y.l[t] += x[k];
+        sum += x[k];
         x[k] *= rel;
       }
+      y.l[t] += sum;
       if (!whole) {  // a key that is not seen has weight 0 on a page of any scale
 #pragma unroll
         for (int k = 0; k < 16; ++k) x[k] = k < left ? x[k] : 0.0f;
@@ -511,13 +516,13 @@ __device__ __forceinline__ void attend_piece(const AttendArgs& a, const Seq& s, 
         z = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[t][0], z, 0, 0, 0);
         z = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[t][1], z, 0, 0, 0);
 #pragma unroll
-        for (int v = 0; v < 4; ++v) y.o[t][d][v] = fmaf(top, z[v], y.o[t][d][v]);
+        for (int v = 0; v < 4; ++v) y.o[t][d][v] = fmaf(lowered, z[v], y.o[t][d][v]);
       }
     }
     if (more) load_values();
   }
 #pragma unroll
-  for (int t = 0; t < NT; ++t) y.l[t] = sum_groups(y.l[t]);
+  for (int t = 0; t < NT; ++t) y.l[t] = sum_groups(y.l[t]) * kLower;
 }
 
 // Whether all pieces of an item are in the workspace. A workgroup sets its own

@@ -123,3 +123,33 @@ def test_small_values_after_zeros_on_large_pages(tiny, new, floor):
     rng, host, tables, n = _tile_scales([ONE] * 6 + [tiny] * 6 + [ONE] * 3, 16, zero=[*range(6), 12, 13, 14])
     got, ref = _attend(rng.standard_normal((new, 1, 64)), host, tables, [n], [new], "bf16", floor, causal=False, top=tiny, **WHOLE[floor])
     assert np.abs(ref).max() > tiny and np.abs(got).max() > tiny
+
+
+def _sink(n, delta, first, d=64, page=16):
+    """One key that takes nearly all weight and has value 0, and n - 1 keys
+    2^-delta below it. Its page's value scale is `first` times the others'."""
+    rng = np.random.default_rng(n + int(delta))
+    count = -(-n // page)
+    k = np.zeros((count, page, 1, d), np.int8)
+    k[:, :, 0, 0] = rng.integers(-3, 4, (count, page))
+    k[0, 0, 0, 0] = 127
+    v = np.clip(np.rint(60 + 40 * rng.standard_normal((count, page, 1, d))), -127, 127).astype(np.int8)
+    v[0] = 0
+    ks, vs = np.full((count, 1), 1 / 127, np.float32), np.ones((count, 1), np.float32)
+    vs[:max(64 // page, 1)] = first  # the whole first tile
+    v[:max(64 // page, 1)] = 0
+    tables = rng.permutation(count).astype(np.int32)
+    place = np.argsort(tables)
+    host = [a[place] for a in (k, v, ks, vs)]
+    return host, tables[None], delta * np.log(2.0)
+
+
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("n,delta", [(20000, 18), (20000, 24), (20000, 26), (131070, 24), (131070, 26)])
+@pytest.mark.parametrize("first", [1.0, 50.0])
+def test_small_weights_beside_a_sink_few_rows(first, n, delta, dtype):
+    host, tables, scale = _sink(n, delta, first)
+    q = np.zeros((1, 2, 64))
+    q[..., 0] = 1
+    _attend(q, host, tables, [n], [1], dtype, FEW, scale=scale, top=1.0, **WHOLE[FEW])
+    _attend(q, host, tables, [n], [1], dtype, FEW, scale=scale, top=1.0)
