@@ -958,9 +958,12 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
 // the wave's halves. Values lie in LDS in the order in which lanes hold P's
 // tokens.
 //
-// A page's value scale goes into P relative to a power of two, `unit`, that
-// follows the scales within 2^6: P keeps fp16's bits whatever the values' size
-// is, and the sums are only rescaled when the unit moves.
+// A page's value scale goes into P relative to a power of two, `unit`, which is
+// what the sums are counted in. A tile's largest scale is kScaleLow to kScaleHigh
+// units, so that P, 2^kLazy high, fills fp16 upwards and a weight is kept down to
+// 2^-30 of the row's largest (2^-33 where the first tile's scale is the usual one).
+// The unit moves no further than a tile asks for: scales within 2^5 of each other
+// settle on one, and the sums are rescaled only when it moves.
 //
 // The work is (sequence, head, row tile, tile of keys), with the tiles past a
 // row tile's last visible key left out; the workgroups take equal shares, and
@@ -977,6 +980,7 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
 // ---------------------------------------------------------------------------
 constexpr int kManyRows = 256;
 constexpr int kManyThreads = 512;
+constexpr float kScaleLow = 0x1p5f, kScaleFirst = 0x1p8f, kScaleHigh = 0x1p11f;
 constexpr int kManyItemCost = 6;  // an item's start and end against a tile, measured
 
 typedef float f16_t __attribute__((ext_vector_type(16)));
@@ -1316,13 +1320,15 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
         const float bottom = fminf(fminf(cs[0], cs[1]), fminf(cs[2], cs[3]));  // -1: a page is missing
         float alpha = 1.0f;
         bool move = false;
-        if (__builtin_expect(!(top * 64.0f >= unit && top <= unit * 64.0f), 0)) {  // the unit moves, or there is none
+        auto fits = [&](float scale) { return scale >= unit * kScaleLow && scale <= unit * kScaleHigh; };
+        if (__builtin_expect(!fits(top), 0)) {  // the unit moves, or there is none
           float t = 0;
 #pragma unroll
           for (int q = 0; q < 4; ++q) t = fmaxf(t, vs[q] < __builtin_huge_valf() ? vs[q] : 0.0f);
-          if (t > 0 && !(t * 64.0f >= unit && t <= unit * 64.0f)) {
+          if (t > 0 && !fits(t)) {
             const float was = unit;
-            unit = fmaxf(floor_pow2(t), 0x1p-120f);
+            const float units = was == 0 ? kScaleFirst : t > was * kScaleHigh ? kScaleHigh / 2 : kScaleLow;
+            unit = fmaxf(floor_pow2(t) / units, 0x1p-126f);
             if (unit < was) {  // not so far that the sums overflow: what such a tile adds is nothing to them
               float most = 0;
 #pragma unroll
@@ -1380,6 +1386,7 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
 #pragma unroll
           for (int d = 0; d < kDt; ++d) o[d] *= alpha;
         }
+        float sum = 0;  // the tile's by itself, as in attend_few
 #pragma unroll
         for (int q = 0; q < 4; ++q)
 #pragma unroll
@@ -1388,7 +1395,7 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const float p = __builtin_amdgcn_exp2f(fmaf(st[q >> 1][8 * (q & 1) + e + i], ck[q], sub));
-              l += p;
+              sum += p;
               w[i] = p * rel[q];
             }
             const h2_t f = first_parts(w[0], w[1]);
@@ -1398,6 +1405,7 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
               pl[q][e + i] = (_Float16)fmaf((float)f[i], -1.0f, w[i]);
             }
           }
+        l += sum;
         if (__builtin_expect(fix, 0)) {  // a key that is not seen has weight 0 on a page of any scale
           asm volatile("" : "+v"(left));
 #pragma unroll

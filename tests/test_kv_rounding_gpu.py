@@ -153,3 +153,13 @@ def test_small_weights_beside_a_sink_few_rows(first, n, delta, dtype):
     q[..., 0] = 1
     _attend(q, host, tables, [n], [1], dtype, FEW, scale=scale, top=1.0, **WHOLE[FEW])
     _attend(q, host, tables, [n], [1], dtype, FEW, scale=scale, top=1.0)
+
+
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("n,delta", [(20000, 18), (20000, 20), (20000, 24)])
+@pytest.mark.parametrize("first", [1.0, 50.0, 1 / 50])
+def test_small_weights_beside_a_sink_many_rows(first, n, delta, dtype):
+    host, tables, scale = _sink(n, delta, first)
+    q = np.zeros((140, 1, 64))
+    q[..., 0] = 1
+    _attend(q, host, tables, [n], [140], dtype, MANY, scale=scale, top=1.0, **WHOLE[MANY])
