@@ -51,6 +51,7 @@ struct AttendArgs {
   float scale_log2;
   int width, tokens, requests, group, bf16, causal;
   int few_rows;  // sequences of more rows are attend_many's
+  int clear;     // this kernel writes the rows of no sequence
 };
 
 // One sequence: its queries, its keys, its row tiles and tiles of keys.
@@ -70,6 +71,29 @@ __device__ __forceinline__ Seq sequence(const AttendArgs& a, int b, int rows_a_t
   s.row_tiles = (rows > a.few_rows) == many ? (rows + rows_a_tile - 1) / rows_a_tile : 0;
   s.tiles = max((s.len + kTile - 1) / kTile, 1);  // an empty sequence's rows are written too
   return s;
+}
+
+// The tokens that belong to a sequence: first <= t < last.
+struct Owned {
+  int first, last;
+};
+__device__ __forceinline__ Owned owned_tokens(const AttendArgs& a) {
+  Owned w{0, a.tokens};
+  if (a.offsets) {
+    w.first = min(max(a.offsets[0], 0), a.tokens);
+    w.last = min(max(a.offsets[a.requests], w.first), a.tokens);
+  }
+  return w;
+}
+
+// The others' rows are zeros, each workgroup's part of them.
+template <int D>
+__device__ __forceinline__ void clear_rows(const AttendArgs& a, const Owned& w, int tid, int threads) {
+  const long long row = (long long)a.c.heads * a.group * (D / 8);  // 16 bytes each
+  const long long before = w.first * row, all = before + (a.tokens - w.last) * row;
+  uint4* out = reinterpret_cast<uint4*>(a.out);
+  for (long long u = (long long)blockIdx.x * threads + tid; u < all; u += (long long)kWorkgroups * threads)
+    out[u < before ? u : u - before + w.last * row] = zero4();
 }
 
 __device__ __forceinline__ h8_t codes_to_f16(uint32_t lo, uint32_t hi) {
@@ -746,6 +770,7 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
   int each_units = 0;  // of every item, if they are one workgroup's each
   auto units_of = [&](const Seq& s) { return each_units ? each_units : s.tiles + kItemCost; };
   auto cost = [&](const Seq& s) { return a.c.heads * s.row_tiles * units_of(s); };
+  const Owned owned = owned_tokens(a);  // asked for along with the lengths
   const int each = (a.requests + 63) / 64;
   int b = lane * each;
   Seq s{};
@@ -770,6 +795,7 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
     upto = items_upto * each_units;
     total = most_items * each_units;
   }
+  if (a.clear) clear_rows<D>(a, owned, tid, F::kThreads);
   const int group_share = share * kWaves;
   if (wg >= (total + group_share - 1) / group_share) return;
   const int begin = wg * group_share + wave * share, end = min(begin + share, total);
@@ -1078,6 +1104,7 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
   const int shift = a.c.page_shift, P = 1 << shift;
 
   // This workgroup's share, found by every wave for itself as in attend_few.
+  const Owned owned = owned_tokens(a);
   const int each = (a.requests + 63) / 64;
   int b = lane * each;
   Seq s{};
@@ -1090,6 +1117,7 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
   const int total = __builtin_amdgcn_readlane(upto, 63);
   const int share = max((int)(((unsigned)total + kWorkgroups - 1) / kWorkgroups), 1);
   const int begin = wg * share, end = min(begin + share, total);
+  if (a.clear) clear_rows<D>(a, owned, tid, kManyThreads);
   if (begin >= end) return;
   int at = __builtin_ctzll(__ballot(begin < upto));
   int base = __builtin_amdgcn_readlane(upto - work, at);
@@ -1634,15 +1662,17 @@ extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
                          requests, num_tokens);
   if (max_query_len < 1)
     return dk::set_error(DK_ERR_INVALID_ARGUMENT, "max_query_len must be >= 1");
-  if (num_tokens == 0 || requests == 0) return DK_OK;
-  if (!q || !out || !seq_lens || (!tables && table_width > 0) || !workspace_ptr)
+  if (num_tokens == 0) return DK_OK;
+  const int group = q_heads / view.heads;
+  const Dispatch d = dispatch(num_tokens, requests, view.heads, group, max_query_len);
+  const size_t need = requests > 0 ? workspace_bytes_of(d, cache->head_size) : 0;
+  if (!q || !out || (requests > 0 && (!seq_lens || (!tables && table_width > 0))) || (!workspace_ptr && need > 0))
     return dk::set_error(DK_ERR_INVALID_ARGUMENT,
                          "q, out, tables, seq_lens and the workspace must not be NULL");
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace_ptr, 16))
     return dk::set_error(DK_ERR_INVALID_ARGUMENT, "q, out and the workspace must be 16-byte aligned");
   if (q_token_stride % 8 || q_head_stride % 8)
     return dk::set_error(DK_ERR_INVALID_ARGUMENT, "the strides of q must be multiples of 8");
-  const int group = q_heads / view.heads;
   // Work is counted in 31 bits: heads, row tiles and tiles of keys.
   const double most = (double)view.heads * ((double)num_tokens * group / 16 + requests) *
                       (((double)table_width * cache->page_size) / dk::kTile + 8);
@@ -1650,10 +1680,8 @@ extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
     return dk::set_error(DK_ERR_UNSUPPORTED, "heads * queries * keys too large");
   if (((double)table_width * cache->page_size + num_tokens + dk::kTile) * group > 1 << 30)
     return dk::set_error(DK_ERR_UNSUPPORTED, "keys * q_heads / heads too large");
-  const Dispatch d = dispatch(num_tokens, requests, view.heads, group, max_query_len);
-  if (workspace_bytes < workspace_bytes_of(d, cache->head_size))
-    return dk::set_error(DK_ERR_INVALID_ARGUMENT, "the workspace has %zu of %zu bytes",
-                         workspace_bytes, workspace_bytes_of(d, cache->head_size));
+  if (workspace_bytes < need)
+    return dk::set_error(DK_ERR_INVALID_ARGUMENT, "the workspace has %zu of %zu bytes", workspace_bytes, need);
   dk::AttendArgs a{};
   a.c = view;
   a.q = static_cast<const uint16_t*>(q);
@@ -1680,11 +1708,13 @@ extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
   };
   if (d.many) {
     a.few_rows = d.few ? kFewRows : 0;
+    a.clear = !d.few;
     if (cache->head_size == 64) launch(dk::attend_many<64>, dk::kManyThreads, dk::kManyRows);
     else launch(dk::attend_many<128>, dk::kManyThreads, dk::kManyRows);
   }
   if (d.few) {
     a.few_rows = d.many ? kFewRows : INT32_MAX;
+    a.clear = 1;
     if (cache->head_size == 64) {
       if (d.nt == 1) launch(dk::attend_few<64, 1>, dk::Few<64, 1>::kThreads, 16);
       else launch(dk::attend_few<64, 2>, dk::Few<64, 2>::kThreads, 32);

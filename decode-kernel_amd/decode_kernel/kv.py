@@ -147,7 +147,8 @@ def attend_kv(
     ``query_offsets[b]:query_offsets[b + 1]``; without query_offsets, one query
     a sequence. The queries are the last tokens of their sequence, their keys
     appended already: with ``causal``, query i of n sees ``seq_lens[b] - n + i
-    + 1`` keys. A query that sees none gives 0. ``max_query_len`` (the most
+    + 1`` keys. A query that sees none gives 0, and so does one of no sequence
+    (a captured step's places past its last token). ``max_query_len`` (the most
     queries a sequence has; default: all of them) picks kernels and changes no
     result beyond the order of its sums. scale: head_size ** -0.5 by default.
     """

@@ -113,8 +113,8 @@ size_t dk_kv_attend_workspace_bytes(int num_tokens, int requests, int q_heads, i
  * num_tokens == requests; offsets do not decrease). With causal, query i of n sees the keys up to
  * seq_lens[b] - n + i: the queries are the sequence's last tokens, and their
  * keys are in the cache already. Keys on a page outside the cache (-1) are
- * not seen. A query that sees no key gives 0, and one that belongs to no
- * sequence is not written.
+ * not seen. A query that sees no key gives 0, and so does one that belongs to no
+ * sequence (before the first offset or from the last one on), which is not read.
  *
  * q and out: DK_KV_F16 or DK_KV_BF16, out contiguous, q with strides (in
  * elements, multiples of 8) of tokens and heads, both 16-byte aligned.
