@@ -54,7 +54,8 @@ struct AttendArgs {
   int clear;     // this kernel writes the rows of no sequence
 };
 
-// One sequence: its queries, its keys, its row tiles and tiles of keys.
+// One sequence: its queries (below 0 of them: offsets that decrease), its keys,
+// its row tiles and tiles of keys.
 struct Seq {
   int q0, n, len, row_tiles, tiles;
 };
@@ -64,10 +65,10 @@ __device__ __forceinline__ Seq sequence(const AttendArgs& a, int b, int rows_a_t
   s.q0 = b, s.n = 1;
   if (a.offsets) {
     s.q0 = min(max(a.offsets[b], 0), a.tokens);
-    s.n = max(min(max(a.offsets[b + 1], 0), a.tokens) - s.q0, 0);
+    s.n = min(max(a.offsets[b + 1], 0), a.tokens) - s.q0;
   }
   s.len = min((long long)max(a.lens[b], 0), (long long)a.width << a.c.page_shift);
-  const int rows = s.n * a.group;
+  const int rows = max(s.n, 0) * a.group;
   s.row_tiles = (rows > a.few_rows) == many ? (rows + rows_a_tile - 1) / rows_a_tile : 0;
   s.tiles = max((s.len + kTile - 1) / kTile, 1);  // an empty sequence's rows are written too
   return s;
@@ -775,8 +776,10 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
   int b = lane * each;
   Seq s{};
   int work = 0, items = 0, longest = 0;
+  bool ordered = true;
   for (int k = 0; k < each && b + k < a.requests; ++k) {
     s = sequence(a, b + k, kRows, false);
+    ordered &= s.n >= 0;
     work += cost(s);
     items += a.c.heads * s.row_tiles;
     longest = max(longest, s.row_tiles ? s.tiles : 0);
@@ -795,7 +798,9 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
     upto = items_upto * each_units;
     total = most_items * each_units;
   }
-  if (a.clear) clear_rows<D>(a, owned, tid, F::kThreads);
+  ordered = __all(ordered);
+  if (a.clear) clear_rows<D>(a, ordered ? owned : Owned{0, 0}, tid, F::kThreads);
+  if (!ordered) return;  // rows of two sequences: more work than is counted in 31 bits
   const int group_share = share * kWaves;
   if (wg >= (total + group_share - 1) / group_share) return;
   const int begin = wg * group_share + wave * share, end = min(begin + share, total);
@@ -1109,16 +1114,19 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
   int b = lane * each;
   Seq s{};
   int work = 0;
+  bool ordered = true;
   for (int k = 0; k < each && b + k < a.requests; ++k) {
     s = sequence(a, b + k, kManyRows, true);
+    ordered &= s.n >= 0;
     work += a.c.heads * head_cost(a, s);
   }
   int upto = wave_scan(work);
   const int total = __builtin_amdgcn_readlane(upto, 63);
   const int share = max((int)(((unsigned)total + kWorkgroups - 1) / kWorkgroups), 1);
   const int begin = wg * share, end = min(begin + share, total);
-  if (a.clear) clear_rows<D>(a, owned, tid, kManyThreads);
-  if (begin >= end) return;
+  ordered = __all(ordered);
+  if (a.clear) clear_rows<D>(a, ordered ? owned : Owned{0, 0}, tid, kManyThreads);
+  if (!ordered || begin >= end) return;
   int at = __builtin_ctzll(__ballot(begin < upto));
   int base = __builtin_amdgcn_readlane(upto - work, at);
   b = at * each;

@@ -144,7 +144,8 @@ def attend_kv(
     q [tokens, q_heads, head_size], fp16 or bf16, q_heads a multiple of the
     cache's heads (query head h reads cache head h // (q_heads / heads)).
     Sequence b has ``seq_lens[b]`` keys and the queries
-    ``query_offsets[b]:query_offsets[b + 1]``; without query_offsets, one query
+    ``query_offsets[b]:query_offsets[b + 1]`` (offsets that decrease anywhere
+    give zeros for all); without query_offsets, one query
     a sequence. The queries are the last tokens of their sequence, their keys
     appended already: with ``causal``, query i of n sees ``seq_lens[b] - n + i
     + 1`` keys. A query that sees none gives 0, and so does one of no sequence

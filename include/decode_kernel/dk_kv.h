@@ -110,7 +110,7 @@ size_t dk_kv_attend_workspace_bytes(int num_tokens, int requests, int q_heads, i
  * of t's sequence, heads hq / (q_heads / heads). Sequence b has seq_lens[b]
  * keys (at most table_width * page_size) and the queries
  * query_offsets[b] .. query_offsets[b + 1] - 1 (NULL: query b alone, and
- * num_tokens == requests; offsets do not decrease). With causal, query i of n sees the keys up to
+ * num_tokens == requests; where offsets decrease, all of out is 0). With causal, query i of n sees the keys up to
  * seq_lens[b] - n + i: the queries are the sequence's last tokens, and their
  * keys are in the cache already. Keys on a page outside the cache (-1) are
  * not seen. A query that sees no key gives 0, and so does one that belongs to no

@@ -71,3 +71,24 @@ def test_no_requests_give_zeros():
         del junk  # the output's memory, most likely
         out = attend_kv(q, KVCache.empty(2, 2, 64, 16), none.view(0, 3), none, torch.zeros(1, dtype=torch.int32, device="cuda"), most)
         assert out.shape == q.shape and not out.any()
+
+
+@pytest.mark.parametrize("requests,tokens,most", [(2, 40, 40), (2, 300, 300), (3, 5, 1), (70, 300, 200), (4096, 4096, 4096), (4096, 4096, 1)])
+def test_offsets_that_decrease_give_zeros(requests, tokens, most):
+    # Sequences that share rows are more work than the counts hold: none is done.
+    rng = np.random.default_rng(requests)
+    heads, group, d = 2, 4, 64
+    tables = np.zeros((requests, 1024), np.int32)
+    host = _random_cache(rng, 3, 16, heads, d)
+    offsets = np.zeros(requests + 1, np.int32)
+    offsets[1::2] = tokens
+    q = _dev(rng.standard_normal((tokens, heads * group, d)).astype(np.float16))
+    out = torch.full_like(q, np.nan)
+    args = _cache(*host), _dev(tables), torch.full((requests,), 16000, dtype=torch.int32, device="cuda")
+    _run_abi(q, *args, _dev(offsets), most, out)
+    assert not out.any()
+    offsets = np.minimum(np.arange(requests + 1), tokens).astype(np.int32)  # one step back among many
+    offsets[-1] = max(int(offsets[-2]) - 1, 0)
+    out.fill_(np.nan)
+    _run_abi(q, *args, _dev(offsets), most, out)
+    assert not out.any()
