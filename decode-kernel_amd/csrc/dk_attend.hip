@@ -1614,6 +1614,19 @@ Dispatch dispatch(int num_tokens, int requests, int heads, int group, int max_qu
   return d;
 }
 
+// The most that a kernel of the call may have to count, in 31 bits: heads, row
+// tiles and tiles of keys with an item's own cost, all sequences as long as the
+// tables are wide. Each kernel's sequences are those of its number of rows.
+double most_work(const Dispatch& d, int num_tokens, int requests, int heads, int group, long long keys) {
+  const double rows = (double)num_tokens * group;
+  const int rows_a_tile = 16 * d.nt;
+  double tiles = 0;
+  if (d.few) tiles = rows / rows_a_tile + requests;
+  if (d.few && d.many) tiles = std::min(tiles, (double)requests * (kFewRows / rows_a_tile));
+  if (d.many) tiles = std::max(tiles, rows / dk::kManyRows + std::min((double)requests, rows / (d.few ? kFewRows : 1) + 1));
+  return heads * tiles * ((double)keys / dk::kTile + 8);
+}
+
 // The number of a call, which never comes again in a process: what its pieces'
 // flags hold when they are set.
 unsigned long long next_call() {
@@ -1681,10 +1694,7 @@ extern "C" int dk_kv_attend(const void* q, int dtype, long long q_token_stride,
     return dk::set_error(DK_ERR_INVALID_ARGUMENT, "q, out and the workspace must be 16-byte aligned");
   if (q_token_stride % 8 || q_head_stride % 8)
     return dk::set_error(DK_ERR_INVALID_ARGUMENT, "the strides of q must be multiples of 8");
-  // Work is counted in 31 bits: heads, row tiles and tiles of keys.
-  const double most = (double)view.heads * ((double)num_tokens * group / 16 + requests) *
-                      (((double)table_width * cache->page_size) / dk::kTile + 8);
-  if (most > 1 << 30)
+  if (most_work(d, num_tokens, requests, view.heads, group, (long long)table_width << view.page_shift) > 1 << 30)
     return dk::set_error(DK_ERR_UNSUPPORTED, "heads * queries * keys too large");
   if (((double)table_width * cache->page_size + num_tokens + dk::kTile) * group > 1 << 30)
     return dk::set_error(DK_ERR_UNSUPPORTED, "keys * q_heads / heads too large");

@@ -119,7 +119,11 @@ size_t dk_kv_attend_workspace_bytes(int num_tokens, int requests, int q_heads, i
  * q and out: DK_KV_F16 or DK_KV_BF16, out contiguous, q with strides (in
  * elements, multiples of 8) of tokens and heads, both 16-byte aligned.
  * max_query_len: the most queries that a sequence has. It only picks
- * kernels; sequences with more are right too. */
+ * kernels; sequences with more are right too. Work is counted in 31 bits: heads
+ * times tiles of 256 rows (queries times the group; of 16 or 32 where all
+ * sequences have up to 128) times tiles of 64 keys (of the tables' width) over
+ * 2^30 is DK_ERR_UNSUPPORTED, and so are keys or num_tokens times the group over
+ * 2^30. */
 int dk_kv_attend(const void* q, int dtype, long long q_token_stride, long long q_head_stride,
                  const dk_kv_cache* cache, const int32_t* tables, int table_width,
                  const int32_t* seq_lens, const int32_t* query_offsets, int num_tokens,
