@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from oracle import kv_oracle
-from test_kv_gpu import _cache, _check, _dev, _random_cache, _tables
+from test_kv_gpu import _attend_case, _cache, _check, _dev, _random_cache, _tables
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +92,41 @@ def test_offsets_that_decrease_give_zeros(requests, tokens, most):
     out.fill_(np.nan)
     _run_abi(q, *args, _dev(offsets), most, out)
     assert not out.any()
+
+
+# --------------------------------------------- prompts among single tokens
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("b,at", [(65, [0]), (65, [64]), (65, [31, 32, 33]), (130, [0, 2, 129]), (130, [65, 66]),
+                                  (257, [0, 4, 5, 128, 256]), (257, [255]), (600, [9, 10, 300])])
+def test_prompts_among_single_tokens(b, at, causal):
+    # More than 64 requests: a lane adds up several, and the prompts stand at
+    # the ends and the middle of what one lane has.
+    rng = np.random.default_rng(b + len(at))
+    new, lens = [1] * b, [int(x) for x in np.exp(rng.uniform(0, np.log(300), b))]
+    for i, p in enumerate(at):
+        new[p] = (70, 150, 33, 257, 129)[i]
+        lens[p] = new[p] + (0, 200, 1000, 5, 64)[i]
+    for p in range(7, b, 19):  # idle places
+        if new[p] == 1:
+            new[p], lens[p] = 0, 0
+    _attend_case(b, lens, new, 1, 4, 64 if causal else 128, 16, "bf16" if b % 2 else "fp16", causal)
+
+
+def test_prompts_in_every_place():
+    # No single tokens at all: every one of 90 requests is attend_many's.
+    rng = np.random.default_rng(3)
+    new = [int(x) for x in rng.integers(33, 60, 90)]
+    _attend_case(4, [n + int(x) for n, x in zip(new, rng.integers(0, 90, 90))], new, 1, 4, 64, 32, "fp16")
+
+
+@pytest.mark.parametrize("before", [0, 100])
+def test_prompt_of_more_than_64_row_tiles(before):
+    # 2100 tokens of 8 query heads: 66 row tiles of 256 a head.
+    _attend_case(5, [2100 + before, 40], [2100, 1], 1, 8, 64, 64, "fp16")
+
+
+@pytest.mark.parametrize("group", [1, 2, 3, 5, 6, 7, 12, 16, 20, 33])
+def test_prompt_by_group(group):
+    # What a row tile's last token sees, for groups that divide its 256 rows and others.
+    n = 1400 // group + 129
+    _attend_case(group, [n + 333, n], [n, n], 1, group, 64, 16, "bf16")
