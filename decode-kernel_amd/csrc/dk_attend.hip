@@ -1032,49 +1032,39 @@ struct Many {
   };
 };
 
-// sum of floor((a i + b) / m) over i < n
-__device__ __forceinline__ int floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
-  unsigned sum = 0;
-  while (n > 0) {
-    if (a >= m) {
-      sum += n * (n - 1) / 2 * (a / m);
-      a %= m;
-    }
-    if (b >= m) {
-      sum += n * (b / m);
-      b %= m;
-    }
-    const unsigned top = a * n + b;
-    if (top < m) break;
-    n = top / m;
-    b = top % m;
-    const unsigned t = m;
-    m = a;
-    a = t;
-  }
-  return (int)sum;
-}
-
 // Whether a sequence's row tiles see different numbers of keys.
 __device__ __forceinline__ bool slanted(const AttendArgs& a, const Seq& s) {
   return a.causal && s.n <= s.len && s.row_tiles > 1;
 }
 
-// Tiles of keys that row tile rt sees: its last row's token sees
-// len - n + ceil((rt + 1) 256 / group) keys, or all.
+// Tiles of keys that row tile rt sees, j = rt + 1: its last row's token sees
+// len - n + ceil(256 j / group) keys, or all, which is a number of tiles of
+//   ceil(((len - n) group + 256 j) / (64 group)) = ceil((c + 4 j) / group),
+// c = ceil((len - n) group / 64).
+__device__ __forceinline__ unsigned keys_before(const AttendArgs& a, const Seq& s) {
+  return ((unsigned)(s.len - s.n) * (unsigned)a.group + kTile - 1) / kTile;
+}
 __device__ __forceinline__ int tiles_seen(const AttendArgs& a, const Seq& s, int rt) {
   if (!slanted(a, s) || rt >= s.row_tiles - 1) return s.tiles;
   const unsigned G = a.group;
-  return ((unsigned)(s.len - s.n) * G + (rt + 1) * kManyRows + kTile * G - 1) / (kTile * G);
+  return (keys_before(a, s) + (kManyRows / kTile) * (rt + 1) + G - 1) / G;
 }
 
-// The work of one head of a sequence.
+// The work of one head of a sequence: the sum of its row tiles'. Every `period`
+// row tiles a row tile sees `rise` tiles of keys more, so those that stand
+// `period` apart are an arithmetic series.
 __device__ __forceinline__ int head_cost(const AttendArgs& a, const Seq& s) {
   if (!slanted(a, s)) return s.row_tiles * (s.tiles + kManyItemCost);
-  const unsigned G = a.group;
-  return s.row_tiles * kManyItemCost + s.tiles +
-         floor_sum(s.row_tiles - 1, kTile * G, kManyRows,
-                   (unsigned)(s.len - s.n) * G + kManyRows + kTile * G - 1);
+  static_assert(kManyRows / kTile == 4, "period and rise");
+  const unsigned G = a.group, common = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
+  const unsigned period = G / common, rise = 4 / common, last = s.row_tiles - 1;
+  const unsigned c = keys_before(a, s);
+  unsigned sum = s.row_tiles * kManyItemCost + s.tiles;
+  for (unsigned j = 1; j <= min(period, last); ++j) {
+    const unsigned terms = (last - j) / period + 1;
+    sum += terms * ((c + 4 * j + G - 1) / G) + rise * (terms * (terms - 1) / 2);
+  }
+  return (int)sum;
 }
 
 // A workgroup barrier for what is in LDS alone: __syncthreads() also waits for
