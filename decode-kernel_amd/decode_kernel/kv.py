@@ -100,7 +100,11 @@ def plan_kv_step(
     off the end of ``free_pages[:free_count]`` and are written into
     ``block_tables`` (int32 [requests, width], in place). Check that
     ``free_count`` did not become negative before trusting the step's last
-    tokens: those without a page are neither stored nor attended to. At most
+    tokens: those without a page are neither stored nor attended to, and a -1 in
+    the tables is not filled in later. Then take those tokens off the next step's
+    ``held`` (or drop their requests), and go on from a count of 0: pages are put
+    back at ``free_pages[0]``, not below it. The five results share one allocation:
+    clone ``seq_lens`` or ``free_count`` to keep them without the slots. At most
     4096 requests.
     """
     return KVStep(*_ext().plan_kv_step(block_tables, held, added, free_pages, free_count,

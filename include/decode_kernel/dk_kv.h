@@ -68,7 +68,11 @@ typedef struct dk_kv_cache {
  * Pages come off the end of free_pages[0 .. *free_count), in the order of
  * the requests. Where none is left the entry is -1, the slots of its tokens
  * are -1 and *free_count_out is negative by what was missing; slots past the
- * table's end are -1 too. Every result is a function of the inputs alone, so
+ * table's end are -1 too. A token without a slot stays without: an entry of -1
+ * is not filled in later. After a shortage take the missing tokens off held
+ * (down to the end of the last page that is there), or drop their requests, and
+ * set the count to 0 before pages are put back from there; a negative one is
+ * subtracted from what comes after it. Every result is a function of the inputs alone, so
  * the same call again gives the same. free_count_out must not be free_count. */
 int dk_kv_plan(int32_t* tables, int table_width, const int32_t* held, const int32_t* added,
                int requests, const int32_t* free_pages, int free_capacity,

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from oracle import kv_oracle
-from test_kv_gpu import _attend_case, _cache, _check, _dev, _random_cache, _tables
+from test_kv_gpu import _attend_case, _back, _cache, _check, _dev, _random_cache, _tables
 
 pytestmark = pytest.mark.gpu
 
@@ -130,3 +130,47 @@ def test_prompt_by_group(group):
     # What a row tile's last token sees, for groups that divide its 256 rows and others.
     n = 1400 // group + 129
     _attend_case(group, [n + 333, n], [n, n], 1, group, 64, 16, "bf16")
+
+
+# ------------------------------------------------------- out of pages
+def test_shortage_then_pages_returned():
+    # What to do when free_count fell below 0: take back the requests that
+    # found no page, set the count to 0, return pages from there.
+    from decode_kernel import KVCache, append_kv, attend_kv, plan_kv_step
+
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    page, heads, d = 16, 1, 64
+    cache = KVCache.empty(6, heads, d, page)
+    tables = torch.full((3, 4), -1, dtype=torch.int32, device="cuda")
+    free, count, held = torch.arange(6, dtype=torch.int32, device="cuda"), i32(6), i32(0, 0, 0)
+    rng = np.random.default_rng(1)
+    make = lambda n, h: _dev(rng.standard_normal((n, h, d)).astype(np.float16))  # noqa: E731
+
+    def step(added):
+        n = sum(added)
+        s = plan_kv_step(tables, held, i32(*added), free, count, page, n)
+        q, k, v = make(n, 2), make(n, 1), make(n, 1)
+        append_kv(cache, k, v, s.slots)
+        o = attend_kv(q, cache, tables, s.seq_lens, s.query_offsets, max(added))
+        ref, spread = kv_oracle.attend(q.float().cpu().numpy(), *_back(cache), tables.cpu().numpy(), s.seq_lens.tolist(),
+                                       s.query_offsets.tolist(), d**-0.5, True)
+        _check(o, ref, spread, 64, 127 * float(cache.v_scales.max()), torch.float16)
+        return s
+
+    s = step([32, 16, 40])  # 2 + 1 + 3 pages: all of them
+    assert s.free_count.tolist() == [0]
+    held, count = s.seq_lens, s.free_count
+    s = step([1, 1, 1])  # two pages are missing: requests 0 and 1 find none
+    assert s.free_count.tolist() == [-2] and s.slots[:2].tolist() == [-1, -1] and int(s.slots[2]) >= 0
+    assert tables[0, 2] == -1 and tables[1, 1] == -1
+    # Request 2 ends and its three pages come back; 0 and 1 take their token back.
+    back = tables[2, :3].clone()
+    tables[2] = -1
+    held = torch.stack([s.seq_lens[0] - 1, s.seq_lens[1] - 1, s.seq_lens[2] * 0])
+    count = s.free_count.clamp(min=0)
+    free[0:3] = back
+    count = count + 3
+    s = step([1, 1, 9])
+    assert s.free_count.tolist() == [0] and (s.slots >= 0).all()
+    assert s.seq_lens.tolist() == [33, 17, 9]
+    assert sorted([int(tables[0, 2]), int(tables[1, 1]), int(tables[2, 0])]) == sorted(back.tolist())
