@@ -114,8 +114,8 @@ def plan_kv_step(
 def append_kv(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Writes k and v [tokens, heads, head_size] (fp16 or bf16) at ``slots``.
 
-    A page's scale for a head is the largest ``amax / 127`` it has seen since
-    its first token was written; where it grows, the page's earlier codes are
+    A page's scale for a head is the largest ``amax * (1 / 127)`` it has seen
+    since its first token was written, a code ``rint(x * (1 / scale))``; where it grows, the page's earlier codes are
     rounded again to the new scale. Tokens of one page stand together and in
     order in ``slots``, as plan_kv_step gives them; slots of -1 are skipped.
     """

@@ -86,13 +86,15 @@ int dk_kv_plan(int32_t* tables, int table_width, const int32_t* held, const int3
  * them (token t + i at slot s + i); slots outside the cache (-1) are skipped,
  * also among them. For each page and head that
  * the step writes, with amax over its new tokens:
- *   scale = max(old scale, amax / 127)    (old scale 0 if token 0 of the page
- *                                          is among the new ones)
- *   code = clamp(rint(x / scale), -127, 127)
+ *   scale = max(old scale, amax * (1 / 127))  (old scale 0 if token 0 of the
+ *                                              page is among the new ones)
+ *   inv = 1 / scale                           (0 for a scale under 2^-126,
+ *                                              which so stores zeros)
+ *   code = clamp(rint(x * inv), -127, 127)
  * and where the scale grows the page's earlier codes become
- * rint(code * old scale / scale). A NaN or infinity makes the scale NaN, and
- * with it every value of the page for that head. A scale under 2^-126 stores
- * zeros. */
+ * clamp(rint(code * (old scale * inv)), -127, 127); each operation is rounded
+ * to fp32. A NaN or infinity makes the scale NaN, and with it every value of
+ * the page for that head. */
 int dk_kv_append(const dk_kv_cache* cache, const void* k, const void* v, int dtype,
                  long long k_token_stride, long long k_head_stride, long long v_token_stride,
                  long long v_head_stride, const int64_t* slots, int num_tokens,
