@@ -994,7 +994,8 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
 // units, so that P, 2^kLazy high, fills fp16 upwards and a weight is kept down to
 // 2^-30 of the row's largest (2^-33 where the first tile's scale is the usual one).
 // The unit moves no further than a tile asks for: scales within 2^5 of each other
-// settle on one, and the sums are rescaled only when it moves.
+// settle on one, and the sums are rescaled only when it moves. A row whose sums
+// are 2^126 under a later tile's scale loses them, where that tile weighs nothing.
 //
 // The work is (sequence, head, row tile, tile of keys), with the tiles past a
 // row tile's last visible key left out; the workgroups take equal shares, and
@@ -1344,35 +1345,8 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
         float ck[4], rel[4];
         const float top = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
         const float bottom = fminf(fminf(cs[0], cs[1]), fminf(cs[2], cs[3]));  // -1: a page is missing
-        float alpha = 1.0f;
-        bool move = false;
-        auto fits = [&](float scale) { return scale >= unit * kScaleLow && scale <= unit * kScaleHigh; };
-        if (__builtin_expect(!fits(top), 0)) {  // the unit moves, or there is none
-          float t = 0;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) t = fmaxf(t, vs[q] < __builtin_huge_valf() ? vs[q] : 0.0f);
-          if (t > 0 && !fits(t)) {
-            const float was = unit;
-            const float units = was == 0 ? kScaleFirst : t > was * kScaleHigh ? kScaleHigh / 2 : kScaleLow;
-            unit = fmaxf(floor_pow2(t) / units, 0x1p-126f);
-            if (unit < was) {  // not so far that the sums overflow: what such a tile adds is nothing to them
-              float most = 0;
-#pragma unroll
-              for (int d = 0; d < kDt; ++d)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(o[d][v]));
-              unit = fminf(fmaxf(unit, floor_pow2(was * (max_halves(most) * 0x1p-99f))), was);
-            }
-            alpha = was / unit;
-            move = unit != was;
-            per_unit = 1.0f / unit;
-          }
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          ck[q] = cs[q] * qs;
-          rel[q] = vs[q] * per_unit;
-        }
+        for (int q = 0; q < 4; ++q) ck[q] = cs[q] * qs;
         bool fix = false;
         // Places of this lane's tokens in the tile: 16 q + 8 (e / 4) + 4 hh + e % 4.
         int left = limit - key0 - 4 * hh;
@@ -1398,16 +1372,44 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
           for (int e = 1; e < 8; ++e) g = fmaxf(g, st[q >> 1][8 * (q & 1) + e]);
           tm = fmaxf(tm, g * ck[q]);
         }
+        float alpha = 1.0f;  // what the sums so far are multiplied by
+        bool move = false;
         if (__builtin_expect(__any(tm > bound), 0)) {
           const float mn = fmaxf(m, max_halves(tm));
-          const float f = mn == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-          l *= f;
-          alpha *= f;
+          alpha = mn == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+          l *= alpha;
           m = mn;
           bound = mn + kLazy;
           sub = mn == kNegInf ? 0.0f : -mn;
           move = true;
         }
+        auto fits = [&](float scale) { return scale >= unit * kScaleLow && scale <= unit * kScaleHigh; };
+        if (__builtin_expect(!fits(top), 0)) {  // the unit moves, or there is none
+          float t = 0;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) t = fmaxf(t, vs[q] < __builtin_huge_valf() ? vs[q] : 0.0f);
+          if (t > 0 && !fits(t)) {
+            const float was = unit;
+            const float units = was == 0 ? kScaleFirst : t > was * kScaleHigh ? kScaleHigh / 2 : kScaleLow;
+            unit = fmaxf(floor_pow2(t) / units, 0x1p-126f);
+            float most = 1.0f;
+            if (unit < was) {  // not so far that the sums overflow: what such a tile adds is nothing to them
+              most = 0;
+#pragma unroll
+              for (int d = 0; d < kDt; ++d)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(o[d][v]));
+              most = max_halves(most) * alpha;
+              const float least = most > 0 ? fmaxf(floor_pow2(was * (most * 0x1p-99f)), was * 0x1p-126f) : 0.0f;
+              unit = fminf(fmaxf(unit, least), was);
+            }
+            if (most > 0) alpha *= was / unit;  // else there is nothing to multiply
+            move |= unit != was;
+            per_unit = 1.0f / unit;
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) rel[q] = vs[q] * per_unit;
         if (__builtin_expect(move, 0)) {
 #pragma unroll
           for (int d = 0; d < kDt; ++d) o[d] *= alpha;

@@ -117,10 +117,11 @@ def test_value_scales_of_any_ratio(which, new, floor, page):
 
 
 @pytest.mark.parametrize("new,floor", [(1, FEW), (140, MANY)])
+@pytest.mark.parametrize("large", [ONE, 1e10])
 @pytest.mark.parametrize("tiny", [1e-20, 1e-30])
-def test_small_values_after_zeros_on_large_pages(tiny, new, floor):
+def test_small_values_after_zeros_on_large_pages(tiny, large, new, floor):
     # Nothing has been summed when the scales fall: what follows is all there is.
-    rng, host, tables, n = _tile_scales([ONE] * 6 + [tiny] * 6 + [ONE] * 3, 16, zero=[*range(6), 12, 13, 14])
+    rng, host, tables, n = _tile_scales([large] * 6 + [tiny] * 6 + [large] * 3, 16, zero=[*range(6), 12, 13, 14])
     got, ref = _attend(rng.standard_normal((new, 1, 64)), host, tables, [n], [new], "bf16", floor, causal=False, top=tiny, **WHOLE[floor])
     assert np.abs(ref).max() > tiny and np.abs(got).max() > tiny
 
@@ -163,3 +164,22 @@ def test_small_weights_beside_a_sink_many_rows(first, n, delta, dtype):
     q = np.zeros((140, 1, 64))
     q[..., 0] = 1
     _attend(q, host, tables, [n], [140], dtype, MANY, scale=scale, top=1.0, **WHOLE[MANY])
+
+
+@pytest.mark.parametrize("new,floor", [(2, FEW), (140, MANY)])
+@pytest.mark.parametrize("scales", [[ONE] * 6 + [1e-34 / 127] * 6, [1e-34 / 127] * 6 + [ONE] * 6,
+                                    [ONE] * 5 + [1e-34 / 127] * 5 + [ONE] * 5 + [1e-34 / 127] * 5])
+def test_rows_that_look_past_large_values(scales, new, floor):
+    # Every other row has all its weight on the pages of small values; the large
+    # ones weigh 2^-200 there, and nothing of them is left.
+    rng, host, tables, n = _tile_scales(scales, 16)
+    small = np.repeat(np.asarray(scales) < 1e-30, 4)
+    host[0][:] = 0
+    host[0][..., 0] = np.where(small, 100, -100)[:, None, None]
+    host[0][..., 1] = rng.integers(-100, 101, host[0].shape[:-1])
+    host[2][:] = 0.01
+    q = np.zeros((new, 1, 64))
+    q[:, 0, 0] = np.where(np.arange(new) % 2, 100, -100) * np.log(2.0)
+    q[:, 0, 1] = 1
+    got, ref = _attend(q, host, tables, [n], [new], "bf16", floor, scale=1.0, causal=False, top=0.0, **WHOLE[floor])
+    assert np.abs(ref[:, 1::2]).max() < 1e-30 and np.abs(ref[:, ::2]).min() > 0.1
