@@ -236,12 +236,15 @@ __device__ __forceinline__ uint16_t* out_row(const AttendArgs& a, const Seq& s, 
 // the keys 16 g .. 16 g + 15 of the tile in both products, and a page's scales
 // are one value a lane. P goes in as two fp16 parts, which costs nothing here.
 //
-// 131071 keys of 8 heads of 128 for one token (8 rows a head): 268 MB in 59 us,
+// 131071 keys of 8 heads of 128 for one token (8 rows a head): 268 MB in 60 us,
 // 4.5 TB/s (a large read has 6.1). The tiles themselves run at 6.9 TB/s; 5 us
 // go by before them (lengths, page numbers, first codes: three trips to
 // memory) and 10 after (joining in LDS, flags, joining 32 workgroups' pieces).
-// 64 ragged sequences in pages of 16: 185 MB in 45 us. 700 keys of 32 heads:
-// 13 us, all of it such trips. Equal shares a workgroup instead of a wave, its
+// 64 ragged sequences in pages of 16: 185 MB in 46 us. 700 keys of 32 heads:
+// 13 us, all of it such trips. With 32 rows and heads of 128 (NT 2) the state
+// takes 256 registers and 112 accumulation registers, one wave a SIMD, and part
+// of it moves between them in the loop; what is uniform and little used lies in
+// vector lanes here and in attend_many (30 to 56 scalar registers). Equal shares a workgroup instead of a wave, its
 // four waves on one item, took 50 us and more where short sequences stand
 // together, and a second launch to join 5 us more.
 // ---------------------------------------------------------------------------
@@ -252,10 +255,10 @@ constexpr int kItemCost = 1;
 // of eight waves; twice as many of four): a tile costs 2.5 us where a wave has
 // few, meeting through the workspace 4 to 7. us, shared / alone, fp16, heads of
 // 128, pages of 64, at 200, 500, 700, 1500 and 3000 keys:
-//    1 sequence, 32 heads                14.9/9.0  14.9/10.8  14.5/13.2  15/19  13/24
-//   16 sequences, 8 x 8 heads            15.7/9.2  15.3/11.1  15.2/13.7  20/-   23/-
-//   32 sequences, 8 x 8 heads            15.8/9.3  19.5/11.7  19.2/15.5  28/22  34/35
-//    8 sequences, 8 x 8, four queries    23.9/16   24.8/19    19.4/20    28/30  26/-
+//    1 sequence, 32 heads                15.1/9.0  14.7/10.9  14.4/13.3  15/19  14/24
+//   16 sequences, 8 x 8 heads            15.7/9.2  15.6/11.2  15.5/14.0  21/20  23/26
+//   32 sequences, 8 x 8 heads            15.7/9.3  20.1/12.0  19.6/15.7  28/23  36/36
+//    8 sequences, 8 x 8, four queries    23.7/16   25.0/19    19.6/20    29/29  26/42
 constexpr int kAloneTiles = 1;
 
 template <int D, int NT>
@@ -1002,13 +1005,14 @@ __global__ __launch_bounds__((Few<D, NT>::kThreads)) void attend_few(AttendArgs 
 // pieces of an item that two or more share meet as those of attend_few do.
 //
 // A prompt of 4096 tokens, 64 query and 8 key/value heads, fp16: 275 GFLOP in
-// 415 us, 660 TFLOP/s, with the products for P's second part on top; 501 tokens
-// on each of three long contexts, bf16: 281 GFLOP in 306 us, 918 TFLOP/s (a
-// large library product has 1200). Per tile the vector instructions of two
-// waves (scores to weights 230, codes 50 each) take about as long as their
-// products, at half of the matrix slots and a clock that falls to 1.7 GHz.
-// Operand loads next to their products, in the compiler's order, cost a
-// quarter; without the halves' shift 383 us instead of 328 for the second.
+// 417 us, 660 TFLOP/s, with the products for P's second part on top (half as
+// many again: 990 of the 1200 that a large library product has); 501 tokens on
+// each of three long contexts, bf16: 281 GFLOP in 405 us. Per tile the vector
+// instructions of two waves (scores to weights about 200, codes 50 each) take
+// about as long as their products, with the matrix units busy 52% and 59% of the
+// time at a clock that falls to 1.8 and 1.7 GHz. With P in one part, operand
+// loads next to their products, in the compiler's order, cost a quarter, and the
+// second took 383 us instead of 328 without the halves' shift.
 // ---------------------------------------------------------------------------
 constexpr int kManyRows = 256;
 constexpr int kManyThreads = 512;
@@ -1087,7 +1091,8 @@ __device__ __forceinline__ const __attribute__((address_space(4))) T* as_constan
 
 // P goes in as two fp16 parts here too, which doubles the second product. With
 // one, results were up to 4.4 (bf16) and 1.6 (fp16) times their own rounding
-// away from 64 bits where few keys carry a row; with two they are not.
+// away from 64 bits where few keys carry a row; with two they are not. The
+// 501-token pieces took 303 us with one, 391 with two.
 template <int D>
 __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
   using M = Many<D>;
@@ -1461,7 +1466,8 @@ __global__ __launch_bounds__(kManyThreads) void attend_many(AttendArgs a) {
         // The workgroup's two halves, a wave of each on every SIMD, run half a
         // tile apart: while one multiplies, the other works out its weights.
         // Both pass the same barriers. Who multiplies issues first: its few
-        // vector instructions would hold its products up (340 against 322 us).
+        // vector instructions would hold its products up (340 against 322 us, P in
+        // one part).
         if (wave >= 4) lds_barrier();
         auto nothing = [](int) {};
         for (int tile = tile0; tile < tile1; ++tile) {
@@ -1582,15 +1588,16 @@ bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % 
 // Which kernels a call runs and what they need. Sequences of at most 128 rows
 // (queries times the group) are attend_few's, larger ones attend_many's. fp16,
 // head size 128, 8 heads, us of the two kernels at 64, 128 and 256 rows:
-//   64 sequences of 4000 keys   182 / 363   354 / 377   704 / 404
-//    8 sequences of 4000 keys    38 / 68     54 / 71     97 / 77
-//    1 sequence of 30000 keys    47 / 115    70 / 117   102 / 122
-//   64 sequences of 500 keys     32 / 59     61 / 66    114 / 79
+//   64 sequences of 4000 keys   181 / 348   356 / 364   709 / 394
+//    8 sequences of 4000 keys    38 / 64     55 / 68     98 / 74
+//    1 sequence of 30000 keys    48 / 114    82 / 116   156 / 121
+//   64 sequences of 500 keys     34 / 57     62 / 66    117 / 77
+// bf16 differs by 4% at most.
 // A call that by its sizes can have one kind alone runs one kernel, which then
 // takes every size. attend_few takes 32 rows at a time where sequences have
 // more than 16 and there are 32 sequences and heads to share the card (64 x 8,
-// 4000 keys, 64 rows: 182 us against 205 for 16 at a time); with fewer, pieces
-// of 16 rows are joined sooner (1 x 8, 30000 keys, 32 rows: 33 against 65).
+// 4000 keys, 64 rows: 181 us against 199 for 16 at a time); with fewer, pieces
+// of 16 rows are joined sooner (1 x 8, 30000 keys, 32 rows: 34 against 66).
 constexpr int kFewRows = 128;
 
 struct Dispatch {

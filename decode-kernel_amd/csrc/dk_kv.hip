@@ -142,12 +142,14 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
 // tokens fall into groups of 16 places of the page. A group's elements stay in
 // a wave's registers from the largest one's search to the codes' store, so
 // they are read once, and everything that a run needs is asked for at once
-// (elements, old scale, codes beside the new ones): two trips to memory after
-// the slots. A workgroup looks for runs that start among its `scan` tokens;
-// runs of few tokens or within one group go to its waves in turn, longer ones
-// to all of them. 8003 prompt tokens, 8 heads of 128, pages of 64: 49.5 MB in
-// 22 us (2.2 TB/s); 10 us would be the rate of a large copy. One wave a run,
-// with the elements read twice, took 53.
+// (elements, old scale, codes beside the new ones). Before that stand four loads
+// of slots, each waiting for the one before: a workgroup's own, those before
+// them, a run's first, those after it. A workgroup looks for runs that start
+// among its `scan` tokens; runs of few tokens or within one group go to its waves
+// in turn, longer ones to all of them. 8003 prompt tokens, 8 heads of 128, pages
+// of 64: 49.5 MB in 22 us (2.2 TB/s); 10 us would be the rate of a large copy, but
+// values are stored 8 or 16 bytes at a time, page_size apart, a page's rows in
+// pieces by several waves. One wave a run, with the elements read twice, took 53.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
   KvView c;
