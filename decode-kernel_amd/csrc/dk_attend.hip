@@ -244,9 +244,9 @@ __device__ __forceinline__ uint16_t* out_row(const AttendArgs& a, const Seq& s, 
 // 13 us, all of it such trips. With 32 rows and heads of 128 (NT 2) the state
 // takes 256 registers and 112 accumulation registers, one wave a SIMD, and part
 // of it moves between them in the loop; what is uniform and little used lies in
-// vector lanes here and in attend_many (30 to 56 scalar registers). Equal shares a workgroup instead of a wave, its
-// four waves on one item, took 50 us and more where short sequences stand
-// together, and a second launch to join 5 us more.
+// vector lanes here and in attend_many (30 to 56 scalar registers). Equal shares
+// a workgroup instead of a wave, its four waves on one item, took 50 us and more
+// where short sequences stand together, and a second launch to join 5 us more.
 // ---------------------------------------------------------------------------
 constexpr int kItemCost = 1;
 

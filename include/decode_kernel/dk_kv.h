@@ -72,8 +72,9 @@ typedef struct dk_kv_cache {
  * is not filled in later. After a shortage take the missing tokens off held
  * (down to the end of the last page that is there), or drop their requests, and
  * set the count to 0 before pages are put back from there; a negative one is
- * subtracted from what comes after it. Every result is a function of the inputs alone, so
- * the same call again gives the same. free_count_out must not be free_count. */
+ * subtracted from what comes after it. Every result is a function of the inputs
+ * alone, so the same call again gives the same. free_count_out must not be
+ * free_count. */
 int dk_kv_plan(int32_t* tables, int table_width, const int32_t* held, const int32_t* added,
                int requests, const int32_t* free_pages, int free_capacity,
                const int32_t* free_count, int page_size, int num_tokens, int64_t* slots,
@@ -84,8 +85,8 @@ int dk_kv_plan(int32_t* tables, int table_width, const int32_t* held, const int3
  * elements of tokens and heads, multiples of 8; 16-byte aligned) at slots.
  * Tokens of one page must stand together and in order, as dk_kv_plan gives
  * them (token t + i at slot s + i); slots outside the cache (-1) are skipped,
- * also among them. For each page and head that
- * the step writes, with amax over its new tokens:
+ * also among them. For each page and head that the step writes, with amax over
+ * its new tokens:
  *   scale = max(old scale, amax * (1 / 127))  (old scale 0 if token 0 of the
  *                                              page is among the new ones)
  *   inv = 1 / scale                           (0 for a scale under 2^-126,
@@ -116,9 +117,9 @@ size_t dk_kv_attend_workspace_bytes(int num_tokens, int requests, int q_heads, i
  * of t's sequence, heads hq / (q_heads / heads). Sequence b has seq_lens[b]
  * keys (at most table_width * page_size) and the queries
  * query_offsets[b] .. query_offsets[b + 1] - 1 (NULL: query b alone, and
- * num_tokens == requests; where offsets decrease, all of out is 0). With causal, query i of n sees the keys up to
- * seq_lens[b] - n + i: the queries are the sequence's last tokens, and their
- * keys are in the cache already. Keys on a page outside the cache (-1) are
+ * num_tokens == requests; where offsets decrease, all of out is 0). With causal,
+ * query i of n sees the keys up to seq_lens[b] - n + i: the queries are the
+ * sequence's last tokens, and their keys are in the cache already. Keys on a page outside the cache (-1) are
  * not seen. A query that sees no key gives 0, and so does one that belongs to no
  * sequence (before the first offset or from the last one on), which is not read.
  *
