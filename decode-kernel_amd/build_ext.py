@@ -35,7 +35,8 @@ ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 ARCH = os.environ.get("DK_OFFLOAD_ARCH", "gfx950")
 
 HIP_SOURCES = [CSRC / "dk_gemv.hip", CSRC / "dk_stream.hip", CSRC / "dk_quant.hip",
-               CSRC / "dk_kv.hip", CSRC / "dk_attend.hip"]
+               CSRC / "dk_kv.hip", CSRC / "dk_attend.hip", CSRC / "dk_delta.hip",
+               CSRC / "dk_delta_chunk.hip", CSRC / "dk_rotary.hip"]
 HIP_FLAGS = [
     f"--offload-arch={ARCH}",
     "-O3",

@@ -61,6 +61,7 @@ void check_gemv_inputs(const torch::Tensor& packed, const torch::Tensor& scales,
 }  // namespace
 
 #include "bindings_kv.hpp"
+#include "bindings_mixing.hpp"
 
 torch::Tensor gemv_common(const torch::Tensor& packed, const torch::Tensor& scales,
                           const torch::Tensor& x, int version, int split_k, bool reuse_weights, int warps_per_row);
@@ -393,5 +394,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("M"), py::arg("K"), py::arg("B"), py::arg("version") = 5, py::arg("split_k") = 4,
         py::arg("reuse_weights") = false, py::arg("warps_per_row") = 1);
   define_kv(m);
+  define_mixing(m);
   m.attr("ABI_VERSION") = dk_abi_version();
 }

@@ -1,0 +1,101 @@
+// Shared by the kernels of the gated delta rule and the short convolution.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "decode_kernel/dk_delta.h"
+#include "dk_kv.hpp"
+
+namespace dk {
+
+constexpr int kChunk = 64;           // tokens that the chunked form takes at once
+constexpr float kUnitEps = 1e-6f;    // added to a squared length
+// Below this a decay's exponential is 0 in fp32 (e^-128 < 2^-149): logarithms
+// are cut there, so that sums over a chunk stay finite and differences exact.
+constexpr float kLowestLog = -128.0f;
+
+// The decay's logarithm as it is summed: cut at kLowestLog, NaN kept.
+__device__ __forceinline__ float cut_log(float g) { return g < kLowestLog ? kLowestLog : g; }
+
+struct DeltaArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  long long q_token, q_head, k_token, k_head, v_token, v_head;
+  const float* log_decay;
+  const float* beta;
+  float* states;
+  const int32_t* held;
+  const int32_t* offsets;
+  uint16_t* out;
+  int tokens, requests, qk_heads, v_heads, group;
+  int limit;  // requests of up to so many tokens go one by one, longer ones in chunks
+  int normalize;
+  float scale;
+};
+
+// Whether offsets grow from at least 0 to at most `tokens`; by one wave.
+__device__ __forceinline__ bool wave_offsets_ok(const int32_t* offsets, int requests, int tokens) {
+  bool bad = false;
+  for (int i = threadIdx.x & 63; i < requests; i += 64) bad |= offsets[i + 1] < offsets[i];
+  if ((threadIdx.x & 63) == 0) bad |= offsets[0] < 0 || offsets[requests] > tokens;
+  return __ballot(bad) == 0;
+}
+
+// A tile of a request's new tokens. Tiles of `tile` tokens have numbers that
+// need no sum over the requests: request b's begin at offsets[b] / tile + b,
+// and since floor(x + n) - floor(x) + 1 >= ceil(n), they end before the next
+// request's do begin. tokens / tile + requests numbers are enough.
+struct Tile {
+  int request;  // -1: the number is nobody's
+  int row;      // its first row
+  int count;    // its rows
+  int index;    // which tile of its request
+};
+
+// By a whole workgroup: the tile with number `number`, and whether offsets
+// are good. shared: 2 ints.
+__device__ __forceinline__ bool find_tile(const int32_t* offsets, int requests, int tokens, int tile,
+                                          int number, int* shared, Tile* out) {
+  int begun = 0;  // requests whose tiles begin at or before the number
+  bool bad = false;
+  for (int i = threadIdx.x; i < requests; i += blockDim.x) {
+    const int from = offsets[i], to = offsets[i + 1];
+    bad |= to < from;
+    begun += from / tile + i <= number;
+  }
+  if (threadIdx.x == 0) {
+    bad |= offsets[0] < 0 || offsets[requests] > tokens;
+    shared[0] = 0;
+    shared[1] = 0;
+  }
+  __syncthreads();
+  const unsigned long long any = __ballot(bad);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) begun += __shfl_xor(begun, d);
+  if ((threadIdx.x & 63) == 0) {
+    atomicAdd(&shared[0], begun);
+    if (any) atomicOr(&shared[1], 1);
+  }
+  __syncthreads();
+  out->request = -1;
+  out->row = out->count = out->index = 0;
+  if (shared[1]) return false;
+  const int b = shared[0] - 1;
+  if (b < 0) return true;
+  const int from = offsets[b], n = offsets[b + 1] - from;
+  const int index = number - (from / tile + b);
+  if ((long long)index * tile >= n) return true;
+  out->request = b;
+  out->row = from + index * tile;
+  out->count = min(tile, n - index * tile);
+  out->index = index;
+  return true;
+}
+
+size_t delta_chunk_bytes(int num_tokens, int requests, int qk_heads, int v_heads, int key_size);
+int delta_chunk_launch(const DeltaArgs& a, int key_size, int value_size, bool bf16, void* workspace,
+                       hipStream_t stream);
+
+}  // namespace dk

@@ -11,7 +11,11 @@ Llama-style MLP decode step on the same kernels (include/decode_kernel/dk_mlp.h)
 `repack_paired` / `gemv_paired` (decode_kernel.layout) use the kernel-native
 paired weight layout. `KVCache`, `plan_kv_step`, `append_kv`, `read_kv` and
 `attend_kv` (decode_kernel.kv) are the paged 8-bit key/value cache and the
-attention over it (include/decode_kernel/dk_kv.h).
+attention over it (include/decode_kernel/dk_kv.h). `delta_rule` and
+`short_conv` (decode_kernel.delta, include/decode_kernel/dk_delta.h) are the
+same place of a layer that keeps a state of fixed size, `Rotary` and
+`rotate_qk` (decode_kernel.rotary, include/decode_kernel/dk_rotary.h) the
+positions of queries and keys.
 """
 
 from __future__ import annotations
@@ -21,19 +25,23 @@ from typing import Optional
 import torch
 
 from ._native import ext as _ext
+from .delta import delta_rule, short_conv
 from .kv import KVCache, KVStep, append_kv, attend_kv, plan_kv_step, read_kv
 from .layout import gemv_paired, repack_paired, unpack_paired
 from .mlp import QuantizedMLP, gate_up_silu, mlp_decode
 from .quantize import GROUP_SIZE, dequantize, quantize_and_pack
+from .rotary import Rotary, rotate_qk
 
 __all__ = [
     "GROUP_SIZE",
     "KVCache",
     "KVStep",
     "QuantizedMLP",
+    "Rotary",
     "append_kv",
     "attend_kv",
     "cuda_available",
+    "delta_rule",
     "dequantize",
     "gate_up_silu",
     "gemv",
@@ -43,6 +51,8 @@ __all__ = [
     "quantize_and_pack",
     "read_kv",
     "repack_paired",
+    "rotate_qk",
+    "short_conv",
     "unpack_paired",
     "w4a16_linear",
 ]

@@ -1,4 +1,5 @@
-"""ctypes view of the C ABI in include/decode_kernel/dk_gemv.h, dk_mlp.h and dk_kv.h.
+"""ctypes view of the C ABI in include/decode_kernel/dk_gemv.h, dk_mlp.h, dk_kv.h,
+dk_delta.h and dk_rotary.h.
 
 This is the binding a non-torch host (or a maintainer wiring the library into
 another runtime) would write: plain pointers, sizes and a hipStream_t handle.
@@ -54,6 +55,19 @@ class KvCache(ctypes.Structure):
         ("heads", ctypes.c_int),
         ("head_size", ctypes.c_int),
         ("page_size", ctypes.c_int),
+    ]
+
+
+class DeltaArgs(ctypes.Structure):
+    """Mirror of dk_delta_args."""
+
+    _fields_ = [
+        *((name, ctypes.c_void_p) for name in ("q", "k", "v")),
+        *((f"{name}_{of}_stride", ctypes.c_longlong) for name in ("q", "k", "v") for of in ("token", "head")),
+        *((name, ctypes.c_void_p) for name in ("log_decay", "beta", "states", "held", "offsets")),
+        *((name, ctypes.c_int) for name in ("dtype", "num_tokens", "requests", "qk_heads", "v_heads", "key_size",
+                                            "value_size", "max_query_len", "normalize")),
+        ("scale", ctypes.c_float),
     ]
 
 
@@ -142,6 +156,20 @@ _SIGNATURES = {
         [_P, ctypes.c_int, ctypes.c_longlong, ctypes.c_longlong, ctypes.POINTER(KvCache), _P,
          ctypes.c_int, _P, _P, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
          ctypes.c_float, ctypes.c_int, _P, _P, ctypes.c_size_t, _P],
+    ),
+    "dk_delta_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 6),
+    "dk_delta_rule": (
+        ctypes.c_int, [ctypes.POINTER(DeltaArgs), _P, _P, ctypes.c_size_t, _P],
+    ),
+    "dk_short_conv": (
+        ctypes.c_int,
+        [_P, ctypes.c_longlong, _P, _P, _P, _P, _P, *[ctypes.c_int] * 7, _P, _P],
+    ),
+    "dk_rotate_qk": (
+        ctypes.c_int,
+        [*[_P, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_int] * 2, ctypes.c_int, ctypes.c_int,
+         ctypes.c_int, _P, ctypes.c_int, ctypes.c_int, _P, _P, ctypes.c_int, ctypes.c_int,
+         ctypes.c_int, _P, _P, _P],
     ),
     "dk_d2d_copy": (ctypes.c_int, [_P, _P, ctypes.c_size_t, _P]),
     "dk_stream_read": (ctypes.c_int, [_P, _P, ctypes.c_size_t, ctypes.c_int, _P]),
