@@ -95,10 +95,11 @@ __device__ __forceinline__ float power2(int e) {  // -126 <= e <= 127
   return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23);
 }
 
-// x as two fp16 parts.
-__device__ __forceinline__ void split2(float x, _Float16* hi, _Float16* lo) {
-  *hi = (_Float16)x;
-  *lo = (_Float16)(x - (float)*hi);
+// x * scale as two fp16 parts, each of one rounding.
+__device__ __forceinline__ void split2(float x, float scale, _Float16* hi, _Float16* lo) {
+  const _Float16 h = (_Float16)(x * scale);
+  *hi = h;
+  *lo = (_Float16)fmaf(x, scale, -(float)h);
 }
 
 // The power of two that brings a column's largest (over this lane's values and
@@ -118,10 +119,10 @@ __device__ __forceinline__ void split_tiles(f4_t x, f4_t y, float scale, h8_t* h
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     _Float16 h, l;
-    split2(x[j] * scale, &h, &l);
+    split2(x[j], scale, &h, &l);
     (*hi)[j] = h;
     (*lo)[j] = l;
-    split2(y[j] * scale, &h, &l);
+    split2(y[j], scale, &h, &l);
     (*hi)[4 + j] = h;
     (*lo)[4 + j] = l;
   }
@@ -361,153 +362,269 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, ChunkSp
 }
 
 // ---------------------------------------------------------------------------
-// One wave 16 columns of one head's state, through a request's chunks.
+// A request's chunks one after another, 32 columns of one head's state a
+// workgroup. Waves 0 and 1 hold 16 columns each and go from state to state;
+// columns do not meet, and a result tile is the next product's operand B, so
+// nothing but the prepared operands comes from outside a wave. Waves 2 and 3
+// compute the same columns' outputs one chunk behind, from the parts of the
+// state and of the corrections that waves 0 and 1 leave in LDS, and bring the
+// next chunk's operands there: what only the outputs need is off the chain
+// that bounds a long prompt.
 // ---------------------------------------------------------------------------
+constexpr int kScanTiles = 2;  // tiles of 16 columns a workgroup holds
+
+using lds_ptr = __attribute__((address_space(3))) void*;
+using global_ptr = __attribute__((address_space(1))) const void*;
+
 template <int kDk, bool kBf16>
-__global__ __launch_bounds__(64, 1) void delta_scan_kernel(DeltaArgs a, ChunkSpace ws, int value_size) {
+__global__ __launch_bounds__(256, 1) void delta_scan_kernel(DeltaArgs a, ChunkSpace ws, int value_size) {
   constexpr int kS = kDk / 32, kTiles = kDk / 16;
   constexpr int kType = kBf16 ? DK_KV_BF16 : DK_KV_F16;
+  constexpr int kKeys = 4 * kS, kInverse = 2 * kFragments, kTurned = 2 * kTiles;  // pieces of 1 KB
   constexpr f4_t kZero{0.f, 0.f, 0.f, 0.f};
-  const int lane = threadIdx.x, i = lane & 15, q4 = lane >> 4;
+  __shared__ h8_t stage[2][kKeys + kInverse + kTurned][64];
+  __shared__ h8_t left_s[2][kScanTiles][2 * kS][64];  // the state's parts
+  __shared__ h8_t left_w[2][kScanTiles][4][64];       // the corrections'
+  __shared__ float left_scale[2][kScanTiles][2][16];  // what both are divided by
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q4 = lane >> 4;
+  const int tile = wave & 1;
   const int h = blockIdx.x % a.v_heads, hq = h / a.group, b = blockIdx.y;
-  const int col = (blockIdx.x / a.v_heads) * 16 + i;
+  const int col = ((blockIdx.x / a.v_heads) * kScanTiles + tile) * 16 + i;
   if (!wave_offsets_ok(a.offsets, a.requests, a.tokens)) return;
   const int from = a.offsets[b], n = a.offsets[b + 1] - from;
   if (n <= a.limit) return;
   const long long slot0 = from / kChunk + b;
-
-  float* state = a.states + ((long long)b * a.v_heads + h) * kDk * value_size + col;
-  f4_t s[kTiles];
-  const bool fresh = a.held && a.held[b] <= 0;
-#pragma unroll
-  for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[t][e] = fresh ? 0.f : state[(long long)(16 * t + 4 * q4 + e) * value_size];
-
   const int chunks = (n + kChunk - 1) / kChunk;
-  for (int c = 0; c < chunks; ++c) {
-    const long long slot = slot0 + c;
-    const int row0 = from + c * kChunk, count = min(kChunk, n - c * kChunk);
-    const size_t qk_at = (slot * a.qk_heads + hq) * (4 * kS * 64) + lane;
-    const size_t v_at = (slot * a.v_heads + h) * (kFragments * 2 * 64) + lane;
-    const float* f = ws.s + (slot * a.v_heads + h) * (kFactors * kChunk);
+  const size_t qk_step = (size_t)a.qk_heads * (4 * kS * 64), v_step = (size_t)a.v_heads * (kInverse * 64);
+  const h8_t* ks = ws.k + slot0 * qk_step + (size_t)hq * (4 * kS * 64) + lane;
+  const h8_t* kts = ws.kt + slot0 * qk_step + (size_t)hq * (4 * kS * 64) + lane;
+  const h8_t* ts = ws.t + slot0 * v_step + (size_t)h * (kInverse * 64) + lane;
+  const float* factors = ws.s + (slot0 * a.v_heads + h) * (kFactors * kChunk) + 4 * q4;
+  const size_t f_step = (size_t)a.v_heads * (kFactors * kChunk);
+  auto rows4 = [&](int c, int which, int y) {
+    return *reinterpret_cast<const f4_t*>(factors + c * f_step + which * kChunk + 16 * y);
+  };
 
-    // K' S and Q' S.
-    float m = 0.f;
+  // Both output waves bring half of chunk c's operands.
+  auto bring = [&](int c) {
+    h8_t* to = &stage[c & 1][0][0];
+    auto one = [&](const h8_t* src, int piece) {
+      __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(to + piece * 64), 16, 0, 0);
+    };
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) m = max4(m, s[t]);
-    int shift = column_shift(m);
-    float up = power2(shift), down = power2(-shift);
-    f4_t x[4] = {kZero, kZero, kZero, kZero}, o[4] = {kZero, kZero, kZero, kZero};
+    for (int p = 0; p < kKeys; p += 2) one(ks + c * qk_step + (p + tile) * 64, p + tile);
 #pragma unroll
-    for (int t = 0; t < kS; ++t) {
-      h8_t hi, lo;
-      split_tiles(s[2 * t], s[2 * t + 1], up, &hi, &lo);
+    for (int p = 0; p < kInverse; p += 2) one(ts + c * v_step + (p + tile) * 64, kKeys + p + tile);
+#pragma unroll
+    for (int p = 0; p < kTurned; p += 2)
+      one(kts + c * qk_step + (p + tile) * 64, kKeys + kInverse + p + tile);
+  };
+
+  if (wave < 2) {
+    float* state = a.states + ((long long)b * a.v_heads + h) * kDk * value_size + col;
+    f4_t s[kTiles];
+    const bool fresh = a.held && a.held[b] <= 0;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[t][e] = fresh ? 0.f : state[(long long)(16 * t + 4 * q4 + e) * value_size];
+    const uint16_t* values = a.v + (long long)from * a.v_token + (long long)h * a.v_head + col;
+    // A chunk's rows are loaded as soon as those of the chunk before are used.
+    uint16_t v[16];
+    f4_t b1[4], b2[4], until[4];
+    auto load_values = [&](int c) {
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
-        const h8_t kf = ws.k[qk_at + (y * kS + t) * 64], qf = ws.q[qk_at + (y * kS + t) * 64];
-        x[y] = mfma(kf, hi, x[y]);
-        x[y] = mfma(kf, lo, x[y]);
-        o[y] = mfma(qf, hi, o[y]);
-        o[y] = mfma(qf, lo, o[y]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)  // past the last token, where b1 and b2 are 0, that one again
+          v[4 * y + e] = values[(long long)min(c * kChunk + 16 * y + 4 * q4 + e, n - 1) * a.v_token];
+        b1[y] = rows4(c, 0, y);
+        b2[y] = rows4(c, 1, y);
+      }
+    };
+    float whole;
+    auto load_until = [&](int c) {
+#pragma unroll
+      for (int y = 0; y < 4; ++y) until[y] = rows4(c, 4, y);
+      whole = factors[c * f_step + 5 * kChunk];
+    };
+    load_values(0);
+    load_until(0);
+    for (int c = 0; c <= chunks; ++c) {
+      __syncthreads();  // chunk c's operands are there, and chunk c - 2's parts read
+      if (c == chunks) break;
+      const int after = min(c + 1, chunks - 1);
+      const h8_t(*keys)[64] = &stage[c & 1][0];
+      const h8_t(*inverse)[64] = &stage[c & 1][kKeys];
+      const h8_t(*turned)[64] = &stage[c & 1][kKeys + kInverse];
+
+      // K' S.
+      float m = 0.f;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) m = max4(m, s[t]);
+      int shift = column_shift(m);
+      float up = power2(shift), down = power2(-shift);
+      if (q4 == 0) left_scale[c & 1][tile][0][i] = down;
+      f4_t x[4] = {kZero, kZero, kZero, kZero};
+#pragma unroll
+      for (int t = 0; t < kS; ++t) {
+        h8_t hi, lo;
+        split_tiles(s[2 * t], s[2 * t + 1], up, &hi, &lo);
+        left_s[c & 1][tile][2 * t][lane] = hi;
+        left_s[c & 1][tile][2 * t + 1][lane] = lo;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) x[y] = mfma(keys[y * kS + t][lane], hi, x[y]);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) x[y] = mfma(keys[y * kS + t][lane], lo, x[y]);
+      }
+      // What each token finds wrong in the state before the chunk.
+      m = 0.f;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          x[y][e] = b1[y][e] * pair_lo<kBf16>(v[4 * y + e]) - b2[y][e] * (down * x[y][e]);
+        m = max4(m, x[y]);
+      }
+      load_values(after);
+      // The corrections w = T x.
+      shift = column_shift(m);
+      up = power2(shift);
+      down = power2(-shift) / kInverseScale;
+      h8_t hi[2], lo[2];
+      split_tiles(x[0], x[1], up, &hi[0], &lo[0]);
+      split_tiles(x[2], x[3], up, &hi[1], &lo[1]);
+      f4_t w[4] = {kZero, kZero, kZero, kZero};
+#pragma unroll
+      for (int part = 0; part < 3; ++part)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int y = 2 * t; y < 4; ++y) {
+            const int piece = (y == 0 ? 0 : y == 1 ? 1 : y == 2 ? 2 : 4) + t;
+            w[y] = mfma(inverse[2 * piece + (part == 2)][lane], part == 1 ? lo[t] : hi[t], w[y]);
+          }
+      float m2 = 0.f;
+      f4_t w2[4];
+      m = 0.f;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        w[y] *= down;
+        w2[y] = w[y] * until[y];
+        m = max4(m, w[y]);
+        m2 = max4(m2, w2[y]);
+      }
+      // The state after the chunk.
+      shift = column_shift(m2);
+      up = power2(shift);
+      down = power2(-shift);
+      split_tiles(w2[0], w2[1], up, &hi[0], &lo[0]);
+      split_tiles(w2[2], w2[3], up, &hi[1], &lo[1]);
+#pragma unroll
+      for (int t = 0; t < kTiles; t += 4) {
+        f4_t add[4] = {kZero, kZero, kZero, kZero};
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+#pragma unroll
+          for (int z = 0; z < 4; ++z) add[z] = mfma(turned[2 * (t + z) + y][lane], hi[y], add[z]);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) add[z] = mfma(turned[2 * (t + z) + y][lane], lo[y], add[z]);
+        }
+#pragma unroll
+        for (int z = 0; z < 4; ++z)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[t + z][e] = fmaf(add[z][e], down, whole * s[t + z][e]);
+      }
+      load_until(after);
+      // The corrections for the outputs.
+      shift = column_shift(m);
+      up = power2(shift);
+      if (q4 == 0) left_scale[c & 1][tile][1][i] = power2(-shift) / kScoreScale;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        split_tiles(w[2 * t], w[2 * t + 1], up, &hi[t], &lo[t]);
+        left_w[c & 1][tile][2 * t][lane] = hi[t];
+        left_w[c & 1][tile][2 * t + 1][lane] = lo[t];
       }
     }
-    // What each token finds wrong in the state before the chunk.
-    m = 0.f;
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const f4_t b1 = *reinterpret_cast<const f4_t*>(f + 16 * y + 4 * q4);
-      const f4_t b2 = *reinterpret_cast<const f4_t*>(f + 64 + 16 * y + 4 * q4);
-      const f4_t since = *reinterpret_cast<const f4_t*>(f + 128 + 16 * y + 4 * q4);
+    for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 16 * y + 4 * q4 + e;
-        float v = 0.f;
-        if (r < count) v = pair_lo<kBf16>(a.v[(long long)(row0 + r) * a.v_token + (long long)h * a.v_head + col]);
-        x[y][e] = b1[e] * v - b2[e] * (down * x[y][e]);
-        o[y][e] *= since[e] * down;
+      for (int e = 0; e < 4; ++e) state[(long long)(16 * t + 4 * q4 + e) * value_size] = s[t][e];
+  } else {
+    const h8_t* qs = ws.q + slot0 * qk_step + (size_t)hq * (4 * kS * 64) + lane;
+    const h8_t* ps = ws.p + slot0 * v_step + (size_t)h * (kInverse * 64) + lane;
+    uint16_t* out = a.out + ((long long)from * a.v_heads + h) * value_size + col;
+    const long long out_token = (long long)a.v_heads * value_size;
+    struct Operands {
+      h8_t q[kKeys], p[kInverse];
+      f4_t since[4], d[4];
+    };
+    auto load = [&](int c) {
+      Operands o;
+#pragma unroll
+      for (int p = 0; p < kKeys; ++p) o.q[p] = qs[c * qk_step + p * 64];
+#pragma unroll
+      for (int p = 0; p < kInverse; ++p) o.p[p] = ps[c * v_step + p * 64];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        o.since[y] = rows4(c, 2, y);
+        o.d[y] = rows4(c, 3, y);
       }
-      m = max4(m, x[y]);
-    }
-    // The corrections w.
-    shift = column_shift(m);
-    up = power2(shift);
-    h8_t hi[2], lo[2];
-    split_tiles(x[0], x[1], up, &hi[0], &lo[0]);
-    split_tiles(x[2], x[3], up, &hi[1], &lo[1]);
-    down = power2(-shift) / kInverseScale;
-    f4_t w[4] = {kZero, kZero, kZero, kZero};
-    m = 0.f;
+      return o;
+    };
+    // Outputs of chunk c - 1, whose operands are in `now`; chunk c's go to `next`.
+    auto outputs = [&](int c, const Operands& now, Operands& next) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // bring()'s pieces are in LDS
+      __syncthreads();
+      h8_t sp[2 * kS], wp[4];
+      float down_s = 0.f, down_w = 0.f;
+      const int at = c - 1;
+      if (c > 0) {
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
+        for (int t = 0; t < 2 * kS; ++t) sp[t] = left_s[at & 1][tile][t][lane];
 #pragma unroll
-      for (int t = 0; t <= y / 2; ++t) {
-        const int piece = (y == 0 ? 0 : y == 1 ? 1 : y == 2 ? 2 : 4) + t;
-        const h8_t th = ws.t[v_at + (2 * piece) * 64], tl = ws.t[v_at + (2 * piece + 1) * 64];
-        w[y] = mfma(th, hi[t], w[y]);
-        w[y] = mfma(th, lo[t], w[y]);
-        w[y] = mfma(tl, hi[t], w[y]);
+        for (int t = 0; t < 4; ++t) wp[t] = left_w[at & 1][tile][t][lane];
+        down_s = left_scale[at & 1][tile][0][i];
+        down_w = left_scale[at & 1][tile][1][i];
       }
-      w[y] *= down;
-      m = max4(m, w[y]);
-    }
-    // Out.
-    shift = column_shift(m);
-    up = power2(shift);
-    down = power2(-shift) / kScoreScale;
-    split_tiles(w[0], w[1], up, &hi[0], &lo[0]);
-    split_tiles(w[2], w[3], up, &hi[1], &lo[1]);
+      if (c + 1 < chunks) bring(c + 1);
+      if (c < chunks) next = load(c);
+      if (c == 0) return;
+      f4_t x[4] = {kZero, kZero, kZero, kZero}, y2[4] = {kZero, kZero, kZero, kZero};
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const f4_t d = *reinterpret_cast<const f4_t*>(f + 192 + 16 * y + 4 * q4);
-      f4_t p = kZero;
+      for (int t = 0; t < kS; ++t) {
 #pragma unroll
-      for (int t = 0; t <= y / 2; ++t) {
-        const int piece = (y == 0 ? 0 : y == 1 ? 1 : y == 2 ? 2 : 4) + t;
-        const h8_t ph = ws.p[v_at + (2 * piece) * 64], pl = ws.p[v_at + (2 * piece + 1) * 64];
-        p = mfma(ph, hi[t], p);
-        p = mfma(ph, lo[t], p);
-        p = mfma(pl, hi[t], p);
+        for (int y = 0; y < 4; ++y) x[y] = mfma(now.q[y * kS + t], sp[2 * t], x[y]);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) x[y] = mfma(now.q[y * kS + t], sp[2 * t + 1], x[y]);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 16 * y + 4 * q4 + e;
-        if (r < count)
-          a.out[((long long)(row0 + r) * a.v_heads + h) * value_size + col] =
-              to_half_bits<kType>(d[e] * fmaf(p[e], down, o[y][e]));
-      }
-    }
-    // The state after the chunk.
-    m = 0.f;
+      for (int part = 0; part < 3; ++part)
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const f4_t until = *reinterpret_cast<const f4_t*>(f + 256 + 16 * y + 4 * q4);
-      w[y] *= until;
-      m = max4(m, w[y]);
-    }
-    shift = column_shift(m);
-    up = power2(shift);
-    down = power2(-shift);
-    split_tiles(w[0], w[1], up, &hi[0], &lo[0]);
-    split_tiles(w[2], w[3], up, &hi[1], &lo[1]);
-    const float whole = f[320];
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      f4_t add = kZero;
+          for (int y = 2 * t; y < 4; ++y) {
+            const int piece = (y == 0 ? 0 : y == 1 ? 1 : y == 2 ? 2 : 4) + t;
+            y2[y] = mfma(now.p[2 * piece + (part == 2)], wp[2 * t + (part == 1)], y2[y]);
+          }
+      const int count = n - at * kChunk;
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const h8_t kt = ws.kt[qk_at + (2 * t + y) * 64];
-        add = mfma(kt, hi[y], add);
-        add = mfma(kt, lo[y], add);
-      }
+      for (int y = 0; y < 4; ++y)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[t][e] = fmaf(add[e], down, whole * s[t][e]);
+        for (int e = 0; e < 4; ++e) {
+          const int row = 16 * y + 4 * q4 + e;
+          const float o = now.d[y][e] * fmaf(y2[y][e], down_w, now.since[y][e] * down_s * x[y][e]);
+          if (row < count) out[(long long)(at * kChunk + row) * out_token] = to_half_bits<kType>(o);
+        }
+    };
+    bring(0);
+    Operands even, odd;  // of chunks c - 1 and c, in turn
+    for (int c = 0; c <= chunks; c += 2) {
+      outputs(c, odd, even);
+      if (c + 1 <= chunks) outputs(c + 1, even, odd);
     }
   }
-#pragma unroll
-  for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) state[(long long)(16 * t + 4 * q4 + e) * value_size] = s[t][e];
 }
 
 }  // namespace
@@ -523,10 +640,10 @@ int delta_chunk_launch(const DeltaArgs& a, int key_size, int value_size, bool bf
   size_t bytes;
   const ChunkSpace ws = chunk_space(workspace, a.tokens, a.requests, a.qk_heads, a.v_heads, key_size, &bytes);
   const dim3 chunks((unsigned)(slots_of(a.tokens, a.requests) * a.v_heads));
-  const dim3 columns((unsigned)(a.v_heads * (value_size / 16)), (unsigned)a.requests);
+  const dim3 columns((unsigned)(a.v_heads * (value_size / (16 * kScanTiles))), (unsigned)a.requests);
   auto launch = [&](auto prepare, auto scan) {
     hipLaunchKernelGGL(prepare, chunks, dim3(256), 0, stream, a, ws);
-    hipLaunchKernelGGL(scan, columns, dim3(64), 0, stream, a, ws, value_size);
+    hipLaunchKernelGGL(scan, columns, dim3(256), 0, stream, a, ws, value_size);
   };
   if (key_size == 64)
     bf16 ? launch(delta_prepare_kernel<64, true>, delta_scan_kernel<64, true>)
