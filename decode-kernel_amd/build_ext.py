@@ -53,6 +53,11 @@ HIP_FLAGS = [
     "-Wno-unused-command-line-argument",
 ]
 
+# Flags that one source alone is compiled with. The chunked delta rule's scan
+# works on its products' results between them: kept in VGPRs, not in the
+# accumulation registers, they need no copies (64 a chunk of 600 instructions).
+SOURCE_FLAGS = {"dk_delta_chunk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+
 LIB = PKG / "libdk_hip.so"
 # Measurement-only kernels (read-floor probes, the load-only ablation, the
 # one-stage and split-K shape variants): dk_bench/libdk_bench.so, never
@@ -82,8 +87,17 @@ def hipcc() -> str:
 
 def build_lib() -> Path:
     tmp = LIB.with_suffix(".so.tmp")
-    _run([hipcc(), *HIP_FLAGS, "-shared", f"-I{INCLUDE}", f"-I{CSRC}",
-          *map(str, HIP_SOURCES), "-o", str(tmp)],
+    BUILD.mkdir(exist_ok=True)
+    objects = []
+    for src in HIP_SOURCES:
+        if src.name not in SOURCE_FLAGS:
+            continue
+        objects.append(BUILD / (src.stem + ".o"))
+        _run([hipcc(), *HIP_FLAGS, *SOURCE_FLAGS[src.name], f"-I{INCLUDE}", f"-I{CSRC}", "-c", str(src),
+              "-o", str(objects[-1])],
+             quiet_warning="packed-fp32-ops' is not a recognized feature")
+    _run([hipcc(), *HIP_FLAGS, "-shared", f"-I{INCLUDE}", f"-I{CSRC}", *map(str, objects),
+          *(str(src) for src in HIP_SOURCES if src.name not in SOURCE_FLAGS), "-o", str(tmp)],
          quiet_warning="packed-fp32-ops' is not a recognized feature")
     os.replace(tmp, LIB)
     return LIB
@@ -103,7 +117,7 @@ def build_asm() -> list[Path]:
     outs = []
     for src in HIP_SOURCES:
         out = BUILD / (src.stem + f"-{ARCH}.s")
-        _run([hipcc(), *HIP_FLAGS, "--cuda-device-only", "-S", f"-I{INCLUDE}", f"-I{CSRC}",
+        _run([hipcc(), *HIP_FLAGS, *SOURCE_FLAGS.get(src.name, []), "--cuda-device-only", "-S", f"-I{INCLUDE}", f"-I{CSRC}",
               str(src), "-o", str(out)],
              quiet_warning="packed-fp32-ops' is not a recognized feature")
         outs.append(out)

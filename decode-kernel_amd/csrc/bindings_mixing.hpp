@@ -57,7 +57,10 @@ torch::Tensor delta_rule(const torch::Tensor& q, const torch::Tensor& k, const t
   a.offsets = offsets ? kv_ints(*offsets, B + 1, device, "query_offsets") : nullptr;
   c10::DeviceGuard guard(device);
   auto out = torch::empty({T, Hv, dv}, v.options());
-  const auto qr = kv_rows(q), kr = kv_rows(k), vr = kv_rows(v);
+  auto rows = [](const torch::Tensor& t) {  // rows too far apart to be counted in 32 bits are copied, too
+    return t.stride(0) > 1 << 24 ? t.clone(at::MemoryFormat::Contiguous) : kv_rows(t);
+  };
+  const auto qr = rows(q), kr = rows(k), vr = rows(v);
   a.q = qr.data_ptr();
   a.k = kr.data_ptr();
   a.v = vr.data_ptr();

@@ -362,6 +362,9 @@ extern "C" int dk_delta_rule(const dk_delta_args* p, void* out, void* workspace,
   if (p->q_token_stride % 8 || p->q_head_stride % 8 || p->k_token_stride % 8 ||
       p->k_head_stride % 8 || p->v_token_stride % 8 || p->v_head_stride % 8)
     return dk::set_error(DK_ERR_INVALID_ARGUMENT, "the strides of q, k and v must be multiples of 8");
+  for (const long long stride : {p->q_token_stride, p->k_token_stride, p->v_token_stride})
+    if (stride < 0 || stride > 1 << 24)  // 64 of them are counted in 32 bits
+      return dk::set_error(DK_ERR_INVALID_ARGUMENT, "the token strides of q, k and v must be in [0, 2^24]");
   // Without offsets a request has one token whatever max_query_len says.
   const bool chunks = p->offsets && p->max_query_len > dk::kStepTokens && p->requests > 0;
   const size_t need = chunks ? dk_delta_workspace_bytes(p->num_tokens, p->requests, p->qk_heads, p->v_heads,

@@ -95,36 +95,35 @@ __device__ __forceinline__ float power2(int e) {  // -126 <= e <= 127
   return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23);
 }
 
-// x * scale as two fp16 parts, each of one rounding.
-__device__ __forceinline__ void split2(float x, float scale, _Float16* hi, _Float16* lo) {
-  const _Float16 h = (_Float16)(x * scale);
-  *hi = h;
-  *lo = (_Float16)fmaf(x, scale, -(float)h);
+// The largest over the lanes l, l + 16, l + 32 and l + 48.
+__device__ __forceinline__ float max_rows(float m) {
+  const uint32_t x = __builtin_bit_cast(uint32_t, m);
+  const auto p = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  const float y = fmaxf(__builtin_bit_cast(float, (uint32_t)p[0]), __builtin_bit_cast(float, (uint32_t)p[1]));
+  const uint32_t z = __builtin_bit_cast(uint32_t, y);
+  const auto q = __builtin_amdgcn_permlane32_swap(z, z, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)q[0]), __builtin_bit_cast(float, (uint32_t)q[1]));
 }
 
 // The power of two that brings a column's largest (over this lane's values and
 // those of the lanes 16, 32 and 48 away) to 2^14 .. 2^15, as an exponent.
-__device__ __forceinline__ int column_shift(float m) {
-  m = fmaxf(m, __shfl_xor(m, 16));
-  m = fmaxf(m, __shfl_xor(m, 32));
-  return min(14 - exponent_of(m), 126);
-}
+__device__ __forceinline__ int column_shift(float m) { return min(14 - exponent_of(max_rows(m)), 126); }
 
 __device__ __forceinline__ float max4(float m, f4_t x) {
-  return fmaxf(fmaxf(m, fmaxf(fabsf(x[0]), fabsf(x[1]))), fmaxf(fabsf(x[2]), fabsf(x[3])));
+  m = fmaxf(fmaxf(m, fabsf(x[0])), fabsf(x[1]));
+  return fmaxf(fmaxf(m, fabsf(x[2])), fabsf(x[3]));
 }
 
-// Two stacked result tiles as an operand B of 32 rows, in two parts.
+// Two stacked result tiles times a power of two as an operand B of 32 rows, in
+// two fp16 parts of one rounding each.
 __device__ __forceinline__ void split_tiles(f4_t x, f4_t y, float scale, h8_t* hi, h8_t* lo) {
+  const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    _Float16 h, l;
-    split2(x[j], scale, &h, &l);
+  for (int j = 0; j < 8; ++j) {
+    // As one instruction of mixed width, not a product and a conversion.
+    const _Float16 h = (_Float16)fmaf(v[j], scale, 0.f);
     (*hi)[j] = h;
-    (*lo)[j] = l;
-    split2(y[j], scale, &h, &l);
-    (*hi)[4 + j] = h;
-    (*lo)[4 + j] = l;
+    (*lo)[j] = (_Float16)fmaf(v[j], scale, -(float)h);
   }
 }
 
@@ -374,10 +373,19 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, ChunkSp
 constexpr int kScanTiles = 2;  // tiles of 16 columns a workgroup holds
 
 using lds_ptr = __attribute__((address_space(3))) void*;
-using global_ptr = __attribute__((address_space(1))) const void*;
+
+// Buffers: a chunk's rows behind the request's last are out of their range, so
+// that they load zeros and store nothing.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
+}
+
+__device__ __forceinline__ h8_t load_piece(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
+  return __builtin_bit_cast(h8_t, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0));
+}
 
 template <int kDk, bool kBf16>
-__global__ __launch_bounds__(256, 1) void delta_scan_kernel(DeltaArgs a, ChunkSpace ws, int value_size) {
+__global__ __launch_bounds__(256, 1) __attribute__((amdgpu_num_vgpr(256))) void delta_scan_kernel(DeltaArgs a, ChunkSpace ws, int value_size) {
   constexpr int kS = kDk / 32, kTiles = kDk / 16;
   constexpr int kType = kBf16 ? DK_KV_BF16 : DK_KV_F16;
   constexpr int kKeys = 4 * kS, kInverse = 2 * kFragments, kTurned = 2 * kTiles;  // pieces of 1 KB
@@ -386,7 +394,8 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(DeltaArgs a, ChunkSp
   __shared__ h8_t left_s[2][kScanTiles][2 * kS][64];  // the state's parts
   __shared__ h8_t left_w[2][kScanTiles][4][64];       // the corrections'
   __shared__ float left_scale[2][kScanTiles][2][16];  // what both are divided by
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, i = lane & 15, q4 = lane >> 4;
   const int tile = wave & 1;
   const int h = blockIdx.x % a.v_heads, hq = h / a.group, b = blockIdx.y;
   const int col = ((blockIdx.x / a.v_heads) * kScanTiles + tile) * 16 + i;
@@ -395,29 +404,36 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(DeltaArgs a, ChunkSp
   if (n <= a.limit) return;
   const long long slot0 = from / kChunk + b;
   const int chunks = (n + kChunk - 1) / kChunk;
-  const size_t qk_step = (size_t)a.qk_heads * (4 * kS * 64), v_step = (size_t)a.v_heads * (kInverse * 64);
-  const h8_t* ks = ws.k + slot0 * qk_step + (size_t)hq * (4 * kS * 64) + lane;
-  const h8_t* kts = ws.kt + slot0 * qk_step + (size_t)hq * (4 * kS * 64) + lane;
-  const h8_t* ts = ws.t + slot0 * v_step + (size_t)h * (kInverse * 64) + lane;
-  const float* factors = ws.s + (slot0 * a.v_heads + h) * (kFactors * kChunk) + 4 * q4;
-  const size_t f_step = (size_t)a.v_heads * (kFactors * kChunk);
-  auto rows4 = [&](int c, int which, int y) {
-    return *reinterpret_cast<const f4_t*>(factors + c * f_step + which * kChunk + 16 * y);
+  // A chunk's operands and factors, whole pieces of 1 KB, 16 bytes a lane.
+  constexpr uint32_t kQkBytes = kKeys * 1024, kVBytes = kInverse * 1024, kFactorBytes = kFactors * kChunk * 4;
+  auto of_qk = [&](const h8_t* base, int c) {
+    return buffer_of(reinterpret_cast<const char*>(base) + ((slot0 + c) * a.qk_heads + hq) * kQkBytes, kQkBytes);
+  };
+  auto of_v = [&](const h8_t* base, int c) {
+    return buffer_of(reinterpret_cast<const char*>(base) + ((slot0 + c) * a.v_heads + h) * kVBytes, kVBytes);
+  };
+  auto of_factors = [&](int c) {
+    return buffer_of(reinterpret_cast<const char*>(ws.s) + ((slot0 + c) * a.v_heads + h) * kFactorBytes, kFactorBytes);
+  };
+  const uint32_t piece_at = lane * 16;
+  auto rows4 = [&](__amdgpu_buffer_rsrc_t r, int which, int y) {
+    return __builtin_bit_cast(
+        f4_t, __builtin_amdgcn_raw_buffer_load_b128(r, 16 * q4 + (which * kChunk + 16 * y) * 4, 0, 0));
   };
 
   // Both output waves bring half of chunk c's operands.
   auto bring = [&](int c) {
     h8_t* to = &stage[c & 1][0][0];
-    auto one = [&](const h8_t* src, int piece) {
-      __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(to + piece * 64), 16, 0, 0);
+    const auto keys = of_qk(ws.k, c), inverse = of_v(ws.t, c), turned = of_qk(ws.kt, c);
+    auto one = [&](__amdgpu_buffer_rsrc_t r, int from, int piece) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(to + piece * 64), 16, piece_at + from * 1024, 0, 0, 0);
     };
 #pragma unroll
-    for (int p = 0; p < kKeys; p += 2) one(ks + c * qk_step + (p + tile) * 64, p + tile);
+    for (int p = 0; p < kKeys; p += 2) one(keys, p + tile, p + tile);
 #pragma unroll
-    for (int p = 0; p < kInverse; p += 2) one(ts + c * v_step + (p + tile) * 64, kKeys + p + tile);
+    for (int p = 0; p < kInverse; p += 2) one(inverse, p + tile, kKeys + p + tile);
 #pragma unroll
-    for (int p = 0; p < kTurned; p += 2)
-      one(kts + c * qk_step + (p + tile) * 64, kKeys + kInverse + p + tile);
+    for (int p = 0; p < kTurned; p += 2) one(turned, p + tile, kKeys + kInverse + p + tile);
   };
 
   if (wave < 2) {
@@ -428,28 +444,37 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(DeltaArgs a, ChunkSp
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[t][e] = fresh ? 0.f : state[(long long)(16 * t + 4 * q4 + e) * value_size];
-    const uint16_t* values = a.v + (long long)from * a.v_token + (long long)h * a.v_head + col;
     // A chunk's rows are loaded as soon as those of the chunk before are used.
+    const uint16_t* values = a.v + (long long)from * a.v_token + (long long)h * a.v_head;
+    uint32_t v_at[16];
+#pragma unroll
+    for (int z = 0; z < 16; ++z) v_at[z] = ((16 * (z >> 2) + (z & 3) + 4 * q4) * (uint32_t)a.v_token + col) * 2;
     uint16_t v[16];
     f4_t b1[4], b2[4], until[4];
     auto load_values = [&](int c) {
+      const uint32_t count = min(n - c * kChunk, kChunk);
+      const auto rows = buffer_of(values + (long long)c * kChunk * a.v_token, ((count - 1) * (uint32_t)a.v_token + value_size) * 2);
+      const auto f = of_factors(c);
+#pragma unroll
+      for (int z = 0; z < 16; ++z) v[z] = __builtin_amdgcn_raw_buffer_load_b16(rows, v_at[z], 0, 0);
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)  // past the last token, where b1 and b2 are 0, that one again
-          v[4 * y + e] = values[(long long)min(c * kChunk + 16 * y + 4 * q4 + e, n - 1) * a.v_token];
-        b1[y] = rows4(c, 0, y);
-        b2[y] = rows4(c, 1, y);
+        b1[y] = rows4(f, 0, y);
+        b2[y] = rows4(f, 1, y);
       }
     };
     float whole;
     auto load_until = [&](int c) {
+      const auto f = of_factors(c);
 #pragma unroll
-      for (int y = 0; y < 4; ++y) until[y] = rows4(c, 4, y);
-      whole = factors[c * f_step + 5 * kChunk];
+      for (int y = 0; y < 4; ++y) until[y] = rows4(f, 4, y);
+      whole = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(f, 5 * kChunk * 4, 0, 0));
     };
     load_values(0);
     load_until(0);
+    float top = 0.f;  // the largest of the state's values here
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) top = max4(top, s[t]);
     for (int c = 0; c <= chunks; ++c) {
       __syncthreads();  // chunk c's operands are there, and chunk c - 2's parts read
       if (c == chunks) break;
@@ -459,10 +484,7 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(DeltaArgs a, ChunkSp
       const h8_t(*turned)[64] = &stage[c & 1][kKeys + kInverse];
 
       // K' S.
-      float m = 0.f;
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) m = max4(m, s[t]);
-      int shift = column_shift(m);
+      int shift = column_shift(top);
       float up = power2(shift), down = power2(-shift);
       if (q4 == 0) left_scale[c & 1][tile][0][i] = down;
       f4_t x[4] = {kZero, kZero, kZero, kZero};
@@ -478,7 +500,7 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(DeltaArgs a, ChunkSp
         for (int y = 0; y < 4; ++y) x[y] = mfma(keys[y * kS + t][lane], lo, x[y]);
       }
       // What each token finds wrong in the state before the chunk.
-      m = 0.f;
+      float m = 0.f;
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
 #pragma unroll
@@ -520,6 +542,7 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(DeltaArgs a, ChunkSp
       down = power2(-shift);
       split_tiles(w2[0], w2[1], up, &hi[0], &lo[0]);
       split_tiles(w2[2], w2[3], up, &hi[1], &lo[1]);
+      top = 0.f;
 #pragma unroll
       for (int t = 0; t < kTiles; t += 4) {
         f4_t add[4] = {kZero, kZero, kZero, kZero};
@@ -531,9 +554,11 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(DeltaArgs a, ChunkSp
           for (int z = 0; z < 4; ++z) add[z] = mfma(turned[2 * (t + z) + y][lane], lo[y], add[z]);
         }
 #pragma unroll
-        for (int z = 0; z < 4; ++z)
+        for (int z = 0; z < 4; ++z) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[t + z][e] = fmaf(add[z][e], down, whole * s[t + z][e]);
+          top = max4(top, s[t + z]);
+        }
       }
       load_until(after);
       // The corrections for the outputs.
@@ -552,77 +577,74 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(DeltaArgs a, ChunkSp
 #pragma unroll
       for (int e = 0; e < 4; ++e) state[(long long)(16 * t + 4 * q4 + e) * value_size] = s[t][e];
   } else {
-    const h8_t* qs = ws.q + slot0 * qk_step + (size_t)hq * (4 * kS * 64) + lane;
-    const h8_t* ps = ws.p + slot0 * v_step + (size_t)h * (kInverse * 64) + lane;
-    uint16_t* out = a.out + ((long long)from * a.v_heads + h) * value_size + col;
-    const long long out_token = (long long)a.v_heads * value_size;
-    struct Operands {
-      h8_t q[kKeys], p[kInverse];
-      f4_t since[4], d[4];
-    };
-    auto load = [&](int c) {
-      Operands o;
+    uint16_t* out = a.out + ((long long)from * a.v_heads + h) * value_size;
+    const uint32_t out_token = a.v_heads * value_size;
+    uint32_t out_at[16];
 #pragma unroll
-      for (int p = 0; p < kKeys; ++p) o.q[p] = qs[c * qk_step + p * 64];
-#pragma unroll
-      for (int p = 0; p < kInverse; ++p) o.p[p] = ps[c * v_step + p * 64];
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        o.since[y] = rows4(c, 2, y);
-        o.d[y] = rows4(c, 3, y);
-      }
-      return o;
-    };
-    // Outputs of chunk c - 1, whose operands are in `now`; chunk c's go to `next`.
-    auto outputs = [&](int c, const Operands& now, Operands& next) {
+    for (int z = 0; z < 16; ++z) out_at[z] = ((16 * (z >> 2) + (z & 3) + 4 * q4) * out_token + col) * 2;
+    h8_t q[kKeys], p[kInverse];
+    bring(0);
+    for (int c = 0; c <= chunks; ++c) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // bring()'s pieces are in LDS
       __syncthreads();
-      h8_t sp[2 * kS], wp[4];
+      const int at = c - 1;  // the chunk whose outputs are computed, of the operands in q and p
+      f4_t x[4] = {kZero, kZero, kZero, kZero}, y2[4] = {kZero, kZero, kZero, kZero};
       float down_s = 0.f, down_w = 0.f;
-      const int at = c - 1;
+      f4_t since[4], d[4];
+      if (c + 1 < chunks) bring(c + 1);
       if (c > 0) {
+        const auto f = of_factors(at);
 #pragma unroll
-        for (int t = 0; t < 2 * kS; ++t) sp[t] = left_s[at & 1][tile][t][lane];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) wp[t] = left_w[at & 1][tile][t][lane];
+        for (int y = 0; y < 4; ++y) {
+          since[y] = rows4(f, 2, y);
+          d[y] = rows4(f, 3, y);
+        }
         down_s = left_scale[at & 1][tile][0][i];
         down_w = left_scale[at & 1][tile][1][i];
-      }
-      if (c + 1 < chunks) bring(c + 1);
-      if (c < chunks) next = load(c);
-      if (c == 0) return;
-      f4_t x[4] = {kZero, kZero, kZero, kZero}, y2[4] = {kZero, kZero, kZero, kZero};
 #pragma unroll
-      for (int t = 0; t < kS; ++t) {
+        for (int t = 0; t < kS; ++t) {
+          const h8_t hi = left_s[at & 1][tile][2 * t][lane], lo = left_s[at & 1][tile][2 * t + 1][lane];
 #pragma unroll
-        for (int y = 0; y < 4; ++y) x[y] = mfma(now.q[y * kS + t], sp[2 * t], x[y]);
+          for (int y = 0; y < 4; ++y) x[y] = mfma(q[y * kS + t], hi, x[y]);
 #pragma unroll
-        for (int y = 0; y < 4; ++y) x[y] = mfma(now.q[y * kS + t], sp[2 * t + 1], x[y]);
-      }
-#pragma unroll
-      for (int part = 0; part < 3; ++part)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int y = 2 * t; y < 4; ++y) {
-            const int piece = (y == 0 ? 0 : y == 1 ? 1 : y == 2 ? 2 : 4) + t;
-            y2[y] = mfma(now.p[2 * piece + (part == 2)], wp[2 * t + (part == 1)], y2[y]);
-          }
-      const int count = n - at * kChunk;
-#pragma unroll
-      for (int y = 0; y < 4; ++y)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = 16 * y + 4 * q4 + e;
-          const float o = now.d[y][e] * fmaf(y2[y][e], down_w, now.since[y][e] * down_s * x[y][e]);
-          if (row < count) out[(long long)(at * kChunk + row) * out_token] = to_half_bits<kType>(o);
+          for (int y = 0; y < 4; ++y) x[y] = mfma(q[y * kS + t], lo, x[y]);
         }
-    };
-    bring(0);
-    Operands even, odd;  // of chunks c - 1 and c, in turn
-    for (int c = 0; c <= chunks; c += 2) {
-      outputs(c, odd, even);
-      if (c + 1 <= chunks) outputs(c + 1, even, odd);
+      }
+      if (c < chunks) {
+        const auto qs = of_qk(ws.q, c);
+#pragma unroll
+        for (int z = 0; z < kKeys; ++z) q[z] = load_piece(qs, piece_at + z * 1024);
+      }
+      if (c > 0) {
+        h8_t wp[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) wp[t] = left_w[at & 1][tile][t][lane];
+#pragma unroll
+        for (int part = 0; part < 3; ++part)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int y = 2 * t; y < 4; ++y) {
+              const int piece = (y == 0 ? 0 : y == 1 ? 1 : y == 2 ? 2 : 4) + t;
+              y2[y] = mfma(p[2 * piece + (part == 2)], wp[2 * t + (part == 1)], y2[y]);
+            }
+      }
+      if (c < chunks) {
+        const auto ps = of_v(ws.p, c);
+#pragma unroll
+        for (int z = 0; z < kInverse; ++z) p[z] = load_piece(ps, piece_at + z * 1024);
+      }
+      if (c > 0) {
+        const uint32_t count = min(n - at * kChunk, kChunk);
+        const auto rows = buffer_of(out + (long long)at * kChunk * out_token, ((count - 1) * out_token + value_size) * 2);
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float o = d[y][e] * fmaf(y2[y][e], down_w, since[y][e] * down_s * x[y][e]);
+            __builtin_amdgcn_raw_buffer_store_b16(to_half_bits<kType>(o), rows, out_at[4 * y + e], 0, 0);
+          }
+      }
     }
   }
 }

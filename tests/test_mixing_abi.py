@@ -43,6 +43,7 @@ def _delta(lib, out=FAKE, ws=FAKE, ws_bytes=1 << 40, **kw):
     (dict(offsets=None), "one token"), (dict(q=None), "NULL"), (dict(beta=None), "NULL"), (dict(states=None), "NULL"),
     (dict(out=None), "NULL"), (dict(q=FAKE + 8), "16-byte"), (dict(states=FAKE + 4), "16-byte"), (dict(out=FAKE + 2), "16-byte"),
     (dict(log_decay=FAKE + 2), "4-byte"), (dict(offsets=FAKE + 1), "4-byte"), (dict(v_head_stride=100), "multiples of 8"),
+    (dict(v_token_stride=2**24 + 8), "token strides"), (dict(q_token_stride=-8), "token strides"),
     (dict(ws=None), "workspace"), (dict(ws=FAKE + 128), "workspace"), (dict(ws_bytes=4096), "workspace"),
 ])
 def test_delta_refuses(lib, kw, text):
