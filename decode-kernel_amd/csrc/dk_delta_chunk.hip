@@ -45,12 +45,13 @@ constexpr int kFragments = 6;  // 16 x 32 pieces of a lower triangle of 64: (0,0
 // lane's 4 values of two stacked result tiles stand in: a product's result is
 // the next one's operand B as it stands.
 struct ChunkSpace {
-  h8_t* k;    // [slot][qk head][4][dk / 32][64]   K', rows = tokens
-  h8_t* q;    // [slot][qk head][4][dk / 32][64]   Q'
-  h8_t* kt;   // [slot][qk head][dk / 16][2][64]   K' transposed, rows = elements
-  h8_t* t;    // [slot][v head][6][2][64]          T' * 512: first and second part
-  h8_t* p;    // [slot][v head][6][2][64]          P * 64, of q' and k'
-  float* s;   // [slot][v head][kFactors * 64]     the rows' factors
+  h8_t* k;    // [qk head][slot][4][dk / 32][64]   K', rows = tokens
+  h8_t* q;    // [qk head][slot][4][dk / 32][64]   Q'
+  h8_t* kt;   // [qk head][slot][dk / 16][2][64]   K' transposed, rows = elements
+  h8_t* t;    // [v head][slot][6][2][64]          T' * 512: first and second part
+  h8_t* p;    // [v head][slot][6][2][64]          P * 64, of q' and k'
+  float* s;   // [v head][slot][kFactors * 64]     the rows' factors
+  long long slots;
 };
 constexpr int kFactors = 6;  // beta c, beta c^2 e^G, e^G, d, e^(G_last - G), e^G_last (all alike)
 
@@ -75,6 +76,7 @@ ChunkSpace chunk_space(void* workspace, int tokens, int requests, int qk_heads, 
   c.t = reinterpret_cast<h8_t*>(take(lower));
   c.p = reinterpret_cast<h8_t*>(take(lower));
   c.s = reinterpret_cast<float*>(take(slots * v_heads * kFactors * kChunk * 4));
+  c.slots = (long long)slots;
   *bytes = (size_t)(at - static_cast<char*>(workspace));
   return c;
 }
@@ -196,7 +198,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, ChunkSp
   float c = 0.f, d = 0.f;  // a row of zeros has no part in anything
   if (ke != INT32_MIN) c = ldexpf(a.normalize ? 1.f / sqrtf(kk + kUnitEps) : 1.f, ke);
   if (qe != INT32_MIN) d = ldexpf(a.normalize ? a.scale / sqrtf(qq + kUnitEps) : a.scale, qe);
-  const size_t qk_at = (slot * a.qk_heads + hq) * (4 * kS * 64);
+  const size_t qk_at = (hq * ws.slots + slot) * (4 * kS * 64);
 #pragma unroll
   for (int s = 0; s < kS; ++s) {
     keys[wave][s][lane] = kf[s];
@@ -231,7 +233,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, ChunkSp
     hi_of[lane] = hi;
     lo_of[lane] = lo;
     b2_of[lane] = beta * cc * cc;
-    float* f = ws.s + (slot * a.v_heads + h) * (kFactors * kChunk) + lane;
+    float* f = ws.s + (h * ws.slots + slot) * (kFactors * kChunk) + lane;
     f[0] = beta * cc;
     f[64] = beta * cc * cc * since;
     f[128] = since;
@@ -285,7 +287,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, ChunkSp
       kkt[j][e] = rr > col ? b2_of[rr] * decay * kkt[j][e] : 0.f;
     }
   }
-  const size_t v_at = (slot * a.v_heads + h) * (kFragments * 2 * 64);
+  const size_t v_at = (h * ws.slots + slot) * (kFragments * 2 * 64);
   const int piece0 = wave == 0 ? 0 : wave == 1 ? 1 : wave == 2 ? 2 : 4;
   auto pieces_out = [&](h8_t* to, float scale) {
     for (int s = 0; s <= wave / 2; ++s) {
@@ -385,7 +387,7 @@ __device__ __forceinline__ h8_t load_piece(__amdgpu_buffer_rsrc_t r, uint32_t of
 }
 
 template <int kDk, bool kBf16>
-__global__ __launch_bounds__(256, 1) __attribute__((amdgpu_num_vgpr(256))) void delta_scan_kernel(DeltaArgs a, ChunkSpace ws, int value_size) {
+__global__ __launch_bounds__(256, 1) void delta_scan_kernel(DeltaArgs a, ChunkSpace ws, int value_size) {
   constexpr int kS = kDk / 32, kTiles = kDk / 16;
   constexpr int kType = kBf16 ? DK_KV_BF16 : DK_KV_F16;
   constexpr int kKeys = 4 * kS, kInverse = 2 * kFragments, kTurned = 2 * kTiles;  // pieces of 1 KB
@@ -407,13 +409,13 @@ __global__ __launch_bounds__(256, 1) __attribute__((amdgpu_num_vgpr(256))) void 
   // A chunk's operands and factors, whole pieces of 1 KB, 16 bytes a lane.
   constexpr uint32_t kQkBytes = kKeys * 1024, kVBytes = kInverse * 1024, kFactorBytes = kFactors * kChunk * 4;
   auto of_qk = [&](const h8_t* base, int c) {
-    return buffer_of(reinterpret_cast<const char*>(base) + ((slot0 + c) * a.qk_heads + hq) * kQkBytes, kQkBytes);
+    return buffer_of(reinterpret_cast<const char*>(base) + (hq * ws.slots + slot0 + c) * kQkBytes, kQkBytes);
   };
   auto of_v = [&](const h8_t* base, int c) {
-    return buffer_of(reinterpret_cast<const char*>(base) + ((slot0 + c) * a.v_heads + h) * kVBytes, kVBytes);
+    return buffer_of(reinterpret_cast<const char*>(base) + (h * ws.slots + slot0 + c) * kVBytes, kVBytes);
   };
   auto of_factors = [&](int c) {
-    return buffer_of(reinterpret_cast<const char*>(ws.s) + ((slot0 + c) * a.v_heads + h) * kFactorBytes, kFactorBytes);
+    return buffer_of(reinterpret_cast<const char*>(ws.s) + (h * ws.slots + slot0 + c) * kFactorBytes, kFactorBytes);
   };
   const uint32_t piece_at = lane * 16;
   auto rows4 = [&](__amdgpu_buffer_rsrc_t r, int which, int y) {
@@ -483,6 +485,12 @@ __global__ __launch_bounds__(256, 1) __attribute__((amdgpu_num_vgpr(256))) void 
       const h8_t(*inverse)[64] = &stage[c & 1][kKeys];
       const h8_t(*turned)[64] = &stage[c & 1][kKeys + kInverse];
 
+      // Operands are read from LDS a product ahead: left to itself the compiler
+      // reads two, waits for them and goes on, 22 times a chunk.
+      h8_t kf[kKeys], tf[kInverse], uf[kTurned];
+#pragma unroll
+      for (int z = 0; z < kKeys; ++z) kf[z] = keys[z][lane];
+      __builtin_amdgcn_sched_barrier(0);
       // K' S.
       int shift = column_shift(top);
       float up = power2(shift), down = power2(-shift);
@@ -495,10 +503,14 @@ __global__ __launch_bounds__(256, 1) __attribute__((amdgpu_num_vgpr(256))) void 
         left_s[c & 1][tile][2 * t][lane] = hi;
         left_s[c & 1][tile][2 * t + 1][lane] = lo;
 #pragma unroll
-        for (int y = 0; y < 4; ++y) x[y] = mfma(keys[y * kS + t][lane], hi, x[y]);
+        for (int y = 0; y < 4; ++y) x[y] = mfma(kf[y * kS + t], hi, x[y]);
 #pragma unroll
-        for (int y = 0; y < 4; ++y) x[y] = mfma(keys[y * kS + t][lane], lo, x[y]);
+        for (int y = 0; y < 4; ++y) x[y] = mfma(kf[y * kS + t], lo, x[y]);
       }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int z = 0; z < kInverse; ++z) tf[z] = inverse[z][lane];
+      __builtin_amdgcn_sched_barrier(0);
       // What each token finds wrong in the state before the chunk.
       float m = 0.f;
 #pragma unroll
@@ -516,6 +528,10 @@ __global__ __launch_bounds__(256, 1) __attribute__((amdgpu_num_vgpr(256))) void 
       h8_t hi[2], lo[2];
       split_tiles(x[0], x[1], up, &hi[0], &lo[0]);
       split_tiles(x[2], x[3], up, &hi[1], &lo[1]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int z = 0; z < kTurned; ++z) uf[z] = turned[z][lane];
+      __builtin_amdgcn_sched_barrier(0);
       f4_t w[4] = {kZero, kZero, kZero, kZero};
 #pragma unroll
       for (int part = 0; part < 3; ++part)
@@ -524,7 +540,7 @@ __global__ __launch_bounds__(256, 1) __attribute__((amdgpu_num_vgpr(256))) void 
 #pragma unroll
           for (int y = 2 * t; y < 4; ++y) {
             const int piece = (y == 0 ? 0 : y == 1 ? 1 : y == 2 ? 2 : 4) + t;
-            w[y] = mfma(inverse[2 * piece + (part == 2)][lane], part == 1 ? lo[t] : hi[t], w[y]);
+            w[y] = mfma(tf[2 * piece + (part == 2)], part == 1 ? lo[t] : hi[t], w[y]);
           }
       float m2 = 0.f;
       f4_t w2[4];
@@ -549,9 +565,9 @@ __global__ __launch_bounds__(256, 1) __attribute__((amdgpu_num_vgpr(256))) void 
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
 #pragma unroll
-          for (int z = 0; z < 4; ++z) add[z] = mfma(turned[2 * (t + z) + y][lane], hi[y], add[z]);
+          for (int z = 0; z < 4; ++z) add[z] = mfma(uf[2 * (t + z) + y], hi[y], add[z]);
 #pragma unroll
-          for (int z = 0; z < 4; ++z) add[z] = mfma(turned[2 * (t + z) + y][lane], lo[y], add[z]);
+          for (int z = 0; z < 4; ++z) add[z] = mfma(uf[2 * (t + z) + y], lo[y], add[z]);
         }
 #pragma unroll
         for (int z = 0; z < 4; ++z) {
@@ -582,69 +598,66 @@ __global__ __launch_bounds__(256, 1) __attribute__((amdgpu_num_vgpr(256))) void 
     uint32_t out_at[16];
 #pragma unroll
     for (int z = 0; z < 16; ++z) out_at[z] = ((16 * (z >> 2) + (z & 3) + 4 * q4) * out_token + col) * 2;
-    h8_t q[kKeys], p[kInverse];
-    bring(0);
-    for (int c = 0; c <= chunks; ++c) {
+    struct Operands {
+      h8_t q[kKeys], p[kInverse];
+    };
+    // Outputs of chunk c - 1, whose operands are in `now`; chunk c's go to `next`,
+    // so that all loads have a chunk's time to arrive.
+    auto outputs = [&](int c, const Operands& now, Operands& next) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // bring()'s pieces are in LDS
       __syncthreads();
-      const int at = c - 1;  // the chunk whose outputs are computed, of the operands in q and p
-      f4_t x[4] = {kZero, kZero, kZero, kZero}, y2[4] = {kZero, kZero, kZero, kZero};
-      float down_s = 0.f, down_w = 0.f;
-      f4_t since[4], d[4];
       if (c + 1 < chunks) bring(c + 1);
-      if (c > 0) {
-        const auto f = of_factors(at);
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          since[y] = rows4(f, 2, y);
-          d[y] = rows4(f, 3, y);
-        }
-        down_s = left_scale[at & 1][tile][0][i];
-        down_w = left_scale[at & 1][tile][1][i];
-#pragma unroll
-        for (int t = 0; t < kS; ++t) {
-          const h8_t hi = left_s[at & 1][tile][2 * t][lane], lo = left_s[at & 1][tile][2 * t + 1][lane];
-#pragma unroll
-          for (int y = 0; y < 4; ++y) x[y] = mfma(q[y * kS + t], hi, x[y]);
-#pragma unroll
-          for (int y = 0; y < 4; ++y) x[y] = mfma(q[y * kS + t], lo, x[y]);
-        }
-      }
       if (c < chunks) {
-        const auto qs = of_qk(ws.q, c);
+        const auto qs = of_qk(ws.q, c), ps = of_v(ws.p, c);
 #pragma unroll
-        for (int z = 0; z < kKeys; ++z) q[z] = load_piece(qs, piece_at + z * 1024);
+        for (int z = 0; z < kKeys; ++z) next.q[z] = load_piece(qs, piece_at + z * 1024);
+#pragma unroll
+        for (int z = 0; z < kInverse; ++z) next.p[z] = load_piece(ps, piece_at + z * 1024);
       }
-      if (c > 0) {
-        h8_t wp[4];
+      if (c == 0) return;
+      const int at = c - 1;
+      f4_t x[4] = {kZero, kZero, kZero, kZero}, y2[4] = {kZero, kZero, kZero, kZero}, since[4], d[4];
+      const auto f = of_factors(at);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) wp[t] = left_w[at & 1][tile][t][lane];
-#pragma unroll
-        for (int part = 0; part < 3; ++part)
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int y = 2 * t; y < 4; ++y) {
-              const int piece = (y == 0 ? 0 : y == 1 ? 1 : y == 2 ? 2 : 4) + t;
-              y2[y] = mfma(p[2 * piece + (part == 2)], wp[2 * t + (part == 1)], y2[y]);
-            }
+      for (int y = 0; y < 4; ++y) {
+        since[y] = rows4(f, 2, y);
+        d[y] = rows4(f, 3, y);
       }
-      if (c < chunks) {
-        const auto ps = of_v(ws.p, c);
+      const float down_s = left_scale[at & 1][tile][0][i], down_w = left_scale[at & 1][tile][1][i];
+      h8_t sp[2 * kS], wp[4];
 #pragma unroll
-        for (int z = 0; z < kInverse; ++z) p[z] = load_piece(ps, piece_at + z * 1024);
-      }
-      if (c > 0) {
-        const uint32_t count = min(n - at * kChunk, kChunk);
-        const auto rows = buffer_of(out + (long long)at * kChunk * out_token, ((count - 1) * out_token + value_size) * 2);
+      for (int t = 0; t < 2 * kS; ++t) sp[t] = left_s[at & 1][tile][t][lane];
 #pragma unroll
-        for (int y = 0; y < 4; ++y)
+      for (int t = 0; t < 4; ++t) wp[t] = left_w[at & 1][tile][t][lane];
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float o = d[y][e] * fmaf(y2[y][e], down_w, since[y][e] * down_s * x[y][e]);
-            __builtin_amdgcn_raw_buffer_store_b16(to_half_bits<kType>(o), rows, out_at[4 * y + e], 0, 0);
+      for (int t = 0; t < 2 * kS; ++t)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) x[y] = mfma(now.q[y * kS + t / 2], sp[t], x[y]);
+#pragma unroll
+      for (int part = 0; part < 3; ++part)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int y = 2 * t; y < 4; ++y) {
+            const int piece = (y == 0 ? 0 : y == 1 ? 1 : y == 2 ? 2 : 4) + t;
+            y2[y] = mfma(now.p[2 * piece + (part == 2)], wp[2 * t + (part == 1)], y2[y]);
           }
-      }
+      const uint32_t count = min(n - at * kChunk, kChunk);
+      const auto rows = buffer_of(out + (long long)at * kChunk * out_token, ((count - 1) * out_token + value_size) * 2);
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float o = d[y][e] * fmaf(y2[y][e], down_w, since[y][e] * down_s * x[y][e]);
+          __builtin_amdgcn_raw_buffer_store_b16(to_half_bits<kType>(o), rows, out_at[4 * y + e], 0, 0);
+        }
+    };
+    bring(0);
+    Operands even, odd;  // of chunks c - 1 and c, in turn
+    for (int c = 0; c <= chunks; c += 2) {
+      outputs(c, odd, even);
+      if (c + 1 <= chunks) outputs(c + 1, even, odd);
     }
   }
 }
