@@ -24,6 +24,8 @@
 //   w = T' (beta c v - beta c^2 e^G (K' S)),  S_after = e^G_last S + sum_j k'_j (e^(..) w_j).
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "dk_delta.hpp"
 #include "dk_host.hpp"
 
@@ -53,7 +55,7 @@ struct ChunkSpace {
   float* s;   // [v head][slot][kFactors * 64]     the rows' factors
   long long slots;
 };
-constexpr int kFactors = 6;  // beta c, beta c^2 e^G, e^G, d, e^(G_last - G), e^G_last (all alike)
+constexpr int kFactors = 8;  // beta c, beta c^2 e^G, e^G, d, e^(G_last - G), e^G_last (all alike), to 2 KB
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -111,21 +113,24 @@ __device__ __forceinline__ float max_rows(float m) {
 // those of the lanes 16, 32 and 48 away) to 2^14 .. 2^15, as an exponent.
 __device__ __forceinline__ int column_shift(float m) { return min(14 - exponent_of(max_rows(m)), 126); }
 
-__device__ __forceinline__ float max4(float m, f4_t x) {
-  m = fmaxf(fmaxf(m, fabsf(x[0])), fabsf(x[1]));
-  return fmaxf(fmaxf(m, fabsf(x[2])), fabsf(x[3]));
+__device__ __forceinline__ float max4(f4_t x) {
+  return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
 }
 
 // Two stacked result tiles times a power of two as an operand B of 32 rows, in
-// two fp16 parts of one rounding each.
+// two fp16 parts of one rounding each: an instruction of mixed width a part.
 __device__ __forceinline__ void split_tiles(f4_t x, f4_t y, float scale, h8_t* hi, h8_t* lo) {
   const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    // As one instruction of mixed width, not a product and a conversion.
-    const _Float16 h = (_Float16)fmaf(v[j], scale, 0.f);
-    (*hi)[j] = h;
-    (*lo)[j] = (_Float16)fmaf(v[j], scale, -(float)h);
+  for (int j = 0; j < 8; j += 2) {
+    const h2_t pair = {(_Float16)fmaf(v[j], scale, 0.f), (_Float16)fmaf(v[j + 1], scale, 0.f)};
+    uint32_t bits = __builtin_bit_cast(uint32_t, pair);
+    asm("" : "+v"(bits));  // or each first part is computed twice, for itself and for the second
+    const h2_t h = as_h2(bits);
+    (*hi)[j] = h[0];
+    (*hi)[j + 1] = h[1];
+    (*lo)[j] = (_Float16)fmaf(v[j], scale, -(float)h[0]);
+    (*lo)[j + 1] = (_Float16)fmaf(v[j + 1], scale, -(float)h[1]);
   }
 }
 
@@ -363,17 +368,16 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, ChunkSp
 }
 
 // ---------------------------------------------------------------------------
-// A request's chunks one after another, 32 columns of one head's state a
-// workgroup. Waves 0 and 1 hold 16 columns each and go from state to state;
-// columns do not meet, and a result tile is the next product's operand B, so
-// nothing but the prepared operands comes from outside a wave. Waves 2 and 3
-// compute the same columns' outputs one chunk behind, from the parts of the
-// state and of the corrections that waves 0 and 1 leave in LDS, and bring the
-// next chunk's operands there: what only the outputs need is off the chain
-// that bounds a long prompt.
+// A request's chunks one after another, kCols tiles of 16 columns of one head's
+// state a workgroup, four waves a tile. Two waves hold half of the tile's rows
+// each and go from state to state: their shares of K' S are added through LDS,
+// the corrections both compute, and each brings its rows of the state forward.
+// Columns do not meet, and a result tile is the next product's operand B as it
+// stands. The other two waves compute half of the tokens' outputs each, one
+// chunk behind, from the parts of the state and the corrections that the first
+// two leave in LDS, and bring the next chunk's operands there: what only the
+// outputs need is off the chain that bounds a long prompt.
 // ---------------------------------------------------------------------------
-constexpr int kScanTiles = 2;  // tiles of 16 columns a workgroup holds
-
 using lds_ptr = __attribute__((address_space(3))) void*;
 
 // Buffers: a chunk's rows behind the request's last are out of their range, so
@@ -386,278 +390,326 @@ __device__ __forceinline__ h8_t load_piece(__amdgpu_buffer_rsrc_t r, uint32_t of
   return __builtin_bit_cast(h8_t, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0));
 }
 
-template <int kDk, bool kBf16>
-__global__ __launch_bounds__(256, 1) void delta_scan_kernel(DeltaArgs a, ChunkSpace ws, int value_size) {
-  constexpr int kS = kDk / 32, kTiles = kDk / 16;
+// Piece (row tile y, columns 32 t ..) of a lower triangle.
+__device__ __forceinline__ constexpr int piece_of(int y, int t) {
+  return (y == 0 ? 0 : y == 1 ? 1 : y == 2 ? 2 : 4) + t;
+}
+
+template <int kDk, int kCols, bool kBf16>
+__global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a, ChunkSpace ws, int value_size) {
+  constexpr int kS = kDk / 32, kHalfS = kS / 2, kHalfTiles = kDk / 32;
   constexpr int kType = kBf16 ? DK_KV_BF16 : DK_KV_F16;
-  constexpr int kKeys = 4 * kS, kInverse = 2 * kFragments, kTurned = 2 * kTiles;  // pieces of 1 KB
+  constexpr int kKeys = 4 * kS, kInverse = 2 * kFragments, kTurned = 4 * kS;  // pieces of 1 KB
+  constexpr int kPieces = kKeys + kInverse + kTurned + 2;
   constexpr f4_t kZero{0.f, 0.f, 0.f, 0.f};
-  __shared__ h8_t stage[2][kKeys + kInverse + kTurned][64];
-  __shared__ h8_t left_s[2][kScanTiles][2 * kS][64];  // the state's parts
-  __shared__ h8_t left_w[2][kScanTiles][4][64];       // the corrections'
-  __shared__ float left_scale[2][kScanTiles][2][16];  // what both are divided by
+  __shared__ h8_t stage[2][kPieces][64];         // a chunk's operands and its rows' factors
+  __shared__ f4_t rows_v[kCols][4][64];          // beta c v of a chunk's rows
+  __shared__ f4_t share[kCols][2][4][64];        // a half's share of K' S
+  __shared__ h8_t left_s[kCols][2 * kS][64];     // the state's parts
+  __shared__ f4_t left_w[kCols][4][64];          // the corrections
+  __shared__ float left_scale[kCols][3][16];     // by which both halves of the state and w are to be multiplied
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, i = lane & 15, q4 = lane >> 4;
-  const int tile = wave & 1;
+  const bool outputs = wave >= 2 * kCols;
+  const int tile = (wave >> 1) & (kCols - 1), half = wave & 1;
   const int h = blockIdx.x % a.v_heads, hq = h / a.group, b = blockIdx.y;
-  const int col = ((blockIdx.x / a.v_heads) * kScanTiles + tile) * 16 + i;
+  const int col = ((blockIdx.x / a.v_heads) * kCols + tile) * 16 + i;
   if (!wave_offsets_ok(a.offsets, a.requests, a.tokens)) return;
   const int from = a.offsets[b], n = a.offsets[b + 1] - from;
   if (n <= a.limit) return;
   const long long slot0 = from / kChunk + b;
   const int chunks = (n + kChunk - 1) / kChunk;
-  // A chunk's operands and factors, whole pieces of 1 KB, 16 bytes a lane.
-  constexpr uint32_t kQkBytes = kKeys * 1024, kVBytes = kInverse * 1024, kFactorBytes = kFactors * kChunk * 4;
-  auto of_qk = [&](const h8_t* base, int c) {
-    return buffer_of(reinterpret_cast<const char*>(base) + (hq * ws.slots + slot0 + c) * kQkBytes, kQkBytes);
-  };
-  auto of_v = [&](const h8_t* base, int c) {
-    return buffer_of(reinterpret_cast<const char*>(base) + (h * ws.slots + slot0 + c) * kVBytes, kVBytes);
-  };
-  auto of_factors = [&](int c) {
-    return buffer_of(reinterpret_cast<const char*>(ws.s) + (h * ws.slots + slot0 + c) * kFactorBytes, kFactorBytes);
-  };
-  const uint32_t piece_at = lane * 16;
-  auto rows4 = [&](__amdgpu_buffer_rsrc_t r, int which, int y) {
-    return __builtin_bit_cast(
-        f4_t, __builtin_amdgcn_raw_buffer_load_b128(r, 16 * q4 + (which * kChunk + 16 * y) * 4, 0, 0));
-  };
 
-  // Both output waves bring half of chunk c's operands.
-  auto bring = [&](int c) {
-    h8_t* to = &stage[c & 1][0][0];
-    const auto keys = of_qk(ws.k, c), inverse = of_v(ws.t, c), turned = of_qk(ws.kt, c);
-    auto one = [&](__amdgpu_buffer_rsrc_t r, int from, int piece) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(to + piece * 64), 16, piece_at + from * 1024, 0, 0, 0);
-    };
-#pragma unroll
-    for (int p = 0; p < kKeys; p += 2) one(keys, p + tile, p + tile);
-#pragma unroll
-    for (int p = 0; p < kInverse; p += 2) one(inverse, p + tile, kKeys + p + tile);
-#pragma unroll
-    for (int p = 0; p < kTurned; p += 2) one(turned, p + tile, kKeys + kInverse + p + tile);
-  };
-
-  if (wave < 2) {
-    float* state = a.states + ((long long)b * a.v_heads + h) * kDk * value_size + col;
-    f4_t s[kTiles];
+  // A chunk takes two barriers. State waves: the first, K' S from the state, the
+  // second, the corrections and the state after. Output waves: the first, P w
+  // and the outputs of the chunk before, the second, Q' S and the next chunk's
+  // loads. Each hands on what the other needs before a barrier and takes it
+  // behind it, so that one buffer of each is enough.
+  if (!outputs) {
+    float* state = a.states + (((long long)b * a.v_heads + h) * kDk + half * (kDk / 2)) * value_size + col;
+    f4_t s[kHalfTiles];
     const bool fresh = a.held && a.held[b] <= 0;
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t)
+    for (int t = 0; t < kHalfTiles; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[t][e] = fresh ? 0.f : state[(long long)(16 * t + 4 * q4 + e) * value_size];
-    // A chunk's rows are loaded as soon as those of the chunk before are used.
-    const uint16_t* values = a.v + (long long)from * a.v_token + (long long)h * a.v_head;
-    uint32_t v_at[16];
-#pragma unroll
-    for (int z = 0; z < 16; ++z) v_at[z] = ((16 * (z >> 2) + (z & 3) + 4 * q4) * (uint32_t)a.v_token + col) * 2;
-    uint16_t v[16];
-    f4_t b1[4], b2[4], until[4];
-    auto load_values = [&](int c) {
-      const uint32_t count = min(n - c * kChunk, kChunk);
-      const auto rows = buffer_of(values + (long long)c * kChunk * a.v_token, ((count - 1) * (uint32_t)a.v_token + value_size) * 2);
-      const auto f = of_factors(c);
-#pragma unroll
-      for (int z = 0; z < 16; ++z) v[z] = __builtin_amdgcn_raw_buffer_load_b16(rows, v_at[z], 0, 0);
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        b1[y] = rows4(f, 0, y);
-        b2[y] = rows4(f, 1, y);
-      }
-    };
-    float whole;
-    auto load_until = [&](int c) {
-      const auto f = of_factors(c);
-#pragma unroll
-      for (int y = 0; y < 4; ++y) until[y] = rows4(f, 4, y);
-      whole = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(f, 5 * kChunk * 4, 0, 0));
-    };
-    load_values(0);
-    load_until(0);
-    float top = 0.f;  // the largest of the state's values here
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) top = max4(top, s[t]);
     for (int c = 0; c <= chunks; ++c) {
-      __syncthreads();  // chunk c's operands are there, and chunk c - 2's parts read
+      __syncthreads();
       if (c == chunks) break;
-      const int after = min(c + 1, chunks - 1);
       const h8_t(*keys)[64] = &stage[c & 1][0];
       const h8_t(*inverse)[64] = &stage[c & 1][kKeys];
       const h8_t(*turned)[64] = &stage[c & 1][kKeys + kInverse];
+      const float* factors = reinterpret_cast<const float*>(&stage[c & 1][kKeys + kInverse + kTurned][0]);
+      auto rows4 = [&](int which, int y) {
+        return *reinterpret_cast<const f4_t*>(factors + which * kChunk + 16 * y + 4 * q4);
+      };
 
-      // Operands are read from LDS a product ahead: left to itself the compiler
-      // reads two, waits for them and goes on, 22 times a chunk.
-      h8_t kf[kKeys], tf[kInverse], uf[kTurned];
+      // Operands are read from LDS well ahead of their products: left to itself
+      // the compiler reads two, waits for them and goes on.
+      h8_t kf[4 * kHalfS], tf[kInverse], uf[2 * kHalfTiles];
 #pragma unroll
-      for (int z = 0; z < kKeys; ++z) kf[z] = keys[z][lane];
+      for (int t = 0; t < kHalfS; ++t)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) kf[y * kHalfS + t] = keys[y * kS + half * kHalfS + t][lane];
       __builtin_amdgcn_sched_barrier(0);
-      // K' S.
-      int shift = column_shift(top);
+      // K' S, this half's share.
+      float m = max4(s[0]);
+#pragma unroll
+      for (int t = 1; t < kHalfTiles; ++t) m = fmaxf(m, max4(s[t]));
+      int shift = column_shift(m);
       float up = power2(shift), down = power2(-shift);
-      if (q4 == 0) left_scale[c & 1][tile][0][i] = down;
       f4_t x[4] = {kZero, kZero, kZero, kZero};
 #pragma unroll
-      for (int t = 0; t < kS; ++t) {
+      for (int t = 0; t < kHalfS; ++t) {
         h8_t hi, lo;
         split_tiles(s[2 * t], s[2 * t + 1], up, &hi, &lo);
-        left_s[c & 1][tile][2 * t][lane] = hi;
-        left_s[c & 1][tile][2 * t + 1][lane] = lo;
+        left_s[tile][2 * (half * kHalfS + t)][lane] = hi;
+        left_s[tile][2 * (half * kHalfS + t) + 1][lane] = lo;
 #pragma unroll
-        for (int y = 0; y < 4; ++y) x[y] = mfma(kf[y * kS + t], hi, x[y]);
+        for (int y = 0; y < 4; ++y) x[y] = mfma(kf[y * kHalfS + t], hi, x[y]);
 #pragma unroll
-        for (int y = 0; y < 4; ++y) x[y] = mfma(kf[y * kS + t], lo, x[y]);
+        for (int y = 0; y < 4; ++y) x[y] = mfma(kf[y * kHalfS + t], lo, x[y]);
       }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int z = 0; z < kInverse; ++z) tf[z] = inverse[z][lane];
-      __builtin_amdgcn_sched_barrier(0);
-      // What each token finds wrong in the state before the chunk.
-      float m = 0.f;
+      if (q4 == 0) left_scale[tile][half][i] = down;
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          x[y][e] = b1[y][e] * pair_lo<kBf16>(v[4 * y + e]) - b2[y][e] * (down * x[y][e]);
-        m = max4(m, x[y]);
+        x[y] *= down;
+        share[tile][half][y][lane] = x[y];
       }
-      load_values(after);
-      // The corrections w = T x.
-      shift = column_shift(m);
+      f4_t bv[4], b2[4], until[4];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        bv[y] = rows_v[tile][y][lane];
+        b2[y] = rows4(1, y);
+      }
+      __syncthreads();
+      f4_t other[4];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) other[y] = share[tile][1 - half][y][lane];
+#pragma unroll
+      for (int z = 0; z < kInverse; ++z) tf[z] = inverse[z][lane];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) until[y] = rows4(4, y);
+      const float whole = factors[5 * kChunk];
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int t = 0; t < kHalfTiles; ++t) uf[2 * t + y] = turned[2 * (half * kHalfTiles + t) + y][lane];
+      __builtin_amdgcn_sched_barrier(0);
+      // What each token finds wrong in the state before the chunk.
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[y][e] = fmaf(-b2[y][e], x[y][e] + other[y][e], bv[y][e]);
+      // The corrections w = T x, times 512 / down.
+      shift = column_shift(fmaxf(fmaxf(max4(x[0]), max4(x[1])), fmaxf(max4(x[2]), max4(x[3]))));
       up = power2(shift);
       down = power2(-shift) / kInverseScale;
       h8_t hi[2], lo[2];
       split_tiles(x[0], x[1], up, &hi[0], &lo[0]);
-      split_tiles(x[2], x[3], up, &hi[1], &lo[1]);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int z = 0; z < kTurned; ++z) uf[z] = turned[z][lane];
-      __builtin_amdgcn_sched_barrier(0);
       f4_t w[4] = {kZero, kZero, kZero, kZero};
 #pragma unroll
       for (int part = 0; part < 3; ++part)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int y = 2 * t; y < 4; ++y) {
-            const int piece = (y == 0 ? 0 : y == 1 ? 1 : y == 2 ? 2 : 4) + t;
-            w[y] = mfma(tf[2 * piece + (part == 2)], part == 1 ? lo[t] : hi[t], w[y]);
-          }
-      float m2 = 0.f;
-      f4_t w2[4];
-      m = 0.f;
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        w[y] *= down;
-        w2[y] = w[y] * until[y];
-        m = max4(m, w[y]);
-        m2 = max4(m2, w2[y]);
-      }
-      // The state after the chunk.
-      shift = column_shift(m2);
-      up = power2(shift);
-      down = power2(-shift);
-      split_tiles(w2[0], w2[1], up, &hi[0], &lo[0]);
-      split_tiles(w2[2], w2[3], up, &hi[1], &lo[1]);
-      top = 0.f;
-#pragma unroll
-      for (int t = 0; t < kTiles; t += 4) {
-        f4_t add[4] = {kZero, kZero, kZero, kZero};
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-#pragma unroll
-          for (int z = 0; z < 4; ++z) add[z] = mfma(uf[2 * (t + z) + y], hi[y], add[z]);
-#pragma unroll
-          for (int z = 0; z < 4; ++z) add[z] = mfma(uf[2 * (t + z) + y], lo[y], add[z]);
-        }
-#pragma unroll
-        for (int z = 0; z < 4; ++z) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[t + z][e] = fmaf(add[z][e], down, whole * s[t + z][e]);
-          top = max4(top, s[t + z]);
-        }
-      }
-      load_until(after);
-      // The corrections for the outputs.
-      shift = column_shift(m);
-      up = power2(shift);
-      if (q4 == 0) left_scale[c & 1][tile][1][i] = power2(-shift) / kScoreScale;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        split_tiles(w[2 * t], w[2 * t + 1], up, &hi[t], &lo[t]);
-        left_w[c & 1][tile][2 * t][lane] = hi[t];
-        left_w[c & 1][tile][2 * t + 1][lane] = lo[t];
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) state[(long long)(16 * t + 4 * q4 + e) * value_size] = s[t][e];
-  } else {
-    uint16_t* out = a.out + ((long long)from * a.v_heads + h) * value_size;
-    const uint32_t out_token = a.v_heads * value_size;
-    uint32_t out_at[16];
-#pragma unroll
-    for (int z = 0; z < 16; ++z) out_at[z] = ((16 * (z >> 2) + (z & 3) + 4 * q4) * out_token + col) * 2;
-    struct Operands {
-      h8_t q[kKeys], p[kInverse];
-    };
-    // Outputs of chunk c - 1, whose operands are in `now`; chunk c's go to `next`,
-    // so that all loads have a chunk's time to arrive.
-    auto outputs = [&](int c, const Operands& now, Operands& next) {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // bring()'s pieces are in LDS
-      __syncthreads();
-      if (c + 1 < chunks) bring(c + 1);
-      if (c < chunks) {
-        const auto qs = of_qk(ws.q, c), ps = of_v(ws.p, c);
-#pragma unroll
-        for (int z = 0; z < kKeys; ++z) next.q[z] = load_piece(qs, piece_at + z * 1024);
-#pragma unroll
-        for (int z = 0; z < kInverse; ++z) next.p[z] = load_piece(ps, piece_at + z * 1024);
-      }
-      if (c == 0) return;
-      const int at = c - 1;
-      f4_t x[4] = {kZero, kZero, kZero, kZero}, y2[4] = {kZero, kZero, kZero, kZero}, since[4], d[4];
-      const auto f = of_factors(at);
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        since[y] = rows4(f, 2, y);
-        d[y] = rows4(f, 3, y);
-      }
-      const float down_s = left_scale[at & 1][tile][0][i], down_w = left_scale[at & 1][tile][1][i];
-      h8_t sp[2 * kS], wp[4];
-#pragma unroll
-      for (int t = 0; t < 2 * kS; ++t) sp[t] = left_s[at & 1][tile][t][lane];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) wp[t] = left_w[at & 1][tile][t][lane];
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int t = 0; t < 2 * kS; ++t)
-#pragma unroll
-        for (int y = 0; y < 4; ++y) x[y] = mfma(now.q[y * kS + t / 2], sp[t], x[y]);
+        for (int y = 0; y < 4; ++y)
+          w[y] = mfma(tf[2 * piece_of(y, 0) + (part == 2)], part == 1 ? lo[0] : hi[0], w[y]);
+      split_tiles(x[2], x[3], up, &hi[1], &lo[1]);
 #pragma unroll
       for (int part = 0; part < 3; ++part)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int y = 2; y < 4; ++y)
+          w[y] = mfma(tf[2 * piece_of(y, 1) + (part == 2)], part == 1 ? lo[1] : hi[1], w[y]);
+      // The state after the chunk.
+      f4_t w2[4];
 #pragma unroll
-          for (int y = 2 * t; y < 4; ++y) {
-            const int piece = (y == 0 ? 0 : y == 1 ? 1 : y == 2 ? 2 : 4) + t;
-            y2[y] = mfma(now.p[2 * piece + (part == 2)], wp[2 * t + (part == 1)], y2[y]);
-          }
-      const uint32_t count = min(n - at * kChunk, kChunk);
-      const auto rows = buffer_of(out + (long long)at * kChunk * out_token, ((count - 1) * out_token + value_size) * 2);
+      for (int y = 0; y < 4; ++y) w2[y] = w[y] * until[y];
+      shift = column_shift(fmaxf(fmaxf(max4(w2[0]), max4(w2[1])), fmaxf(max4(w2[2]), max4(w2[3]))));
+      up = power2(shift);
+      f4_t add[kHalfTiles];
 #pragma unroll
-      for (int y = 0; y < 4; ++y)
+      for (int z = 0; z < kHalfTiles; ++z) add[z] = kZero;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float o = d[y][e] * fmaf(y2[y][e], down_w, since[y][e] * down_s * x[y][e]);
-          __builtin_amdgcn_raw_buffer_store_b16(to_half_bits<kType>(o), rows, out_at[4 * y + e], 0, 0);
-        }
+      for (int y = 0; y < 2; ++y) {
+        split_tiles(w2[2 * y], w2[2 * y + 1], up, &hi[y], &lo[y]);
+#pragma unroll
+        for (int z = 0; z < kHalfTiles; ++z) add[z] = mfma(uf[2 * z + y], hi[y], add[z]);
+#pragma unroll
+        for (int z = 0; z < kHalfTiles; ++z) add[z] = mfma(uf[2 * z + y], lo[y], add[z]);
+      }
+      if (half == 0) {  // one half of the tokens' corrections each
+        left_w[tile][0][lane] = w[0];
+        left_w[tile][1][lane] = w[1];
+        if (q4 == 0) left_scale[tile][2][i] = down;
+      } else {
+        left_w[tile][2][lane] = w[2];
+        left_w[tile][3][lane] = w[3];
+      }
+      down *= power2(-shift);
+#pragma unroll
+      for (int z = 0; z < kHalfTiles; ++z)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[z][e] = fmaf(add[z][e], down, whole * s[z][e]);
+    }
+#pragma unroll
+    for (int t = 0; t < kHalfTiles; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) state[(long long)(16 * t + 4 * q4 + e) * value_size] = s[t][e];
+  } else {
+    // A chunk's operands and factors, whole pieces of 1 KB, 16 bytes a lane.
+    constexpr uint32_t kQkBytes = kKeys * 1024, kVBytes = kInverse * 1024, kFactorBytes = kFactors * kChunk * 4;
+    auto of_qk = [&](const h8_t* base, int c) {
+      return buffer_of(reinterpret_cast<const char*>(base) + (hq * ws.slots + slot0 + c) * kQkBytes, kQkBytes);
     };
+    auto of_v = [&](const h8_t* base, int c) {
+      return buffer_of(reinterpret_cast<const char*>(base) + (h * ws.slots + slot0 + c) * kVBytes, kVBytes);
+    };
+    auto of_factors = [&](int c) {
+      return buffer_of(reinterpret_cast<const char*>(ws.s) + (h * ws.slots + slot0 + c) * kFactorBytes, kFactorBytes);
+    };
+    const uint32_t piece_at = lane * 16;
+    // The rows 32 half .. 32 half + 31 of a chunk are this wave's.
+    auto rows4 = [&](__amdgpu_buffer_rsrc_t r, int which, int y) {
+      return __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                                          r, 16 * q4 + (which * kChunk + 32 * half + 16 * y) * 4, 0, 0));
+    };
+    const uint16_t* values = a.v + (long long)from * a.v_token + (long long)h * a.v_head;
+    uint16_t* out = a.out + ((long long)from * a.v_heads + h) * value_size;
+    const uint32_t out_token = a.v_heads * value_size;
+    uint32_t v_at[8], out_at[8];
+#pragma unroll
+    for (int z = 0; z < 8; ++z) {
+      const uint32_t row = 32 * half + 16 * (z >> 2) + (z & 3) + 4 * q4;
+      v_at[z] = (row * (uint32_t)a.v_token + col) * 2;
+      out_at[z] = (row * out_token + col) * 2;
+    }
+    // All output waves bring a chunk's operands, each its share of the pieces.
+    auto bring = [&](int c) {
+      h8_t* to = &stage[c & 1][0][0];
+      auto some = [&](__amdgpu_buffer_rsrc_t r, int first, int count) {
+#pragma unroll
+        for (int p = 0; p < count; p += 2 * kCols)
+          if (count % (2 * kCols) == 0 || p + wave - 2 * kCols < count)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(to + (first + p + wave - 2 * kCols) * 64), 16,
+                                                     piece_at + (p + wave - 2 * kCols) * 1024, 0, 0, 0);
+      };
+      some(of_qk(ws.k, c), 0, kKeys);
+      some(of_v(ws.t, c), kKeys, kInverse);
+      some(of_qk(ws.kt, c), kKeys + kInverse, kTurned);
+      some(of_factors(c), kKeys + kInverse + kTurned, 2);
+    };
+    uint16_t v[8];
+    f4_t b1[2], since[2], d[2];
+    h8_t q[2 * kS], p[8];
+    auto load_values = [&](int c) {
+      const uint32_t count = min(n - c * kChunk, kChunk);
+      const auto r =
+          buffer_of(values + (long long)c * kChunk * a.v_token, ((count - 1) * (uint32_t)a.v_token + value_size) * 2);
+      const auto f = of_factors(c);
+#pragma unroll
+      for (int z = 0; z < 8; ++z) v[z] = __builtin_amdgcn_raw_buffer_load_b16(r, v_at[z], 0, 0);
+#pragma unroll
+      for (int y = 0; y < 2; ++y) b1[y] = rows4(f, 0, y);
+    };
+    auto give_values = [&] {
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        f4_t x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = b1[y][e] * pair_lo<kBf16>(v[4 * y + e]);
+        rows_v[tile][2 * half + y][lane] = x;
+      }
+    };
+    auto load_queries = [&](int c) {
+      const auto qs = of_qk(ws.q, c);
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int t = 0; t < kS; ++t) q[y * kS + t] = load_piece(qs, piece_at + ((2 * half + y) * kS + t) * 1024);
+    };
+    load_values(0);
     bring(0);
-    Operands even, odd;  // of chunks c - 1 and c, in turn
-    for (int c = 0; c <= chunks; c += 2) {
-      outputs(c, odd, even);
-      if (c + 1 <= chunks) outputs(c + 1, even, odd);
+    load_queries(0);
+    give_values();
+    f4_t x[2][2], y2[2];
+    for (int c = 0; c <= chunks; ++c) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // bring()'s pieces are in LDS
+      __syncthreads();
+      if (c > 0) {
+        const int at = c - 1;
+        f4_t wv[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) wv[t] = left_w[tile][t][lane];
+        const float ds0 = left_scale[tile][0][i], ds1 = left_scale[tile][1][i];
+        float down = left_scale[tile][2][i];
+        float m = fmaxf(max4(wv[0]), max4(wv[1]));
+        if (half) m = fmaxf(m, fmaxf(max4(wv[2]), max4(wv[3])));
+        const int shift = column_shift(m);
+        const float up = power2(shift);
+        down *= power2(-shift) / kScoreScale;
+        y2[0] = y2[1] = kZero;
+        h8_t hi, lo;
+        split_tiles(wv[0], wv[1], up, &hi, &lo);
+        // Rows 0 .. 31 have pieces 0 and 1, rows 32 .. 63 have 2 to 5, two parts each.
+        if (half) {
+#pragma unroll
+          for (int part = 0; part < 3; ++part)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) y2[y] = mfma(p[4 * y + (part == 2)], part == 1 ? lo : hi, y2[y]);
+          split_tiles(wv[2], wv[3], up, &hi, &lo);
+#pragma unroll
+          for (int part = 0; part < 3; ++part)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) y2[y] = mfma(p[4 * y + 2 + (part == 2)], part == 1 ? lo : hi, y2[y]);
+        } else {
+#pragma unroll
+          for (int part = 0; part < 3; ++part)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) y2[y] = mfma(p[2 * y + (part == 2)], part == 1 ? lo : hi, y2[y]);
+        }
+        const uint32_t count = min(n - at * kChunk, kChunk);
+        const auto r = buffer_of(out + (long long)at * kChunk * out_token, ((count - 1) * out_token + value_size) * 2);
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float held = fmaf(ds0, x[0][y][e], ds1 * x[1][y][e]);
+            const float o = d[y][e] * fmaf(y2[y][e], down, since[y][e] * held);
+            __builtin_amdgcn_raw_buffer_store_b16(to_half_bits<kType>(o), r, out_at[4 * y + e], 0, 0);
+          }
+      }
+      if (c == chunks) break;
+      __syncthreads();
+      h8_t sp[2 * kS];
+#pragma unroll
+      for (int t = 0; t < 2 * kS; ++t) sp[t] = left_s[tile][t][lane];
+      const bool more = c + 1 < chunks;
+      if (more) {
+        load_values(c + 1);
+        bring(c + 1);
+      }
+      {
+        const auto ps = of_v(ws.p, c), f = of_factors(c);
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          since[y] = rows4(f, 2, y);
+          d[y] = rows4(f, 3, y);
+        }
+#pragma unroll
+        for (int z = 0; z < 8; ++z)
+          if (z < 4 || half) p[z] = load_piece(ps, piece_at + (4 * half + z) * 1024);
+      }
+#pragma unroll
+      for (int y = 0; y < 2; ++y) x[0][y] = x[1][y] = kZero;
+#pragma unroll
+      for (int t = 0; t < kS; ++t)
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) x[t / kHalfS][y] = mfma(q[y * kS + t], sp[2 * t + part], x[t / kHalfS][y]);
+      if (more) {
+        load_queries(c + 1);
+        give_values();
+      }
     }
   }
 }
@@ -675,17 +727,26 @@ int delta_chunk_launch(const DeltaArgs& a, int key_size, int value_size, bool bf
   size_t bytes;
   const ChunkSpace ws = chunk_space(workspace, a.tokens, a.requests, a.qk_heads, a.v_heads, key_size, &bytes);
   const dim3 chunks((unsigned)(slots_of(a.tokens, a.requests) * a.v_heads));
-  const dim3 columns((unsigned)(a.v_heads * (value_size / (16 * kScanTiles))), (unsigned)a.requests);
-  auto launch = [&](auto prepare, auto scan) {
+  // Tiles of 16 columns: two a workgroup where one each would not be at work at
+  // once (its LDS leaves one workgroup a CU).
+  const long long tiles = (long long)a.requests * a.v_heads * (value_size / 16);
+  const int cols = tiles > 256 ? 2 : 1;
+  const dim3 columns((unsigned)(a.v_heads * (value_size / (16 * cols))), (unsigned)a.requests);
+  auto launch = [&](auto prepare, auto one, auto two) {
     hipLaunchKernelGGL(prepare, chunks, dim3(256), 0, stream, a, ws);
-    hipLaunchKernelGGL(scan, columns, dim3(256), 0, stream, a, ws, value_size);
+    if (cols == 1) hipLaunchKernelGGL(one, columns, dim3(256), 0, stream, a, ws, value_size);
+    else hipLaunchKernelGGL(two, columns, dim3(512), 0, stream, a, ws, value_size);
   };
+  auto pick = [&](auto dk, auto type) {
+    constexpr int d = decltype(dk)::value;
+    constexpr bool t = decltype(type)::value;
+    launch(delta_prepare_kernel<d, t>, delta_scan_kernel<d, 1, t>, delta_scan_kernel<d, 2, t>);
+  };
+  using std::integral_constant;
   if (key_size == 64)
-    bf16 ? launch(delta_prepare_kernel<64, true>, delta_scan_kernel<64, true>)
-         : launch(delta_prepare_kernel<64, false>, delta_scan_kernel<64, false>);
+    bf16 ? pick(integral_constant<int, 64>{}, std::true_type{}) : pick(integral_constant<int, 64>{}, std::false_type{});
   else
-    bf16 ? launch(delta_prepare_kernel<128, true>, delta_scan_kernel<128, true>)
-         : launch(delta_prepare_kernel<128, false>, delta_scan_kernel<128, false>);
+    bf16 ? pick(integral_constant<int, 128>{}, std::true_type{}) : pick(integral_constant<int, 128>{}, std::false_type{});
   return check_launch("delta_rule launch");
 }
 
