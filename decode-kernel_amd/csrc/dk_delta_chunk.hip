@@ -395,6 +395,10 @@ __device__ __forceinline__ constexpr int piece_of(int y, int t) {
   return (y == 0 ? 0 : y == 1 ? 1 : y == 2 ? 2 : 4) + t;
 }
 
+// A barrier for what was read from and written to LDS: __syncthreads() waits for
+// loads to LDS too, which the output waves have under way across it.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 template <int kDk, int kCols, bool kBf16>
 __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a, ChunkSpace ws, int value_size) {
   constexpr int kS = kDk / 32, kHalfS = kS / 2, kHalfTiles = kDk / 32;
@@ -403,7 +407,7 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
   constexpr int kPieces = kKeys + kInverse + kTurned + 2;
   constexpr f4_t kZero{0.f, 0.f, 0.f, 0.f};
   __shared__ h8_t stage[2][kPieces][64];         // a chunk's operands and its rows' factors
-  __shared__ f4_t rows_v[kCols][4][64];          // beta c v of a chunk's rows
+  __shared__ f4_t rows_v[2][kCols][4][64];       // beta c v of a chunk's rows
   __shared__ f4_t share[kCols][2][4][64];        // a half's share of K' S
   __shared__ h8_t left_s[kCols][2 * kS][64];     // the state's parts
   __shared__ f4_t left_w[kCols][4][64];          // the corrections
@@ -434,7 +438,7 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[t][e] = fresh ? 0.f : state[(long long)(16 * t + 4 * q4 + e) * value_size];
     for (int c = 0; c <= chunks; ++c) {
-      __syncthreads();
+      lds_barrier();
       if (c == chunks) break;
       const h8_t(*keys)[64] = &stage[c & 1][0];
       const h8_t(*inverse)[64] = &stage[c & 1][kKeys];
@@ -479,10 +483,10 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
       f4_t bv[4], b2[4], until[4];
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
-        bv[y] = rows_v[tile][y][lane];
+        bv[y] = rows_v[c & 1][tile][y][lane];
         b2[y] = rows4(1, y);
       }
-      __syncthreads();
+      lds_barrier();
       f4_t other[4];
 #pragma unroll
       for (int y = 0; y < 4; ++y) other[y] = share[tile][1 - half][y][lane];
@@ -567,23 +571,17 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
       return buffer_of(reinterpret_cast<const char*>(ws.s) + (h * ws.slots + slot0 + c) * kFactorBytes, kFactorBytes);
     };
     const uint32_t piece_at = lane * 16;
-    // The rows 32 half .. 32 half + 31 of a chunk are this wave's.
-    auto rows4 = [&](__amdgpu_buffer_rsrc_t r, int which, int y) {
-      return __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(
-                                          r, 16 * q4 + (which * kChunk + 32 * half + 16 * y) * 4, 0, 0));
-    };
     const uint16_t* values = a.v + (long long)from * a.v_token + (long long)h * a.v_head;
     uint16_t* out = a.out + ((long long)from * a.v_heads + h) * value_size;
     const uint32_t out_token = a.v_heads * value_size;
-    uint32_t v_at[8], out_at[8];
+    // Of a chunk's outputs the rows 32 half .. 32 half + 31 are this wave's, and of
+    // its values, a row a lane, the columns 8 half .. 8 half + 7.
+    uint32_t out_at[8];
 #pragma unroll
-    for (int z = 0; z < 8; ++z) {
-      const uint32_t row = 32 * half + 16 * (z >> 2) + (z & 3) + 4 * q4;
-      v_at[z] = (row * (uint32_t)a.v_token + col) * 2;
-      out_at[z] = (row * out_token + col) * 2;
-    }
+    for (int z = 0; z < 8; ++z) out_at[z] = ((32 * half + 16 * (z >> 2) + (z & 3) + 4 * q4) * out_token + col) * 2;
+    const uint32_t v_at = (lane * (uint32_t)a.v_token + col - i + 8 * half) * 2;
     // All output waves bring a chunk's operands, each its share of the pieces.
-    auto bring = [&](int c) {
+    auto bring = [&](int c, int which) {
       h8_t* to = &stage[c & 1][0][0];
       auto some = [&](__amdgpu_buffer_rsrc_t r, int first, int count) {
 #pragma unroll
@@ -592,31 +590,31 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
             __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(to + (first + p + wave - 2 * kCols) * 64), 16,
                                                      piece_at + (p + wave - 2 * kCols) * 1024, 0, 0, 0);
       };
-      some(of_qk(ws.k, c), 0, kKeys);
-      some(of_v(ws.t, c), kKeys, kInverse);
-      some(of_qk(ws.kt, c), kKeys + kInverse, kTurned);
-      some(of_factors(c), kKeys + kInverse + kTurned, 2);
+      if (which == 0) {
+        some(of_qk(ws.k, c), 0, kKeys);
+      } else {
+        some(of_v(ws.t, c), kKeys, kInverse);
+        some(of_qk(ws.kt, c), kKeys + kInverse, kTurned);
+        some(of_factors(c), kKeys + kInverse + kTurned, 2);
+      }
     };
-    uint16_t v[8];
-    f4_t b1[2], since[2], d[2];
+    uint4 v;
+    float b1;
     h8_t q[2 * kS], p[8];
     auto load_values = [&](int c) {
       const uint32_t count = min(n - c * kChunk, kChunk);
       const auto r =
           buffer_of(values + (long long)c * kChunk * a.v_token, ((count - 1) * (uint32_t)a.v_token + value_size) * 2);
-      const auto f = of_factors(c);
-#pragma unroll
-      for (int z = 0; z < 8; ++z) v[z] = __builtin_amdgcn_raw_buffer_load_b16(r, v_at[z], 0, 0);
-#pragma unroll
-      for (int y = 0; y < 2; ++y) b1[y] = rows4(f, 0, y);
+      v = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, v_at, 0, 0));
+      b1 = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(of_factors(c), lane * 4, 0, 0));
     };
-    auto give_values = [&] {
+    auto give_values = [&](int c) {  // to where a result tile has row `lane`
+      float* to = reinterpret_cast<float*>(&rows_v[c & 1][tile][lane >> 4][8 * half + 16 * ((lane & 15) >> 2)]) + (lane & 3);
+      const uint32_t pairs[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        f4_t x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = b1[y][e] * pair_lo<kBf16>(v[4 * y + e]);
-        rows_v[tile][2 * half + y][lane] = x;
+      for (int j = 0; j < 4; ++j) {
+        to[8 * j] = b1 * pair_lo<kBf16>(pairs[j]);
+        to[8 * j + 4] = b1 * pair_hi<kBf16>(pairs[j]);
       }
     };
     auto load_queries = [&](int c) {
@@ -627,18 +625,29 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
         for (int t = 0; t < kS; ++t) q[y * kS + t] = load_piece(qs, piece_at + ((2 * half + y) * kS + t) * 1024);
     };
     load_values(0);
-    bring(0);
+    bring(0, 0);
+    bring(0, 1);
     load_queries(0);
-    give_values();
+    give_values(0);
     f4_t x[2][2], y2[2];
     for (int c = 0; c <= chunks; ++c) {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // bring()'s pieces are in LDS
-      __syncthreads();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0);  // bring()'s pieces are in LDS
+      lds_barrier();
+      const bool more = c + 1 < chunks;
+      if (more) load_values(c + 1);
       if (c > 0) {
         const int at = c - 1;
         f4_t wv[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) wv[t] = left_w[tile][t][lane];
+        const float* factors = reinterpret_cast<const float*>(&stage[at & 1][kKeys + kInverse + kTurned][0]);
+        f4_t since[2], d[2];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          since[y] = *reinterpret_cast<const f4_t*>(factors + 2 * kChunk + 32 * half + 16 * y + 4 * q4);
+          d[y] = *reinterpret_cast<const f4_t*>(factors + 3 * kChunk + 32 * half + 16 * y + 4 * q4);
+        }
         const float ds0 = left_scale[tile][0][i], ds1 = left_scale[tile][1][i];
         float down = left_scale[tile][2][i];
         float m = fmaxf(max4(wv[0]), max4(wv[1]));
@@ -678,26 +687,18 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
           }
       }
       if (c == chunks) break;
-      __syncthreads();
+      if (more) {
+        // Stores to LDS and reads of it behind bring() would wait for what it
+        // asked for. The state waves are through with chunk c - 1's keys.
+        give_values(c + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        bring(c + 1, 0);
+      }
+      lds_barrier();
       h8_t sp[2 * kS];
 #pragma unroll
       for (int t = 0; t < 2 * kS; ++t) sp[t] = left_s[tile][t][lane];
-      const bool more = c + 1 < chunks;
-      if (more) {
-        load_values(c + 1);
-        bring(c + 1);
-      }
-      {
-        const auto ps = of_v(ws.p, c), f = of_factors(c);
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          since[y] = rows4(f, 2, y);
-          d[y] = rows4(f, 3, y);
-        }
-#pragma unroll
-        for (int z = 0; z < 8; ++z)
-          if (z < 4 || half) p[z] = load_piece(ps, piece_at + (4 * half + z) * 1024);
-      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int y = 0; y < 2; ++y) x[0][y] = x[1][y] = kZero;
 #pragma unroll
@@ -706,10 +707,15 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
         for (int part = 0; part < 2; ++part)
 #pragma unroll
           for (int y = 0; y < 2; ++y) x[t / kHalfS][y] = mfma(q[y * kS + t], sp[2 * t + part], x[t / kHalfS][y]);
+      __builtin_amdgcn_sched_barrier(0);
       if (more) {
         load_queries(c + 1);
-        give_values();
+        bring(c + 1, 1);
       }
+      const auto ps = of_v(ws.p, c);
+#pragma unroll
+      for (int z = 0; z < 8; ++z)
+        if (z < 4 || half) p[z] = load_piece(ps, piece_at + (4 * half + z) * 1024);
     }
   }
 }
