@@ -185,7 +185,6 @@ __global__ __launch_bounds__(256) void short_conv_kernel(ConvArgs a) {
   constexpr int kEach = kWide ? 8 : 1, kPast = kWidth - 1;
   constexpr int kType = kBf16 ? DK_KV_BF16 : DK_KV_F16;
   using Part = typename std::conditional<kWide, uint4, uint16_t>::type;
-  __shared__ int shared[2];
   const int c = (blockIdx.y * 256 + threadIdx.x) * kEach;
   const bool mine = c < a.channels;
   auto clear = [&](long long from, long long to) {
@@ -196,7 +195,7 @@ __global__ __launch_bounds__(256) void short_conv_kernel(ConvArgs a) {
   if (a.offsets) {
     const long long part = (long long)blockIdx.x * kConvTile;
     if (a.requests == 0 ||
-        !find_tile(a.offsets, a.requests, a.tokens, kConvTile, blockIdx.x, shared, &tile)) {
+        !find_tile(a.offsets, a.requests, a.tokens, kConvTile, blockIdx.x, &tile)) {
       clear(min(part, (long long)a.tokens), min(part + kConvTile, (long long)a.tokens));
       return;
     }

@@ -54,35 +54,27 @@ struct Tile {
   int index;    // which tile of its request
 };
 
-// By a whole workgroup: the tile with number `number`, and whether offsets
-// are good. shared: 2 ints.
+// The tile with number `number`, and whether offsets are good; by each wave for
+// itself, with the same answer in all.
 __device__ __forceinline__ bool find_tile(const int32_t* offsets, int requests, int tokens, int tile,
-                                          int number, int* shared, Tile* out) {
+                                          int number, Tile* out) {
+  const int lane = threadIdx.x & 63;
   int begun = 0;  // requests whose tiles begin at or before the number
-  bool bad = false;
-  for (int i = threadIdx.x; i < requests; i += blockDim.x) {
-    const int from = offsets[i], to = offsets[i + 1];
-    bad |= to < from;
-    begun += from / tile + i <= number;
+  bool bad = lane == 0 && (offsets[0] < 0 || offsets[requests] > tokens);
+  for (int first = 0; first < requests; first += 64) {
+    const int i = first + lane;
+    bool before = false;
+    if (i < requests) {
+      const int from = offsets[i];
+      bad |= offsets[i + 1] < from;
+      before = from / tile + i <= number;
+    }
+    begun += __popcll(__ballot(before));
   }
-  if (threadIdx.x == 0) {
-    bad |= offsets[0] < 0 || offsets[requests] > tokens;
-    shared[0] = 0;
-    shared[1] = 0;
-  }
-  __syncthreads();
-  const unsigned long long any = __ballot(bad);
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) begun += __shfl_xor(begun, d);
-  if ((threadIdx.x & 63) == 0) {
-    atomicAdd(&shared[0], begun);
-    if (any) atomicOr(&shared[1], 1);
-  }
-  __syncthreads();
   out->request = -1;
   out->row = out->count = out->index = 0;
-  if (shared[1]) return false;
-  const int b = shared[0] - 1;
+  if (__ballot(bad)) return false;
+  const int b = begun - 1;
   if (b < 0) return true;
   const int from = offsets[b], n = offsets[b + 1] - from;
   const int index = number - (from / tile + b);

@@ -91,6 +91,11 @@ __device__ __forceinline__ f4_t mfma32(float a, float b, f4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
+// Piece (row tile y, columns 32 t ..) of a lower triangle.
+__device__ __forceinline__ constexpr int piece_of(int y, int t) {
+  return (y == 0 ? 0 : y == 1 ? 1 : y == 2 ? 2 : 4) + t;
+}
+
 __device__ __forceinline__ int exponent_of(float m) {
   return (int)(__builtin_bit_cast(uint32_t, m) >> 23 & 0xFF) - 127;
 }
@@ -140,104 +145,109 @@ __device__ __forceinline__ void split_tiles(f4_t x, f4_t y, float scale, h8_t* h
 constexpr int kPad = 68;  // floats a row of 64 takes in LDS
 
 template <int kDk, bool kBf16>
-__global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, ChunkSpace ws) {
+__global__ __launch_bounds__(256, 4) void delta_prepare_kernel(DeltaArgs a, ChunkSpace ws) {
   constexpr int kS = kDk / 32;
   __shared__ h8_t keys[4][kS][64];
   __shared__ float m[kChunk][kPad];
-  __shared__ float c_of[kChunk], d_of[kChunk], hi_of[kChunk], lo_of[kChunk], b2_of[kChunk];
-  __shared__ int found[2];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, i = lane & 15, q4 = lane >> 4;
+  __shared__ float c_of[kChunk], d_of[kChunk], beta_of[kChunk], hi_of[kChunk], lo_of[kChunk];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, i = lane & 15, q4 = lane >> 4;
   const long long slot = blockIdx.x / a.v_heads;
   const int h = blockIdx.x % a.v_heads, hq = h / a.group;
   Tile tile;
-  if (!find_tile(a.offsets, a.requests, a.tokens, kChunk, (int)slot, found, &tile)) return;
+  if (!find_tile(a.offsets, a.requests, a.tokens, kChunk, (int)slot, &tile)) return;
   if (tile.request < 0) return;
   if (a.offsets[tile.request + 1] - a.offsets[tile.request] <= a.limit) return;
   const bool first_of_group = h % a.group == 0;
 
-  // Rows of keys and queries, scaled to fp16.
+  // Every load first; rows behind the last are row 0 again, and zeros below.
   const int r = 16 * wave + i;
   const bool real = r < tile.count;
+  const long long row = tile.row + (real ? r : 0);
+  const uint16_t* kp = a.k + row * a.k_token + (long long)hq * a.k_head + 4 * q4;
+  const uint16_t* qp = a.q + row * a.q_token + (long long)hq * a.q_head + 4 * q4;
+  uint2 k_raw[2 * kS], q_raw[2 * kS];
+#pragma unroll
+  for (int s = 0; s < 2 * kS; ++s) k_raw[s] = *reinterpret_cast<const uint2*>(kp + 16 * s);
+#pragma unroll
+  for (int s = 0; s < 2 * kS; ++s) q_raw[s] = *reinterpret_cast<const uint2*>(qp + 16 * s);
+  const bool live = lane < tile.count;
+  double g = 0.0;
+  float beta = 0.f;
+  if (wave == 0) {
+    const long long at = (long long)(tile.row + (live ? lane : 0)) * a.v_heads + h;
+    g = (double)cut_log(a.log_decay[at]);
+    beta = a.beta[at];
+  }
+
+  // Rows of keys and queries, scaled to fp16.
   h8_t kf[kS], qf[kS];
-  auto rows = [&](const uint16_t* x, h8_t(&f)[kS], float* length2) {
-    uint2 raw[kS][2];
-#pragma unroll
-    for (int s = 0; s < kS; ++s)
-#pragma unroll
-      for (int p = 0; p < 2; ++p)
-        raw[s][p] = real ? *reinterpret_cast<const uint2*>(x + 32 * s + 16 * p + 4 * q4) : make_uint2(0u, 0u);
+  auto rows = [&](const uint2(&raw)[2 * kS], h8_t(&f)[kS], float* length2) {
     float top = 0.f, sum = 0.f;
+    float e[kS][8];
 #pragma unroll
-    for (int s = 0; s < kS; ++s)
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const float e[4] = {pair_lo<kBf16>(raw[s][p].x), pair_hi<kBf16>(raw[s][p].x),
-                            pair_lo<kBf16>(raw[s][p].y), pair_hi<kBf16>(raw[s][p].y)};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          top = fmaxf(top, fabsf(e[j]));
-          sum = fmaf(e[j], e[j], sum);
-        }
-      }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
+    for (int s = 0; s < 2 * kS; ++s) {
+      const uint32_t x = real ? raw[s].x : 0u, y = real ? raw[s].y : 0u;
+      float* to = e[s >> 1] + 4 * (s & 1);
+      to[0] = pair_lo<kBf16>(x);
+      to[1] = pair_hi<kBf16>(x);
+      to[2] = pair_lo<kBf16>(y);
+      to[3] = pair_hi<kBf16>(y);
+      top = fmaxf(fmaxf(top, fmaxf(fabsf(to[0]), fabsf(to[1]))), fmaxf(fabsf(to[2]), fabsf(to[3])));
+      sum += fmaf(to[0], to[0], to[1] * to[1]) + fmaf(to[2], to[2], to[3] * to[3]);
+    }
+    top = max_rows(top);
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
     const int e2 = exponent_of(top);
 #pragma unroll
     for (int s = 0; s < kS; ++s)
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        f[s][4 * p] = (_Float16)ldexpf(pair_lo<kBf16>(raw[s][p].x), -e2);
-        f[s][4 * p + 1] = (_Float16)ldexpf(pair_hi<kBf16>(raw[s][p].x), -e2);
-        f[s][4 * p + 2] = (_Float16)ldexpf(pair_lo<kBf16>(raw[s][p].y), -e2);
-        f[s][4 * p + 3] = (_Float16)ldexpf(pair_hi<kBf16>(raw[s][p].y), -e2);
-      }
+      for (int j = 0; j < 8; ++j) f[s][j] = (_Float16)ldexpf(e[s][j], -e2);
     *length2 = sum;
     return top == 0.f ? INT32_MIN : e2;  // NaN has an exponent too
   };
-  const long long row = tile.row + (real ? r : 0);
   float kk, qq;
-  const int ke = rows(a.k + row * a.k_token + (long long)hq * a.k_head, kf, &kk);
-  const int qe = rows(a.q + row * a.q_token + (long long)hq * a.q_head, qf, &qq);
-  float c = 0.f, d = 0.f;  // a row of zeros has no part in anything
-  if (ke != INT32_MIN) c = ldexpf(a.normalize ? 1.f / sqrtf(kk + kUnitEps) : 1.f, ke);
-  if (qe != INT32_MIN) d = ldexpf(a.normalize ? a.scale / sqrtf(qq + kUnitEps) : a.scale, qe);
+  const int ke = rows(k_raw, kf, &kk);
   const size_t qk_at = (hq * ws.slots + slot) * (4 * kS * 64);
 #pragma unroll
   for (int s = 0; s < kS; ++s) {
     keys[wave][s][lane] = kf[s];
-    if (first_of_group) {
-      ws.k[qk_at + (wave * kS + s) * 64 + lane] = kf[s];
-      ws.q[qk_at + (wave * kS + s) * 64 + lane] = qf[s];
-    }
+    if (first_of_group) ws.k[qk_at + (wave * kS + s) * 64 + lane] = kf[s];
   }
+  const int qe = rows(q_raw, qf, &qq);
+  if (first_of_group)
+#pragma unroll
+    for (int s = 0; s < kS; ++s) ws.q[qk_at + (wave * kS + s) * 64 + lane] = qf[s];
+  float c = 0.f, d = 0.f;  // a row of zeros has no part in anything
+  if (ke != INT32_MIN) c = ldexpf(a.normalize ? 1.f / sqrtf(kk + kUnitEps) : 1.f, ke);
+  if (qe != INT32_MIN) d = ldexpf(a.normalize ? a.scale / sqrtf(qq + kUnitEps) : a.scale, qe);
   if (q4 == 0) {
     c_of[r] = c;
     d_of[r] = d;
   }
-  __syncthreads();
-
   // Sums of the decays' logarithms, in 64 bits: a sum's difference to another
   // has to be exact where both are large. Kept as two fp32, to the base 2.
+  float hi = 0.f, lo = 0.f, until = 0.f;
   if (wave == 0) {
-    const bool live = lane < tile.count;
-    const long long at = (long long)(tile.row + (live ? lane : 0)) * a.v_heads + h;
-    const float beta = live ? a.beta[at] : 0.f;
-    double g = live ? (double)cut_log(a.log_decay[at]) : 0.0;
+    if (!live) g = 0.0, beta = 0.f;
 #pragma unroll
     for (int dd = 1; dd < 64; dd *= 2) {
       const double o = __shfl_up(g, dd);
       if (lane >= dd) g += o;
     }
     g *= 1.4426950408889634074;  // log2(e)
-    const double rest = __shfl(g, 63) - g;
-    const float hi = (float)g, lo = (float)(g - (double)hi);
-    const float cc = c_of[lane], since = exp2f(hi) * fmaf(lo, 0.69314718f, 1.f);
-    const float until = exp2f((float)rest);
+    until = exp2f((float)(__shfl(g, 63) - g));
+    hi = (float)g;
+    lo = (float)(g - (double)hi);
     hi_of[lane] = hi;
     lo_of[lane] = lo;
-    b2_of[lane] = beta * cc * cc;
+    beta_of[lane] = beta;
+  }
+  __syncthreads();
+
+  if (wave == 0) {
+    const float cc = c_of[lane], since = exp2f(hi) * fmaf(lo, 0.69314718f, 1.f);
     float* f = ws.s + (h * ws.slots + slot) * (kFactors * kChunk) + lane;
     f[0] = beta * cc;
     f[64] = beta * cc * cc * since;
@@ -245,6 +255,81 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, ChunkSp
     f[192] = d_of[lane];
     f[256] = until;
     f[320] = __shfl(since, 63);
+  }
+  // Decayed products of the wave's rows with those before them.
+  const size_t v_at = (h * ws.slots + slot) * (kFragments * 2 * 64);
+  const int piece0 = piece_of(wave, 0);
+  auto pieces_out = [&](h8_t* to, float scale) {
+    for (int s = 0; s <= wave / 2; ++s) {
+      h8_t first, second;
+      const f4_t x = *reinterpret_cast<const f4_t*>(&m[16 * wave + i][32 * s + 4 * q4]);
+      const f4_t y = *reinterpret_cast<const f4_t*>(&m[16 * wave + i][32 * s + 16 + 4 * q4]);
+      split_tiles(x, y, scale, &first, &second);
+      to[v_at + (2 * (piece0 + s)) * 64 + lane] = first;
+      to[v_at + (2 * (piece0 + s) + 1) * 64 + lane] = second;
+    }
+  };
+  const int rr0 = 16 * wave + 4 * q4;
+  float hr[4], lr[4], b2[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    hr[e] = hi_of[rr0 + e];
+    lr[e] = lo_of[rr0 + e];
+    b2[e] = beta_of[rr0 + e] * c_of[rr0 + e] * c_of[rr0 + e];
+  }
+  f4_t kkt[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    f4_t qkt{0.f, 0.f, 0.f, 0.f};
+    kkt[j] = f4_t{0.f, 0.f, 0.f, 0.f};
+    const int col = 16 * j + i;
+    if (j <= wave) {
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        const h8_t b = keys[j][s][lane];
+        kkt[j] = mfma(kf[s], b, kkt[j]);
+        qkt = mfma(qf[s], b, qkt);
+      }
+      const float hc = hi_of[col], lc = lo_of[col];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float decay = exp2f((hr[e] - hc) + (lr[e] - lc));
+        qkt[e] = rr0 + e >= col ? decay * qkt[e] : 0.f;
+        kkt[j][e] = rr0 + e > col ? b2[e] * decay * kkt[j][e] : 0.f;
+      }
+    }
+    if (j <= (wave | 1))
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m[rr0 + e][col] = qkt[e];
+  }
+  // A wave's rows of m are its own until the barrier: P goes out from there, then
+  // A comes in.
+  pieces_out(ws.p, kScoreScale);
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (j <= (wave | 1))
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m[rr0 + e][16 * j + i] = kkt[j][e];
+
+  // T = (1 + A)^-1: the blocks of 16 on the diagonal by substitution, a lane a
+  // column, then the blocks below from them, a wave a column of blocks, with
+  // 32-bit matrix products:  T_ij = -T_ii sum_(j <= k < i) A_ik T_kj.
+  {
+    float t[16];
+    const int base = 16 * wave;
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      float even = x == i ? 1.f : 0.f, odd = 0.f;
+#pragma unroll
+      for (int k = 0; k < x; ++k) {
+        float& sum = k & 1 ? odd : even;
+        sum = fmaf(-m[base + x][base + k], t[k], sum);
+      }
+      t[x] = even + odd;
+    }
+    if (q4 == 0)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) m[base + x][base + i] = t[x];
   }
   // The transposed keys, element by element out of the operands' order.
   if (first_of_group) {
@@ -263,73 +348,6 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, ChunkSp
       }
       ws.kt[qk_at + f * 64 + lane] = x.v;
     }
-  }
-  f4_t kkt[4], qkt[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    kkt[j] = qkt[j] = f4_t{0.f, 0.f, 0.f, 0.f};
-    if (j <= wave) {
-#pragma unroll
-      for (int s = 0; s < kS; ++s) {
-        const h8_t b = keys[j][s][lane];
-        kkt[j] = mfma(kf[s], b, kkt[j]);
-        qkt[j] = mfma(qf[s], b, qkt[j]);
-      }
-    }
-  }
-  __syncthreads();
-
-  // Decayed products: P to LDS and out; A stays here.
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int col = 16 * j + i;
-    const float hc = hi_of[col], lc = lo_of[col];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int rr = 16 * wave + 4 * q4 + e;
-      const float decay = exp2f((hi_of[rr] - hc) + (lo_of[rr] - lc));
-      m[rr][col] = rr >= col ? decay * qkt[j][e] : 0.f;
-      kkt[j][e] = rr > col ? b2_of[rr] * decay * kkt[j][e] : 0.f;
-    }
-  }
-  const size_t v_at = (h * ws.slots + slot) * (kFragments * 2 * 64);
-  const int piece0 = wave == 0 ? 0 : wave == 1 ? 1 : wave == 2 ? 2 : 4;
-  auto pieces_out = [&](h8_t* to, float scale) {
-    for (int s = 0; s <= wave / 2; ++s) {
-      h8_t hi, lo;
-      const f4_t x = *reinterpret_cast<const f4_t*>(&m[16 * wave + i][32 * s + 4 * q4]);
-      const f4_t y = *reinterpret_cast<const f4_t*>(&m[16 * wave + i][32 * s + 16 + 4 * q4]);
-      split_tiles(x, y, scale, &hi, &lo);
-      to[v_at + (2 * (piece0 + s)) * 64 + lane] = hi;
-      to[v_at + (2 * (piece0 + s) + 1) * 64 + lane] = lo;
-    }
-  };
-  __syncthreads();
-  pieces_out(ws.p, kScoreScale);
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) m[16 * wave + 4 * q4 + e][16 * j + i] = kkt[j][e];
-  __syncthreads();
-
-  // T = (1 + A)^-1: the blocks of 16 on the diagonal by substitution, a lane a
-  // column, then the blocks below from them, a wave a column of blocks, with
-  // 32-bit matrix products:  T_ij = -T_ii sum_(j <= k < i) A_ik T_kj.
-  {
-    float t[16];
-    const int base = 16 * wave;
-#pragma unroll
-    for (int x = 0; x < 16; ++x) {
-      float sum = x == i ? 1.f : 0.f;
-#pragma unroll
-      for (int k = 0; k < x; ++k) sum = fmaf(-m[base + x][base + k], t[k], sum);
-      t[x] = sum;
-    }
-    __builtin_amdgcn_wave_barrier();
-    if (q4 == 0)
-#pragma unroll
-      for (int x = 0; x < 16; ++x) m[base + x][base + i] = t[x];
   }
   __syncthreads();
   f4_t below[4];
@@ -388,11 +406,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* base, ui
 
 __device__ __forceinline__ h8_t load_piece(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
   return __builtin_bit_cast(h8_t, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0));
-}
-
-// Piece (row tile y, columns 32 t ..) of a lower triangle.
-__device__ __forceinline__ constexpr int piece_of(int y, int t) {
-  return (y == 0 ? 0 : y == 1 ? 1 : y == 2 ? 2 : 4) + t;
 }
 
 // A barrier for what was read from and written to LDS: __syncthreads() waits for
