@@ -495,14 +495,14 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
       }
       f4_t bv[4], b2[4], until[4];
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        bv[y] = rows_v[c & 1][tile][y][lane];
-        b2[y] = rows4(1, y);
-      }
+      for (int y = 0; y < 4; ++y) bv[y] = rows_v[c & 1][tile][y][lane];
       lds_barrier();
       f4_t other[4];
 #pragma unroll
-      for (int y = 0; y < 4; ++y) other[y] = share[tile][1 - half][y][lane];
+      for (int y = 0; y < 4; ++y) {
+        other[y] = share[tile][1 - half][y][lane];
+        b2[y] = rows4(1, y);
+      }
 #pragma unroll
       for (int z = 0; z < kInverse; ++z) tf[z] = inverse[z][lane];
 #pragma unroll
@@ -638,30 +638,24 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
         for (int t = 0; t < kS; ++t) q[y * kS + t] = load_piece(qs, piece_at + ((2 * half + y) * kS + t) * 1024);
     };
     load_values(0);
+    give_values(0);
+    if (chunks > 1) load_values(1);
     bring(0, 0);
     bring(0, 1);
     load_queries(0);
-    give_values(0);
-    f4_t x[2][2], y2[2];
+    if (chunks > 1) bring(1, 0);
+    f4_t x[2], d[2], y2[2];  // of the last chunk: e^G Q' S, and the queries' factors
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0);  // chunk 0's operands are in LDS
+    asm volatile("" ::: "memory");
     for (int c = 0; c <= chunks; ++c) {
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_waitcnt(0);  // bring()'s pieces are in LDS
       lds_barrier();
       const bool more = c + 1 < chunks;
-      if (more) load_values(c + 1);
       if (c > 0) {
         const int at = c - 1;
         f4_t wv[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) wv[t] = left_w[tile][t][lane];
-        const float* factors = reinterpret_cast<const float*>(&stage[at & 1][kKeys + kInverse + kTurned][0]);
-        f4_t since[2], d[2];
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          since[y] = *reinterpret_cast<const f4_t*>(factors + 2 * kChunk + 32 * half + 16 * y + 4 * q4);
-          d[y] = *reinterpret_cast<const f4_t*>(factors + 3 * kChunk + 32 * half + 16 * y + 4 * q4);
-        }
-        const float ds0 = left_scale[tile][0][i], ds1 = left_scale[tile][1][i];
         float down = left_scale[tile][2][i];
         float m = fmaxf(max4(wv[0]), max4(wv[1]));
         if (half) m = fmaxf(m, fmaxf(max4(wv[2]), max4(wv[3])));
@@ -688,47 +682,68 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
 #pragma unroll
             for (int y = 0; y < 2; ++y) y2[y] = mfma(p[2 * y + (part == 2)], part == 1 ? lo : hi, y2[y]);
         }
+        if (more) give_values(c + 1);
+        __builtin_amdgcn_sched_barrier(0);
         const uint32_t count = min(n - at * kChunk, kChunk);
         const auto r = buffer_of(out + (long long)at * kChunk * out_token, ((count - 1) * out_token + value_size) * 2);
 #pragma unroll
         for (int y = 0; y < 2; ++y)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float held = fmaf(ds0, x[0][y][e], ds1 * x[1][y][e]);
-            const float o = d[y][e] * fmaf(y2[y][e], down, since[y][e] * held);
+            const float o = d[y][e] * fmaf(y2[y][e], down, x[y][e]);
             __builtin_amdgcn_raw_buffer_store_b16(to_half_bits<kType>(o), r, out_at[4 * y + e], 0, 0);
           }
       }
       if (c == chunks) break;
-      if (more) {
-        // Stores to LDS and reads of it behind bring() would wait for what it
-        // asked for. The state waves are through with chunk c - 1's keys.
-        give_values(c + 1);
-        __builtin_amdgcn_sched_barrier(0);
-        bring(c + 1, 0);
+      // All that was asked for in the last turn is there, but not yet the 8 stores
+      // above have to be.
+      if (c > 0) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xF78);  // vmcnt(8)
+        asm volatile("" ::: "memory");
+      } else if (more) {
+        give_values(1);
       }
       lds_barrier();
       h8_t sp[2 * kS];
 #pragma unroll
       for (int t = 0; t < 2 * kS; ++t) sp[t] = left_s[tile][t][lane];
+      const float ds0 = left_scale[tile][0][i], ds1 = left_scale[tile][1][i];
+      const float* factors = reinterpret_cast<const float*>(&stage[c & 1][kKeys + kInverse + kTurned][0]);
+      f4_t since[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        since[y] = *reinterpret_cast<const f4_t*>(factors + 2 * kChunk + 32 * half + 16 * y + 4 * q4);
+        d[y] = *reinterpret_cast<const f4_t*>(factors + 3 * kChunk + 32 * half + 16 * y + 4 * q4);
+      }
       __builtin_amdgcn_sched_barrier(0);
+      f4_t x0[2] = {kZero, kZero}, x1[2] = {kZero, kZero};  // of the state's halves
 #pragma unroll
-      for (int y = 0; y < 2; ++y) x[0][y] = x[1][y] = kZero;
-#pragma unroll
-      for (int t = 0; t < kS; ++t)
+      for (int t = 0; t < kHalfS; ++t)
 #pragma unroll
         for (int part = 0; part < 2; ++part)
 #pragma unroll
-          for (int y = 0; y < 2; ++y) x[t / kHalfS][y] = mfma(q[y * kS + t], sp[2 * t + part], x[t / kHalfS][y]);
+          for (int y = 0; y < 2; ++y) {
+            x0[y] = mfma(q[y * kS + t], sp[2 * t + part], x0[y]);
+            x1[y] = mfma(q[y * kS + kHalfS + t], sp[2 * (kHalfS + t) + part], x1[y]);
+          }
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[y][e] = since[y][e] * fmaf(ds0, x0[y][e], ds1 * x1[y][e]);
       __builtin_amdgcn_sched_barrier(0);
-      if (more) {
-        load_queries(c + 1);
-        bring(c + 1, 1);
-      }
+      // In the order in which it is waited for. The state waves are through with
+      // this chunk's keys and with all of the last one's operands.
       const auto ps = of_v(ws.p, c);
 #pragma unroll
       for (int z = 0; z < 8; ++z)
         if (z < 4 || half) p[z] = load_piece(ps, piece_at + (4 * half + z) * 1024);
+      if (more) {
+        if (c + 2 < chunks) load_values(c + 2);
+        bring(c + 1, 1);
+        load_queries(c + 1);
+        if (c + 2 < chunks) bring(c + 2, 0);
+      }
     }
   }
 }
