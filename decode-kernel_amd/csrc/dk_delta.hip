@@ -164,10 +164,8 @@ __global__ __launch_bounds__(64) void delta_step_kernel(DeltaArgs a, int value_s
 // that each input is read once but for the width - 1 before a tile. The tile
 // that holds a request's first tokens is the only reader of its window, so
 // the same threads write it. Bound by HBM for prompts and by latency for
-// single tokens.
+// single tokens: every load is asked for before the first is waited for.
 // ---------------------------------------------------------------------------
-constexpr int kConvTile = 16;
-
 struct ConvArgs {
   const uint16_t* x;
   long long x_token;
@@ -180,7 +178,14 @@ struct ConvArgs {
   int tokens, requests, channels, silu;
 };
 
-template <int kWidth, bool kBf16, bool kWide>
+// z / (1 + e^-z) on the hardware's exponential and reciprocal, 1 ulp each: with
+// a division and expf() the arithmetic of 67 million elements takes as long as
+// their bytes (62 of 80 us).
+__device__ __forceinline__ float silu_of(float z) {
+  return z * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f));
+}
+
+template <int kWidth, int kTile, bool kBf16, bool kWide>
 __global__ __launch_bounds__(256) void short_conv_kernel(ConvArgs a) {
   constexpr int kEach = kWide ? 8 : 1, kPast = kWidth - 1;
   constexpr int kType = kBf16 ? DK_KV_BF16 : DK_KV_F16;
@@ -192,17 +197,18 @@ __global__ __launch_bounds__(256) void short_conv_kernel(ConvArgs a) {
       for (long long t = from; t < to; ++t) *reinterpret_cast<Part*>(a.y + t * a.channels + c) = Part{};
   };
   Tile tile{(int)blockIdx.x, (int)blockIdx.x, 1, 0};
+  int n = 1;  // the request's new tokens
   if (a.offsets) {
-    const long long part = (long long)blockIdx.x * kConvTile;
-    if (a.requests == 0 ||
-        !find_tile(a.offsets, a.requests, a.tokens, kConvTile, blockIdx.x, &tile)) {
-      clear(min(part, (long long)a.tokens), min(part + kConvTile, (long long)a.tokens));
+    const long long part = (long long)blockIdx.x * kTile;
+    if (a.requests == 0 || !find_tile(a.offsets, a.requests, a.tokens, kTile, blockIdx.x, &tile)) {
+      clear(min(part, (long long)a.tokens), min(part + kTile, (long long)a.tokens));
       return;
     }
     const long long head = a.offsets[0], end = a.offsets[a.requests];
-    clear(min(part, head), min(part + kConvTile, head));
-    clear(min(end + part, (long long)a.tokens), min(end + part + kConvTile, (long long)a.tokens));
+    clear(min(part, head), min(part + kTile, head));
+    clear(min(end + part, (long long)a.tokens), min(end + part + kTile, (long long)a.tokens));
     if (tile.request < 0) return;
+    n = a.offsets[tile.request + 1] - a.offsets[tile.request];
   }
   if (!mine) return;
 
@@ -218,44 +224,48 @@ __global__ __launch_bounds__(256) void short_conv_kernel(ConvArgs a) {
       f[0] = pair_lo<kBf16>(p);
     }
   };
+  // Rows before the request's first come from the window, those behind the
+  // tile's last are that one again.
   const uint16_t* x = a.x + (long long)tile.row * a.x_token + c;
-  Part in[kPast + kConvTile];  // the inputs before the tile, then its own
-#pragma unroll
-  for (int i = 0; i < kConvTile; ++i)
-    in[kPast + i] = i < tile.count ? *reinterpret_cast<const Part*>(x + (long long)i * a.x_token) : Part{};
   uint16_t* window = a.windows + (long long)tile.request * kPast * a.channels + c;
-  if (tile.index == 0) {
-    const bool fresh = a.held && a.held[tile.request] <= 0;
+  const bool first = tile.index == 0;
+  Part in[kPast + kTile];
+#pragma unroll
+  for (int i = 0; i < kPast; ++i)
+    in[i] = *reinterpret_cast<const Part*>(first ? window + (long long)i * a.channels
+                                                 : x + (long long)(i - kPast) * a.x_token);
+#pragma unroll
+  for (int i = 0; i < kTile; ++i)
+    in[kPast + i] = *reinterpret_cast<const Part*>(x + (long long)min(i, tile.count - 1) * a.x_token);
+  Part w_raw[kWidth];
+#pragma unroll
+  for (int i = 0; i < kWidth; ++i)  // 8 channels' weights are kWidth pieces of 16 bytes in a row
+    w_raw[i] = *reinterpret_cast<const Part*>(a.weight + (long long)c * kWidth + kEach * i);
+  if (first) {
+    if (a.held && a.held[tile.request] <= 0)
+#pragma unroll
+      for (int i = 0; i < kPast; ++i) in[i] = Part{};
+    // The window's row i is then the request's new row n - kPast + i, or, where
+    // that is below 0, its own row n + i.
+    Part keep[kPast];
 #pragma unroll
     for (int i = 0; i < kPast; ++i)
-      in[i] = fresh ? Part{} : *reinterpret_cast<const Part*>(window + (long long)i * a.channels);
-    const int n = a.offsets ? a.offsets[tile.request + 1] - tile.row : 1;
+      keep[i] = *reinterpret_cast<const Part*>(x + (long long)max(n - kPast + i, 0) * a.x_token);
 #pragma unroll
     for (int i = 0; i < kPast; ++i) {
-      // Place n - kPast + i among the request's new tokens; below 0 it is the
-      // window's, and its number there (n + i) is small.
-      const int at = n - kPast + i;
-      Part w{};
-      if (at >= 0) w = *reinterpret_cast<const Part*>(x + (long long)at * a.x_token);
 #pragma unroll
       for (int j = 0; j < kPast; ++j)
-        if (at < 0 && at + kPast == j) w = in[j];
-      *reinterpret_cast<Part*>(window + (long long)i * a.channels) = w;
+        if (n + i == j) keep[i] = in[j];
+      *reinterpret_cast<Part*>(window + (long long)i * a.channels) = keep[i];
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kPast; ++i)
-      in[i] = *reinterpret_cast<const Part*>(x + (long long)(i - kPast) * a.x_token);
   }
 
   float w[kEach][kWidth], bias[kEach];
   if constexpr (kWide) {
-    // 8 channels' weights are kWidth pieces of 16 bytes in a row.
     uint16_t flat[8 * kWidth];
 #pragma unroll
     for (int i = 0; i < kWidth; ++i) {
-      const uint4 p = *reinterpret_cast<const uint4*>(a.weight + (long long)c * kWidth + 8 * i);
-      const uint32_t pw[4] = {p.x, p.y, p.z, p.w};
+      const uint32_t pw[4] = {w_raw[i].x, w_raw[i].y, w_raw[i].z, w_raw[i].w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         flat[8 * i + 2 * j] = (uint16_t)pw[j];
@@ -268,7 +278,7 @@ __global__ __launch_bounds__(256) void short_conv_kernel(ConvArgs a) {
       for (int j = 0; j < kWidth; ++j) w[e][j] = pair_lo<kBf16>(flat[e * kWidth + j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < kWidth; ++j) w[0][j] = pair_lo<kBf16>(a.weight[(long long)c * kWidth + j]);
+    for (int j = 0; j < kWidth; ++j) w[0][j] = pair_lo<kBf16>(w_raw[j]);
   }
 #pragma unroll
   for (int e = 0; e < kEach; ++e) bias[e] = a.bias ? pair_lo<kBf16>(a.bias[c + e]) : 0.f;
@@ -278,7 +288,7 @@ __global__ __launch_bounds__(256) void short_conv_kernel(ConvArgs a) {
   for (int i = 0; i < kPast; ++i) get(in[i], past[i]);
   uint16_t* y = a.y + (long long)tile.row * a.channels + c;
 #pragma unroll
-  for (int i = 0; i < kConvTile; ++i) {
+  for (int i = 0; i < kTile; ++i) {
     get(in[kPast + i], past[kPast]);
     uint16_t o[kEach];
 #pragma unroll
@@ -286,8 +296,7 @@ __global__ __launch_bounds__(256) void short_conv_kernel(ConvArgs a) {
       float z = bias[e];
 #pragma unroll
       for (int j = 0; j < kWidth; ++j) z = fmaf(past[j][e], w[e][j], z);
-      if (a.silu) z = z / (1.f + expf(-z));
-      o[e] = to_half_bits<kType>(z);
+      o[e] = to_half_bits<kType>(a.silu ? silu_of(z) : z);
     }
     if (i < tile.count) {
       if constexpr (kWide) {
@@ -436,7 +445,10 @@ extern "C" int dk_short_conv(const void* x, long long x_token_stride, const void
       !aligned(y, 2) || !aligned(held, 4) || !aligned(offsets, 4))
     return dk::set_error(DK_ERR_INVALID_ARGUMENT,
                          "short_conv's arrays must be aligned as their elements");
-  const long long tiles = offsets ? (long long)num_tokens / dk::kConvTile + requests + 1 : requests;
+  // Tokens of a request that a workgroup takes: as many as it has where they are
+  // few, since a tile's arithmetic runs over all its places.
+  const int tile = !offsets ? 1 : max_query_len <= 4 ? 4 : 16;
+  const long long tiles = offsets ? (long long)num_tokens / tile + requests + 1 : requests;
   const bool wide = channels % 8 == 0 && x_token_stride % 8 == 0 && aligned(x, 16) &&
                     aligned(weight, 16) && aligned(windows, 16) && aligned(y, 16);
   const long long blocks = ((long long)channels - 1) / (wide ? 2048 : 256) + 1;
@@ -452,7 +464,9 @@ extern "C" int dk_short_conv(const void* x, long long x_token_stride, const void
   auto pick = [&](auto bf16, auto w) {
     constexpr bool b = decltype(bf16)::value;
     constexpr int n = decltype(w)::value;
-    wide ? launch(dk::short_conv_kernel<n, b, true>) : launch(dk::short_conv_kernel<n, b, false>);
+    if (tile == 1) wide ? launch(dk::short_conv_kernel<n, 1, b, true>) : launch(dk::short_conv_kernel<n, 1, b, false>);
+    else if (tile == 4) wide ? launch(dk::short_conv_kernel<n, 4, b, true>) : launch(dk::short_conv_kernel<n, 4, b, false>);
+    else wide ? launch(dk::short_conv_kernel<n, 16, b, true>) : launch(dk::short_conv_kernel<n, 16, b, false>);
   };
   auto by_width = [&](auto bf16) {
     if (width == 2) pick(bf16, std::integral_constant<int, 2>{});

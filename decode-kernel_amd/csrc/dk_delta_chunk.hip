@@ -397,6 +397,7 @@ __global__ __launch_bounds__(256, 4) void delta_prepare_kernel(DeltaArgs a, Chun
 // outputs need is off the chain that bounds a long prompt.
 // ---------------------------------------------------------------------------
 using lds_ptr = __attribute__((address_space(3))) void*;
+using lds_float_ptr = __attribute__((address_space(3))) float*;
 
 // Buffers: a chunk's rows behind the request's last are out of their range, so
 // that they load zeros and store nothing.
@@ -593,9 +594,12 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
 #pragma unroll
     for (int z = 0; z < 8; ++z) out_at[z] = ((32 * half + 16 * (z >> 2) + (z & 3) + 4 * q4) * out_token + col) * 2;
     const uint32_t v_at = (lane * (uint32_t)a.v_token + col - i + 8 * half) * 2;
-    // All output waves bring a chunk's operands, each its share of the pieces.
-    auto bring = [&](int c, int which) {
-      h8_t* to = &stage[c & 1][0][0];
+    // All output waves bring a chunk's operands, each its share of the pieces. Past
+    // the last chunk it is that one again, into a buffer that nobody reads: the
+    // compiler counts what is on its way only where every turn asks for as much.
+    auto bring = [&](int chunk, int which) {
+      h8_t* to = &stage[chunk & 1][0][0];
+      const int c = min(chunk, chunks - 1);
       auto some = [&](__amdgpu_buffer_rsrc_t r, int first, int count) {
 #pragma unroll
         for (int p = 0; p < count; p += 2 * kCols)
@@ -611,10 +615,15 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
         some(of_factors(c), kKeys + kInverse + kTurned, 2);
       }
     };
+    auto in_order = [] {
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
     uint4 v;
     float b1;
     h8_t q[2 * kS], p[8];
-    auto load_values = [&](int c) {
+    auto load_values = [&](int chunk) {
+      const int c = min(chunk, chunks - 1);
       const uint32_t count = min(n - c * kChunk, kChunk);
       const auto r =
           buffer_of(values + (long long)c * kChunk * a.v_token, ((count - 1) * (uint32_t)a.v_token + value_size) * 2);
@@ -624,13 +633,18 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
     auto give_values = [&](int c) {  // to where a result tile has row `lane`
       float* to = reinterpret_cast<float*>(&rows_v[c & 1][tile][lane >> 4][8 * half + 16 * ((lane & 15) >> 2)]) + (lane & 3);
       const uint32_t pairs[4] = {v.x, v.y, v.z, v.w};
+      const uint32_t at = (uint32_t)(uintptr_t)(lds_float_ptr)to;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        to[8 * j] = b1 * pair_lo<kBf16>(pairs[j]);
-        to[8 * j + 4] = b1 * pair_hi<kBf16>(pairs[j]);
+        // Before a store to LDS the compiler waits for all loads to LDS, also where
+        // they go elsewhere.
+        asm volatile("ds_write_b32 %0, %1 offset:%2" ::"v"(at), "v"(b1 * pair_lo<kBf16>(pairs[j])), "n"(32 * j) : "memory");
+        asm volatile("ds_write_b32 %0, %1 offset:%2" ::"v"(at), "v"(b1 * pair_hi<kBf16>(pairs[j])), "n"(32 * j + 16)
+                     : "memory");
       }
     };
-    auto load_queries = [&](int c) {
+    auto load_queries = [&](int chunk) {
+      const int c = min(chunk, chunks - 1);
       const auto qs = of_qk(ws.q, c);
 #pragma unroll
       for (int y = 0; y < 2; ++y)
@@ -639,18 +653,17 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
     };
     load_values(0);
     give_values(0);
-    if (chunks > 1) load_values(1);
+    load_values(1);
     bring(0, 0);
     bring(0, 1);
     load_queries(0);
-    if (chunks > 1) bring(1, 0);
+    bring(1, 0);
     f4_t x[2], d[2], y2[2];  // of the last chunk: e^G Q' S, and the queries' factors
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0);  // chunk 0's operands are in LDS
     asm volatile("" ::: "memory");
     for (int c = 0; c <= chunks; ++c) {
       lds_barrier();
-      const bool more = c + 1 < chunks;
       if (c > 0) {
         const int at = c - 1;
         f4_t wv[4];
@@ -682,7 +695,7 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
 #pragma unroll
             for (int y = 0; y < 2; ++y) y2[y] = mfma(p[2 * y + (part == 2)], part == 1 ? lo : hi, y2[y]);
         }
-        if (more) give_values(c + 1);
+        give_values(c + 1);
         __builtin_amdgcn_sched_barrier(0);
         const uint32_t count = min(n - at * kChunk, kChunk);
         const auto r = buffer_of(out + (long long)at * kChunk * out_token, ((count - 1) * out_token + value_size) * 2);
@@ -695,13 +708,14 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
           }
       }
       if (c == chunks) break;
-      // All that was asked for in the last turn is there, but not yet the 8 stores
-      // above have to be.
+      // What the state waves read behind the barrier is there; the next chunk's
+      // keys and queries, asked for last, and the 8 stores above may be under way.
       if (c > 0) {
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0xF78);  // vmcnt(8)
+        constexpr int kLate = 8 + 2 * kS + kKeys / (2 * kCols);
+        __builtin_amdgcn_s_waitcnt((kLate & 15) | (kLate >> 4 << 14) | 0xF70);  // vmcnt(kLate)
         asm volatile("" ::: "memory");
-      } else if (more) {
+      } else {
         give_values(1);
       }
       lds_barrier();
@@ -735,16 +749,20 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
       // In the order in which it is waited for. The state waves are through with
       // this chunk's keys and with all of the last one's operands.
       const auto ps = of_v(ws.p, c);
+      if (half)
 #pragma unroll
-      for (int z = 0; z < 8; ++z)
-        if (z < 4 || half) p[z] = load_piece(ps, piece_at + (4 * half + z) * 1024);
-      if (more) {
-        if (c + 2 < chunks) load_values(c + 2);
-        bring(c + 1, 1);
-        load_queries(c + 1);
-        if (c + 2 < chunks) bring(c + 2, 0);
-      }
+        for (int z = 4; z < 8; ++z) p[z] = load_piece(ps, piece_at + (4 + z) * 1024);
+#pragma unroll
+      for (int z = 0; z < 4; ++z) p[z] = load_piece(ps, piece_at + (4 * half + z) * 1024);
+      load_values(c + 2);
+      bring(c + 1, 1);
+      in_order();  // kLate counts what comes behind this
+      load_queries(c + 1);
+      in_order();
+      bring(c + 2, 0);
+      in_order();
     }
+    __builtin_amdgcn_s_waitcnt(0);  // nothing is on its way to LDS behind the end
   }
 }
 
