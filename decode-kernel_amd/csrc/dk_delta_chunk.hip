@@ -49,7 +49,6 @@ constexpr int kFragments = 6;  // 16 x 32 pieces of a lower triangle of 64: (0,0
 struct ChunkSpace {
   h8_t* k;    // [qk head][slot][4][dk / 32][64]   K', rows = tokens
   h8_t* q;    // [qk head][slot][4][dk / 32][64]   Q'
-  h8_t* kt;   // [qk head][slot][dk / 16][2][64]   K' transposed, rows = elements
   h8_t* t;    // [v head][slot][6][2][64]          T' * 512: first and second part
   h8_t* p;    // [v head][slot][6][2][64]          P * 64, of q' and k'
   float* s;   // [v head][slot][kFactors * 64]     the rows' factors
@@ -74,7 +73,6 @@ ChunkSpace chunk_space(void* workspace, int tokens, int requests, int qk_heads, 
   const size_t rows = slots * qk_heads * kChunk * dk * 2, lower = slots * v_heads * kFragments * 2 * 1024;
   c.k = reinterpret_cast<h8_t*>(take(rows));
   c.q = reinterpret_cast<h8_t*>(take(rows));
-  c.kt = reinterpret_cast<h8_t*>(take(rows));
   c.t = reinterpret_cast<h8_t*>(take(lower));
   c.p = reinterpret_cast<h8_t*>(take(lower));
   c.s = reinterpret_cast<float*>(take(slots * v_heads * kFactors * kChunk * 4));
@@ -331,24 +329,6 @@ __global__ __launch_bounds__(256, 4) void delta_prepare_kernel(DeltaArgs a, Chun
 #pragma unroll
       for (int x = 0; x < 16; ++x) m[base + x][base + i] = t[x];
   }
-  // The transposed keys, element by element out of the operands' order.
-  if (first_of_group) {
-    const uint16_t* flat = reinterpret_cast<const uint16_t*>(&keys[0][0][0]);
-    for (int f = wave; f < kDk / 16 * 2; f += 4) {
-      const int e = 16 * (f >> 1) + i;  // the element
-      union {
-        uint16_t u[8];
-        h8_t v;
-      } x;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int t = 32 * (f & 1) + 16 * (j >> 2) + 4 * q4 + (j & 3);
-        x.u[j] = flat[(((t >> 4) * kS + (e >> 5)) * 64 + (t & 15) + 16 * ((e & 15) >> 2)) * 8 +
-                      ((e >> 4) & 1) * 4 + (e & 3)];
-      }
-      ws.kt[qk_at + f * 64 + lane] = x.v;
-    }
-  }
   __syncthreads();
   f4_t below[4];
 #pragma unroll
@@ -397,6 +377,9 @@ __global__ __launch_bounds__(256, 4) void delta_prepare_kernel(DeltaArgs a, Chun
 // outputs need is off the chain that bounds a long prompt.
 // ---------------------------------------------------------------------------
 using lds_ptr = __attribute__((address_space(3))) void*;
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+using lds_short4_ptr = __attribute__((address_space(3))) short4_t*;
 using lds_float_ptr = __attribute__((address_space(3))) float*;
 
 // Buffers: a chunk's rows behind the request's last are out of their range, so
@@ -417,8 +400,8 @@ template <int kDk, int kCols, bool kBf16>
 __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a, ChunkSpace ws, int value_size) {
   constexpr int kS = kDk / 32, kHalfS = kS / 2, kHalfTiles = kDk / 32;
   constexpr int kType = kBf16 ? DK_KV_BF16 : DK_KV_F16;
-  constexpr int kKeys = 4 * kS, kInverse = 2 * kFragments, kTurned = 4 * kS;  // pieces of 1 KB
-  constexpr int kPieces = kKeys + kInverse + kTurned + 2;
+  constexpr int kKeys = 4 * kS, kInverse = 2 * kFragments;  // pieces of 1 KB
+  constexpr int kPieces = kKeys + kInverse + 2;
   constexpr f4_t kZero{0.f, 0.f, 0.f, 0.f};
   __shared__ h8_t stage[2][kPieces][64];         // a chunk's operands and its rows' factors
   __shared__ f4_t rows_v[2][kCols][4][64];       // beta c v of a chunk's rows
@@ -456,8 +439,7 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
       if (c == chunks) break;
       const h8_t(*keys)[64] = &stage[c & 1][0];
       const h8_t(*inverse)[64] = &stage[c & 1][kKeys];
-      const h8_t(*turned)[64] = &stage[c & 1][kKeys + kInverse];
-      const float* factors = reinterpret_cast<const float*>(&stage[c & 1][kKeys + kInverse + kTurned][0]);
+      const float* factors = reinterpret_cast<const float*>(&stage[c & 1][kKeys + kInverse][0]);
       auto rows4 = [&](int which, int y) {
         return *reinterpret_cast<const f4_t*>(factors + which * kChunk + 16 * y + 4 * q4);
       };
@@ -488,6 +470,23 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
 #pragma unroll
         for (int y = 0; y < 4; ++y) x[y] = mfma(kf[y * kHalfS + t], lo, x[y]);
       }
+      __builtin_amdgcn_sched_barrier(0);
+      // The keys once more, transposed: rows are elements 16 z .. of this half, and
+      // the columns tokens in the order of an operand. Of each 16 lanes lane 4 r +
+      // c reads the elements 4 c .. 4 c + 3 of token r, and lane l receives
+      // element l of tokens 0 .. 3.
+#pragma unroll
+      for (int z = 0; z < kHalfTiles; ++z)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int e = half * kHalfTiles + z;
+          const h8_t* from = &keys[y * kS + (e >> 1)][4 * q4 + (i >> 2) + 16 * (i & 3)];
+          const h4_t part = __builtin_bit_cast(
+              h4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_ptr)(reinterpret_cast<const uint16_t*>(from) + 4 * (e & 1))));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) uf[2 * z + (y >> 1)][4 * (y & 1) + j] = part[j];
+        }
+      __builtin_amdgcn_sched_barrier(0);
       if (q4 == 0) left_scale[tile][half][i] = down;
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
@@ -509,10 +508,6 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
 #pragma unroll
       for (int y = 0; y < 4; ++y) until[y] = rows4(4, y);
       const float whole = factors[5 * kChunk];
-#pragma unroll
-      for (int y = 0; y < 2; ++y)
-#pragma unroll
-        for (int t = 0; t < kHalfTiles; ++t) uf[2 * t + y] = turned[2 * (half * kHalfTiles + t) + y][lane];
       __builtin_amdgcn_sched_barrier(0);
       // What each token finds wrong in the state before the chunk.
 #pragma unroll
@@ -611,8 +606,7 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
         some(of_qk(ws.k, c), 0, kKeys);
       } else {
         some(of_v(ws.t, c), kKeys, kInverse);
-        some(of_qk(ws.kt, c), kKeys + kInverse, kTurned);
-        some(of_factors(c), kKeys + kInverse + kTurned, 2);
+        some(of_factors(c), kKeys + kInverse, 2);
       }
     };
     auto in_order = [] {
@@ -723,7 +717,7 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
 #pragma unroll
       for (int t = 0; t < 2 * kS; ++t) sp[t] = left_s[tile][t][lane];
       const float ds0 = left_scale[tile][0][i], ds1 = left_scale[tile][1][i];
-      const float* factors = reinterpret_cast<const float*>(&stage[c & 1][kKeys + kInverse + kTurned][0]);
+      const float* factors = reinterpret_cast<const float*>(&stage[c & 1][kKeys + kInverse][0]);
       f4_t since[2];
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
