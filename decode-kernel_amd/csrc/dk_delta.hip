@@ -19,12 +19,17 @@ namespace dk {
 // A lane has 4 columns (16 bytes of a row) of dk / 8 rows that follow one
 // another; 8 lanes read a line of 128 bytes, and sums over the rows go over
 // the other three lane bits. One new token a request is bound by reading and
-// writing its state once.
+// writing its state once: 61 requests of 32 heads of 128 x 128, 250 MB, take 49.8
+// us, 5.0 TB/s, where a copy reaches 5.1. More tokens are bound by the chain from
+// token to token.
 // ---------------------------------------------------------------------------
 constexpr int kStepColumns = 32;
 
 __device__ __forceinline__ float sum_rows(float v) {
   v += dpp<0x128>(v);  // row_ror:8: the lane 8 away in its row of 16
+  // Through LDS, 22 of them on their way at once: swaps of register halves
+  // (v_permlane*_swap) take one wait each, 13.0 against 11.8 us for 4 tokens of
+  // 96 requests.
   v += __shfl_xor(v, 16);
   v += __shfl_xor(v, 32);
   return v;
@@ -315,8 +320,10 @@ __global__ __launch_bounds__(256) void short_conv_kernel(ConvArgs a) {
   }
 }
 
-// Requests of up to so many tokens go token by token: a chunk costs its 64
-// tokens' work also where few are there.
+// Requests of up to so many tokens go token by token, 1.2 us each; a chunk costs
+// its 64 tokens' work also where few are there. 17 tokens, token by token and as
+// a chunk, us: 1 request of 32 heads 24 and 16, 8 of them 29 and 37, 64 of 4 heads
+// 27 and 40; 32 tokens 41 and 16, 48 and 37, 47 and 41.
 constexpr int kStepTokens = 16;
 
 }  // namespace dk
@@ -445,13 +452,16 @@ extern "C" int dk_short_conv(const void* x, long long x_token_stride, const void
       !aligned(y, 2) || !aligned(held, 4) || !aligned(offsets, 4))
     return dk::set_error(DK_ERR_INVALID_ARGUMENT,
                          "short_conv's arrays must be aligned as their elements");
-  // Tokens of a request that a workgroup takes: as many as it has where they are
-  // few, since a tile's arithmetic runs over all its places.
-  const int tile = !offsets ? 1 : max_query_len <= 4 ? 4 : 16;
-  const long long tiles = offsets ? (long long)num_tokens / tile + requests + 1 : requests;
   const bool wide = channels % 8 == 0 && x_token_stride % 8 == 0 && aligned(x, 16) &&
                     aligned(weight, 16) && aligned(windows, 16) && aligned(y, 16);
   const long long blocks = ((long long)channels - 1) / (wide ? 2048 : 256) + 1;
+  // Tokens of a request that a workgroup takes. Where there are many, 8: each
+  // input is read 11 times in 8, not 7 in 4 (8192 tokens of 8192 channels 50.6
+  // against 55.8 us; with 16 fewer loads are on their way at once, 60.2). Where 8
+  // would leave the chip few workgroups, or requests have few tokens, 4 (4100
+  // tokens of 1544 channels 10.1 against 11.5 us).
+  const int tile = !offsets ? 1 : max_query_len <= 4 || (long long)num_tokens / 8 * blocks < 1024 ? 4 : 8;
+  const long long tiles = offsets ? (long long)num_tokens / tile + requests + 1 : requests;
   if (tiles > INT32_MAX || blocks > 65535)
     return dk::set_error(DK_ERR_UNSUPPORTED, "too many tokens or channels for one call");
   const dk::ConvArgs a{static_cast<const uint16_t*>(x), x_token_stride,
@@ -466,7 +476,7 @@ extern "C" int dk_short_conv(const void* x, long long x_token_stride, const void
     constexpr int n = decltype(w)::value;
     if (tile == 1) wide ? launch(dk::short_conv_kernel<n, 1, b, true>) : launch(dk::short_conv_kernel<n, 1, b, false>);
     else if (tile == 4) wide ? launch(dk::short_conv_kernel<n, 4, b, true>) : launch(dk::short_conv_kernel<n, 4, b, false>);
-    else wide ? launch(dk::short_conv_kernel<n, 16, b, true>) : launch(dk::short_conv_kernel<n, 16, b, false>);
+    else wide ? launch(dk::short_conv_kernel<n, 8, b, true>) : launch(dk::short_conv_kernel<n, 8, b, false>);
   };
   auto by_width = [&](auto bf16) {
     if (width == 2) pick(bf16, std::integral_constant<int, 2>{});
