@@ -613,6 +613,16 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
       asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
     };
+    // Until no more than so many of this wave's loads and stores are under way: they
+    // come back in the order in which they were asked for.
+    auto wait_but = [&](auto count) {
+      constexpr int k = decltype(count)::value;
+      static_assert(k < 64, "what vmcnt holds");
+      in_order();
+      __builtin_amdgcn_s_waitcnt((k & 15) | (k >> 4 << 14) | 0xF70);
+      in_order();
+    };
+    constexpr int kLateLoads = 2 * kS + kKeys / (2 * kCols);  // queries, and a share of keys
     uint4 v;
     float b1;
     h8_t q[2 * kS], p[8];
@@ -704,14 +714,8 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
       if (c == chunks) break;
       // What the state waves read behind the barrier is there; the next chunk's
       // keys and queries, asked for last, and the 8 stores above may be under way.
-      if (c > 0) {
-        asm volatile("" ::: "memory");
-        constexpr int kLate = 8 + 2 * kS + kKeys / (2 * kCols);
-        __builtin_amdgcn_s_waitcnt((kLate & 15) | (kLate >> 4 << 14) | 0xF70);  // vmcnt(kLate)
-        asm volatile("" ::: "memory");
-      } else {
-        give_values(1);
-      }
+      if (c > 0) wait_but(std::integral_constant<int, 8 + kLateLoads>{});
+      else give_values(1);
       lds_barrier();
       h8_t sp[2 * kS];
 #pragma unroll
@@ -750,11 +754,15 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
       for (int z = 0; z < 4; ++z) p[z] = load_piece(ps, piece_at + (4 * half + z) * 1024);
       load_values(c + 2);
       bring(c + 1, 1);
-      in_order();  // kLate counts what comes behind this
+      in_order();  // kLateLoads counts what comes behind this
       load_queries(c + 1);
       in_order();
       bring(c + 2, 0);
       in_order();
+      // Chunk c + 1's keys, asked for before the last turn's stores, are there:
+      // at least so many more were asked for since.
+      constexpr int kSince = 8 + 4 + 2 + kInverse / (2 * kCols) + (kCols == 1 ? 1 : 0) + kLateLoads;
+      wait_but(std::integral_constant<int, kSince>{});
     }
     __builtin_amdgcn_s_waitcnt(0);  // nothing is on its way to LDS behind the end
   }
