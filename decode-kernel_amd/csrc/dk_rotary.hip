@@ -6,8 +6,10 @@
 // frequency's angle is a 64-bit product reduced to a part of one turn there,
 // so that only that part is rounded to fp32 (a position of 10^6 has 20 bits
 // before the point, which a 32-bit angle would lose behind it). Each element
-// is read and written once, 32 bytes a lane: bound by HBM for prompts and by
-// latency for a decode step.
+// is read and written once, 32 bytes a lane: bound by HBM for prompts (8192
+// tokens of 72 heads of 128, 302 MB, 53 us with the result's memory used again and
+// 64 into new memory, where a copy takes 59) and by latency for a decode step (64
+// tokens 3.3 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
