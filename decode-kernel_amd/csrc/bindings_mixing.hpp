@@ -166,7 +166,14 @@ std::tuple<torch::Tensor, torch::Tensor> rotate_qk(const torch::Tensor& q, const
     return t.stride(2) == 1 || t.numel() == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
   };
   const auto qr = rows(q), kr = rows(k);
-  auto qo = torch::empty(q.sizes(), q.options()), ko = torch::empty(k.sizes(), k.options());
+  // One allocation for both, k's part from a multiple of 16 bytes: a decode step
+  // takes as long as its host work does.
+  const int64_t k_at = (q.numel() + 7) / 8 * 8;
+  auto qo = torch::empty({k_at + k.numel()}, q.options());
+  auto ko = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(qo.storage()), qo.key_set(), qo.dtype());
+  ko.unsafeGetTensorImpl()->set_storage_offset(k_at);
+  ko.unsafeGetTensorImpl()->set_sizes_contiguous(k.sizes());
+  qo.unsafeGetTensorImpl()->set_sizes_contiguous(q.sizes());
   if (D == 0) return {qo, ko};
   check_status(
       dk_rotate_qk(qr.data_ptr(), qr.stride(0), qr.stride(1), static_cast<int>(q.size(1)), kr.data_ptr(),

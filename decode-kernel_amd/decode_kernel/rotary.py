@@ -72,6 +72,7 @@ def rotate_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rotary:
     becomes (a cos - b sin, a sin + b cos); elements past the rotary's pairs are
     copied. inverse turns back, which is also what the gradient of the results
     goes through. Angles are formed in 64 bits: a position in the millions is as
-    exact as a small one. q and k may be slices of one projection.
+    exact as a small one. q and k may be slices of one projection. The two results
+    share one allocation.
     """
     return _ext().rotate_qk(q, k, positions, rotary.frequencies, rotary.axes, rotary.adjacent, inverse)
