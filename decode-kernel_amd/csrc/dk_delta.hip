@@ -413,6 +413,7 @@ extern "C" int dk_delta_rule(const dk_delta_args* p, void* out, void* workspace,
                         p->v_heads,
                         p->v_heads / p->qk_heads,
                         chunks ? dk::kStepTokens : INT32_MAX,
+                        p->max_query_len,
                         p->normalize,
                         p->scale};
   const bool bf16 = p->dtype == DK_KV_BF16;

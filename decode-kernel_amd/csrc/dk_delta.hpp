@@ -31,6 +31,7 @@ struct DeltaArgs {
   uint16_t* out;
   int tokens, requests, qk_heads, v_heads, group;
   int limit;  // requests of up to so many tokens go one by one, longer ones in chunks
+  int longest;  // max_query_len
   int normalize;
   float scale;
 };
@@ -41,6 +42,22 @@ __device__ __forceinline__ bool wave_offsets_ok(const int32_t* offsets, int requ
   for (int i = threadIdx.x & 63; i < requests; i += 64) bad |= offsets[i + 1] < offsets[i];
   if ((threadIdx.x & 63) == 0) bad |= offsets[0] < 0 || offsets[requests] > tokens;
   return __ballot(bad) == 0;
+}
+
+// The request that is number `rank` (from 0) of those with more than `limit`
+// tokens, or -1; by one wave. Offsets have to be good.
+__device__ __forceinline__ int find_long(const int32_t* offsets, int requests, int limit, int rank) {
+  for (int first = 0; first < requests; first += 64) {
+    const int i = first + (threadIdx.x & 63);
+    unsigned long long is = __ballot(i < requests && offsets[min(i, requests - 1) + 1] - offsets[min(i, requests - 1)] > limit);
+    const int count = __popcll(is);
+    if (rank < count) {
+      for (; rank > 0; --rank) is &= is - 1;
+      return first + __ffsll(is) - 1;
+    }
+    rank -= count;
+  }
+  return -1;
 }
 
 // A tile of a request's new tokens. Tiles of `tile` tokens have numbers that

@@ -24,6 +24,7 @@
 //   w = T' (beta c v - beta c^2 e^G (K' S)),  S_after = e^G_last S + sum_j k'_j (e^(..) w_j).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "dk_delta.hpp"
@@ -416,14 +417,20 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
   __shared__ f4_t left_w[kCols][4][64];          // the corrections
   __shared__ float left_scale[kCols][3][16];     // by which both halves of the state and w are to be multiplied
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63, i = lane & 15, q4 = lane >> 4;
   const bool outputs = wave >= 2 * kCols;
   const int tile = (wave >> 1) & (kCols - 1), half = wave & 1;
-  const int h = blockIdx.x % a.v_heads, hq = h / a.group, b = blockIdx.y;
-  const int col = ((blockIdx.x / a.v_heads) * kCols + tile) * 16 + i;
+  const int h = blockIdx.x % a.v_heads, hq = h / a.group;
   if (!wave_offsets_ok(a.offsets, a.requests, a.tokens)) return;
-  const int from = a.offsets[b], n = a.offsets[b + 1] - from;
-  if (n <= a.limit) return;
+  // The grid has room for as many long requests as there seem to be; where there
+  // are more, a workgroup takes several, one after another.
+  for (int rank = blockIdx.y;; rank += gridDim.y) {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // or all addresses of both kinds of waves are kept across requests
+  const int i = lane & 15, q4 = lane >> 4, col = ((blockIdx.x / a.v_heads) * kCols + tile) * 16 + i;
+  const int b = __builtin_amdgcn_readfirstlane(find_long(a.offsets, a.requests, a.limit, rank));
+  if (b < 0) return;
+  const int from = __builtin_amdgcn_readfirstlane(a.offsets[b]);
+  const int n = __builtin_amdgcn_readfirstlane(a.offsets[b + 1]) - from;
   const long long slot0 = from / kChunk + b;
   const int chunks = (n + kChunk - 1) / kChunk;
 
@@ -772,6 +779,8 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
     }
     __builtin_amdgcn_s_waitcnt(0);  // nothing is on its way to LDS behind the end
   }
+  lds_barrier();  // the next request's first stores to LDS are behind this one's last reads
+  }
 }
 
 }  // namespace
@@ -790,9 +799,14 @@ int delta_chunk_launch(const DeltaArgs& a, int key_size, int value_size, bool bf
   // Tiles of 16 columns: two a workgroup where one each would not be at work at
   // once (its LDS leaves one workgroup a CU). One and two, us: 256 tiles (a prompt
   // of 8192 tokens of 32 heads) 264 and 353, 896 (7 prompts of 16 heads) 57 and 42.
-  const long long tiles = (long long)a.requests * a.v_heads * (value_size / 16);
+  // Room for as many long requests as there may well be: workgroups take several
+  // where there are more, and one without any costs its turn on a CU (61 single
+  // tokens and a prompt of 2048, 32 heads: 122 us, and 154 with room for 62 of them).
+  const long long seem = std::max(1LL, 2LL * a.tokens / a.longest);
+  const unsigned longs = (unsigned)std::max(1LL, std::min({seem, (long long)a.requests, (long long)a.tokens / (a.limit + 1)}));
+  const long long tiles = (long long)std::min(longs, (unsigned)std::max(1, a.tokens / a.longest)) * a.v_heads * (value_size / 16);
   const int cols = tiles > 256 ? 2 : 1;
-  const dim3 columns((unsigned)(a.v_heads * (value_size / (16 * cols))), (unsigned)a.requests);
+  const dim3 columns((unsigned)(a.v_heads * (value_size / (16 * cols))), longs);
   auto launch = [&](auto prepare, auto one, auto two) {
     hipLaunchKernelGGL(prepare, chunks, dim3(256), 0, stream, a, ws);
     if (cols == 1) hipLaunchKernelGGL(one, columns, dim3(256), 0, stream, a, ws, value_size);

@@ -141,6 +141,14 @@ def test_max_query_len_only_picks_kernels():
         check(c, max_query_len=most)
 
 
+@pytest.mark.parametrize("most", [None, 17, 600, 10**6])
+def test_more_prompts_than_seem_to_be(most):
+    """One long prompt among many short ones: the workgroups are counted by the
+    longest and take several prompts each."""
+    lens = [600] + [20, 0, 3] * 12 + [65, 1, 129]
+    check(case(lens, 1, 2, 64, 64, BF16, seed=33), max_query_len=most)
+
+
 def test_split_steps_are_one_step():
     """A prompt in two steps and then tokens one by one ends where one step does."""
     c = case([90], 2, 1, 128, 128, BF16, seed=7, held=[0])
