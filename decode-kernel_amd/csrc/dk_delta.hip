@@ -56,10 +56,10 @@ __global__ __launch_bounds__(64) void delta_step_kernel(DeltaArgs a, int value_s
   if (!ok) {
     clear(0, a.tokens);
   } else if (a.offsets) {
+    first = a.offsets[b];
+    last = a.offsets[b + 1];
     ok = wave_offsets_ok(a.offsets, a.requests, a.tokens);
     if (ok) {
-      first = a.offsets[b];
-      last = a.offsets[b + 1];
       if (b == 0) clear(0, first);
       if (b == a.requests - 1) clear(last, a.tokens);
     } else if (b == 0) {
@@ -202,19 +202,16 @@ __global__ __launch_bounds__(256) void short_conv_kernel(ConvArgs a) {
     if (mine)
       for (long long t = from; t < to; ++t) *reinterpret_cast<Part*>(a.y + t * a.channels + c) = Part{};
   };
-  Tile tile{(int)blockIdx.x, (int)blockIdx.x, 1, 0};
-  int n = 1;  // the request's new tokens
+  Tile tile{(int)blockIdx.x, (int)blockIdx.x, 1, 0, 1, 0, 0};
   if (a.offsets) {
     const long long part = (long long)blockIdx.x * kTile;
     if (a.requests == 0 || !find_tile(a.offsets, a.requests, a.tokens, kTile, blockIdx.x, &tile)) {
       clear(min(part, (long long)a.tokens), min(part + kTile, (long long)a.tokens));
       return;
     }
-    const long long head = a.offsets[0], end = a.offsets[a.requests];
-    clear(min(part, head), min(part + kTile, head));
-    clear(min(end + part, (long long)a.tokens), min(end + part + kTile, (long long)a.tokens));
+    clear(min(part, (long long)tile.head), min(part + kTile, (long long)tile.head));
+    clear(min(tile.end + part, (long long)a.tokens), min(tile.end + part + kTile, (long long)a.tokens));
     if (tile.request < 0) return;
-    n = a.offsets[tile.request + 1] - a.offsets[tile.request];
   }
   if (!mine) return;
 
@@ -235,6 +232,7 @@ __global__ __launch_bounds__(256) void short_conv_kernel(ConvArgs a) {
   const uint16_t* x = a.x + (long long)tile.row * a.x_token + c;
   uint16_t* window = a.windows + (long long)tile.request * kPast * a.channels + c;
   const bool first = tile.index == 0;
+  const int n = tile.total;
   Part in[kPast + kTile];
 #pragma unroll
   for (int i = 0; i < kPast; ++i)

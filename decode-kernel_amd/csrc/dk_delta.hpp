@@ -65,41 +65,47 @@ __device__ __forceinline__ int find_long(const int32_t* offsets, int requests, i
 // and since floor(x + n) - floor(x) + 1 >= ceil(n), they end before the next
 // request's do begin. tokens / tile + requests numbers are enough.
 struct Tile {
-  int request;  // -1: the number is nobody's
-  int row;      // its first row
-  int count;    // its rows
-  int index;    // which tile of its request
+  int request;    // -1: the number is nobody's
+  int row;        // its first row
+  int count;      // its rows
+  int index;      // which tile of its request
+  int total;      // its request's rows
+  int head, end;  // the first row of all requests, and one past the last
 };
 
 // The tile with number `number`, and whether offsets are good; by each wave for
-// itself, with the same answer in all.
+// itself, with the same answer in all. Offsets are loaded once, 64 requests at
+// a time, and what is needed of them is taken from other lanes: a load that
+// waits for another costs 1 to 2 us next to stores of a full chip.
 __device__ __forceinline__ bool find_tile(const int32_t* offsets, int requests, int tokens, int tile,
                                           int number, Tile* out) {
   const int lane = threadIdx.x & 63;
-  int begun = 0;  // requests whose tiles begin at or before the number
-  bool bad = lane == 0 && (offsets[0] < 0 || offsets[requests] > tokens);
+  int b = -1, from_b = 0, to_b = 0, head = 0, end = 0;
+  bool bad = false;
   for (int first = 0; first < requests; first += 64) {
-    const int i = first + lane;
-    bool before = false;
-    if (i < requests) {
-      const int from = offsets[i];
-      bad |= offsets[i + 1] < from;
-      before = from / tile + i <= number;
+    const int i = min(first + lane, requests - 1);
+    const int from = offsets[i], to = offsets[i + 1];
+    bad |= to < from;
+    const unsigned long long before = __ballot(first + lane < requests && from / tile + i <= number);
+    if (before) {  // requests' tiles begin one after another: the last that does before the number
+      const int at = 63 - __clzll(before);
+      b = first + at;
+      from_b = __builtin_amdgcn_readlane(from, at);
+      to_b = __builtin_amdgcn_readlane(to, at);
     }
-    begun += __popcll(__ballot(before));
+    if (first == 0) head = __builtin_amdgcn_readlane(from, 0);
+    end = __builtin_amdgcn_readlane(to, 63);  // of the last request: i ends there
   }
-  out->request = -1;
-  out->row = out->count = out->index = 0;
-  if (__ballot(bad)) return false;
-  const int b = begun - 1;
+  *out = Tile{-1, 0, 0, 0, 0, head, end};
+  if (__ballot(bad) || head < 0 || end > tokens) return false;
   if (b < 0) return true;
-  const int from = offsets[b], n = offsets[b + 1] - from;
-  const int index = number - (from / tile + b);
+  const int n = to_b - from_b, index = number - (from_b / tile + b);
   if ((long long)index * tile >= n) return true;
   out->request = b;
-  out->row = from + index * tile;
+  out->row = from_b + index * tile;
   out->count = min(tile, n - index * tile);
   out->index = index;
+  out->total = n;
   return true;
 }
 

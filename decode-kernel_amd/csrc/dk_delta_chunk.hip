@@ -140,9 +140,9 @@ __device__ __forceinline__ void split_tiles(f4_t x, f4_t y, float scale, h8_t* h
 
 // ---------------------------------------------------------------------------
 // One workgroup a chunk and head; wave w has its rows 16 w .. 16 w + 15. 8192
-// tokens of 32 heads of 128 (16 of keys), 4096 workgroups, take 66 us: 74 MB read
-// from memory and 170 written, and between them substitution (120 dependent
-// operations) and up to 36 products of 32 bits in a row, four workgroups a CU.
+// tokens of 32 heads of 128 (16 of keys), 4096 workgroups, take 65 us: 74 MB read
+// from memory and 170 written, 3.7 TB/s, which bounds it; a workgroup alone would
+// take 8 us, and next to others' stores its first loads take 4 of 13.
 // ---------------------------------------------------------------------------
 constexpr int kPad = 68;  // floats a row of 64 takes in LDS
 
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(256, 4) void delta_prepare_kernel(DeltaArgs a, Chun
   Tile tile;
   if (!find_tile(a.offsets, a.requests, a.tokens, kChunk, (int)slot, &tile)) return;
   if (tile.request < 0) return;
-  if (a.offsets[tile.request + 1] - a.offsets[tile.request] <= a.limit) return;
+  if (tile.total <= a.limit) return;
   const bool first_of_group = h % a.group == 0;
 
   // Every load first; rows behind the last are row 0 again, and zeros below.

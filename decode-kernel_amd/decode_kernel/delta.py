@@ -55,8 +55,8 @@ def delta_rule(
 
     q, k [tokens, qk_heads, key_size] and v [tokens, v_heads, value_size] in
     fp16 or bf16, v_heads a multiple of qk_heads (head h has the keys of head h
-    // (v_heads / qk_heads)), sizes of 64 or 128; log_decay and beta fp32
-    [tokens, v_heads]; states fp32 [requests, v_heads, key_size, value_size].
+    // (v_heads / qk_heads)), sizes of 64 or 128; log_decay (at most 0,
+    -inf empties the state) and beta fp32 [tokens, v_heads]; states fp32 [requests, v_heads, key_size, value_size].
     Request b has the rows ``query_offsets[b]:query_offsets[b + 1]`` (offsets
     that decrease anywhere, or leave the rows, give zeros for all and update
     nothing); without query_offsets, one row a request. ``held[b]`` of 0 or less
@@ -66,7 +66,9 @@ def delta_rule(
     default: all) picks kernels and changes no result beyond rounding.
     ``normalize`` divides q and k by sqrt(|x|^2 + 1e-6). scale: key_size ** -0.5
     by default. States, sums and decays are 32 bits, whichever kernel runs. The
-    rule wants beta * |k|^2 of at most 2; beyond, it amplifies what it holds.
+    rule wants beta * |k|^2 of at most 2; beyond, it amplifies what it holds. A NaN
+    or infinity stays in its request (one in v in its column); in a prompt it may
+    also reach up to 63 tokens before its own.
     """
     if scale is None:
         scale = q.shape[-1] ** -0.5

@@ -39,9 +39,7 @@ extern "C" {
 /* What dk_delta_rule works on. q and k: [num_tokens, qk_heads, key_size], v:
  * [num_tokens, v_heads, value_size], of type dtype (DK_KV_F16 or DK_KV_BF16),
  * strides in elements of tokens (0 .. 2^24) and heads, multiples of 8, 16-byte
- * aligned;
- * log_decay and beta: fp32 [num_tokens, v_heads]; states: fp32
- * [requests, v_heads, key_size, value_size], 16-byte aligned. v_heads is a
+ * aligned; log_decay and beta: fp32 [num_tokens, v_heads]; states: fp32 [requests, v_heads, key_size, value_size], 16-byte aligned. v_heads is a
  * multiple of qk_heads (head h has the keys of head h / (v_heads / qk_heads)),
  * key_size and value_size are 64 or 128. */
 typedef struct dk_delta_args {
@@ -81,11 +79,14 @@ size_t dk_delta_workspace_bytes(int num_tokens, int requests, int qk_heads, int 
  *   out = scale S^T q
  * with S as it is after the last token written back. out: dtype, contiguous
  * [num_tokens, v_heads, value_size], 16-byte aligned; it and states are
- * apart from all inputs. A log_decay of -infinity empties the state. With
+ * apart from all inputs. log_decay is at most 0 (over a chunk of 64 tokens its sum
+ * has to stay in fp32's exponents); -infinity empties the state. With
  * beta |k|^2 over 2 (over 2 of normalised keys' beta) the rule itself
  * amplifies what the state holds; long prompts then leave fp32's range sooner
  * than tokens one by one would. Sums and states are fp32. A NaN or infinity
- * stays in its request, and one in v in its column of the state. The
+ * stays in its request, and one in v in its column of the state; in a prompt it
+ * may reach the results of up to 63 tokens before its own, too (a chunk's
+ * products multiply what comes later by 0). The
  * workspace is 256-byte aligned, needs no clearing and holds nothing between
  * calls; calls that overlap in time need workspaces of their own. Over 2^31 -
  * 1 chunks times heads is DK_ERR_UNSUPPORTED. */
@@ -99,7 +100,7 @@ int dk_delta_rule(const dk_delta_args* args, void* out, void* workspace, size_t 
  * channels] (the oldest first), which then hold the last width - 1 inputs. act
  * is z / (1 + exp(-z)) with silu nonzero, else nothing. x, weight [channels,
  * width], bias (or NULL), windows and y have type dtype (F16 or BF16); sums
- * are fp32. x has a stride of tokens, y is contiguous; both, weight and
+ * are fp32. x has a stride of tokens, y is contiguous; max_query_len as in dk_delta_args; both, weight and
  * windows aligned as their elements are (16-byte rows of x, y and windows,
  * and 16-byte weights, take the wide loads). y and windows are apart from all
  * inputs. */

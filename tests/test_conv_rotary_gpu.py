@@ -84,6 +84,20 @@ def test_conv_ragged(channels, width, dtype):
     conv_check(conv_case(lens, channels, width, dtype, bias=False, seed=2), silu=False)
 
 
+def test_conv_hundreds_of_requests():
+    """Offsets are looked through 64 at a time."""
+    lens = [(0, 1, 3, 17, 0, 2)[b % 6] for b in range(200)]
+    for b in (0, 62, 63, 64, 65, 127, 128, 191, 192, 199):
+        lens[b] = 30
+    conv_check(conv_case(lens, 40, 4, seed=12, lead=1, tail=3))
+    conv_check(conv_case(lens, 40, 4, seed=13), most=4)
+
+
+def test_conv_many_tokens():
+    """Where the chip is full anyway a workgroup takes 8 tokens."""
+    conv_check(conv_case([5000, 1, 3200], 264, 4, BF16, seed=14, tail=5))
+
+
 @pytest.mark.parametrize("most", [1, 4, 5, 16, 300])
 def test_conv_max_query_len_only_picks_kernels(most):
     conv_check(conv_case([1, 40, 3, 4, 5], 72, 4, seed=3), most)

@@ -149,6 +149,16 @@ def test_more_prompts_than_seem_to_be(most):
     check(case(lens, 1, 2, 64, 64, BF16, seed=33), max_query_len=most)
 
 
+@pytest.mark.parametrize("most", [1, 70])
+def test_hundreds_of_requests(most):
+    """Offsets are looked through 64 at a time: long requests at either side of
+    those borders, and empty ones."""
+    lens = [(0, 1, 3, 17, 0, 2)[b % 6] for b in range(200)]
+    for b in (0, 62, 63, 64, 65, 127, 128, 191, 192, 199):
+        lens[b] = 70
+    check(case(lens, 1, 1, 64, 64, seed=34, lead=1, tail=3), max_query_len=most)
+
+
 def test_split_steps_are_one_step():
     """A prompt in two steps and then tokens one by one ends where one step does."""
     c = case([90], 2, 1, 128, 128, BF16, seed=7, held=[0])
