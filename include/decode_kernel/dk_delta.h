@@ -39,7 +39,8 @@ extern "C" {
 /* What dk_delta_rule works on. q and k: [num_tokens, qk_heads, key_size], v:
  * [num_tokens, v_heads, value_size], of type dtype (DK_KV_F16 or DK_KV_BF16),
  * strides in elements of tokens (0 .. 2^24) and heads, multiples of 8, 16-byte
- * aligned; log_decay and beta: fp32 [num_tokens, v_heads]; states: fp32 [requests, v_heads, key_size, value_size], 16-byte aligned. v_heads is a
+ * aligned; log_decay and beta: fp32 [num_tokens, v_heads]; states: fp32
+ * [requests, v_heads, key_size, value_size], 16-byte aligned. v_heads is a
  * multiple of qk_heads (head h has the keys of head h / (v_heads / qk_heads)),
  * key_size and value_size are 64 or 128. */
 typedef struct dk_delta_args {
