@@ -380,8 +380,8 @@ __global__ __launch_bounds__(256, 4) void delta_prepare_kernel(DeltaArgs a, Chun
 // two leave in LDS, and bring the next chunk's operands there: what only the
 // outputs need is off the chain that bounds a long prompt. That chain, K' S, the
 // corrections, what they add, each with its largest value, a scale and two parts
-// before it, is 415 instructions a chunk in 1.85 us: one prompt of 8192 tokens of
-// 32 heads takes 237 us on 256 workgroups, 7 of 3001 tokens of 16 heads 41.
+// before it, is 415 instructions a chunk in 1.8 us: one prompt of 8192 tokens of
+// 32 heads takes 231 us on 256 workgroups, 7 of 3001 tokens of 16 heads 42.
 // ---------------------------------------------------------------------------
 using lds_ptr = __attribute__((address_space(3))) void*;
 typedef short short4_t __attribute__((ext_vector_type(4)));
