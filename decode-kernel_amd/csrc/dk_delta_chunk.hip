@@ -13,13 +13,23 @@
 // chunks one after another, with the state in registers.
 //
 // Precision: the state is fp32 and keeps what 32-bit products would give. The
-// matrix cores take fp16, so an fp32 operand goes in as two fp16 parts, 22
-// bits together, after its column (one element of v's axis) was scaled by a
-// power of two to just below fp16's top: a part's own range then reaches 2^-39
-// of the column's largest. Keys and queries are exact in one part: a row is
-// scaled by a power of two (k = 2^e k'), which takes bf16's range away and
-// leaves its 8 bits. The power and the length that a row is divided by go into
-// the rows' factors: with c_i = 2^e / |k_i| and w_i = c_i u_i,
+// matrix cores take 16 bits, and what stands behind a sum decides how an fp32
+// operand goes in.
+//  - Where all terms of a sum belong to one moment (the state in K S and Q S, the
+//    corrections that are added to it, decayed to the chunk's end), what counts is
+//    the largest of a column (one element of v's axis): two fp16 parts, 22 bits
+//    together, after the column was scaled by a power of two to just below fp16's
+//    top; their range reaches 2^-39 of the column's largest.
+//  - Where a sum goes over tokens (T and what it multiplies, P and the
+//    corrections), a decay of 2^-40 may meet a value 2^40 times its neighbours', and
+//    neither has a scale that fits the others: three bf16 parts, which
+//    are the fp32 number in all its bits and all its range. Of the nine products of
+//    parts the six largest are taken, which leaves 2^-24 of a term.
+//  - Keys and queries are one fp16 part: a row is scaled by a power of two (k = 2^e
+//    k') that brings its largest to 1 .. 2, and elements keep all of their bits
+//    down to 2^-14 (fp16's 11) or 2^-17 (bf16's 8) of that, below it 2^-25 of it.
+// The power and the length that a row is divided by go into the rows' factors: with
+// c_i = 2^e / |k_i| and w_i = c_i u_i,
 //   A'_ij = beta_i c_i^2 e^(G_i - G_j) k'_i.k'_j,
 //   w = T' (beta c v - beta c^2 e^G (K' S)),  S_after = e^G_last S + sum_j k'_j (e^(..) w_j).
 #include <hip/hip_runtime.h>
@@ -34,13 +44,16 @@ namespace dk {
 
 namespace {
 
-// What T and P are multiplied by before they become two fp16 parts, so that the
-// second part of a small entry is not lost below fp16's smallest: elements of
-// k' and q' are under 2, so P stays under 4 * 128 * 64 = 2^15, and T under 2 *
-// 22.7 * 512 = 2^14.5 where beta |k|^2 is at most 2 (an entry is at most beta
-// |k_i| |k_j| in the rule's own keys, and k' of 1 to 22.7 in length).
-constexpr float kInverseScale = 512.f, kScoreScale = 64.f;
-constexpr int kFragments = 6;  // 16 x 32 pieces of a lower triangle of 64: (0,0) (1,0) (2,0) (2,1) (3,0) (3,1)
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+
+// A lower triangle of 64 as pieces of 16 rows (tile y) and 32 columns (from 32 t): in
+// 1 .. 4 (1,0) (2,0) (3,0) (3,1), and in 0 what there is of (0,0) and (2,1), the 16
+// columns up to the diagonal: a lane's first 8 bytes are of the one and its last of the
+// other. Without the empty halves the operands of 8192 tokens of 32 heads are 200 MB,
+// not 225, and stay in the last cache: 2.0 and 2.3 us a chunk.
+constexpr int kTriangle = 5;
+constexpr int kParts = 3;  // bf16 parts of an entry of T and P
 
 // The prepared operands of a chunk, as matrix operands A: for a piece of 16
 // rows and 32 columns lane l holds row l % 16 and the columns 4 q .. 4 q + 3
@@ -50,12 +63,12 @@ constexpr int kFragments = 6;  // 16 x 32 pieces of a lower triangle of 64: (0,0
 struct ChunkSpace {
   h8_t* k;    // [qk head][slot][4][dk / 32][64]   K', rows = tokens
   h8_t* q;    // [qk head][slot][4][dk / 32][64]   Q'
-  h8_t* t;    // [v head][slot][6][2][64]          T' * 512: first and second part
-  h8_t* p;    // [v head][slot][6][2][64]          P * 64, of q' and k'
+  b8_t* t;    // [v head][slot][kTriangle][kParts][64]  T'
+  b8_t* p;    // [v head][slot][kTriangle][kParts][64]  P, of q' and k'
   float* s;   // [v head][slot][kFactors * 64]     the rows' factors
   long long slots;
 };
-constexpr int kFactors = 8;  // beta c, beta c^2 e^G, e^G, d, e^(G_last - G), e^G_last (all alike), to 2 KB
+constexpr int kFactors = 5;  // beta c^2 e^G, e^G (the last one is the chunk's), d, e^(G_last - G): a piece of 1 KB; beta c
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -71,11 +84,11 @@ ChunkSpace chunk_space(void* workspace, int tokens, int requests, int qk_heads, 
     return p;
   };
   ChunkSpace c;
-  const size_t rows = slots * qk_heads * kChunk * dk * 2, lower = slots * v_heads * kFragments * 2 * 1024;
+  const size_t rows = slots * qk_heads * kChunk * dk * 2, lower = slots * v_heads * kTriangle * kParts * 1024;
   c.k = reinterpret_cast<h8_t*>(take(rows));
   c.q = reinterpret_cast<h8_t*>(take(rows));
-  c.t = reinterpret_cast<h8_t*>(take(lower));
-  c.p = reinterpret_cast<h8_t*>(take(lower));
+  c.t = reinterpret_cast<b8_t*>(take(lower));
+  c.p = reinterpret_cast<b8_t*>(take(lower));
   c.s = reinterpret_cast<float*>(take(slots * v_heads * kFactors * kChunk * 4));
   c.slots = (long long)slots;
   *bytes = (size_t)(at - static_cast<char*>(workspace));
@@ -86,13 +99,18 @@ __device__ __forceinline__ f4_t mfma(h8_t a, h8_t b, f4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-__device__ __forceinline__ f4_t mfma32(float a, float b, f4_t c) {
-  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+__device__ __forceinline__ f4_t mfma(b8_t a, b8_t b, f4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// Piece (row tile y, columns 32 t ..) of a lower triangle.
-__device__ __forceinline__ constexpr int piece_of(int y, int t) {
-  return (y == 0 ? 0 : y == 1 ? 1 : y == 2 ? 2 : 4) + t;
+// The same of 16 columns, a lane's 4 q .. 4 q + 3: the first half of a piece.
+__device__ __forceinline__ f4_t mfma(short4_t a, b8_t b, f4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
+      a, __builtin_bit_cast(short4_t, __builtin_shufflevector(b, b, 0, 1, 2, 3)), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ f4_t mfma32(float a, float b, f4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
 __device__ __forceinline__ int exponent_of(float m) {
@@ -138,10 +156,60 @@ __device__ __forceinline__ void split_tiles(f4_t x, f4_t y, float scale, h8_t* h
   }
 }
 
+// Two stacked result tiles as an operand of 32 rows in three bf16 parts: one of the
+// number, one of what that leaves, and the rest, which has no more than 8 bits.
+// kNearest: the nearest ones, each at most 2^-9 of the one before and of either sign;
+// for T and P, where nothing waits. Else the upper 16 bits, at most 2^-7 of the one
+// before, an instruction less (1.68 and 1.74 us a chunk). What the products left
+// out then are is as small and of either sign. (An infinity's second part is NaN.)
+struct Split {
+  b8_t part[kParts];
+};
+template <bool kNearest>
+__device__ __forceinline__ Split split_exact(f4_t x, f4_t y) {
+  float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+  uint32_t bits[kParts][4];
+#pragma unroll
+  for (int p = 0; p < kParts; ++p)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t a = __builtin_bit_cast(uint32_t, v[2 * j]), b = __builtin_bit_cast(uint32_t, v[2 * j + 1]);
+      if constexpr (kNearest) {
+        a = (uint32_t)f2bf(v[2 * j]) << 16;
+        b = (uint32_t)f2bf(v[2 * j + 1]) << 16;
+      }
+      bits[p][j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+      v[2 * j] -= __builtin_bit_cast(float, a & 0xFFFF0000u);
+      v[2 * j + 1] -= __builtin_bit_cast(float, b & 0xFFFF0000u);
+    }
+  Split s;
+#pragma unroll
+  for (int p = 0; p < kParts; ++p)
+    s.part[p] = __builtin_bit_cast(b8_t, make_uint4(bits[p][0], bits[p][1], bits[p][2], bits[p][3]));
+  return s;
+}
+
+__device__ __forceinline__ uint2 first_half(b8_t x) {
+  const uint4 w = __builtin_bit_cast(uint4, x);
+  return make_uint2(w.x, w.y);
+}
+
+// The products of parts that are taken: of the first with all, and of the second with two.
+constexpr int kProducts = 6;
+__device__ constexpr int kLeft[kProducts] = {0, 0, 1, 1, 0, 2}, kRight[kProducts] = {0, 1, 0, 1, 2, 0};
+
+// 2^(a - b) of two sums of logarithms in two fp32 parts each, a below b: the
+// difference of the first parts is not exact, and what it leaves counts, since a
+// difference of 40 has steps of 2^-18.
+__device__ __forceinline__ float decay_of(float a, float a_rest, float b, float b_rest) {
+  const float d = a - b;
+  return exp2f(d) * fmaf((a - d) - b + (a_rest - b_rest), 0.69314718f, 1.f);
+}
+
 // ---------------------------------------------------------------------------
 // One workgroup a chunk and head; wave w has its rows 16 w .. 16 w + 15. 8192
-// tokens of 32 heads of 128 (16 of keys), 4096 workgroups, take 65 us: 74 MB read
-// from memory and 170 written, 3.7 TB/s, which bounds it; a workgroup alone would
+// tokens of 32 heads of 128 (16 of keys), 4096 workgroups, take 69 us: 74 MB read
+// from memory and 198 written, 3.9 TB/s, which bounds it; a workgroup alone would
 // take 8 us, and next to others' stores its first loads take 4 of 13.
 // ---------------------------------------------------------------------------
 constexpr int kPad = 68;  // floats a row of 64 takes in LDS
@@ -239,9 +307,9 @@ __global__ __launch_bounds__(256, 4) void delta_prepare_kernel(DeltaArgs a, Chun
       if (lane >= dd) g += o;
     }
     g *= 1.4426950408889634074;  // log2(e)
-    until = exp2f((float)(__shfl(g, 63) - g));
     hi = (float)g;
     lo = (float)(g - (double)hi);
+    until = decay_of(__shfl(hi, 63), __shfl(lo, 63), hi, lo);
     hi_of[lane] = hi;
     lo_of[lane] = lo;
     beta_of[lane] = beta;
@@ -249,26 +317,28 @@ __global__ __launch_bounds__(256, 4) void delta_prepare_kernel(DeltaArgs a, Chun
   __syncthreads();
 
   if (wave == 0) {
-    const float cc = c_of[lane], since = exp2f(hi) * fmaf(lo, 0.69314718f, 1.f);
+    const float cc = c_of[lane], since = decay_of(hi, lo, 0.f, 0.f);
     float* f = ws.s + (h * ws.slots + slot) * (kFactors * kChunk) + lane;
-    f[0] = beta * cc;
-    f[64] = beta * cc * cc * since;
-    f[128] = since;
-    f[192] = d_of[lane];
-    f[256] = until;
-    f[320] = __shfl(since, 63);
+    f[0] = beta * cc * cc * since;
+    f[64] = since;
+    f[128] = d_of[lane];
+    f[192] = until;
+    f[256] = beta * cc;
   }
   // Decayed products of the wave's rows with those before them.
-  const size_t v_at = (h * ws.slots + slot) * (kFragments * 2 * 64);
-  const int piece0 = piece_of(wave, 0);
-  auto pieces_out = [&](h8_t* to, float scale) {
+  const size_t v_at = (h * ws.slots + slot) * (kTriangle * kParts * 64);
+  auto pieces_out = [&](b8_t* to) {
     for (int s = 0; s <= wave / 2; ++s) {
-      h8_t first, second;
+      const bool alone = (wave & 1) == 0 && s == wave / 2;
       const f4_t x = *reinterpret_cast<const f4_t*>(&m[16 * wave + i][32 * s + 4 * q4]);
-      const f4_t y = *reinterpret_cast<const f4_t*>(&m[16 * wave + i][32 * s + 16 + 4 * q4]);
-      split_tiles(x, y, scale, &first, &second);
-      to[v_at + (2 * (piece0 + s)) * 64 + lane] = first;
-      to[v_at + (2 * (piece0 + s) + 1) * 64 + lane] = second;
+      f4_t y{0.f, 0.f, 0.f, 0.f};
+      if (!alone) y = *reinterpret_cast<const f4_t*>(&m[16 * wave + i][32 * s + 16 + 4 * q4]);
+      const Split e = split_exact<true>(x, y);
+      b8_t* at = to + v_at + (alone ? 0 : wave + s) * (kParts * 64) + lane;
+#pragma unroll
+      for (int p = 0; p < kParts; ++p)
+        if (alone) reinterpret_cast<uint2*>(at + p * 64)[s] = first_half(e.part[p]);
+        else at[p * 64] = e.part[p];
     }
   };
   const int rr0 = 16 * wave + 4 * q4;
@@ -295,21 +365,21 @@ __global__ __launch_bounds__(256, 4) void delta_prepare_kernel(DeltaArgs a, Chun
       const float hc = hi_of[col], lc = lo_of[col];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float decay = exp2f((hr[e] - hc) + (lr[e] - lc));
+        const float decay = decay_of(hr[e], lr[e], hc, lc);
         qkt[e] = rr0 + e >= col ? decay * qkt[e] : 0.f;
         kkt[j][e] = rr0 + e > col ? b2[e] * decay * kkt[j][e] : 0.f;
       }
     }
-    if (j <= (wave | 1))
+    if (j <= wave)
 #pragma unroll
       for (int e = 0; e < 4; ++e) m[rr0 + e][col] = qkt[e];
   }
   // A wave's rows of m are its own until the barrier: P goes out from there, then
   // A comes in.
-  pieces_out(ws.p, kScoreScale);
+  pieces_out(ws.p);
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    if (j <= (wave | 1))
+    if (j <= wave)
 #pragma unroll
       for (int e = 0; e < 4; ++e) m[rr0 + e][16 * j + i] = kkt[j][e];
 
@@ -366,7 +436,7 @@ __global__ __launch_bounds__(256, 4) void delta_prepare_kernel(DeltaArgs a, Chun
       for (int e = 0; e < 4; ++e) m[16 * x + 4 * q4 + e][16 * j + i] = below[x][e];
   }
   __syncthreads();
-  pieces_out(ws.t, kInverseScale);
+  pieces_out(ws.t);
 }
 
 // ---------------------------------------------------------------------------
@@ -378,13 +448,13 @@ __global__ __launch_bounds__(256, 4) void delta_prepare_kernel(DeltaArgs a, Chun
 // stands. The other two waves compute half of the tokens' outputs each, one
 // chunk behind, from the parts of the state and the corrections that the first
 // two leave in LDS, and bring the next chunk's operands there: what only the
-// outputs need is off the chain that bounds a long prompt. That chain, K' S, the
-// corrections, what they add, each with its largest value, a scale and two parts
-// before it, is 415 instructions a chunk in 1.8 us: one prompt of 8192 tokens of
-// 32 heads takes 231 us on 256 workgroups, 7 of 3001 tokens of 16 heads 42.
+// outputs need is off the chain that bounds a long prompt. That chain is K' S and
+// what the corrections add, each with its largest value, a scale and two parts
+// before it, and between them the corrections, with three: 1.95 us a chunk (1.8 with
+// two fp16 parts there, too). One prompt of 8192 tokens of 32 heads takes 250 us on
+// 256 workgroups, 7 of 3001 tokens of 16 heads 44.
 // ---------------------------------------------------------------------------
 using lds_ptr = __attribute__((address_space(3))) void*;
-typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
 using lds_short4_ptr = __attribute__((address_space(3))) short4_t*;
 using lds_float_ptr = __attribute__((address_space(3))) float*;
@@ -395,8 +465,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* base, ui
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
 }
 
-__device__ __forceinline__ h8_t load_piece(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
-  return __builtin_bit_cast(h8_t, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0));
+template <typename Piece>
+__device__ __forceinline__ Piece load_piece(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
+  return __builtin_bit_cast(Piece, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0));
 }
 
 // A barrier for what was read from and written to LDS: __syncthreads() waits for
@@ -407,15 +478,15 @@ template <int kDk, int kCols, bool kBf16>
 __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a, ChunkSpace ws, int value_size) {
   constexpr int kS = kDk / 32, kHalfS = kS / 2, kHalfTiles = kDk / 32;
   constexpr int kType = kBf16 ? DK_KV_BF16 : DK_KV_F16;
-  constexpr int kKeys = 4 * kS, kInverse = 2 * kFragments;  // pieces of 1 KB
-  constexpr int kPieces = kKeys + kInverse + 2;
+  constexpr int kKeys = 4 * kS, kInverse = kParts * kTriangle;  // pieces of 1 KB
+  constexpr int kPieces = kKeys + kInverse + 1;
   constexpr f4_t kZero{0.f, 0.f, 0.f, 0.f};
   __shared__ h8_t stage[2][kPieces][64];         // a chunk's operands and its rows' factors
   __shared__ f4_t rows_v[2][kCols][4][64];       // beta c v of a chunk's rows
   __shared__ f4_t share[kCols][2][4][64];        // a half's share of K' S
   __shared__ h8_t left_s[kCols][2 * kS][64];     // the state's parts
   __shared__ f4_t left_w[kCols][4][64];          // the corrections
-  __shared__ float left_scale[kCols][3][16];     // by which both halves of the state and w are to be multiplied
+  __shared__ float left_scale[kCols][2][16];     // by which both halves of the state are to be multiplied
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool outputs = wave >= 2 * kCols;
   const int tile = (wave >> 1) & (kCols - 1), half = wave & 1;
@@ -459,7 +530,9 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
 
       // Operands are read from LDS well ahead of their products: left to itself
       // the compiler reads two, waits for them and goes on.
-      h8_t kf[4 * kHalfS], tf[kInverse], uf[2 * kHalfTiles];
+      h8_t kf[4 * kHalfS], uf[2 * kHalfTiles];
+      short4_t t_first[2][kParts];  // of (0,0) and (2,1)
+      b8_t t_whole[4][kParts];      // (1,0) (2,0) (3,0) (3,1)
 #pragma unroll
       for (int t = 0; t < kHalfS; ++t)
 #pragma unroll
@@ -514,43 +587,51 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         other[y] = share[tile][1 - half][y][lane];
-        b2[y] = rows4(1, y);
+        b2[y] = rows4(0, y);
       }
 #pragma unroll
-      for (int z = 0; z < kInverse; ++z) tf[z] = inverse[z][lane];
+      for (int n = 0; n < kParts; ++n) {
+        t_first[0][n] = *reinterpret_cast<const short4_t*>(&inverse[n][lane]);
 #pragma unroll
-      for (int y = 0; y < 4; ++y) until[y] = rows4(4, y);
-      const float whole = factors[5 * kChunk];
+        for (int z = 0; z < 3; ++z) t_whole[z][n] = __builtin_bit_cast(b8_t, inverse[(z + 1) * kParts + n][lane]);
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) until[y] = rows4(3, y);
+      const float whole = factors[2 * kChunk - 1];
       __builtin_amdgcn_sched_barrier(0);
       // What each token finds wrong in the state before the chunk.
 #pragma unroll
       for (int y = 0; y < 4; ++y)
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[y][e] = fmaf(-b2[y][e], x[y][e] + other[y][e], bv[y][e]);
-      // The corrections w = T x, times 512 / down.
-      shift = column_shift(fmaxf(fmaxf(max4(x[0]), max4(x[1])), fmaxf(max4(x[2]), max4(x[3]))));
-      up = power2(shift);
-      down = power2(-shift) / kInverseScale;
-      h8_t hi[2], lo[2];
-      split_tiles(x[0], x[1], up, &hi[0], &lo[0]);
+      // The corrections w = T x.
       f4_t w[4] = {kZero, kZero, kZero, kZero};
+      const Split x01 = split_exact<false>(x[0], x[1]);
 #pragma unroll
-      for (int part = 0; part < 3; ++part)
+      for (int n = 0; n < kParts; ++n) {
+        t_first[1][n] = *(reinterpret_cast<const short4_t*>(&inverse[n][lane]) + 1);
+        t_whole[3][n] = __builtin_bit_cast(b8_t, inverse[4 * kParts + n][lane]);
+      }
 #pragma unroll
-        for (int y = 0; y < 4; ++y)
-          w[y] = mfma(tf[2 * piece_of(y, 0) + (part == 2)], part == 1 ? lo[0] : hi[0], w[y]);
-      split_tiles(x[2], x[3], up, &hi[1], &lo[1]);
+      for (int n = 0; n < kProducts; ++n) {
+        w[0] = mfma(t_first[0][kLeft[n]], x01.part[kRight[n]], w[0]);
 #pragma unroll
-      for (int part = 0; part < 3; ++part)
+        for (int y = 1; y < 4; ++y) w[y] = mfma(t_whole[y - 1][kLeft[n]], x01.part[kRight[n]], w[y]);
+      }
+      const Split x23 = split_exact<false>(x[2], x[3]);
 #pragma unroll
-        for (int y = 2; y < 4; ++y)
-          w[y] = mfma(tf[2 * piece_of(y, 1) + (part == 2)], part == 1 ? lo[1] : hi[1], w[y]);
+      for (int n = 0; n < kProducts; ++n) {
+        w[2] = mfma(t_first[1][kLeft[n]], x23.part[kRight[n]], w[2]);
+        w[3] = mfma(t_whole[3][kLeft[n]], x23.part[kRight[n]], w[3]);
+      }
       // The state after the chunk.
       f4_t w2[4];
 #pragma unroll
       for (int y = 0; y < 4; ++y) w2[y] = w[y] * until[y];
       shift = column_shift(fmaxf(fmaxf(max4(w2[0]), max4(w2[1])), fmaxf(max4(w2[2]), max4(w2[3]))));
       up = power2(shift);
+      down = power2(-shift);
+      h8_t hi[2], lo[2];
       f4_t add[kHalfTiles];
 #pragma unroll
       for (int z = 0; z < kHalfTiles; ++z) add[z] = kZero;
@@ -565,12 +646,10 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
       if (half == 0) {  // one half of the tokens' corrections each
         left_w[tile][0][lane] = w[0];
         left_w[tile][1][lane] = w[1];
-        if (q4 == 0) left_scale[tile][2][i] = down;
       } else {
         left_w[tile][2][lane] = w[2];
         left_w[tile][3][lane] = w[3];
       }
-      down *= power2(-shift);
 #pragma unroll
       for (int z = 0; z < kHalfTiles; ++z)
 #pragma unroll
@@ -586,7 +665,7 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
     auto of_qk = [&](const h8_t* base, int c) {
       return buffer_of(reinterpret_cast<const char*>(base) + (hq * ws.slots + slot0 + c) * kQkBytes, kQkBytes);
     };
-    auto of_v = [&](const h8_t* base, int c) {
+    auto of_v = [&](const b8_t* base, int c) {
       return buffer_of(reinterpret_cast<const char*>(base) + (h * ws.slots + slot0 + c) * kVBytes, kVBytes);
     };
     auto of_factors = [&](int c) {
@@ -608,18 +687,19 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
     auto bring = [&](int chunk, int which) {
       h8_t* to = &stage[chunk & 1][0][0];
       const int c = min(chunk, chunks - 1);
-      auto some = [&](__amdgpu_buffer_rsrc_t r, int first, int count) {
+      auto some = [&](__amdgpu_buffer_rsrc_t r, int first, int count, int turn) {
 #pragma unroll
         for (int p = 0; p < count; p += 2 * kCols)
-          if (count % (2 * kCols) == 0 || p + wave - 2 * kCols < count)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(to + (first + p + wave - 2 * kCols) * 64), 16,
-                                                     piece_at + (p + wave - 2 * kCols) * 1024, 0, 0, 0);
+          if (count % (2 * kCols) == 0 || p + turn < count)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(to + (first + p + turn) * 64), 16,
+                                                     piece_at + (p + turn) * 1024, 0, 0, 0);
       };
+      const int turn = wave - 2 * kCols;
       if (which == 0) {
-        some(of_qk(ws.k, c), 0, kKeys);
-      } else {
-        some(of_v(ws.t, c), kKeys, kInverse);
-        some(of_factors(c), kKeys + kInverse, 2);
+        some(of_qk(ws.k, c), 0, kKeys, turn);
+      } else {  // as many for each wave: the last has one of T less and the factors
+        some(of_v(ws.t, c), kKeys, kInverse, turn);
+        some(of_factors(c), kKeys + kInverse, 1, 2 * kCols - 1 - turn);
       }
     };
     auto in_order = [] {
@@ -638,14 +718,16 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
     constexpr int kLateLoads = 2 * kS + kKeys / (2 * kCols);  // queries, and a share of keys
     uint4 v;
     float b1;
-    h8_t q[2 * kS], p[8];
+    h8_t q[2 * kS];
+    short4_t p_first[kParts];  // of (0,0) or (2,1)
+    b8_t p[3 * kParts];        // (1,0), or (2,0) (3,0) (3,1)
     auto load_values = [&](int chunk) {
       const int c = min(chunk, chunks - 1);
       const uint32_t count = min(n - c * kChunk, kChunk);
       const auto r =
           buffer_of(values + (long long)c * kChunk * a.v_token, ((count - 1) * (uint32_t)a.v_token + value_size) * 2);
       v = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, v_at, 0, 0));
-      b1 = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(of_factors(c), lane * 4, 0, 0));
+      b1 = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(of_factors(c), (4 * kChunk + lane) * 4, 0, 0));
     };
     auto give_values = [&](int c) {  // to where a result tile has row `lane`
       float* to = reinterpret_cast<float*>(&rows_v[c & 1][tile][lane >> 4][8 * half + 16 * ((lane & 15) >> 2)]) + (lane & 3);
@@ -666,7 +748,7 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
 #pragma unroll
       for (int y = 0; y < 2; ++y)
 #pragma unroll
-        for (int t = 0; t < kS; ++t) q[y * kS + t] = load_piece(qs, piece_at + ((2 * half + y) * kS + t) * 1024);
+        for (int t = 0; t < kS; ++t) q[y * kS + t] = load_piece<h8_t>(qs, piece_at + ((2 * half + y) * kS + t) * 1024);
     };
     load_values(0);
     give_values(0);
@@ -686,31 +768,25 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
         f4_t wv[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) wv[t] = left_w[tile][t][lane];
-        float down = left_scale[tile][2][i];
-        float m = fmaxf(max4(wv[0]), max4(wv[1]));
-        if (half) m = fmaxf(m, fmaxf(max4(wv[2]), max4(wv[3])));
-        const int shift = column_shift(m);
-        const float up = power2(shift);
-        down *= power2(-shift) / kScoreScale;
         y2[0] = y2[1] = kZero;
-        h8_t hi, lo;
-        split_tiles(wv[0], wv[1], up, &hi, &lo);
-        // Rows 0 .. 31 have pieces 0 and 1, rows 32 .. 63 have 2 to 5, two parts each.
+        const Split w01 = split_exact<false>(wv[0], wv[1]);
         if (half) {
 #pragma unroll
-          for (int part = 0; part < 3; ++part)
+          for (int n = 0; n < kProducts; ++n)
 #pragma unroll
-            for (int y = 0; y < 2; ++y) y2[y] = mfma(p[4 * y + (part == 2)], part == 1 ? lo : hi, y2[y]);
-          split_tiles(wv[2], wv[3], up, &hi, &lo);
+            for (int y = 0; y < 2; ++y) y2[y] = mfma(p[kParts * y + kLeft[n]], w01.part[kRight[n]], y2[y]);
+          const Split w23 = split_exact<false>(wv[2], wv[3]);
 #pragma unroll
-          for (int part = 0; part < 3; ++part)
-#pragma unroll
-            for (int y = 0; y < 2; ++y) y2[y] = mfma(p[4 * y + 2 + (part == 2)], part == 1 ? lo : hi, y2[y]);
+          for (int n = 0; n < kProducts; ++n) {
+            y2[0] = mfma(p_first[kLeft[n]], w23.part[kRight[n]], y2[0]);
+            y2[1] = mfma(p[kParts * 2 + kLeft[n]], w23.part[kRight[n]], y2[1]);
+          }
         } else {
 #pragma unroll
-          for (int part = 0; part < 3; ++part)
-#pragma unroll
-            for (int y = 0; y < 2; ++y) y2[y] = mfma(p[2 * y + (part == 2)], part == 1 ? lo : hi, y2[y]);
+          for (int n = 0; n < kProducts; ++n) {
+            y2[0] = mfma(p_first[kLeft[n]], w01.part[kRight[n]], y2[0]);
+            y2[1] = mfma(p[kLeft[n]], w01.part[kRight[n]], y2[1]);
+          }
         }
         give_values(c + 1);
         __builtin_amdgcn_sched_barrier(0);
@@ -720,7 +796,7 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
         for (int y = 0; y < 2; ++y)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float o = d[y][e] * fmaf(y2[y][e], down, x[y][e]);
+            const float o = d[y][e] * (y2[y][e] + x[y][e]);
             __builtin_amdgcn_raw_buffer_store_b16(to_half_bits<kType>(o), r, out_at[4 * y + e], 0, 0);
           }
       }
@@ -738,8 +814,8 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
       f4_t since[2];
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        since[y] = *reinterpret_cast<const f4_t*>(factors + 2 * kChunk + 32 * half + 16 * y + 4 * q4);
-        d[y] = *reinterpret_cast<const f4_t*>(factors + 3 * kChunk + 32 * half + 16 * y + 4 * q4);
+        since[y] = *reinterpret_cast<const f4_t*>(factors + kChunk + 32 * half + 16 * y + 4 * q4);
+        d[y] = *reinterpret_cast<const f4_t*>(factors + 2 * kChunk + 32 * half + 16 * y + 4 * q4);
       }
       __builtin_amdgcn_sched_barrier(0);
       f4_t x0[2] = {kZero, kZero}, x1[2] = {kZero, kZero};  // of the state's halves
@@ -762,9 +838,12 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
       const auto ps = of_v(ws.p, c);
       if (half)
 #pragma unroll
-        for (int z = 4; z < 8; ++z) p[z] = load_piece(ps, piece_at + (4 + z) * 1024);
+        for (int z = kParts; z < 3 * kParts; ++z) p[z] = load_piece<b8_t>(ps, piece_at + (2 * kParts + z) * 1024);
 #pragma unroll
-      for (int z = 0; z < 4; ++z) p[z] = load_piece(ps, piece_at + (4 * half + z) * 1024);
+      for (int z = 0; z < kParts; ++z) {
+        p_first[z] = __builtin_bit_cast(short4_t, __builtin_amdgcn_raw_buffer_load_b64(ps, piece_at + z * 1024 + 8 * half, 0, 0));
+        p[z] = load_piece<b8_t>(ps, piece_at + (kParts * (1 + half) + z) * 1024);
+      }
       load_values(c + 2);
       bring(c + 1, 1);
       in_order();  // kLateLoads counts what comes behind this
@@ -774,7 +853,8 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
       in_order();
       // Chunk c + 1's keys, asked for before the last turn's stores, are there:
       // at least so many more were asked for since.
-      constexpr int kSince = 8 + 4 + 2 + kInverse / (2 * kCols) + (kCols == 1 ? 1 : 0) + kLateLoads;
+      static_assert((kInverse + 1) % (2 * kCols) == 0, "every wave brings as much");
+      constexpr int kSince = 8 + 2 * kParts + 2 + (kInverse + 1) / (2 * kCols) + kLateLoads;
       wait_but(std::integral_constant<int, kSince>{});
     }
     __builtin_amdgcn_s_waitcnt(0);  // nothing is on its way to LDS behind the end

@@ -84,7 +84,12 @@ size_t dk_delta_workspace_bytes(int num_tokens, int requests, int qk_heads, int 
  * has to stay in fp32's exponents); -infinity empties the state. With
  * beta |k|^2 over 2 (over 2 of normalised keys' beta) the rule itself
  * amplifies what the state holds; long prompts then leave fp32's range sooner
- * than tokens one by one would. Sums and states are fp32. A NaN or infinity
+ * than tokens one by one would. Sums and states are fp32, and a result is off by
+ * their roundings at the token's own time, whatever came before or comes later:
+ * in a prompt's products the state has 22 bits, counted from the largest value of
+ * its column, and values, decays and corrections have 24 of their own. With beta
+ * |k|^2 near 2 and keys that hardly differ the corrections of a prompt's 64 tokens
+ * cancel, and up to 2e-3 of values and state is lost (1e-4 token by token). A NaN or infinity
  * stays in its request, and one in v in its column of the state; in a prompt it
  * may reach the results of up to 63 tokens before its own, too (a chunk's
  * products multiply what comes later by 0). The

@@ -407,3 +407,60 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="multiple"):
         delta_rule(c["q"], c["k"], torch.zeros(2, 3, 64, device="cuda").half(), torch.zeros(2, 3, device="cuda"),
                    torch.zeros(2, 3, device="cuda"), three)
+
+
+def rows_apart(n, dtype, first, then, log_decay, seed):
+    """Requests whose values are `first` in size for 20 tokens of every 50 and
+    `then` in the others, with a decay before each change to `then`."""
+    c = case([n], 2, 1, 64, 64, dtype, seed=seed, held=[1])
+    t = torch.arange(n, device="cuda") % 50
+    size = torch.where(t < 20, first, then).view(n, 1, 1)
+    c["v"] = (c["v"].float() * size).to(dtype)
+    c["log_decay"][t == 20] = log_decay
+    return c
+
+
+@pytest.mark.parametrize("n", [9, 60, 130])
+@pytest.mark.parametrize("dtype,first,then,log_decay", [
+    (F16, 1e4, 1e-3, -16.0), (F16, 1e4, 1e-3, -float("inf")), (F16, 1e-3, 1e4, 0.0), (BF16, 1e6, 1.0, -14.0), (BF16, 1e12, 1.0, -28.0),
+    (BF16, 1e12, 1.0, -float("inf")), (BF16, 1.0, 1e12, 0.0), (BF16, 1e25, 1e-5, -69.0), (BF16, 1e-20, 1e10, -1.0)])
+def test_rows_of_values_far_apart(n, dtype, first, then, log_decay):
+    """What a decay leaves of large values next to small ones, and small values
+    before large ones: a token's error is that of the state as it is then, so
+    that the bounds of outputs and states stand as they are."""
+    check(rows_apart(n, dtype, first, then, log_decay, seed=35))
+
+
+@pytest.mark.parametrize("n", [12, 64, 200])
+def test_rows_and_decays_of_every_size(n):
+    """Values of eight powers of ten, each token's its own, and decays from none to all."""
+    c = case([n], 2, 2, 128, 64, BF16, seed=36, held=[1])
+    g = torch.Generator().manual_seed(37)
+    c["v"] = (c["v"].float() * (10.0 ** (8 * torch.rand(n, 4, 1, generator=g) - 4)).cuda()).to(BF16)
+    strong = (torch.rand(n, 4, generator=g) < 0.2).cuda()
+    c["log_decay"] = torch.where(strong, -(40 * torch.rand(n, 4, generator=g)).cuda(), c["log_decay"])
+    c["log_decay"][(torch.rand(n, 4, generator=g) < 0.03).cuda()] = -float("inf")
+    check(c)
+
+
+@pytest.mark.parametrize("size", [64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_one_key_at_beta_two_keeps_what_is_promised(size, dtype):
+    """What 64 tokens of one key with beta 2 cost in a chunk: T = (1 + A)^-1 has
+    entries of up to 2 throughout, A's are off by four roundings (the key's
+    length twice, beta, the product), and a correction goes through up to 64
+    rows and 64 columns of them: 64 * 64 * 2 * 4 * 2^-24 = 2e-3 of the values and
+    the column, which is what the interface says. Tokens one by one keep 1e-4."""
+    for n, most, promised in ((150, None, 2e-3), (150, 1, 1e-4)):
+        c = case([n], 2, 1, size, 64, dtype, seed=38, held=[1])
+        c["k"][:] = c["k"][:1].clone()
+        c["beta"].fill_(2.0)
+        c["log_decay"].zero_()
+        o, states = run(c, most)
+        want_o, want_s, reach = expect(c)
+        column = np.sqrt((want_s**2).sum(-2, keepdims=True))
+        most_v = np.abs(c["v"].double().cpu().numpy()).max(0)[None, :, None]
+        bound = promised * (column + most_v)
+        assert (np.abs(states.double().cpu().numpy() - want_s) <= bound).all()
+        bound_o = torch.finfo(dtype).eps / 2 * np.abs(want_o) + promised * (reach + most_v[:, :, 0] * size**-0.5) + 2.0**-25
+        assert (np.abs(o.double().cpu().numpy() - want_o) <= bound_o).all()
