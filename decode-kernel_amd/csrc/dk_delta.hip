@@ -386,8 +386,8 @@ extern "C" int dk_delta_rule(const dk_delta_args* p, void* out, void* workspace,
   const size_t need = chunks ? dk_delta_workspace_bytes(p->num_tokens, p->requests, p->qk_heads, p->v_heads,
                                                         p->key_size, p->max_query_len) : 0;
   if (chunks) {
-    if ((p->num_tokens / (long long)dk::kChunk + p->requests) * p->v_heads > INT32_MAX)
-      return dk::set_error(DK_ERR_UNSUPPORTED, "too large: chunks times heads must fit in int32");
+    if (!dk::fits_launch((p->num_tokens / (long long)dk::kChunk + p->requests) * p->v_heads, dk::kPrepareThreads))
+      return dk::set_error(DK_ERR_UNSUPPORTED, "too large: chunks times heads must be under 2^24");
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < need)
       return dk::set_error(DK_ERR_INVALID_ARGUMENT,
                            "workspace must be 256-byte aligned and of %zu bytes", need);
@@ -464,7 +464,7 @@ extern "C" int dk_short_conv(const void* x, long long x_token_stride, const void
   // tokens of 1544 channels 10.1 against 11.5 us).
   const int tile = !offsets ? 1 : max_query_len <= 4 || (long long)num_tokens / 8 * blocks < 1024 ? 4 : 8;
   const long long tiles = offsets ? (long long)num_tokens / tile + requests + 1 : requests;
-  if (tiles > INT32_MAX || blocks > 65535)
+  if (!dk::fits_launch(tiles, 256) || blocks > 65535)
     return dk::set_error(DK_ERR_UNSUPPORTED, "too many tokens or channels for one call");
   const dk::ConvArgs a{static_cast<const uint16_t*>(x), x_token_stride,
                        static_cast<const uint16_t*>(weight), static_cast<const uint16_t*>(bias),

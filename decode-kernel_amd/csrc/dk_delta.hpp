@@ -10,6 +10,7 @@
 namespace dk {
 
 constexpr int kChunk = 64;           // tokens that the chunked form takes at once
+constexpr int kPrepareThreads = 256; // of the workgroup that prepares a chunk and head
 constexpr float kUnitEps = 1e-6f;    // added to a squared length
 // Below this a decay's exponential is 0 in fp32 (e^-128 < 2^-149): logarithms
 // are cut there, so that sums over a chunk stay finite and differences exact.

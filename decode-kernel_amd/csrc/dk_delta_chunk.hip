@@ -215,7 +215,7 @@ __device__ __forceinline__ float decay_of(float a, float a_rest, float b, float 
 constexpr int kPad = 68;  // floats a row of 64 takes in LDS
 
 template <int kDk, bool kBf16>
-__global__ __launch_bounds__(256, 4) void delta_prepare_kernel(DeltaArgs a, ChunkSpace ws) {
+__global__ __launch_bounds__(kPrepareThreads, 4) void delta_prepare_kernel(DeltaArgs a, ChunkSpace ws) {
   constexpr int kS = kDk / 32;
   __shared__ h8_t keys[4][kS][64];
   __shared__ float m[kChunk][kPad];
@@ -888,7 +888,7 @@ int delta_chunk_launch(const DeltaArgs& a, int key_size, int value_size, bool bf
   const int cols = tiles > 256 ? 2 : 1;
   const dim3 columns((unsigned)(a.v_heads * (value_size / (16 * cols))), longs);
   auto launch = [&](auto prepare, auto one, auto two) {
-    hipLaunchKernelGGL(prepare, chunks, dim3(256), 0, stream, a, ws);
+    hipLaunchKernelGGL(prepare, chunks, dim3(kPrepareThreads), 0, stream, a, ws);
     if (cols == 1) hipLaunchKernelGGL(one, columns, dim3(256), 0, stream, a, ws, value_size);
     else hipLaunchKernelGGL(two, columns, dim3(512), 0, stream, a, ws, value_size);
   };

@@ -5,6 +5,9 @@
 
 namespace dk {
 
+// What a launch takes along x: workgroups times their threads in 32 bits.
+inline bool fits_launch(long long workgroups, int threads) { return workgroups <= 0xFFFFFFFFLL / threads; }
+
 // Record a formatted message for dk_last_error() on this thread; returns code.
 int set_error(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 

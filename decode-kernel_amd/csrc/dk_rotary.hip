@@ -218,6 +218,8 @@ extern "C" int dk_rotate_qk(const void* q, long long q_token_stride, long long q
   }
   const long long groups = ((long long)num_tokens + tokens_each - 1) / tokens_each;
   const unsigned splits = (unsigned)((heads + heads_each - 1) / heads_each);
+  if (!dk::fits_launch(groups, dk::kRotaryThreads))
+    return dk::set_error(DK_ERR_UNSUPPORTED, "too many tokens for one call");
   if (splits > 65535)
     return dk::set_error(DK_ERR_UNSUPPORTED, "too many heads for this head size");
   const dk::RotaryArgs a{{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k)},

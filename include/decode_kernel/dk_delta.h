@@ -94,8 +94,8 @@ size_t dk_delta_workspace_bytes(int num_tokens, int requests, int qk_heads, int 
  * may reach the results of up to 63 tokens before its own, too (a chunk's
  * products multiply what comes later by 0). The
  * workspace is 256-byte aligned, needs no clearing and holds nothing between
- * calls; calls that overlap in time need workspaces of their own. Over 2^31 -
- * 1 chunks times heads is DK_ERR_UNSUPPORTED. */
+ * calls; calls that overlap in time need workspaces of their own. From 2^24
+ * chunks of 64 tokens (one more a request) times heads on it is DK_ERR_UNSUPPORTED. */
 int dk_delta_rule(const dk_delta_args* args, void* out, void* workspace, size_t workspace_bytes,
                   hipStream_t stream);
 
@@ -109,7 +109,8 @@ int dk_delta_rule(const dk_delta_args* args, void* out, void* workspace, size_t 
  * are fp32. x has a stride of tokens, y is contiguous; max_query_len as in dk_delta_args; both, weight and
  * windows aligned as their elements are (16-byte rows of x, y and windows,
  * and 16-byte weights, take the wide loads). y and windows are apart from all
- * inputs. */
+ * inputs. A call takes fewer than 2^24 tiles of 4 or 8 tokens (one more a request;
+ * of one token without offsets), else it is DK_ERR_UNSUPPORTED. */
 int dk_short_conv(const void* x, long long x_token_stride, const void* weight, const void* bias,
                   void* windows, const int32_t* held, const int32_t* offsets, int dtype,
                   int num_tokens, int requests, int channels, int width, int max_query_len,

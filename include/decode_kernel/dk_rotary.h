@@ -42,7 +42,8 @@ extern "C" {
  * [num_frequencies], values outside 0 .. num_axes - 1 taken as the nearest of
  * them, NULL for all 0. The angle is formed in 64 bits and reduced to one turn
  * there, so far positions cost no accuracy; cos, sin and the products are fp32.
- * q or k may have 0 heads. Outputs are apart from all inputs. */
+ * q or k may have 0 heads. Outputs are apart from all inputs. From 2^26 - 3 tokens
+ * on it is DK_ERR_UNSUPPORTED. */
 int dk_rotate_qk(const void* q, long long q_token_stride, long long q_head_stride, int q_heads,
                  const void* k, long long k_token_stride, long long k_head_stride, int k_heads,
                  int dtype, int head_size, int num_tokens, const void* positions, int positions64,

@@ -70,6 +70,16 @@ def test_delta_workspace(lib):
     assert 0 < one < two and one % 256 == 0
 
 
+def test_more_than_a_launch_takes(lib):
+    """A launch has fewer than 2^32 threads along x, and a call whose second launch
+    would have more has changed the states in its first: refused before any."""
+    _refused(lib, _delta(lib, num_tokens=64 * (2**22 - 2), max_query_len=2**28), "too large", _abi.DK_ERR_UNSUPPORTED)
+    _refused(lib, _conv(lib, tokens=2**24, requests=2**24, offsets=None, channels=8), "too many", _abi.DK_ERR_UNSUPPORTED)
+    _refused(lib, _conv(lib, tokens=8 * (2**24 - 3), channels=8), "too many", _abi.DK_ERR_UNSUPPORTED)
+    _refused(lib, _rotate(lib, tokens=2**26 - 3, qh=1, kh=0, k=None, k_out=None), "too many", _abi.DK_ERR_UNSUPPORTED)
+    _refused(lib, _rotate(lib, tokens=2**26 - 3, qh=64, kh=8), "too many", _abi.DK_ERR_UNSUPPORTED)
+
+
 def _conv(lib, x=FAKE, stride=16, weight=FAKE, bias=None, windows=FAKE, held=None, offsets=FAKE, dtype=0, tokens=9, requests=2,
           channels=16, width=4, most=9, silu=1, y=FAKE):
     return lib.dk_short_conv(x, stride, weight, bias, windows, held, offsets, dtype, tokens, requests, channels, width, most,
