@@ -342,7 +342,7 @@ extern "C" size_t dk_delta_workspace_bytes(int num_tokens, int requests, int qk_
   if (num_tokens <= 0 || requests <= 0 || qk_heads <= 0 || v_heads <= 0 || v_heads % qk_heads ||
       !delta_size(key_size) || max_query_len <= dk::kStepTokens)
     return 0;
-  return dk::delta_chunk_bytes(num_tokens, requests, qk_heads, v_heads, key_size);
+  return dk::delta_chunk_bytes(num_tokens, requests, dk::kStepTokens, qk_heads, v_heads, key_size);
 }
 
 extern "C" int dk_delta_rule(const dk_delta_args* p, void* out, void* workspace,
@@ -386,7 +386,7 @@ extern "C" int dk_delta_rule(const dk_delta_args* p, void* out, void* workspace,
   const size_t need = chunks ? dk_delta_workspace_bytes(p->num_tokens, p->requests, p->qk_heads, p->v_heads,
                                                         p->key_size, p->max_query_len) : 0;
   if (chunks) {
-    if (!dk::fits_launch((p->num_tokens / (long long)dk::kChunk + p->requests) * p->v_heads, dk::kPrepareThreads))
+    if (!dk::fits_launch(dk::chunk_slots(p->num_tokens, p->requests, dk::kStepTokens) * p->v_heads, dk::kPrepareThreads))
       return dk::set_error(DK_ERR_UNSUPPORTED, "too large: chunks times heads must be under 2^24");
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < need)
       return dk::set_error(DK_ERR_INVALID_ARGUMENT,

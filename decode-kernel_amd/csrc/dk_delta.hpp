@@ -64,7 +64,9 @@ __device__ __forceinline__ int find_long(const int32_t* offsets, int requests, i
 // A tile of a request's new tokens. Tiles of `tile` tokens have numbers that
 // need no sum over the requests: request b's begin at offsets[b] / tile + b,
 // and since floor(x + n) - floor(x) + 1 >= ceil(n), they end before the next
-// request's do begin. tokens / tile + requests numbers are enough.
+// request's do begin. tokens / tile + requests numbers are enough. Where only
+// requests of more than `limit` tokens have tiles, b is the request's number
+// among those.
 struct Tile {
   int request;    // -1: the number is nobody's
   int row;        // its first row
@@ -74,23 +76,39 @@ struct Tile {
   int head, end;  // the first row of all requests, and one past the last
 };
 
-// The tile with number `number`, and whether offsets are good; by each wave for
+// Numbers that the chunks of requests of more than `limit` tokens take.
+inline long long chunk_slots(int tokens, int requests, int limit) {
+  const int longs = tokens / (limit + 1);
+  return (long long)(tokens / kChunk) + (requests < longs ? requests : longs);
+}
+
+// The tile with number `number` (kLong: of requests of more than `limit` tokens), and whether offsets are good; by each wave for
 // itself, with the same answer in all. Offsets are loaded once, 64 requests at
 // a time, and what is needed of them is taken from other lanes: a load that
 // waits for another costs 1 to 2 us next to stores of a full chip.
+template <bool kLong = false>
 __device__ __forceinline__ bool find_tile(const int32_t* offsets, int requests, int tokens, int tile,
-                                          int number, Tile* out) {
+                                          int number, Tile* out, int limit = 0) {
   const int lane = threadIdx.x & 63;
-  int b = -1, from_b = 0, to_b = 0, head = 0, end = 0;
+  int b = -1, rank_b = 0, from_b = 0, to_b = 0, head = 0, end = 0, longs = 0;
   bool bad = false;
   for (int first = 0; first < requests; first += 64) {
     const int i = min(first + lane, requests - 1);
     const int from = offsets[i], to = offsets[i + 1];
     bad |= to < from;
-    const unsigned long long before = __ballot(first + lane < requests && from / tile + i <= number);
+    bool has = first + lane < requests;
+    int rank = i;
+    if constexpr (kLong) {
+      has = has && to - from > limit;
+      const unsigned long long is = __ballot(has);
+      rank = longs + __builtin_amdgcn_mbcnt_hi((uint32_t)(is >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)is, 0));
+      longs += __popcll(is);
+    }
+    const unsigned long long before = __ballot(has && from / tile + rank <= number);
     if (before) {  // requests' tiles begin one after another: the last that does before the number
       const int at = 63 - __clzll(before);
       b = first + at;
+      rank_b = kLong ? __builtin_amdgcn_readlane(rank, at) : b;
       from_b = __builtin_amdgcn_readlane(from, at);
       to_b = __builtin_amdgcn_readlane(to, at);
     }
@@ -100,7 +118,7 @@ __device__ __forceinline__ bool find_tile(const int32_t* offsets, int requests, 
   *out = Tile{-1, 0, 0, 0, 0, head, end};
   if (__ballot(bad) || head < 0 || end > tokens) return false;
   if (b < 0) return true;
-  const int n = to_b - from_b, index = number - (from_b / tile + b);
+  const int n = to_b - from_b, index = number - (from_b / tile + rank_b);
   if ((long long)index * tile >= n) return true;
   out->request = b;
   out->row = from_b + index * tile;
@@ -110,7 +128,7 @@ __device__ __forceinline__ bool find_tile(const int32_t* offsets, int requests, 
   return true;
 }
 
-size_t delta_chunk_bytes(int num_tokens, int requests, int qk_heads, int v_heads, int key_size);
+size_t delta_chunk_bytes(int num_tokens, int requests, int limit, int qk_heads, int v_heads, int key_size);
 int delta_chunk_launch(const DeltaArgs& a, int key_size, int value_size, bool bf16, void* workspace,
                        hipStream_t stream);
 

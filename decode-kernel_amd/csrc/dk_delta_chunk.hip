@@ -72,11 +72,7 @@ constexpr int kFactors = 5;  // beta c^2 e^G, e^G (the last one is the chunk's),
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-long long slots_of(int tokens, int requests) { return (long long)tokens / kChunk + requests; }
-
-ChunkSpace chunk_space(void* workspace, int tokens, int requests, int qk_heads, int v_heads, int dk,
-                       size_t* bytes) {
-  const size_t slots = (size_t)slots_of(tokens, requests);
+ChunkSpace chunk_space(void* workspace, size_t slots, int qk_heads, int v_heads, int dk, size_t* bytes) {
   char* at = static_cast<char*>(workspace);
   auto take = [&](size_t n) {
     char* p = at;
@@ -225,9 +221,8 @@ __global__ __launch_bounds__(kPrepareThreads, 4) void delta_prepare_kernel(Delta
   const long long slot = blockIdx.x / a.v_heads;
   const int h = blockIdx.x % a.v_heads, hq = h / a.group;
   Tile tile;
-  if (!find_tile(a.offsets, a.requests, a.tokens, kChunk, (int)slot, &tile)) return;
+  if (!find_tile<true>(a.offsets, a.requests, a.tokens, kChunk, (int)slot, &tile, a.limit)) return;
   if (tile.request < 0) return;
-  if (tile.total <= a.limit) return;
   const bool first_of_group = h % a.group == 0;
 
   // Every load first; rows behind the last are row 0 again, and zeros below.
@@ -502,7 +497,7 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
   if (b < 0) return;
   const int from = __builtin_amdgcn_readfirstlane(a.offsets[b]);
   const int n = __builtin_amdgcn_readfirstlane(a.offsets[b + 1]) - from;
-  const long long slot0 = from / kChunk + b;
+  const long long slot0 = from / kChunk + rank;
   const int chunks = (n + kChunk - 1) / kChunk;
 
   // A chunk takes two barriers. State waves: the first, K' S from the state, the
@@ -865,17 +860,18 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
 
 }  // namespace
 
-size_t delta_chunk_bytes(int num_tokens, int requests, int qk_heads, int v_heads, int key_size) {
+size_t delta_chunk_bytes(int num_tokens, int requests, int limit, int qk_heads, int v_heads, int key_size) {
   size_t bytes;
-  chunk_space(nullptr, num_tokens, requests, qk_heads, v_heads, key_size, &bytes);
+  chunk_space(nullptr, chunk_slots(num_tokens, requests, limit), qk_heads, v_heads, key_size, &bytes);
   return bytes;
 }
 
 int delta_chunk_launch(const DeltaArgs& a, int key_size, int value_size, bool bf16, void* workspace,
                        hipStream_t stream) {
   size_t bytes;
-  const ChunkSpace ws = chunk_space(workspace, a.tokens, a.requests, a.qk_heads, a.v_heads, key_size, &bytes);
-  const dim3 chunks((unsigned)(slots_of(a.tokens, a.requests) * a.v_heads));
+  const long long slots = chunk_slots(a.tokens, a.requests, a.limit);
+  const ChunkSpace ws = chunk_space(workspace, slots, a.qk_heads, a.v_heads, key_size, &bytes);
+  const dim3 chunks((unsigned)(slots * a.v_heads));
   // Tiles of 16 columns: two a workgroup where one each would not be at work at
   // once (its LDS leaves one workgroup a CU). One and two, us: 256 tiles (a prompt
   // of 8192 tokens of 32 heads) 264 and 353, 896 (7 prompts of 16 heads) 57 and 42.

@@ -464,3 +464,21 @@ def test_one_key_at_beta_two_keeps_what_is_promised(size, dtype):
         assert (np.abs(states.double().cpu().numpy() - want_s) <= bound).all()
         bound_o = torch.finfo(dtype).eps / 2 * np.abs(want_o) + promised * (reach + most_v[:, :, 0] * size**-0.5) + 2.0**-25
         assert (np.abs(o.double().cpu().numpy() - want_o) <= bound_o).all()
+
+
+@pytest.mark.parametrize("places", [(0, 1, 2, 3, 4, 5), (63, 64, 127, 128, 400, 699), (694, 695, 696, 697, 698, 699)])
+def test_prompts_among_hundreds_of_single_tokens(places):
+    """Chunks are numbered by the requests that have any: those before, between and
+    behind them take no number."""
+    lens = [1] * 700
+    for b, n in zip(places, (17, 64, 65, 130, 300, 128)):
+        lens[b] = n
+    lens[350] = 0
+    check(case(lens, 1, 1, 64, 64, BF16, seed=39, lead=60, tail=9), max_query_len=300)
+
+
+def test_as_many_prompts_as_there_is_room_for():
+    """Requests of 17 tokens alone, the most that tokens can be of, and empty ones:
+    the numbers' end."""
+    check(case([17, 0] * 70, 1, 1, 64, 64, seed=40), max_query_len=17)
+    check(case([0, 17, 0], 1, 1, 64, 64, seed=41), max_query_len=17)

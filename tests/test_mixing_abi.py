@@ -80,6 +80,14 @@ def test_more_than_a_launch_takes(lib):
     _refused(lib, _rotate(lib, tokens=2**26 - 3, qh=64, kh=8), "too many", _abi.DK_ERR_UNSUPPORTED)
 
 
+def test_delta_workspace_goes_by_requests_in_chunks(lib):
+    """Requests of up to 16 tokens have no chunk: 3071 tokens can be those of 180
+    others at most, whatever the batch's places are."""
+    size = lib.dk_delta_workspace_bytes
+    assert size(3071, 1024, 16, 32, 128, 2048) == size(3071, 180, 16, 32, 128, 2048) > size(3071, 179, 16, 32, 128, 2048)
+    assert size(2048, 1, 16, 32, 128, 2048) < size(2048, 2, 16, 32, 128, 2048)
+
+
 def _conv(lib, x=FAKE, stride=16, weight=FAKE, bias=None, windows=FAKE, held=None, offsets=FAKE, dtype=0, tokens=9, requests=2,
           channels=16, width=4, most=9, silu=1, y=FAKE):
     return lib.dk_short_conv(x, stride, weight, bias, windows, held, offsets, dtype, tokens, requests, channels, width, most,
