@@ -68,6 +68,7 @@ struct ChunkSpace {
   float* s;   // [v head][slot][kFactors * 64]     the rows' factors
   long long slots;
 };
+constexpr int kCus = 256;
 constexpr int kFactors = 5;  // beta c^2 e^G, e^G (the last one is the chunk's), d, e^(G_last - G): a piece of 1 KB; beta c
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -487,8 +488,8 @@ __global__ __launch_bounds__(256 * kCols, 1) void delta_scan_kernel(DeltaArgs a,
   const int tile = (wave >> 1) & (kCols - 1), half = wave & 1;
   const int h = blockIdx.x % a.v_heads, hq = h / a.group;
   if (!wave_offsets_ok(a.offsets, a.requests, a.tokens)) return;
-  // The grid has room for as many long requests as there seem to be; where there
-  // are more, a workgroup takes several, one after another.
+  // The grid has room for so many long requests; where there are more, a workgroup
+  // takes several, one after another.
   for (int rank = blockIdx.y;; rank += gridDim.y) {
   int lane = threadIdx.x & 63;
   asm volatile("" : "+v"(lane));  // or all addresses of both kinds of waves are kept across requests
@@ -873,16 +874,26 @@ int delta_chunk_launch(const DeltaArgs& a, int key_size, int value_size, bool bf
   const ChunkSpace ws = chunk_space(workspace, slots, a.qk_heads, a.v_heads, key_size, &bytes);
   const dim3 chunks((unsigned)(slots * a.v_heads));
   // Tiles of 16 columns: two a workgroup where one each would not be at work at
-  // once (its LDS leaves one workgroup a CU). One and two, us: 256 tiles (a prompt
-  // of 8192 tokens of 32 heads) 264 and 353, 896 (7 prompts of 16 heads) 57 and 42.
-  // Room for as many long requests as there may well be: workgroups take several
-  // where there are more, and one without any costs its turn on a CU (61 single
-  // tokens and a prompt of 2048, 32 heads: 122 us, and 154 with room for 62 of them).
-  const long long seem = std::max(1LL, 2LL * a.tokens / a.longest);
-  const unsigned longs = (unsigned)std::max(1LL, std::min({seem, (long long)a.requests, (long long)a.tokens / (a.limit + 1)}));
-  const long long tiles = (long long)std::min(longs, (unsigned)std::max(1, a.tokens / a.longest)) * a.v_heads * (value_size / 16);
-  const int cols = tiles > 256 ? 2 : 1;
-  const dim3 columns((unsigned)(a.v_heads * (value_size / (16 * cols))), longs);
+  // once (its LDS leaves one workgroup a CU). One and two, us: 256 tiles (61 single
+  // tokens and a prompt of 2048 of 32 heads) 124 and 144, 512 (4 prompts of 2048 of
+  // 16 heads) 162 and 131, 1920 (60 prompts of 100 of 4 heads) 78 and 60. How many
+  // requests are at work at once goes by the longest, or, where max_query_len says
+  // no more than the number of tokens does, by their average (and is one where that
+  // is under a chunk: single tokens and a prompt).
+  const long long average = a.tokens / a.requests;
+  const long long each = a.longest < a.tokens ? a.longest : average >= kChunk ? average : a.tokens;
+  const long long at_once = std::min((long long)a.requests, std::max(1LL, a.tokens / each));
+  const int cols = at_once * a.v_heads * (value_size / 16) > kCus ? 2 : 1;
+  // Room for three times the requests that fill the chip, whatever max_query_len is:
+  // workgroups take several where there are more, and one without any costs its
+  // turn on a CU. Once, three times and room for all, us: 7 ragged prompts of 16
+  // heads 77, 66 and 66; 8192 tokens and 100 prompts of 80 of 4 heads 316, 267 and
+  // 242; the 62 requests above 126, 124 and 187; 64 prompts of 128 of 32 heads 411,
+  // 411 and 471.
+  const int workgroups = a.v_heads * (value_size / (16 * cols));
+  const long long longs = std::min((long long)a.requests, (long long)a.tokens / (a.limit + 1));
+  const unsigned room = (unsigned)std::max(1LL, std::min(longs, 3LL * ((kCus + workgroups - 1) / workgroups)));
+  const dim3 columns((unsigned)workgroups, room);
   auto launch = [&](auto prepare, auto one, auto two) {
     hipLaunchKernelGGL(prepare, chunks, dim3(kPrepareThreads), 0, stream, a, ws);
     if (cols == 1) hipLaunchKernelGGL(one, columns, dim3(256), 0, stream, a, ws, value_size);

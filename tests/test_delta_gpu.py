@@ -482,3 +482,37 @@ def test_as_many_prompts_as_there_is_room_for():
     the numbers' end."""
     check(case([17, 0] * 70, 1, 1, 64, 64, seed=40), max_query_len=17)
     check(case([0, 17, 0], 1, 1, 64, 64, seed=41), max_query_len=17)
+
+
+def test_a_loose_max_query_len_costs_little():
+    """60 prompts of 100 tokens: how long a call takes hardly depends on whether
+    max_query_len is the longest, all tokens (its default) or a model's limit. The
+    least of several measurements, and a factor of 2 for the machine's own noise;
+    where prompts waited for one another it was 3.2 and 6."""
+    c = case([100] * 60, 4, 1, 128, 128, BF16, seed=42)
+    states, offsets, held = c["states"].clone(), ints(*c["offsets"]), ints(*c["held"])
+    args = [c[x] for x in ("q", "k", "v", "log_decay", "beta")]
+
+    def least(most):
+        times = []
+        for _ in range(6):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()
+            for _ in range(20):
+                delta_rule(*args, states, held, offsets, most)
+            end.record()
+            end.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times)
+
+    least(100)
+    exact = least(100)
+    assert least(None) < 2 * exact and least(32768) < 2 * exact
+
+
+@pytest.mark.parametrize("most", [None, 500, 10**6])
+def test_workgroups_that_take_several_prompts(most):
+    """More prompts than there is room for, of lengths around chunks and with short
+    requests between: 50 of 16 heads, where 12 fill the chip three times."""
+    lens = [(17, 64, 130, 1, 40, 65, 0, 128)[b % 8] for b in range(64)] + [500]
+    check(case(lens, 8, 2, 128, 64, F16, seed=43, lead=2, tail=5), max_query_len=most)
