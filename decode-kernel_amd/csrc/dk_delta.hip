@@ -321,10 +321,12 @@ __global__ __launch_bounds__(256) void short_conv_kernel(ConvArgs a) {
   }
 }
 
-// Requests of up to so many tokens go token by token, 1.2 us each; a chunk costs
+// Requests of up to so many tokens go token by token, 1.1 us each; a chunk costs
 // its 64 tokens' work also where few are there. 17 tokens, token by token and as
-// a chunk, us: 1 request of 32 heads 24 and 16, 8 of them 29 and 37, 64 of 4 heads
-// 27 and 40; 32 tokens 41 and 16, 48 and 37, 47 and 41.
+// a chunk, us: 1 request of 32 heads 22 and 17, 8 of them 27 and 43, 64 of 4 heads
+// 25 and 48, 200 of 8 heads 110 and 197; 32 tokens 37 and 18, 44 and 42, 43 and 48,
+// 165 and 209. One line for all: where it is wrong, for a single request or for
+// many with 17 to about 40 tokens each, a call takes up to twice as long.
 constexpr int kStepTokens = 16;
 
 }  // namespace dk

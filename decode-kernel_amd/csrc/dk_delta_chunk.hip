@@ -51,7 +51,7 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 // 1 .. 4 (1,0) (2,0) (3,0) (3,1), and in 0 what there is of (0,0) and (2,1), the 16
 // columns up to the diagonal: a lane's first 8 bytes are of the one and its last of the
 // other. Without the empty halves the operands of 8192 tokens of 32 heads are 200 MB,
-// not 225, and stay in the last cache: 2.0 and 2.3 us a chunk.
+// not 225, and a chunk's factors one piece, not two: 255 us instead of 287.
 constexpr int kTriangle = 5;
 constexpr int kParts = 3;  // bf16 parts of an entry of T and P
 
@@ -205,8 +205,8 @@ __device__ __forceinline__ float decay_of(float a, float a_rest, float b, float 
 
 // ---------------------------------------------------------------------------
 // One workgroup a chunk and head; wave w has its rows 16 w .. 16 w + 15. 8192
-// tokens of 32 heads of 128 (16 of keys), 4096 workgroups, take 69 us: 74 MB read
-// from memory and 198 written, 3.9 TB/s, which bounds it; a workgroup alone would
+// tokens of 32 heads of 128 (16 of keys), 4096 workgroups, take 70 us: 76 MB read
+// from memory and 199 written, 3.9 TB/s, which bounds it; a workgroup alone would
 // take 8 us, and next to others' stores its first loads take 4 of 13.
 // ---------------------------------------------------------------------------
 constexpr int kPad = 68;  // floats a row of 64 takes in LDS
@@ -446,9 +446,10 @@ __global__ __launch_bounds__(kPrepareThreads, 4) void delta_prepare_kernel(Delta
 // two leave in LDS, and bring the next chunk's operands there: what only the
 // outputs need is off the chain that bounds a long prompt. That chain is K' S and
 // what the corrections add, each with its largest value, a scale and two parts
-// before it, and between them the corrections, with three: 1.95 us a chunk (1.8 with
-// two fp16 parts there, too). One prompt of 8192 tokens of 32 heads takes 250 us on
-// 256 workgroups, 7 of 3001 tokens of 16 heads 44.
+// before it, and between them the corrections, with three: 1.65 us a chunk where the
+// chip has room, 1.95 to 2 on all of its CUs (1.5 and 1.8 with two fp16 parts
+// there, too). One prompt of 8192 tokens of 32 heads takes 255 us on 256
+// workgroups, of 4 heads 211 on 32, and 7 prompts of 3001 tokens of 16 heads 45.
 // ---------------------------------------------------------------------------
 using lds_ptr = __attribute__((address_space(3))) void*;
 typedef _Float16 h4_t __attribute__((ext_vector_type(4)));

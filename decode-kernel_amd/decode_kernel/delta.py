@@ -63,13 +63,14 @@ def delta_rule(
     starts from a state of zeros (without held, all go on from theirs). A request
     without rows keeps its state; rows of no request (a captured step's places
     past its last token) give 0. ``max_query_len`` (the most rows a request has;
-    default: all) picks kernels and changes no result beyond rounding.
+    default: all) picks kernels, the better the closer it is, and changes no result
+    beyond rounding.
     ``normalize`` divides q and k by sqrt(|x|^2 + 1e-6). scale: key_size ** -0.5
     by default. States, sums and decays are 32 bits, whichever kernel runs (in a
     prompt's products a state's element has 22 bits, counted from the largest of its
     column). The rule wants beta * |k|^2 of at most 2; beyond, it amplifies what it
-    holds, and near 2 with keys that hardly differ a prompt keeps 2e-3 of values and
-    state, where tokens one by one keep 1e-4. A NaN
+    holds, and near 2 with keys that hardly differ nothing fades and 64 tokens of a
+    prompt can lose 2e-3 of values and state (150 tokens one by one 1e-4). A NaN
     or infinity stays in its request (one in v in its column); in a prompt it may
     also reach up to 63 tokens before its own.
     """

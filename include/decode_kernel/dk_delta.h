@@ -63,7 +63,8 @@ typedef struct dk_delta_args {
   int key_size;
   int value_size;
   int max_query_len; /* the most tokens that a request gets. It only picks
-                        kernels; requests with more are right too */
+                        kernels, the better the closer it is; requests with
+                        more are right too */
   int normalize;     /* nonzero: q and k as x / sqrt(|x|^2 + 1e-6) */
   float scale;
 } dk_delta_args;
@@ -88,8 +89,9 @@ size_t dk_delta_workspace_bytes(int num_tokens, int requests, int qk_heads, int 
  * their roundings at the token's own time, whatever came before or comes later:
  * in a prompt's products the state has 22 bits, counted from the largest value of
  * its column, and values, decays and corrections have 24 of their own. With beta
- * |k|^2 near 2 and keys that hardly differ the corrections of a prompt's 64 tokens
- * cancel, and up to 2e-3 of values and state is lost (1e-4 token by token). A NaN or infinity
+ * |k|^2 near 2 and keys that hardly differ nothing fades, and the corrections of a
+ * prompt's 64 tokens cancel: they can lose up to 2e-3 of values and state (150
+ * tokens one by one up to 1e-4). A NaN or infinity
  * stays in its request, and one in v in its column of the state; in a prompt it
  * may reach the results of up to 63 tokens before its own, too (a chunk's
  * products multiply what comes later by 0). The
